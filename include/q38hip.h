@@ -261,6 +261,120 @@ int q38hip_attention_rows(float *attention, Q38Q8KBlock *attention_q8k, const fl
                           float *value_cache, uint32_t context_length, uint32_t position,
                           uint32_t rows, void *stream);
 
+/* ---- 3. paged 8-bit key/value cache ---------------------------------------
+ *
+ * Library extension (no counterpart in the reference, whose cache is fp32 and
+ * belongs to one sequence): keys and values of many sequences as 8-bit codes
+ * in pages that sequences can share.  Everything lives in device memory that
+ * the caller owns and describes by a Q38KVPages; the calls enqueue on
+ * `stream`, allocate nothing, read nothing back and can be captured into a
+ * HIP graph.  Calls on one cache have to be ordered (one stream, or events).
+ *
+ *   data    [layers][pages][2][kv_heads][page_tokens * head_dim] codes, 16-byte
+ *           aligned: keys (half 0) are [token][channel], values (half 1)
+ *           [channel][token]
+ *   scales  [layers][pages][2][kv_heads] powers of two; a code c stands for
+ *           c * scale (int8: -127 .. 127; e4m3: OCP float8, up to 448)
+ *   refs    [pages]: the sequences that a page belongs to; 0 is a free page
+ *   tables  [sequences][table_entries]: page of tokens entry * page_tokens ..;
+ *           -1 behind a sequence's last page
+ *   lengths [sequences]: tokens
+ *   status  [1]: Q38_KV_* bits that calls set (never clear) for what they find
+ *           in device memory; a host program reads it when it likes
+ *
+ * page_tokens is 16, 32, 64 or 128, head_dim 64, 128 or 256, table_entries *
+ * page_tokens below 2^31.  A page serves all layers.  All ids are 32-bit words
+ * in device memory.  Ids and pages outside the cache are never followed: they
+ * set a status bit, and what they stand for holds no tokens. */
+enum { Q38_KV_INT8 = 0, Q38_KV_E4M3 = 1 };
+enum {
+    Q38_KV_BAD_SEQUENCE = 1,   /* an id outside the cache, or twice in one call */
+    Q38_KV_POOL_FULL = 2,      /* extend: fewer free pages than asked for; nothing was done */
+    Q38_KV_TABLE_FULL = 4,     /* extend: longer than a table holds; nothing was done */
+    Q38_KV_BAD_PAGE = 8,       /* a page outside the pool */
+    Q38_KV_NOT_EMPTY = 16      /* fork: the child holds tokens; that pair was left out */
+};
+typedef struct {
+    uint8_t *data;
+    float *scales;
+    int32_t *refs;
+    int32_t *tables;
+    int32_t *lengths;
+    int32_t *status;
+    uint32_t layers, pages, page_tokens, kv_heads, head_dim, sequences, table_entries, type;
+} Q38KVPages;
+
+/* An empty cache: every page free, every table -1, lengths and status 0. */
+int q38hip_kv_reset(const Q38KVPages *cache, void *stream);
+
+/* Bytes of the workspace that extend and compact take (16-byte aligned device
+ * memory, one call at a time); 0 for a bad cache. */
+uint64_t q38hip_kv_workspace_bytes(const Q38KVPages *cache);
+
+/* sequences[i] grows by rows[i] tokens (count <= 1024, distinct ids): its
+ * table gets the pages, lowest free page first in the order of the items, and
+ * its length the sum.  A partly filled last page that other sequences share,
+ * after the items before i took their copies, is copied in all layers first,
+ * so what append writes is the sequence's own.  All items or none: see the
+ * status bits. */
+int q38hip_kv_extend(const Q38KVPages *cache, const int32_t *sequences, const int32_t *rows, uint32_t count,
+                     void *workspace, void *stream);
+
+/* Sequence children[i], which has to be empty, becomes the first lengths[i]
+ * tokens of parents[i] (all of them where lengths is NULL) and shares their
+ * pages.  Children are distinct and none is a parent in the same call. */
+int q38hip_kv_fork(const Q38KVPages *cache, const int32_t *parents, const int32_t *children, const int32_t *lengths,
+                   uint32_t count, void *stream);
+
+/* sequences[i] keeps its first lengths[i] tokens (0: it is freed; more than it
+ * has: unchanged); pages that no sequence holds any more are free. */
+int q38hip_kv_truncate(const Q38KVPages *cache, const int32_t *sequences, const int32_t *lengths, uint32_t count,
+                       void *stream);
+
+/* The pages in use move to the front of the pool, in place: with n in use, the
+ * j-th of them at or above n goes to the j-th free page below n.  The first
+ * two words of the workspace then hold the number of moves and n. */
+int q38hip_kv_compact(const Q38KVPages *cache, void *workspace, void *stream);
+
+/* Pages sources[i] to pages targets[i], codes and scales of all layers
+ * (a negative id: no copy); a target is no other pair's source or target. */
+int q38hip_kv_copy(const Q38KVPages *cache, const int32_t *sources, const int32_t *targets, uint32_t count,
+                   void *stream);
+
+/* Rows of the attention calls: sequences[i] owns rows row_starts[i] ..
+ * row_starts[i + 1] - 1 of total_rows (device words, non-decreasing), or
+ * total_rows / count rows each where row_starts is NULL.  They are the last
+ * rows of the sequence's tokens: row t of r stands at position
+ * length - r + t.  type is the GGML id of the rows: F32 0, F16 1, BF16 30. */
+
+/* Quantises the rows' keys and values ([kv_heads][head_dim], rows row_stride
+ * elements apart) into the pages of one layer.  Per page, head and half: with
+ * a the largest magnitude among its new tokens and k >= -100 the least with a
+ * <= M 2^k (M = 127 or 448), the scale becomes 2^k where the page holds no
+ * older token, else the larger of 2^k and what it was, and older codes are
+ * rounded to a scale that grew; new codes are value / scale, rounded to
+ * nearest, ties to even.  A value that is not finite makes the scale NaN. */
+int q38hip_kv_append(const Q38KVPages *cache, uint32_t layer, const void *key, const void *value, uint32_t type,
+                     uint64_t row_stride, const int32_t *sequences, const int32_t *row_starts, uint32_t count,
+                     uint32_t total_rows, void *stream);
+
+/* Causal attention of the rows' queries over their sequences' tokens in one
+ * layer: output[row][head] = sum softmax(scale q.k) v over positions 0 ..
+ * length - r + t, times sigmoid(gate) where gate is not NULL; zeros for a row
+ * that sees nothing.  Query head h reads key/value head h / (heads /
+ * kv_heads).  Head h of a row begins at row * query_row_stride + h *
+ * query_head_stride elements of query and of gate; output rows are
+ * output_row_stride elements apart, heads head_dim.  Sums and softmax are in
+ * fp32; fp32 rows keep 22 bits of queries and weights in the products.
+ * q38hip_kv_attention_workspace_bytes: device memory for the call (16-byte
+ * aligned; 0: none needed, or a bad call). */
+uint64_t q38hip_kv_attention_workspace_bytes(const Q38KVPages *cache, uint32_t type, uint32_t heads, uint32_t count,
+                                             uint32_t total_rows);
+int q38hip_kv_attention(const Q38KVPages *cache, uint32_t layer, void *output, const void *query, const void *gate,
+                        uint32_t type, uint32_t heads, uint64_t query_row_stride, uint64_t query_head_stride,
+                        uint64_t output_row_stride, float scale, const int32_t *sequences, const int32_t *row_starts,
+                        uint32_t count, uint32_t total_rows, void *workspace, void *stream);
+
 /* Last argument error of the calling thread ("" when none). */
 const char *q38hip_last_error(void);
 

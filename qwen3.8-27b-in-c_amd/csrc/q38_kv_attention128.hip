@@ -1,0 +1,6 @@
+/* Paged 8-bit attention of 128-wide heads. */
+#include "q38_kv_attention_launch.h"
+
+namespace q38 {
+template bool launch_kv_attention_width<128>(const KVAttention &, hipStream_t);
+}

@@ -1,0 +1,207 @@
+"""What the paged cache refuses on the host, and its index arithmetic
+(csrc/q38_kv.h) compiled for the CPU: work slots of ragged batches, bad ids and
+pages, scale exponents."""
+import ctypes
+import os
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+import kv_cases as kc
+import q38hip
+from q38hip import kv
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def _cache(**change):
+    words = ctypes.create_string_buffer(4096 + 16)
+    at = (ctypes.addressof(words) + 15) // 16 * 16
+    fields = dict(data=at, scales=at, refs=at, tables=at, lengths=at, status=at, layers=1, pages=4, page_tokens=16, kv_heads=2,
+                  head_dim=64, sequences=2, table_entries=2, type=0)
+    fields.update(change)
+    cache = kv.Pages(**fields)
+    cache.keep = words
+    return cache
+
+
+BAD_CACHES = [dict(data=0), dict(status=0), dict(layers=0), dict(pages=0), dict(kv_heads=0), dict(sequences=0),
+              dict(table_entries=0), dict(page_tokens=8), dict(page_tokens=48), dict(page_tokens=256), dict(head_dim=32),
+              dict(head_dim=96), dict(head_dim=512), dict(type=2), dict(pages=0x80000000), dict(table_entries=0x10000000),
+              dict(kv_heads=40000), dict(layers=70000), dict(sequences=0x80000000)]
+
+
+@pytest.mark.parametrize("change", BAD_CACHES, ids=str)
+def test_bad_caches_are_refused(change):
+    lib, p = kv._lib(), 4096
+    cache = ctypes.byref(_cache(**change))
+    calls = (lambda: lib.q38hip_kv_reset(cache, None), lambda: lib.q38hip_kv_workspace_bytes(cache),
+             lambda: lib.q38hip_kv_extend(cache, p, p, 1, p, None), lambda: lib.q38hip_kv_fork(cache, p, p, None, 1, None),
+             lambda: lib.q38hip_kv_truncate(cache, p, p, 1, None), lambda: lib.q38hip_kv_compact(cache, p, None),
+             lambda: lib.q38hip_kv_copy(cache, p, p, 1, None),
+             lambda: lib.q38hip_kv_append(cache, 0, p, p, 0, 128, p, None, 1, 1, None),
+             lambda: lib.q38hip_kv_attention_workspace_bytes(cache, 0, 2, 1, 1),
+             lambda: lib.q38hip_kv_attention(cache, 0, p, p, None, 0, 2, 128, 64, 128, 1.0, p, None, 1, 1, p, None))
+    for call in calls:
+        assert call() == 0 and q38hip.last_error()
+
+
+def test_bad_arguments_are_refused():
+    lib, p = kv._lib(), 4096
+    cache = ctypes.byref(_cache())
+    append = dict(layer=0, key=p, value=p, type=0, stride=128, ids=p, starts=None, count=1, total=1)
+    for change in (dict(key=None), dict(value=None), dict(type=2), dict(layer=1), dict(ids=None), dict(count=0), dict(total=0),
+                   dict(total=3, count=2), dict(total=2, stride=127), dict(total=1 << 25), dict(count=1 << 25, starts=p)):
+        a = dict(append, **change)
+        assert not lib.q38hip_kv_append(cache, a["layer"], a["key"], a["value"], a["type"], a["stride"], a["ids"], a["starts"],
+                                        a["count"], a["total"], None), change
+    good = dict(layer=0, out=p, query=p, gate=None, type=0, heads=4, row=256, head=64, to=256, ids=p, starts=None, count=1,
+                total=1, work=p)
+    for change in (dict(out=None), dict(query=None), dict(type=8), dict(heads=3), dict(heads=0), dict(layer=5), dict(head=63),
+                   dict(total=2, to=255), dict(ids=None), dict(total=0), dict(count=0), dict(total=5, count=2), dict(work=None),
+                   dict(work=p + 4)):
+        a = dict(good, **change)
+        assert not lib.q38hip_kv_attention(cache, a["layer"], a["out"], a["query"], a["gate"], a["type"], a["heads"], a["row"],
+                                           a["head"], a["to"], 1.0, a["ids"], a["starts"], a["count"], a["total"], a["work"],
+                                           None) or change.get("work", p) is None and not \
+            lib.q38hip_kv_attention_workspace_bytes(cache, 0, 4, 1, 1), change
+    assert not lib.q38hip_kv_extend(cache, p, p, 1025, p, None)
+    assert not lib.q38hip_kv_extend(cache, p, None, 1, p, None)
+    assert not lib.q38hip_kv_extend(cache, p, p, 1, None, None)
+    assert not lib.q38hip_kv_fork(cache, p, None, None, 1, None)
+    assert not lib.q38hip_kv_truncate(cache, p, None, 1, None)
+    assert not lib.q38hip_kv_compact(cache, None, None)
+    assert not lib.q38hip_kv_copy(cache, p, p, 0, None)
+
+
+def test_python_checks():
+    plain = kc.Cache(1, 4, 16, 2, 64, 2, 2, "int8").to("cpu")
+    ids = kc.words([0], "cpu")
+    row = torch.zeros(1, 2, 64)
+    for call in (lambda: kv.KVPages(plain.data, plain.scales, plain.refs, plain.tables, plain.lengths, plain.status, "int4"),
+                 lambda: kv.KVPages(plain.data[0], plain.scales, plain.refs, plain.tables, plain.lengths, plain.status, "int8"),
+                 lambda: kv.KVPages(plain.data, plain.scales[:, :2], plain.refs, plain.tables, plain.lengths, plain.status, "int8"),
+                 lambda: kv.KVPages(plain.data, plain.scales, plain.refs.long(), plain.tables, plain.lengths, plain.status, "int8"),
+                 lambda: plain.append(0, row, row.half(), ids), lambda: plain.append(0, row.double(), row.double(), ids),
+                 lambda: plain.append(0, row[:, :1], row, ids), lambda: plain.append(0, row, row, ids.long()),
+                 lambda: plain.append(0, torch.zeros(3, 2, 64), torch.zeros(3, 2, 64), kc.words([0, 1], "cpu")),
+                 lambda: plain.append(0, row, row, ids, kc.words([0], "cpu")),
+                 lambda: plain.attention(0, row[..., :32], ids), lambda: plain.attention(0, row.int(), ids),
+                 lambda: plain.attention(0, row, ids, gate=row.half()), lambda: plain.attention(0, row, ids, out=row.half()),
+                 lambda: plain.attention(0, row[0], ids), lambda: plain.extend(ids, kc.words([1, 2], "cpu")),
+                 lambda: plain.fork(ids, ids.long()), lambda: plain.truncate(ids, kc.words([], "cpu"))):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_exports():
+    declared = open(os.path.join(ROOT, "include", "q38hip.h")).read()
+    for name in kv.EXPORTS:
+        assert name + "(" in declared and hasattr(q38hip.lib(), name)
+    assert ctypes.sizeof(kv.Pages) == 6 * 8 + 8 * 4
+
+
+INDEX_CHECK = r"""
+#include <cstdio>
+#include <cstdlib>
+#include <cmath>
+#include <vector>
+#include "q38_kv.h"
+using namespace q38;
+#define CHECK(x) do { if (!(x)) { std::printf("line %d: %s\n", __LINE__, #x); return 1; } } while (0)
+static uint32_t state = 12345;
+static uint32_t draw(uint32_t n) { state = state * 1664525u + 1013904223u; return (state >> 8) % n; }
+int main()
+{
+    /* every item of every sequence has a slot of its own sequence, and the slots suffice */
+    for (int trial = 0; trial < 3000; ++trial) {
+        const uint32_t count = 1 + draw(40), per_row = 1 + draw(12), unit = 1u << draw(8), T = 16u << draw(4);
+        std::vector<int32_t> starts(1, 0), ids(count, 0);
+        for (uint32_t i = 0; i < count; ++i) starts.push_back(starts.back() + draw(trial % 3 ? 4 : 200));
+        const uint32_t total = starts.back();
+        if (!total) continue;
+        const KVRows rows{ids.data(), starts.data(), count, total, total / count};
+        for (uint32_t i = 0; i < count; ++i) {
+            const uint32_t b = kv_row_start(rows, i), e = kv_row_start(rows, i + 1);
+            const uint32_t items = ((e - b) * per_row + unit - 1) / unit;
+            CHECK(kv_slot_base(b, i, per_row, unit, 1) + items <= kv_slot_base(e, i + 1, per_row, unit, 1));
+            for (uint32_t first = 0; first < 2 * T; ++first) {
+                const uint32_t pages = e > b ? (first + e - b + T - 1) / T - first / T : 0;
+                CHECK(kv_slot_base(b, i, 1, T, 2) + pages <= kv_slot_base(e, i + 1, 1, T, 2));
+            }
+        }
+        CHECK(kv_slot_base(total, count, per_row, unit, 1) <= kv_slots(total, count, per_row, unit, 1));
+        CHECK(kv_slot_base(total, count, 1, T, 2) <= kv_slots(total, count, 1, T, 2));
+    }
+    /* offsets that are not: never past the rows */
+    int32_t odd[4] = {-7, 3, 1 << 30, 2}, id = 0;
+    const KVRows rows{&id, odd, 3, 10, 3};
+    for (uint32_t i = 0; i < 4; ++i) CHECK(kv_row_start(rows, i) <= 10);
+    const KVRows even{&id, nullptr, 3, 12, 4};
+    for (uint32_t i = 0; i < 4; ++i) CHECK(kv_row_start(even, i) == 4 * i);
+    /* ids, lengths and pages outside the cache */
+    int32_t tables[6] = {0, 4, 5, -1, 0x7fffffff, (int32_t)0x80000000}, lengths[2] = {33, 1000};
+    Q38KVPages c{};
+    c.tables = tables;
+    c.lengths = lengths;
+    c.pages = 5;
+    c.page_tokens = 16;
+    c.sequences = 2;
+    c.table_entries = 3;
+    c.kv_heads = 4;
+    c.head_dim = 256;
+    CHECK(kv_tokens(c, 0) == 33 && kv_tokens(c, 1) == 48 && kv_tokens(c, 2) == 0 && kv_tokens(c, -1) == 0);
+    lengths[0] = -3;
+    CHECK(kv_tokens(c, 0) == 0);
+    CHECK(kv_page(c, 0, 0) == 0 && kv_page(c, 0, 1) == 4 && kv_page(c, 0, 2) == -1 && kv_page(c, 0, 3) == -1);
+    CHECK(kv_page(c, 1, 0) == -1 && kv_page(c, 1, 1) == -1 && kv_page(c, 1, 2) == -1);
+    CHECK(kv_page_bytes(c) == 2 * 4 * 16 * 256 && kv_block(c, 0x7ffffffe, 1, 3) == (0x7ffffffeull * 2 + 1) * 4 + 3);
+    /* scale exponents: the least that holds the value */
+    for (int e4m3 = 0; e4m3 < 2; ++e4m3) {
+        const double most = e4m3 ? 448 : 127;
+        for (uint32_t bits = 0; bits < 0x7f800000u; bits += 9973) {
+            float v;
+            __builtin_memcpy(&v, &bits, 4);
+            const int k = kv_scale_exponent(bits, e4m3);
+            CHECK(v <= std::ldexp(most, k) && k >= -100 && k <= 122);
+            CHECK(k == -100 || v > std::ldexp(most, k - 1));
+        }
+        for (int e = -80; e < 110; ++e)
+            for (int step = -1; step <= 1; ++step) {
+                float v = (float)std::ldexp(most, e);
+                uint32_t bits;
+                __builtin_memcpy(&bits, &v, 4);
+                CHECK(kv_scale_exponent(bits + step, e4m3) == (step > 0 ? e + 1 : e));
+            }
+    }
+    std::puts("ok");
+    return 0;
+}
+"""
+
+
+def test_index_arithmetic(tmp_path):
+    source, program = tmp_path / "kv_index.cpp", tmp_path / "kv_index"
+    source.write_text(INDEX_CHECK)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror",
+                    "-I", os.path.join(ROOT, "include"), "-I", os.path.join(ROOT, "qwen3.8-27b-in-c_amd", "csrc"), str(source),
+                    "-o", str(program)], check=True)
+    assert subprocess.run([str(program)], capture_output=True, text=True, timeout=120).stdout == "ok\n"
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_model_of_the_codes(kind):
+    """the plain model's own encoding: every code stands for itself, and borders go to even"""
+    codes = np.arange(256, dtype=np.uint8)
+    values = kc.decode(codes, kind)
+    fine = np.isfinite(values) & ((values != -128) | (kind != "int8"))
+    assert np.array_equal(kc.decode(kc.encode(values[fine], kind), kind), values[fine])
+    steps = np.unique(values[fine])
+    middle = (steps[1:] + steps[:-1]) / 2
+    got = kc.decode(kc.encode(middle, kind), kind)
+    assert np.isin(got, steps).all() and (np.abs(got - middle) == (steps[1:] - steps[:-1]) / 2).all()
+    want = torch.from_numpy(middle).float()
+    want = want.round() if kind == "int8" else want.to(torch.float8_e4m3fn).float()
+    assert np.array_equal(got, want.double().numpy())
