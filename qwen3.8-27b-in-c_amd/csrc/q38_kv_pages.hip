@@ -197,7 +197,7 @@ __global__ __launch_bounds__(256) void kv_copy_kernel(Q38KVPages c, const int32_
 __global__ __launch_bounds__(256) void kv_fork_kernel(Q38KVPages c, const int32_t *parents, const int32_t *children,
                                                       const int32_t *lengths, uint32_t count)
 {
-    __shared__ uint32_t bad;
+    __shared__ uint32_t bad, taken;
     const int32_t parent = parents[blockIdx.x], child = children[blockIdx.x];
     if (threadIdx.x == 0)
         bad = parent < 0 || (uint32_t)parent >= c.sequences || child < 0 || (uint32_t)child >= c.sequences;
@@ -213,9 +213,9 @@ __global__ __launch_bounds__(256) void kv_fork_kernel(Q38KVPages c, const int32_
     const uint32_t held = kv_tokens(c, parent);
     const uint32_t tokens = lengths ? (uint32_t)min((int64_t)held, max((int64_t)0, (int64_t)lengths[blockIdx.x])) : held;
     if (!tokens) return;
-    if (threadIdx.x == 0 && atomicCAS(&c.lengths[child], 0, (int32_t)tokens) != 0) bad = 1;
+    if (threadIdx.x == 0) taken = atomicCAS(&c.lengths[child], 0, (int32_t)tokens) != 0;
     __syncthreads();
-    if (bad) {
+    if (taken) {
         if (threadIdx.x == 0) atomicOr(c.status, Q38_KV_NOT_EMPTY);
         return;
     }
