@@ -52,6 +52,13 @@ __device__ __forceinline__ float kv_other_rows(float v, bool maximum)
     auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return maximum ? fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1])) : __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
+/* l 2^d, d <= 0: a total counts pages without their value scales, so it can be
+ * as large as 2^d is small, and 2^d alone may leave fp32 */
+__device__ __forceinline__ float kv_lower(float l, float d)
+{
+    const float half = exp2f(0.5f * d);
+    return l * half * half;
+}
 /* lane n ^ 8 of the same 16 lanes (row rotation by 8) */
 __device__ __forceinline__ float kv_partner(float v)
 {
@@ -338,9 +345,9 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(KVAttention a)
             most = kv_other_rows(most, true);
             if (__any(most > m[t] + kKVMaximumSlack)) {
                 const float now = fmaxf(m[t], most);
-                const float keep = m[t] == now ? 1.0f : exp2f(m[t] - now);
+                const float by = m[t] == now ? 0.0f : m[t] - now, keep = exp2f(by);
                 m[t] = now;
-                l[t] *= keep;
+                l[t] = kv_lower(l[t], by);
 #pragma unroll
                 for (int c = 0; c < kChannels; ++c) o[t][c] *= keep;
             }
@@ -353,7 +360,18 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(KVAttention a)
                 const _Float16 high = (_Float16)w;
                 weight[t][e / 8][e & 7] = SPLIT && n >= 8 ? (_Float16)(w - (float)high) : high;
             }
-            l[t] = fmaf(sum, inverse, l[t]);
+            /* weights of a page whose value scale lies that far below the sums'
+             * largest leave fp32 before they leave the total: theirs is taken
+             * without the scale */
+            if (__any(value_log < m[t] - 64.0f && page >= 0)) {
+                const float back = value_scale == value_scale ? offset - value_log : offset;
+                sum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(u[e] + back);
+                l[t] += sum;
+            } else {
+                l[t] = fmaf(sum, inverse, l[t]);
+            }
         }
         if (!whole) {
             /* codes of tokens that no column of the slot sees may be any bytes */
@@ -443,7 +461,7 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(KVAttention a)
             for (int w = 0; w < 4; ++w) {
                 const float mw = merge_m[(w * NT + t) * kTile + c];
                 if (mw == -INFINITY) continue;
-                total += merge_l[(w * NT + t) * kTile + c] * exp2f(mw - top);
+                total += kv_lower(merge_l[(w * NT + t) * kTile + c], mw - top);
                 sum += *reinterpret_cast<const kv_float4 *>(&merge_o[(w * kTile + c) * kPitch + d]);
             }
             if (parts == 1) {

@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KVAttention a, uint32_t le
         const float m = stats[2 * row];
         if (m == -INFINITY) continue;
         const float keep = exp2f(m - top);
-        total = fmaf(stats[2 * row + 1], keep, total);
+        total += kv_lower(stats[2 * row + 1], m - top);
         sum += *reinterpret_cast<const kv_float4 *>(a.partial + row * D + d) * keep;
     }
     const uint32_t column = s.column + c;

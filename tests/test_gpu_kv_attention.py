@@ -114,6 +114,23 @@ def test_large_and_small_scales(device):
     _compare(got, want, mass, size, F32, 300)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_values_of_zero_beside_large_ones(device, dtype):
+    """pages of zeros (the least scale there is) still count in the total"""
+    rng = np.random.default_rng(17)
+    cache = kc.filled(rng, [200], "int8", 16, 1, 64)
+    for entry in range(cache.pages(200)):
+        page = cache.tables[0, entry]
+        if entry % 2:
+            cache.scales[0, page, 1, 0] *= 2.0 ** 60
+        else:
+            cache.data[0, page, 1], cache.scales[0, page, 1] = 0, 2.0 ** -100
+    q = torch.from_numpy(rng.normal(size=(3, 2, 64))).to(dtype).to(device)
+    got = cache.to(device).attention(0, q, kc.words([0], device))
+    want, mass, size = cache.attention(0, q.double().cpu().numpy(), [0], [0, 3], 0.125)
+    _compare(got, want, mass, size, dtype, 200)
+
+
 def test_offsets_past_32_bits(device):
     """pages that begin more than 4 GiB into a layer, and a second layer behind it"""
     from q38hip import kv
