@@ -90,6 +90,23 @@ Q38_HD int kv_scale_exponent(uint32_t abs_bits, bool e4m3)
     return k > kMinScaleExponent ? k : kMinScaleExponent;
 }
 
+struct KVAttention {
+    Q38KVPages cache;      /* data and scales moved to the layer */
+    KVRows rows;
+    const void *query, *gate;
+    void *output;
+    float *partial;        /* the workspace (q38_kv_attention.h) */
+    uint64_t query_row, query_head, output_row;
+    uint32_t group, page_shift;
+    uint32_t columns, slots;               /* columns of a slot, at most that many slots */
+    uint32_t workgroups, shift, least;     /* per key/value head; steps of a unit (log2); units of a workgroup at least */
+    int type;
+    float scale;           /* softmax scale times log2(e) */
+};
+/* the split of a call: fills columns, slots, workgroups, shift and least;
+ * returns the bytes of `partial` (0 where no slot is cut) */
+uint64_t plan_kv_attention(KVAttention &call);
+
 }  // namespace q38
 
 #if defined(__HIPCC__)
@@ -117,20 +134,6 @@ __device__ __forceinline__ int kv_find_sequence(const KVRows &rows, uint32_t slo
 bool launch_kv_append(const Q38KVPages &cache, uint32_t layer, const void *key, const void *value, int type,
                       uint64_t row_stride, const KVRows &rows, hipStream_t stream);
 
-struct KVAttention {
-    Q38KVPages cache;      /* data and scales moved to the layer */
-    KVRows rows;
-    const void *query, *gate;
-    void *output;
-    float *partial;        /* [slots][kv_heads][parts][columns][head_dim], then the same rows' (maximum, sum) */
-    uint64_t query_row, query_head, output_row;
-    uint32_t group, page_shift, slots, parts, columns;
-    int type;
-    bool vector;           /* query and gate rows are 16-byte aligned */
-    float scale;           /* softmax scale times log2(e) */
-};
-/* the split of a call: fills slots, parts and columns; returns the bytes of `partial` */
-uint64_t plan_kv_attention(KVAttention &call);
 bool launch_kv_attention(const KVAttention &call, hipStream_t stream);
 
 bool launch_kv_reset(const Q38KVPages &cache, hipStream_t stream);

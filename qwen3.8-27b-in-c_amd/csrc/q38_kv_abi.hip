@@ -189,9 +189,6 @@ extern "C" int q38hip_kv_attention(const Q38KVPages *cache, uint32_t layer, void
     a.query_head = query_head_stride;
     a.output_row = output_row_stride;
     a.page_shift = (uint32_t)__builtin_ctz(cache->page_tokens);
-    const uint64_t lane = type == (uint32_t)q38::kElementF32 ? 4 : 8;
-    a.vector = query_row_stride % lane == 0 && query_head_stride % lane == 0 &&
-               ((reinterpret_cast<uintptr_t>(query) | reinterpret_cast<uintptr_t>(gate)) & 15) == 0;
     a.scale = scale * 1.44269504088896340736f;
     return q38::launch_kv_attention(a, static_cast<hipStream_t>(stream)) ? 1
                                                                          : abi_fail("paged attention kernels failed");

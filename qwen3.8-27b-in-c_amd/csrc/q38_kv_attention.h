@@ -11,25 +11,29 @@
  *
  * Everything stays transposed: S^T = K Q^T and O^T = V^T W^T, on
  * v_mfma_f32_16x16x32_f16.  Lane (n = lane & 15, g = lane >> 4) holds column
- * n in the results of both, so maximum, sum and rescaling are the lane's own
- * (one exchange over g for the maximum).  Row m of the i-th of four key tiles
- * is token 16 (m / 4) + 4 i + m % 4 of a 64-token step: lane g then has the
- * scores of tokens 16 g .. 16 g + 15, which are both its slice of the second
- * product and 16 consecutive bytes of a value channel.  Keys and values come
- * straight from memory as 16-byte loads, in the order the products use them:
- * no LDS and no exchange in the loop.
+ * n in the results of both, so maximum, sum and rescaling are the lane's own.
+ * Row m of the i-th of four key tiles is token 16 (m / 4) + 4 i + m % 4 of a
+ * 64-token step: lane g then has the scores of tokens 16 g .. 16 g + 15, which
+ * are both its slice of the second product and 16 consecutive bytes of a value
+ * channel.
+ *
+ * Codes go from memory straight into LDS (global_load_lds, 1 KiB each, whole
+ * rows of keys or values, so requests are contiguous and no register waits for
+ * them), in 16-byte pieces whose place in a row is exclusive-ored with the row
+ * so that the 16 lanes that read one piece of 16 rows use all banks.
  *
  * 8-bit codes are exact in fp16, and so is a 16-bit query once its row is
- * scaled by a power of two to a maximum of 2^13..2^14.  For fp32 calls
- * (SPLIT) a column takes two lanes: n < 8 works with the fp16 value of its
- * queries and weights, n + 8 with what that leaves, 22 bits together.  16-bit
- * calls keep the fp16 weight alone: its error, 2^-12 of the weight, is an
- * eighth of a bf16 output's own rounding and, over many tokens, below an
- * fp16 output's. */
+ * scaled by a power of two to a maximum of 2^13..2^14 (but for what lies 2^37
+ * below it).  For fp32 calls (SPLIT) a column takes two lanes: n < 8 works
+ * with the fp16 value of its queries and weights, n + 8 with what that leaves,
+ * 22 bits together.  16-bit calls keep the fp16 weight alone: its error, 2^-12
+ * of the weight, is an eighth of a bf16 output's own rounding and, over many
+ * tokens, below an fp16 output's. */
 #pragma once
 
 #include "q38_device.h"
 #include "q38_kv.h"
+#include "q38_kv_plan.h"
 
 namespace q38 {
 
@@ -37,7 +41,6 @@ using kv_half2 = _Float16 __attribute__((ext_vector_type(2)));
 using kv_half8 = _Float16 __attribute__((ext_vector_type(8)));
 using kv_float4 = float __attribute__((ext_vector_type(4)));
 
-constexpr int kKVStep = 64;               /* tokens of a step */
 /* exponent of the largest weight, and how far a column's maximum may be
  * passed before its sums are rescaled: weights stay below 2^15 (fp16 holds
  * 2^16) and one 2^20 below the largest is still a normal fp16 value */
@@ -63,6 +66,17 @@ __device__ __forceinline__ float kv_lower(float l, float d)
 __device__ __forceinline__ float kv_partner(float v)
 {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, false));
+}
+
+using kv_float2 = float __attribute__((ext_vector_type(2)));
+/* two values to fp16; LOW: what fp16 leaves of them in the lanes of `mask` -1 */
+template <bool LOW>
+__device__ __forceinline__ kv_half2 kv_round2(float a, float b, uint32_t mask)
+{
+    const kv_half2 high = __builtin_convertvector((kv_float2){a, b}, kv_half2);
+    if constexpr (!LOW) return high;
+    const kv_half2 taken = __builtin_bit_cast(kv_half2, __builtin_bit_cast(uint32_t, high) & mask);
+    return __builtin_convertvector((kv_float2){a - (float)taken[0], b - (float)taken[1]}, kv_half2);
 }
 
 /* eight codes -> fp16, exactly */
@@ -91,61 +105,120 @@ __device__ __forceinline__ kv_half8 kv_decode8(uint32_t lo, uint32_t hi)
     return r.all;
 }
 
-__device__ __forceinline__ float kv_element(const void *base, uint64_t at, int type)
+/* sums times keep where `some` (uniform).  The branch is within the assembly, so
+ * that the sums are one value on both ways and stay in their accumulation
+ * registers; 18 wait states cover a matrix product that may still write them. */
+__device__ __forceinline__ void kv_scale(kv_float4 &x, kv_float4 &y, float keep, uint64_t some)
 {
-    if (type == kElementF32) return static_cast<const float *>(base)[at];
-    const uint16_t bits = static_cast<const uint16_t *>(base)[at];
-    return type == kElementF16 ? f16_to_f32(bits) : __uint_as_float((uint32_t)bits << 16);
+    float a = x[0], b = x[1], c = x[2], d = x[3], e = y[0], f = y[1], g = y[2], h = y[3], t;
+    asm volatile("s_cmp_eq_u64 %10, 0\n\ts_cbranch_scc1 1f\n\ts_nop 15\n\ts_nop 3\n\t"
+                 "v_accvgpr_read_b32 %8, %0\n\tv_mul_f32 %8, %8, %9\n\tv_accvgpr_write_b32 %0, %8\n\t"
+                 "v_accvgpr_read_b32 %8, %1\n\tv_mul_f32 %8, %8, %9\n\tv_accvgpr_write_b32 %1, %8\n\t"
+                 "v_accvgpr_read_b32 %8, %2\n\tv_mul_f32 %8, %8, %9\n\tv_accvgpr_write_b32 %2, %8\n\t"
+                 "v_accvgpr_read_b32 %8, %3\n\tv_mul_f32 %8, %8, %9\n\tv_accvgpr_write_b32 %3, %8\n\t"
+                 "v_accvgpr_read_b32 %8, %4\n\tv_mul_f32 %8, %8, %9\n\tv_accvgpr_write_b32 %4, %8\n\t"
+                 "v_accvgpr_read_b32 %8, %5\n\tv_mul_f32 %8, %8, %9\n\tv_accvgpr_write_b32 %5, %8\n\t"
+                 "v_accvgpr_read_b32 %8, %6\n\tv_mul_f32 %8, %8, %9\n\tv_accvgpr_write_b32 %6, %8\n\t"
+                 "v_accvgpr_read_b32 %8, %7\n\tv_mul_f32 %8, %8, %9\n\tv_accvgpr_write_b32 %7, %8\n\t"
+                 "s_nop 3\n1:"
+                 : "+a"(a), "+a"(b), "+a"(c), "+a"(d), "+a"(e), "+a"(f), "+a"(g), "+a"(h), "=&v"(t)
+                 : "v"(keep), "s"(some)
+                 : "scc");
+    x = {a, b, c, d};
+    y = {e, f, g, h};
 }
 
-/* elements at .. at + 7 as fp32 */
-__device__ __forceinline__ void kv_elements8(float *x, const void *base, uint64_t at, int type, bool vector)
+/* 16, 8 and 4 bytes at any alignment of the element */
+struct __attribute__((packed, aligned(2))) KVBytes16 {
+    uint32_t word[4];
+};
+struct __attribute__((packed, aligned(2))) KVBytes8 {
+    uint32_t word[2];
+};
+struct __attribute__((packed, aligned(4))) KVFloats4 {
+    float v[4];
+};
+
+__device__ __forceinline__ float kv_half(uint32_t bits, int type)
 {
-    if (!vector) {
-        for (int e = 0; e < 8; ++e) x[e] = kv_element(base, at + e, type);
-    } else if (type == kElementF32) {
-        const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at);
-        const float4 a = p[0], b = p[1];
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    return type == kElementF16 ? f16_to_f32(bits) : __uint_as_float(bits << 16);
+}
+
+/* elements at .. at + 7 as stored: fp32 eight words, 16-bit types four */
+template <bool F32>
+__device__ __forceinline__ void kv_load8(uint32_t *raw, const void *base, uint64_t at)
+{
+    if constexpr (F32) {
+        const KVFloats4 *p = reinterpret_cast<const KVFloats4 *>(static_cast<const float *>(base) + at);
+        const KVFloats4 a = p[0], b = p[1];
+        for (int e = 0; e < 4; ++e) raw[e] = __float_as_uint(a.v[e]), raw[4 + e] = __float_as_uint(b.v[e]);
     } else {
-        const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + at);
-        const uint32_t word[4] = {v.x, v.y, v.z, v.w};
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t bits = e & 1 ? word[e / 2] >> 16 : word[e / 2] & 0xffffu;
-            x[e] = type == kElementF16 ? f16_to_f32(bits) : __uint_as_float(bits << 16);
-        }
+        const KVBytes16 v = *reinterpret_cast<const KVBytes16 *>(static_cast<const uint16_t *>(base) + at);
+        for (int e = 0; e < 4; ++e) raw[e] = v.word[e];
     }
 }
+template <bool F32>
+__device__ __forceinline__ float kv_element8(const uint32_t *raw, int e, int type)
+{
+    if constexpr (F32) return __uint_as_float(raw[e]);
+    else return kv_half(e & 1 ? raw[e / 2] >> 16 : raw[e / 2] & 0xffffu, type);
+}
 
+/* elements at .. at + 3 */
+__device__ __forceinline__ kv_float4 kv_load4(const void *base, uint64_t at, int type)
+{
+    if (type == kElementF32) {
+        const KVFloats4 v = *reinterpret_cast<const KVFloats4 *>(static_cast<const float *>(base) + at);
+        return {v.v[0], v.v[1], v.v[2], v.v[3]};
+    }
+    const KVBytes8 v = *reinterpret_cast<const KVBytes8 *>(static_cast<const uint16_t *>(base) + at);
+    return {kv_half(v.word[0] & 0xffffu, type), kv_half(v.word[0] >> 16, type), kv_half(v.word[1] & 0xffffu, type),
+            kv_half(v.word[1] >> 16, type)};
+}
 /* four consecutive outputs, rounded once */
 __device__ __forceinline__ void kv_store4(void *base, uint64_t at, int type, const kv_float4 v)
 {
     if (type == kElementF32) {
-        float *p = static_cast<float *>(base) + at;
-        for (int e = 0; e < 4; ++e) p[e] = v[e];
+        *reinterpret_cast<KVFloats4 *>(static_cast<float *>(base) + at) = {{v[0], v[1], v[2], v[3]}};
     } else {
-        uint16_t *p = static_cast<uint16_t *>(base) + at;
+        uint32_t bits[4];
         for (int e = 0; e < 4; ++e)
-            p[e] = type == kElementF16 ? __builtin_bit_cast(uint16_t, (_Float16)v[e])
-                                       : __builtin_bit_cast(uint16_t, (__bf16)v[e]);
+            bits[e] = type == kElementF16 ? __builtin_bit_cast(uint16_t, (_Float16)v[e])
+                                          : __builtin_bit_cast(uint16_t, (__bf16)v[e]);
+        *reinterpret_cast<KVBytes8 *>(static_cast<uint16_t *>(base) + at) = {{bits[0] | bits[1] << 16, bits[2] | bits[3] << 16}};
     }
+}
+
+/* 1 / (1 + e^-x) within 2^-22 of itself: x log2(e) in two parts, so the error
+ * does not grow with x */
+__device__ __forceinline__ float kv_sigmoid(float x)
+{
+    constexpr float kHigh = 1.44269502f, kLow = 1.92596299e-8f;
+    float t = -x * kHigh;
+    const float rest = fmaf(-x, kHigh, -t) - x * kLow;
+    if (t > 126.0f) t = 126.0f;
+    const float e = __builtin_amdgcn_exp2f(t), d = 1.0f + fmaf(e, rest * 0.693147182f, e);
+    const float inverse = __builtin_amdgcn_rcpf(d);
+    return fmaf(inverse, fmaf(-d, inverse, 1.0f), inverse);
 }
 
 /* out[row][head][d .. d + 3] = O / l, times sigmoid(gate); 0 where the row saw nothing */
 __device__ __forceinline__ void kv_finish4(const KVAttention &a, uint32_t row, uint32_t head, uint32_t d, kv_float4 o,
                                            float l)
 {
-    const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-    for (int e = 0; e < 4; ++e) o[e] *= inverse;
+    o *= l == 0.0f ? 0.0f : 1.0f / l;
     if (a.gate) {
-        const uint64_t at = row * a.query_row + head * a.query_head + d;
-        for (int e = 0; e < 4; ++e) o[e] = o[e] / (1.0f + expf(-kv_element(a.gate, at + e, a.type)));
+        const kv_float4 gate = kv_load4(a.gate, row * a.query_row + head * a.query_head + d, a.type);
+        for (int e = 0; e < 4; ++e) o[e] *= kv_sigmoid(gate[e]);
     }
     kv_store4(a.output, row * a.output_row + (uint64_t)head * a.cache.head_dim + d, a.type, o);
 }
 
-/* what a work slot covers; false for a slot with nothing to do */
+/* ---- work ---------------------------------------------------------------------- */
+
+/* A slot: up to a.columns columns of one sequence. */
 struct KVSlot {
+    uint32_t index;                              /* among the call's slots */
     uint32_t first_row, rows, column, columns;   /* columns column .. column + columns - 1 of the sequence's rows x group */
     int32_t sequence, tokens;                    /* sequence -1 where the id is bad */
     int32_t seen;                                /* tokens the slot's last row sees */
@@ -154,328 +227,578 @@ struct KVSlot {
         return tokens - (int32_t)rows + (int32_t)(column_at / group) + 1;
     }
 };
-__device__ __forceinline__ bool kv_slot(const KVAttention &a, uint32_t slot, KVSlot &s)
-{
-    const int i = kv_find_sequence(a.rows, slot, a.group, a.columns, 1);
-    if (i < 0) return false;
-    const uint32_t begin = kv_row_start(a.rows, i), end = kv_row_start(a.rows, i + 1);
-    s.first_row = begin;
-    s.rows = end > begin ? end - begin : 0;
-    s.column = (slot - kv_slot_base(begin, i, a.group, a.columns, 1)) * a.columns;
-    if (s.column >= s.rows * a.group) return false;
-    s.columns = min(a.columns, s.rows * a.group - s.column);
-    const int32_t id = a.rows.sequences[i];
-    s.tokens = (int32_t)kv_tokens(a.cache, id);
-    s.sequence = s.tokens > 0 ? id : -1;
-    s.seen = max(0, s.seen_by(s.column + s.columns - 1, a.group));
-    return true;
-}
-/* parts of the token axis that a slot is worked on in: at least
- * `least` steps each */
-__device__ __forceinline__ uint32_t kv_parts(const KVAttention &a, uint32_t steps, uint32_t least)
-{
-    return max(1u, min(a.parts, (steps + least - 1) / least));
-}
-constexpr uint32_t kKVLeastStepsTokens = 4;   /* one per wavefront */
-constexpr uint32_t kKVLeastStepsColumns = 8;
 
-/* One workgroup of four wavefronts per (slot, part, key/value head).
+/* 64 sequences of the call, one per lane, and the prefix sums of their slots
+ * and units (kv_slot_units) */
+struct KVLanes {
+    uint32_t first, count;                       /* of the block; sequences of the call */
+    uint32_t begin, end, slots, each;            /* the lane's; units of each slot */
+    int32_t id, tokens;
+    uint32_t slots_upto, units_upto;             /* inclusive, within the block */
+    bool good;                                   /* the block's row offsets do not decrease */
+
+    __device__ __forceinline__ void load(const KVAttention &a, uint32_t at)
+    {
+        const uint32_t lane = threadIdx.x & 63, i = at + lane;
+        first = at;
+        begin = end = slots = each = 0;
+        id = -1;
+        tokens = 0;
+        if (i < a.rows.count) {
+            id = a.rows.sequences[i];
+            begin = kv_row_start(a.rows, i);
+            end = kv_row_start(a.rows, i + 1);
+            tokens = (int32_t)kv_tokens(a.cache, id);
+            slots = ((end - begin) * a.group + a.columns - 1) / a.columns;
+            each = kv_slot_units(kv_steps((uint32_t)tokens), a.shift);
+        }
+        good = __all(begin <= end);
+        slots_upto = slots;
+        units_upto = slots * each;
+        for (int by = 1; by < 64; by *= 2) {
+            const uint32_t s = (uint32_t)__shfl_up((int)slots_upto, by), u = (uint32_t)__shfl_up((int)units_upto, by);
+            if (lane >= (uint32_t)by) slots_upto += s, units_upto += u;
+        }
+    }
+    static __device__ __forceinline__ uint32_t of(uint32_t v, int lane)
+    {
+        return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+    }
+};
+
+/* What a workgroup does.  The slots' units, one after another, are cut into
+ * equal ranges, one per workgroup (and key/value head); a slot of few units
+ * goes whole to the range that it begins in. */
+struct KVWalk {
+    KVLanes block;
+    uint32_t block_slots, block_units;           /* of the sequences before the block */
+    uint32_t total_slots, total_units, chunk, small, at, end;
+
+    __device__ __forceinline__ void start(const KVAttention &a, uint32_t workgroup)
+    {
+        total_slots = total_units = block_slots = block_units = 0;
+        bool good = true;
+        for (uint32_t first = (a.rows.count - 1) / 64 * 64 + 64; first; ) {
+            first -= 64;
+            block.load(a, first);
+            total_slots += KVLanes::of(block.slots_upto, 63);
+            total_units += KVLanes::of(block.units_upto, 63);
+            good = good && block.good;
+        }
+        if (!good) {
+            /* the sums mean nothing, and the workspace need not hold the slots */
+            if (threadIdx.x == 0) atomicOr(a.cache.status, Q38_KV_BAD_ROWS);
+            total_slots = total_units = 0;
+        }
+        chunk = kv_chunk(total_units, a.workgroups, a.least);
+        small = kv_small(chunk);
+        at = min((uint64_t)workgroup * chunk, (uint64_t)total_units);
+        end = min((uint64_t)at + chunk, (uint64_t)total_units);
+    }
+
+    /* the next piece of a slot; false when there is none */
+    __device__ __forceinline__ bool next(const KVAttention &a, KVSlot &s, KVPiece &piece)
+    {
+        const uint32_t from = at;
+        while (at < end) {
+            while (at - block_units >= KVLanes::of(block.units_upto, 63)) {
+                block_slots += KVLanes::of(block.slots_upto, 63);
+                block_units += KVLanes::of(block.units_upto, 63);
+                block.load(a, block.first + 64);
+            }
+            const int i = __popcll(__ballot(block.units_upto <= at - block_units));
+            const uint32_t slots = KVLanes::of(block.slots, i), each = KVLanes::of(block.each, i);
+            const uint32_t base = block_units + KVLanes::of(block.units_upto, i) - slots * each;
+            const uint32_t j = slots == 1 ? 0 : (at - base) / each, slot_at = base + j * each;
+            s.first_row = KVLanes::of(block.begin, i);
+            s.rows = KVLanes::of(block.end, i) - s.first_row;
+            s.index = block_slots + KVLanes::of(block.slots_upto, i) - slots + j;
+            s.column = j * a.columns;
+            s.columns = min(a.columns, s.rows * a.group - s.column);
+            s.tokens = (int32_t)KVLanes::of((uint32_t)block.tokens, i);
+            s.sequence = s.tokens > 0 ? (int32_t)KVLanes::of((uint32_t)block.id, i) : -1;
+            s.seen = max(0, s.seen_by(s.column + s.columns - 1, a.group));
+            at = slot_at + each;
+            piece = kv_piece(slot_at, each, kv_steps((uint32_t)s.seen), from, end, small, a.shift);
+            if (piece.some) return true;
+        }
+        return false;
+    }
+};
+
+/* Workspace of a call whose slots may be cut: one KVRecord per slot (record 0
+ * is the number of slots), then the sums of the pieces, then their (maximum,
+ * total). */
+struct KVRecord {
+    uint32_t pieces, first_piece, first_row, column, columns, unused[3];
+};
+__device__ __forceinline__ KVRecord *kv_records(const KVAttention &a) { return reinterpret_cast<KVRecord *>(a.partial); }
+__device__ __forceinline__ float *kv_partial(const KVAttention &a, uint64_t piece, uint32_t head)
+{
+    return a.partial + (a.slots + 1) * (sizeof(KVRecord) / 4) + (piece * a.cache.kv_heads + head) * a.columns * a.cache.head_dim;
+}
+__device__ __forceinline__ float *kv_stats(const KVAttention &a, uint64_t piece, uint32_t head)
+{
+    return kv_partial(a, (uint64_t)a.workgroups + a.slots, 0) + (piece * a.cache.kv_heads + head) * a.columns * 2;
+}
+
+/* ---- codes to LDS -------------------------------------------------------------- */
+
+__device__ __forceinline__ uint32_t kv_lds(const void *p)
+{
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
+}
+/* 16 (4) bytes per lane to LDS at `to` + 16 (4) lane.  Inline assembly keeps
+ * the compiler's wait counts out of it: callers wait. */
+__device__ __forceinline__ void kv_copy16(const void *from, uint32_t to)
+{
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory", "m0");
+}
+__device__ __forceinline__ void kv_copy4(const void *from, uint32_t to)
+{
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(to) : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void kv_wait()
+{
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+/* the wavefront's LDS reads have returned: what they read may be overwritten */
+__device__ __forceinline__ void kv_reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void kv_barrier()
+{
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+/* The 64 tokens of a step as D * 64 bytes of keys and as many of values.
+ * Key row r = 16 i + n (token 16 (n / 4) + 4 i + n % 4) holds its 16-byte
+ * pieces p at p ^ kv_key_turn(n); value row (channel) its four at p ^ (n / 4),
+ * n the channel's low four bits. */
+template <int D>
+__device__ __forceinline__ uint32_t kv_key_turn(uint32_t n)
+{
+    return D == 256 ? n : D == 128 ? n >> 1 : n >> 2;
+}
+
+/* One workgroup of four wavefronts per (range of work, key/value head).
  * COLUMNS false: the wavefronts take steps of the tokens in turn, over the
- * same NT tiles of columns, and are joined at the end.  COLUMNS true (prompt
- * chunks): every wavefront has NT column tiles of its own over all steps. */
+ * same NT tiles of columns, each with its own step in LDS, and are joined at
+ * the end.  COLUMNS true (prompt chunks): every wavefront has NT column tiles
+ * of its own over all steps, which all four read from one pair of buffers. */
+template <int D, bool COLUMNS>
+constexpr int kv_ring_bytes() { return (COLUMNS ? 2 : 4) * 128 * D; }
+constexpr int kKVMetaBytes = 4 * 2 * 256;
+template <int D, int TILE, bool COLUMNS>
+constexpr int kv_lds_bytes()
+{
+    constexpr int merge = 4 * TILE * (D + 4) * 4;
+    return (kv_ring_bytes<D, COLUMNS>() > merge ? kv_ring_bytes<D, COLUMNS>() : merge) + kKVMetaBytes;
+}
+
 template <bool E4M3, int D, int NT, bool SPLIT, bool COLUMNS>
-__global__ __launch_bounds__(256) void kv_attention_kernel(KVAttention a)
+__global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_kernel(KVAttention a)
 {
     constexpr int kTile = SPLIT ? 8 : 16;
+    constexpr bool kAccumulators = kv_waves(D, NT, COLUMNS) == 1;  /* more registers than VGPRs: sums in AGPRs */
     constexpr int kChunks = D / 64, kChannels = D / 16;
     constexpr int kPitch = D + 4;
-    __shared__ float merge_o[COLUMNS ? 1 : 4 * kTile * kPitch];
-    __shared__ float merge_m[COLUMNS ? 1 : 4 * NT * kTile], merge_l[COLUMNS ? 1 : 4 * NT * kTile];
+    constexpr int kCopies = D / 16;                                /* copies of 1 KiB of a step's keys or values */
+    constexpr int kRuns = D / 64;                                  /* of 16-token groups that a lane copies keys of */
+    __shared__ __attribute__((aligned(16))) uint8_t ring[kv_lds_bytes<D, kTile, COLUMNS>()];
+    __shared__ float merge_m[4 * NT * kTile], merge_l[4 * NT * kTile];
 
-    const uint32_t slot = blockIdx.x, head = blockIdx.y, part = blockIdx.z;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    const uint32_t T = a.cache.page_tokens;
+    const uint32_t head = blockIdx.y;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    const uint32_t T = a.cache.page_tokens, low_half = n >= 8 ? 0xffffffffu : 0u;
+    uint8_t *mine = ring + (COLUMNS ? 0 : wave * 128 * D);        /* the (first) keys; values 64 D behind */
+    float *meta = reinterpret_cast<float *>(ring + kv_lds_bytes<D, kTile, COLUMNS>() - kKVMetaBytes) + wave * 128;
+
+    /* LDS places of the lane's reads */
+    uint32_t key_at[kChunks];
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) key_at[j] = n * D + (((uint32_t)(4 * j + g) ^ kv_key_turn<D>(n)) & (D / 16 - 1)) * 16;
+    const uint32_t value_at = 64 * D + n * 64 + (g ^ (n >> 2)) * 16;
+    /* what the lane copies.  Keys: copy d = kRuns i + run is rows 16 i + (64 /
+     * D..) of the tile: within a run every i is four tokens further on */
+    constexpr int kLanesPerRow = D / 16, kRowsPerCopy = 64 / kLanesPerRow;
+    const uint32_t copy_row = lane / kLanesPerRow;                /* + run * kRowsPerCopy = n of the row */
+    const uint32_t value_group = (lane & 3) ^ ((lane >> 4) & 3);
+
+    KVWalk walk;
+    walk.start(a, blockIdx.x);
+    if (a.workgroups > 1 && blockIdx.x == 0 && head == 0 && threadIdx.x == 0) kv_records(a)->pieces = walk.total_slots;
     KVSlot s;
-    if (!kv_slot(a, slot, s)) return;
-    const uint32_t steps = (s.seen + kKVStep - 1) / kKVStep;
-    const uint32_t parts = kv_parts(a, steps, COLUMNS ? kKVLeastStepsColumns : kKVLeastStepsTokens);
-    if (part >= parts) return;
-    uint32_t step = (uint64_t)steps * part / parts, end = (uint64_t)steps * (part + 1) / parts;
-
-    /* the wavefront's columns */
-    uint32_t column[NT];
-    int32_t seen[NT], seen_least = 0x7fffffff, seen_most = 0;
-    float to_u[NT];
-    kv_half8 q[NT][2 * kChunks];
+    KVPiece piece;
+    while (walk.next(a, s, piece)) {
+        /* the wavefront's columns */
+        uint32_t column[NT];
+        int32_t seen[NT], seen_least = 0x7fffffff, seen_most = 0;
+        float to_u[NT];
+        kv_half8 q[NT][2 * kChunks];
+        constexpr int kRaw = SPLIT ? 8 : 4;
+        uint32_t raw[NT][2 * kChunks][kRaw];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        column[t] = ((COLUMNS ? wave * NT : 0) + t) * kTile + (SPLIT ? n & 7 : n);
-        const bool held = column[t] < s.columns;
-        const uint32_t at = s.column + (held ? column[t] : 0);
-        seen[t] = held ? s.seen_by(at, a.group) : 0;
-        float x[kChunks * 16];
-        uint32_t largest = 0;
-        const uint64_t from = (s.first_row + at / a.group) * a.query_row + (head * a.group + at % a.group) * a.query_head;
+        for (int t = 0; t < NT; ++t) {
+            column[t] = ((COLUMNS ? wave * NT : 0) + t) * kTile + (SPLIT ? n & 7 : n);
+            const bool held = column[t] < s.columns;
+            const uint32_t at = s.column + (held ? column[t] : 0);
+            seen[t] = held ? s.seen_by(at, a.group) : 0;
+            const uint64_t from = (s.first_row + at / a.group) * a.query_row + (head * a.group + at % a.group) * a.query_head;
 #pragma unroll
-        for (int c = 0; c < 2 * kChunks; ++c) {
-            kv_elements8(x + 8 * c, a.query, from + (c / 2) * 64 + g * 16 + (c & 1) * 8, a.type, a.vector);
+            for (int c = 0; c < 2 * kChunks; ++c) kv_load8<SPLIT>(raw[t][c], a.query, from + (c / 2) * 64 + g * 16 + (c & 1) * 8);
+        }
+        /* least and most over the wavefront's columns: columns are in row order */
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if (!held) x[8 * c + e] = 0.0f;
-                largest = max(largest, __float_as_uint(x[8 * c + e]) & 0x7fffffffu);
+        for (int t = 0; t < NT; ++t) {
+            const uint32_t first = ((COLUMNS ? wave * NT : 0) + t) * kTile;
+            if (first < s.columns) {
+                seen_least = min(seen_least, s.seen_by(s.column + first, a.group));
+                seen_most = max(seen_most, s.seen_by(s.column + min(first + kTile, s.columns) - 1, a.group));
             }
         }
-        /* non-negative floats order as their bits; NaN is above all of them */
-        {
-            auto r = __builtin_amdgcn_permlane16_swap(largest, largest, false, false);
-            largest = max(r[0], r[1]);
-            r = __builtin_amdgcn_permlane32_swap(largest, largest, false, false);
-            largest = max(r[0], r[1]);
-        }
-        const uint32_t exponent = max(largest >> 23, 30u);
-        const float scale = __uint_as_float((267u - exponent) << 23);       /* largest * scale in 2^13..2^14 */
-        to_u[t] = a.scale * __uint_as_float((exponent - 13u) << 23);
+        constexpr uint32_t kStride = COLUMNS ? 1 : 4;
+        uint32_t step = piece.first + (COLUMNS ? 0 : wave);
+        const uint32_t end = piece.last, own_end = COLUMNS ? min(end, kv_steps((uint32_t)max(seen_most, 0))) : end;
+
+        /* pages of 16 steps: lane l has that of tokens 16 (l % 4) .. of the
+         * step that is l / 4 turns after the first; their scales go to LDS */
+        int32_t pages = -1;
+        uint32_t turn = 0;
+        auto load_pages = [&](uint32_t first) {
+            const uint32_t at = first + (lane >> 2) * kStride, token = at * kKVStep + 16 * (lane & 3);
+            pages = -1;
+            if (at < end && s.sequence >= 0 && token < (uint32_t)s.seen)
+                pages = kv_page(a.cache, s.sequence, token >> a.page_shift);
+            turn = 0;
+            const float *scales = a.cache.scales + kv_block(a.cache, max(pages, 0), 0, head);
+            kv_copy4(scales, kv_lds(meta));
+            kv_copy4(scales + a.cache.kv_heads, kv_lds(meta + 64));
+        };
+        auto copy_keys = [&](uint32_t at, uint32_t to, int first, int count) {
 #pragma unroll
-        for (int c = 0; c < 2 * kChunks; ++c)
+            for (int run = 0; run < kRuns; ++run) {
+                const uint32_t row = run * kRowsPerCopy + copy_row;            /* n */
+                const uint32_t chunk = ((lane % kLanesPerRow) ^ kv_key_turn<D>(row)) & (kLanesPerRow - 1);
+                const uint32_t token = at * kKVStep + 16 * (row >> 2) + (row & 3);
+                const int32_t page = max(__shfl(pages, (int)(4 * turn + (row >> 2))), 0);
+                const uint8_t *from = a.cache.data + kv_block(a.cache, page, 0, head) * (T * D) + (token & (T - 1)) * D + chunk * 16;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float v = x[8 * c + e] * scale;
-                const _Float16 high = (_Float16)v;
-                q[t][c][e] = SPLIT && n >= 8 ? (_Float16)(v - (float)high) : high;
+                for (int i = first; i < first + count; ++i) kv_copy16(from + 4 * i * D, to + (kRuns * i + run) * 1024);
             }
-    }
-    /* least and most over the wavefront's columns: columns are in row order */
-    for (int t = 0; t < NT; ++t) {
-        const uint32_t first = ((COLUMNS ? wave * NT : 0) + t) * kTile;
-        if (first < s.columns) {
-            seen_least = min(seen_least, s.seen_by(s.column + first, a.group));
-            seen_most = max(seen_most, s.seen_by(s.column + min(first + kTile, s.columns) - 1, a.group));
-        }
-    }
-    if (COLUMNS) end = min(end, (uint32_t)(max(seen_most, 0) + kKVStep - 1) / kKVStep);
+        };
+        auto copy_values = [&](uint32_t at, uint32_t to, int first, int count) {
+            const int32_t page = max(__shfl(pages, (int)(4 * turn + value_group)), 0);
+            const uint8_t *from = a.cache.data + kv_block(a.cache, page, 1, head) * (T * D) + (first * 16 + (lane >> 2)) * T +
+                                  ((at * kKVStep + 16 * value_group) & (T - 1));
+#pragma unroll
+            for (int c = 0; c < count; ++c) kv_copy16(from + c * 16 * T, to + (first + c) * 1024);
+        };
 
-    kv_float4 o[NT][kChannels];
-    float m[NT], l[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        m[t] = -INFINITY;
-        l[t] = 0.0f;
-#pragma unroll
-        for (int c = 0; c < kChannels; ++c) o[t][c] = {0.0f, 0.0f, 0.0f, 0.0f};
-    }
-
-    constexpr uint32_t kStride = COLUMNS ? 1 : 4;
-    if (!COLUMNS) step += wave;
-    /* the page of the 16 tokens of lane group `part_of` of a step; -1: none */
-    auto page_of = [&](uint32_t at, int part_of) -> int32_t {
-        const uint32_t token = at * kKVStep + 16 * part_of;
-        if (s.sequence < 0 || token >= (uint32_t)s.seen) return -1;
-        return kv_page(a.cache, s.sequence, token >> a.page_shift);
-    };
-    uint4 k[4][kChunks];
-    auto load_keys = [&](uint32_t at, int32_t page) {
-        const uint32_t token = at * kKVStep + 16 * (n >> 2);
-        const uint8_t *from = a.cache.data + kv_block(a.cache, max(page, 0), 0, head) * (T * D) +
-                              ((token & (T - 1)) + (n & 3)) * D + g * 16;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < kChunks; ++j) k[i][j] = *reinterpret_cast<const uint4 *>(from + 4 * i * D + j * 64);
-    };
-    int32_t key_page = step < end ? page_of(step, n >> 2) : -1, page = step < end ? page_of(step, g) : -1;
-    if (step < end) load_keys(step, key_page);
-    for (; step < end; step += kStride) {
-        const uint32_t token = step * kKVStep + 16 * g;
-        /* this step's values and scales */
-        const uint64_t block = kv_block(a.cache, max(page, 0), 1, head);
-        uint4 v[kChannels];
-        {
-            const uint8_t *from = a.cache.data + block * (T * D) + n * T + (token & (T - 1));
-#pragma unroll
-            for (int c = 0; c < kChannels; ++c) v[c] = *reinterpret_cast<const uint4 *>(from + c * 16 * T);
+        load_pages(step);
+        if (step < end) {
+            if (COLUMNS) {
+                copy_keys(step, kv_lds(mine), wave, 1);
+                copy_values(step, kv_lds(mine) + 64 * D, wave * (kCopies / 4), kCopies / 4);
+            } else {
+                copy_keys(step, kv_lds(mine), 0, 4);
+                copy_values(step, kv_lds(mine) + 64 * D, 0, kCopies);
+            }
         }
-        float key_scale = 1.0f, value_scale = 1.0f;
-        if (page >= 0) {
-            key_scale = a.cache.scales[block - a.cache.kv_heads];
-            value_scale = a.cache.scales[block];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            uint32_t largest = 0;
+            const bool held = column[t] < s.columns;
+#pragma unroll
+            for (int c = 0; c < 2 * kChunks; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    largest = max(largest, __float_as_uint(kv_element8<SPLIT>(raw[t][c], e, a.type)) & 0x7fffffffu);
+            /* non-negative floats order as their bits; NaN is above all of them */
+            {
+                auto r = __builtin_amdgcn_permlane16_swap(largest, largest, false, false);
+                largest = max(r[0], r[1]);
+                r = __builtin_amdgcn_permlane32_swap(largest, largest, false, false);
+                largest = max(r[0], r[1]);
+            }
+            if (!held) largest = 0;
+            const uint32_t exponent = max(largest >> 23, 30u);
+            const float scale = held ? __uint_as_float((267u - exponent) << 23) : 0.0f;   /* largest * scale in 2^13..2^14 */
+            to_u[t] = a.scale * __uint_as_float((exponent - 13u) << 23);
+#pragma unroll
+            for (int c = 0; c < 2 * kChunks; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const kv_half2 pair = kv_round2<SPLIT>(kv_element8<SPLIT>(raw[t][c], e, a.type) * scale,
+                                                           kv_element8<SPLIT>(raw[t][c], e + 1, a.type) * scale, low_half);
+                    q[t][c][e] = pair[0], q[t][c][e + 1] = pair[1];
+                }
         }
-        const bool next = step + kStride < end;
-        const int32_t next_key_page = next ? page_of(step + kStride, n >> 2) : -1;
-        const int32_t next_page = next ? page_of(step + kStride, g) : -1;
 
-        kv_float4 score[NT][4];
+        kv_float4 o[NT][kChannels];
+        float m[NT], l[NT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int t = 0; t < NT; ++t) {
+            m[t] = -INFINITY;
+            l[t] = 0.0f;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) score[t][i] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int c = 0; c < kChannels; ++c) o[t][c] = {0.0f, 0.0f, 0.0f, 0.0f};
+        }
+
+        /* one step's columns: keys and values of `tile` */
+        uint32_t tile = 0;
+        while (step < end) {
+            const bool more = step + kStride < end;
+            kv_wait<COLUMNS ? 0 : kCopies>();                     /* the keys are there */
+            if (COLUMNS) kv_barrier();
+            const int32_t page = __shfl(pages, (int)(4 * turn + g));
+            float key_scale = meta[4 * turn + g], value_scale = meta[64 + 4 * turn + g];
+            if (page < 0) key_scale = value_scale = 1.0f;
+            const bool refresh = turn == 15;
+            if (COLUMNS && more) {
+                kv_reads_done();
+                ++turn;
+                if (refresh) load_pages(step + kStride);
+                const uint32_t to = kv_lds(mine) + (tile ^ (128 * D));
+                copy_keys(step + kStride, to, wave, 1);
+                copy_values(step + kStride, to + 64 * D, wave * (kCopies / 4), kCopies / 4);
+            }
+            const uint8_t *codes = mine + tile;
+            if (!COLUMNS || step < own_end) {
+                kv_float4 score[NT][4];
 #pragma unroll
-            for (int j = 0; j < kChunks; ++j) {
-                const kv_half8 low = kv_decode8<E4M3>(k[i][j].x, k[i][j].y), high = kv_decode8<E4M3>(k[i][j].z, k[i][j].w);
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) score[t][i] = {0.0f, 0.0f, 0.0f, 0.0f};
+                {
+                    /* pieces in the order (j, i), read two ahead; the fences keep the
+                     * compiler from reading all of them first, for which there are no registers */
+                    uint4 raw_codes[3];
+#pragma unroll
+                    for (int p = 0; p < 2; ++p)
+                        raw_codes[p] = *reinterpret_cast<const uint4 *>(codes + key_at[p / 4] + p % 4 * 16 * D);
+#pragma unroll
+                    for (int p = 0; p < 4 * kChunks; ++p) {
+                        const int i = p % 4, j = p / 4, ahead = p + 2;
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (ahead < 4 * kChunks)
+                            raw_codes[ahead % 3] = *reinterpret_cast<const uint4 *>(codes + key_at[ahead / 4] + ahead % 4 * 16 * D);
+                        const uint4 k = raw_codes[p % 3];
+                        const kv_half8 low = kv_decode8<E4M3>(k.x, k.y), high = kv_decode8<E4M3>(k.z, k.w);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+                            score[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(low, q[t][2 * j], score[t][i], 0, 0, 0);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+                            score[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(high, q[t][2 * j + 1], score[t][i], 0, 0, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (!COLUMNS && more) {
+                    kv_reads_done();
+                    ++turn;
+                    if (refresh) load_pages(step + kStride);
+                    copy_keys(step + kStride, kv_lds(mine), 0, 4);
+                }
+
+                const uint32_t token = step * kKVStep + 16 * g;
+                const uint32_t scale_bits = __float_as_uint(value_scale);
+                const float value_log = value_scale == value_scale ? (float)((int)(scale_bits >> 23) - 127) : value_scale;
+                const float inverse = __uint_as_float((254u << 23) - scale_bits);
+                const bool whole = step * kKVStep + kKVStep <= (uint32_t)max(seen_least, 0) && __all(page >= 0);
+                kv_half8 weight[NT][2];
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    score[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(low, q[t][2 * j], score[t][i], 0, 0, 0);
-                    score[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(high, q[t][2 * j + 1], score[t][i], 0, 0, 0);
+                    const float factor = to_u[t] * key_scale;
+                    const float base = value_log + kKVWeightExponent - m[t];
+                    float u[16], most = -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        if (SPLIT) score[t][e / 4][e & 3] += kv_partner(score[t][e / 4][e & 3]);
+                        u[e] = fmaf(score[t][e / 4][e & 3], factor, base);
+                    }
+                    if (!whole) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (page < 0 || (int32_t)(token + e) >= seen[t]) u[e] = score[t][e / 4][e & 3] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) most = fmaxf(most, u[e]);
+                    const uint64_t passed = __ballot(most > kKVWeightExponent + kKVMaximumSlack);
+                    float keep = 1.0f;
+                    if (passed) {
+                        /* a maximum was passed by that much (m = -inf: the first tokens): sums follow the new one */
+                        most = -INFINITY;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const bool hidden = score[t][e / 4][e & 3] == -INFINITY;
+                            u[e] = hidden ? -INFINITY : fmaf(score[t][e / 4][e & 3], factor, value_log);
+                            most = fmaxf(most, u[e]);
+                        }
+                        most = kv_other_rows(most, true);
+                        const float now = fmaxf(m[t], most);
+                        const float by = m[t] == now ? 0.0f : m[t] - now;
+                        keep = exp2f(by);
+                        m[t] = now;
+                        l[t] = kv_lower(l[t], by);
+                        if (!kAccumulators)
+#pragma unroll
+                            for (int c = 0; c < kChannels; ++c) o[t][c] *= keep;
+                        const float offset = kKVWeightExponent - (now == -INFINITY ? 0.0f : now);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) u[e] += offset;
+                    }
+#pragma unroll
+                    for (int c = 0; kAccumulators && c < kChannels; c += 2) kv_scale(o[t][c], o[t][c + 1], keep, passed);
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const float w = __builtin_amdgcn_exp2f(u[e]), v = __builtin_amdgcn_exp2f(u[e + 1]);
+                        sum += w;
+                        sum += v;
+                        const kv_half2 pair = kv_round2<SPLIT>(w, v, low_half);
+                        weight[t][e / 8][e & 7] = pair[0], weight[t][e / 8][(e & 7) + 1] = pair[1];
+                    }
+                    /* weights of a page whose value scale lies that far below the sums'
+                     * largest leave fp32 before they leave the total: theirs is taken
+                     * without the scale */
+                    if (__any(value_log < m[t] - 64.0f && page >= 0)) {
+                        const float back = value_scale == value_scale ? -value_log : 0.0f;
+                        sum = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(u[e] + back);
+                        l[t] += sum;
+                    } else {
+                        l[t] = fmaf(sum, inverse, l[t]);
+                    }
+                }
+
+                if (!COLUMNS) {
+                    if (more) kv_wait<kCopies>();                 /* the values are there; the next keys may not be */
+                    else kv_wait<0>();
+                }
+                if (E4M3 && !whole) {
+                    /* codes of tokens that no column of the slot sees may be any bytes, NaN among
+                     * them: made zero (the wavefronts that share the tile write the same) */
+                    const int32_t good = page < 0 ? 0 : min(16, max(0, s.seen - (int32_t)token));
+                    if (__any(good < 16))
+#pragma unroll 1
+                        for (int c = 0; c < kChannels; ++c) {
+                            uint4 *at = reinterpret_cast<uint4 *>(mine + tile + value_at + c * 1024);
+                            uint4 v = *at;
+                            uint32_t word[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int b = 0; b < 4; ++b) {
+                                const int left = good - 4 * b;
+                                word[b] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+                            }
+                            *at = make_uint4(word[0], word[1], word[2], word[3]);
+                        }
+                }
+                {
+                    uint4 raw_codes[3];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) raw_codes[c] = *reinterpret_cast<const uint4 *>(codes + value_at + c * 1024);
+#pragma unroll
+                    for (int c = 0; c < kChannels; ++c) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (c + 2 < kChannels)
+                            raw_codes[(c + 2) % 3] = *reinterpret_cast<const uint4 *>(codes + value_at + (c + 2) * 1024);
+                        const uint4 v = raw_codes[c % 3];
+                        const kv_half8 low = kv_decode8<E4M3>(v.x, v.y), high = kv_decode8<E4M3>(v.z, v.w);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+                            o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(low, weight[t][0], o[t][c], 0, 0, 0);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+                            o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(high, weight[t][1], o[t][c], 0, 0, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (!COLUMNS && more) {
+                    kv_reads_done();
+                    copy_values(step + kStride, kv_lds(mine) + 64 * D, 0, kCopies);
                 }
             }
+            if (COLUMNS) tile ^= 128 * D;
+            step += kStride;
         }
-        if (next) load_keys(step + kStride, next_key_page);
 
-        const uint32_t scale_bits = __float_as_uint(value_scale);
-        const float value_log = value_scale == value_scale ? (float)((int)(scale_bits >> 23) - 127) : value_scale;
-        const float inverse = __uint_as_float((254u << 23) - scale_bits);
-        const bool whole = step * kKVStep + kKVStep <= (uint32_t)max(seen_least, 0) && __all(page >= 0);
-        kv_half8 weight[NT][2];
+        kv_wait<0>();                               /* nothing is on its way to LDS */
+
+        const uint64_t index = (uint64_t)blockIdx.x + s.index;
+        float *partial = kv_partial(a, index, head), *stats = kv_stats(a, index, head);
+        if (a.workgroups > 1 && head == 0 && piece.first_piece && threadIdx.x == 0)
+            kv_records(a)[1 + s.index] = {piece.whole ? 1 : kv_pieces(piece.units, walk.chunk, walk.at, piece.each),
+                                          (uint32_t)index, s.first_row, s.column, s.columns, {0, 0, 0}};
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const float factor = to_u[t] * key_scale;
-            float u[16], most = -INFINITY;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                float dot = score[t][e / 4][e & 3];
-                if (SPLIT) dot += kv_partner(dot);
-                u[e] = fmaf(dot, factor, value_log);
-            }
-            if (!whole) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (page < 0 || (int32_t)(token + e) >= seen[t]) u[e] = -INFINITY;
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) most = fmaxf(most, u[e]);
-            most = kv_other_rows(most, true);
-            if (__any(most > m[t] + kKVMaximumSlack)) {
-                const float now = fmaxf(m[t], most);
-                const float by = m[t] == now ? 0.0f : m[t] - now, keep = exp2f(by);
-                m[t] = now;
-                l[t] = kv_lower(l[t], by);
-#pragma unroll
-                for (int c = 0; c < kChannels; ++c) o[t][c] *= keep;
-            }
-            const float offset = kKVWeightExponent - (m[t] == -INFINITY ? 0.0f : m[t]);
-            float sum = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float w = __builtin_amdgcn_exp2f(u[e] + offset);
-                sum += w;
-                const _Float16 high = (_Float16)w;
-                weight[t][e / 8][e & 7] = SPLIT && n >= 8 ? (_Float16)(w - (float)high) : high;
-            }
-            /* weights of a page whose value scale lies that far below the sums'
-             * largest leave fp32 before they leave the total: theirs is taken
-             * without the scale */
-            if (__any(value_log < m[t] - 64.0f && page >= 0)) {
-                const float back = value_scale == value_scale ? offset - value_log : offset;
-                sum = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(u[e] + back);
-                l[t] += sum;
-            } else {
-                l[t] = fmaf(sum, inverse, l[t]);
+            l[t] = kv_other_rows(l[t], false);
+            if (l[t] != l[t]) m[t] = INFINITY;      /* a NaN outweighs the other parts */
+            if (g == 0 && (!SPLIT || n < 8)) {
+                merge_m[(wave * NT + t) * kTile + n] = m[t];
+                merge_l[(wave * NT + t) * kTile + n] = l[t];
             }
         }
-        if (!whole) {
-            /* codes of tokens that no column of the slot sees may be any bytes */
-            const int32_t good = page < 0 ? 0 : min(16, max(0, s.seen - (int32_t)token));
-#pragma unroll
-            for (int c = 0; c < kChannels; ++c) {
-                uint32_t word[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const int left = good - 4 * b;
-                    word[b] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
-                }
-                v[c] = make_uint4(word[0], word[1], word[2], word[3]);
-            }
-        }
-#pragma unroll
-        for (int c = 0; c < kChannels; ++c) {
-            const kv_half8 low = kv_decode8<E4M3>(v[c].x, v[c].y), high = kv_decode8<E4M3>(v[c].z, v[c].w);
+        __syncthreads();                            /* also: every wavefront is done with its codes */
+        /* tile by tile through LDS: rows of one column, from there on whole rows */
+        float *merge_o = reinterpret_cast<float *>(ring);
+        const uint32_t tiles = COLUMNS ? NT : (s.columns + kTile - 1) / kTile;
+#pragma unroll 1
+        for (uint32_t tile_at = 0; tile_at < tiles; ++tile_at) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(low, weight[t][0], o[t][c], 0, 0, 0);
-                o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(high, weight[t][1], o[t][c], 0, 0, 0);
-            }
-        }
-        key_page = next_key_page;
-        page = next_page;
-    }
-
-    const uint64_t partial = (((uint64_t)slot * a.cache.kv_heads + head) * a.parts + part) * a.columns;
-    float *stats = a.partial + (uint64_t)a.slots * a.cache.kv_heads * a.parts * a.columns * D;
+                if (tile_at != t) continue;
+                float keep = 1.0f;
+                if (!COLUMNS) {
+                    float top = -INFINITY;
+                    for (int w = 0; w < 4; ++w) top = fmaxf(top, merge_m[(w * NT + t) * kTile + (SPLIT ? n & 7 : n)]);
+                    keep = m[t] == top ? (m[t] == -INFINITY ? 0.0f : 1.0f) : exp2f(m[t] - top);
+                }
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        l[t] = kv_other_rows(l[t], false);
-        if (l[t] != l[t]) m[t] = INFINITY;      /* a NaN outweighs the other parts */
-        if (SPLIT)
+                for (int c = 0; c < kChannels; ++c) {
+                    kv_float4 sum = o[t][c];
+                    if (SPLIT)
 #pragma unroll
-            for (int c = 0; c < kChannels; ++c)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[t][c][e] += kv_partner(o[t][c][e]);
-    }
-    if (COLUMNS) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            if (column[t] >= s.columns || (SPLIT && n >= 8)) continue;
-            const uint32_t at = s.column + column[t];
-            if (parts == 1) {
-#pragma unroll
-                for (int c = 0; c < kChannels; ++c)
-                    kv_finish4(a, s.first_row + at / a.group, head * a.group + at % a.group, c * 16 + 4 * g, o[t][c], l[t]);
-            } else {
-                float *to = a.partial + (partial + column[t]) * D + 4 * g;
-#pragma unroll
-                for (int c = 0; c < kChannels; ++c) *reinterpret_cast<kv_float4 *>(to + c * 16) = o[t][c];
-                if (g == 0) {
-                    stats[2 * (partial + column[t])] = m[t];
-                    stats[2 * (partial + column[t]) + 1] = l[t];
+                        for (int e = 0; e < 4; ++e) sum[e] += kv_partner(sum[e]);
+                    if (!SPLIT || n < 8)
+                        *reinterpret_cast<kv_float4 *>(&merge_o[(wave * kTile + n) * kPitch + c * 16 + 4 * g]) = sum * keep;
                 }
             }
-        }
-        return;
-    }
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-        if (g == 0 && (!SPLIT || n < 8)) {
-            merge_m[(wave * NT + t) * kTile + n] = m[t];
-            merge_l[(wave * NT + t) * kTile + n] = l[t];
-        }
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        if (t * kTile >= s.columns) break;
-        if (!SPLIT || n < 8) {
-            float top = -INFINITY;
-            for (int w = 0; w < 4; ++w) top = fmaxf(top, merge_m[(w * NT + t) * kTile + n]);
-            const float keep = m[t] == top ? (m[t] == -INFINITY ? 0.0f : 1.0f) : exp2f(m[t] - top);
-#pragma unroll
-            for (int c = 0; c < kChannels; ++c)
-                *reinterpret_cast<kv_float4 *>(&merge_o[(wave * kTile + n) * kPitch + c * 16 + 4 * g]) = o[t][c] * keep;
-        }
-        __syncthreads();
-        for (uint32_t at = threadIdx.x; at < kTile * (D / 4); at += 256) {
-            const uint32_t c = at / (D / 4), d = at % (D / 4) * 4, of = t * kTile + c;
-            if (of >= s.columns) break;
-            float top = -INFINITY, total = 0.0f;
-            kv_float4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (int w = 0; w < 4; ++w) top = fmaxf(top, merge_m[(w * NT + t) * kTile + c]);
-            for (int w = 0; w < 4; ++w) {
-                const float mw = merge_m[(w * NT + t) * kTile + c];
-                if (mw == -INFINITY) continue;
-                total += kv_lower(merge_l[(w * NT + t) * kTile + c], mw - top);
-                sum += *reinterpret_cast<const kv_float4 *>(&merge_o[(w * kTile + c) * kPitch + d]);
-            }
-            if (parts == 1) {
-                const uint32_t col = s.column + of;
-                kv_finish4(a, s.first_row + col / a.group, head * a.group + col % a.group, d, sum, total);
-            } else {
-                *reinterpret_cast<kv_float4 *>(a.partial + (partial + of) * D + d) = sum;
-                if (d == 0) {
-                    stats[2 * (partial + of)] = top;
-                    stats[2 * (partial + of) + 1] = total;
+            if (COLUMNS) kv_reads_done();           /* the wavefront's own rows; the writes too */
+            else __syncthreads();
+            const uint32_t first = COLUMNS ? (wave * NT + tile_at) * kTile : tile_at * kTile;
+            for (uint32_t at = COLUMNS ? lane : threadIdx.x; at < kTile * (D / 4); at += COLUMNS ? 64 : 256) {
+                const uint32_t c = at / (D / 4), d = at % (D / 4) * 4, of = first + c;
+                if (of >= s.columns) break;
+                float top = -INFINITY, total = 0.0f;
+                kv_float4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (COLUMNS) {
+                    top = merge_m[of];
+                    total = merge_l[of];
+                    sum = *reinterpret_cast<const kv_float4 *>(&merge_o[(wave * kTile + c) * kPitch + d]);
+                } else {
+                    for (int w = 0; w < 4; ++w) top = fmaxf(top, merge_m[w * NT * kTile + of]);
+                    for (int w = 0; w < 4; ++w) {
+                        const float mw = merge_m[w * NT * kTile + of];
+                        if (mw == -INFINITY) continue;
+                        total += kv_lower(merge_l[w * NT * kTile + of], mw - top);
+                        sum += *reinterpret_cast<const kv_float4 *>(&merge_o[(w * kTile + c) * kPitch + d]);
+                    }
+                }
+                if (piece.whole) {
+                    const uint32_t col = s.column + of;
+                    kv_finish4(a, s.first_row + col / a.group, head * a.group + col % a.group, d, sum, total);
+                } else {
+                    *reinterpret_cast<kv_float4 *>(partial + of * D + d) = sum;
+                    if (d == 0) {
+                        stats[2 * of] = top;
+                        stats[2 * of + 1] = total;
+                    }
                 }
             }
+            if (!COLUMNS) __syncthreads();
         }
-        __syncthreads();
+        if (COLUMNS) __syncthreads();               /* the tiles are free for the next piece */
     }
 }
 

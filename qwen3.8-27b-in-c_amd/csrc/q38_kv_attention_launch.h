@@ -10,15 +10,15 @@ namespace q38 {
 template <bool E4M3, int D, bool SPLIT>
 bool launch_kv_attention_typed(const KVAttention &a, hipStream_t stream)
 {
-    const dim3 grid(a.slots, a.cache.kv_heads, a.parts), block(256);
-    switch (kv_variant(a)) {
-    case KVVariant::kOneTile:
-        return launch_kernel(kv_attention_kernel<E4M3, D, 1, SPLIT, false>, grid, block, stream, a);
-    case KVVariant::kTwoTiles:
-        return launch_kernel(kv_attention_kernel<E4M3, D, 2, SPLIT, false>, grid, block, stream, a);
-    default:
-        return launch_kernel(kv_attention_kernel<E4M3, D, 2, SPLIT, true>, grid, block, stream, a);
-    }
+    const dim3 grid(a.workgroups, a.cache.kv_heads), block(256);
+    const KVShape shape = kv_shape(a);
+    if (shape.columns)
+        return launch_kernel(shape.tiles == 1 ? kv_attention_kernel<E4M3, D, 1, SPLIT, true> : kv_attention_kernel<E4M3, D, 2, SPLIT, true>,
+                             grid, block, stream, a);
+    if constexpr (kv_token_tiles(D) == 3)
+        if (shape.tiles == 3) return launch_kernel(kv_attention_kernel<E4M3, D, 3, SPLIT, false>, grid, block, stream, a);
+    return launch_kernel(shape.tiles == 1 ? kv_attention_kernel<E4M3, D, 1, SPLIT, false> : kv_attention_kernel<E4M3, D, 2, SPLIT, false>,
+                         grid, block, stream, a);
 }
 
 template <int D>

@@ -1,21 +1,77 @@
-/* How a paged attention call is cut into work: by sizes that the host knows. */
+/* How a paged attention call is cut into work.  The host knows the sizes of
+ * the call and of the cache, the device the lengths; the functions are plain
+ * C++, so they are checked on the CPU too. */
 #pragma once
 
 #include "q38_kv.h"
 
 namespace q38 {
 
-enum class KVVariant { kOneTile, kTwoTiles, kColumns };
+constexpr int kKVStep = 64;               /* tokens of a step */
+/* units of a slot beside those of its steps: queries, joining and output take
+ * about as long as that many steps */
+constexpr uint32_t kKVSlotOverhead = 2;
 
-/* columns of a sequence, on average over the call */
-inline uint64_t kv_columns_each(const KVAttention &a)
+Q38_HD uint32_t kv_steps(uint32_t tokens) { return (tokens + kKVStep - 1) / kKVStep; }
+/* units of a slot of a sequence with that many steps, 2^shift steps each */
+Q38_HD uint32_t kv_slot_units(uint32_t steps, uint32_t shift)
 {
-    return ((uint64_t)a.rows.total_rows * a.group + a.rows.count - 1) / a.rows.count;
+    return ((steps + (1u << shift) - 1) >> shift) + kKVSlotOverhead;
 }
-inline KVVariant kv_variant(const KVAttention &a)
+/* units of a workgroup's range, and of a slot that is never cut */
+Q38_HD uint32_t kv_chunk(uint32_t units, uint32_t workgroups, uint32_t least)
 {
-    const uint64_t tile = a.type == kElementF32 ? 8 : 16, columns = kv_columns_each(a);
-    return columns <= tile ? KVVariant::kOneTile : columns <= 4 * tile ? KVVariant::kTwoTiles : KVVariant::kColumns;
+    const uint32_t each = units / workgroups + (units % workgroups ? 1 : 0);
+    return each > least ? each : least;
+}
+Q38_HD uint32_t kv_small(uint32_t chunk) { return chunk / 4; }
+
+/* What a range of units begin .. end - 1 holds of the slot whose `each` units
+ * (of `steps` steps) begin at `slot` < end: steps first .. last - 1.  A slot of
+ * no steps is one piece without any. */
+struct KVPiece {
+    uint32_t first, last, units, each;        /* units that hold the slot's steps, and all of its units */
+    bool some, first_piece, whole;
+};
+Q38_HD KVPiece kv_piece(uint32_t slot, uint32_t each, uint32_t steps, uint32_t begin, uint32_t end, uint32_t small,
+                        uint32_t shift)
+{
+    uint32_t units = (steps + (1u << shift) - 1) >> shift;
+    if (!units) units = 1;
+    if (each <= small) return {0, steps, units, each, slot >= begin, true, true};
+    const uint32_t low = begin > slot ? begin - slot : 0, high = end - slot < units ? end - slot : units;
+    const uint64_t last = (uint64_t)high << shift;
+    return {low << shift, last < steps ? (uint32_t)last : steps, units, each, low < high, low == 0, low == 0 && high == units};
+}
+/* pieces of a slot that is cut and ends (with all its units) before `behind` */
+Q38_HD uint32_t kv_pieces(uint32_t units, uint32_t chunk, uint32_t behind, uint32_t each)
+{
+    const uint32_t slot = behind - each;
+    return (slot + units - 1) / chunk - slot / chunk + 1;
+}
+
+/* Column tiles (of 8 fp32 or 16 other columns): up to kv_token_tiles in a
+ * workgroup whose wavefronts share the tokens, else one or two in each
+ * wavefront. */
+constexpr int kv_token_tiles(int head_dim) { return head_dim == 128 ? 2 : 3; }
+/* wavefronts that share a SIMD's registers: one has 512, of two each 256 */
+constexpr int kv_waves(int head_dim, int tiles, bool columns)
+{
+    return head_dim == 256 && (!columns || tiles == 2) ? 1 : 2;
+}
+
+struct KVShape {
+    int tiles;
+    bool columns;          /* tiles of each wavefront's own */
+};
+inline KVShape kv_shape(const KVAttention &a)
+{
+    const uint64_t tile = a.type == kElementF32 ? 8 : 16;
+    /* columns of a sequence, on average over the call */
+    const uint64_t columns = ((uint64_t)a.rows.total_rows * a.group + a.rows.count - 1) / a.rows.count;
+    const uint64_t shared = (columns + tile - 1) / tile;
+    if (shared <= (uint64_t)kv_token_tiles(a.cache.head_dim)) return {(int)shared, false};
+    return {columns <= 16 * tile ? 1 : 2, true};
 }
 
 }  // namespace q38

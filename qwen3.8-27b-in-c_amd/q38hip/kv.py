@@ -16,7 +16,7 @@ import ctypes
 
 from . import _check, _stream, lib
 
-BAD_SEQUENCE, POOL_FULL, TABLE_FULL, BAD_PAGE, NOT_EMPTY = 1, 2, 4, 8, 16
+BAD_SEQUENCE, POOL_FULL, TABLE_FULL, BAD_PAGE, NOT_EMPTY, BAD_ROWS = 1, 2, 4, 8, 16, 32
 KINDS = {"int8": 0, "e4m3": 1}
 EXPORTS = ("q38hip_kv_reset", "q38hip_kv_workspace_bytes", "q38hip_kv_extend", "q38hip_kv_fork", "q38hip_kv_truncate",
            "q38hip_kv_compact", "q38hip_kv_copy", "q38hip_kv_append", "q38hip_kv_attention_workspace_bytes",
@@ -143,7 +143,7 @@ class KVPages:
         if bits:
             self.status.zero_()
             names = ("bad sequence id", "page pool full", "table full", "page outside the pool", "fork into a sequence "
-                     "that is not empty")
+                     "that is not empty", "row offsets that decrease")
             raise RuntimeError("paged cache: " + ", ".join(n for i, n in enumerate(names) if bits >> i & 1))
 
     # ---- pages -------------------------------------------------------------------

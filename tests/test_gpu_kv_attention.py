@@ -179,3 +179,17 @@ def test_same_bits_every_time(device):
     first = dev.attention(0, q, ids)
     for _ in range(5):
         assert torch.equal(dev.attention(0, q, ids), first)
+
+
+def test_row_offsets_that_decrease(device):
+    """nothing is done, and the status says so"""
+    from q38hip import kv
+    rng = np.random.default_rng(11)
+    dev = kc.filled(rng, [48, 48, 20], "int8", 16, 2, 64).to(device)
+    q = torch.from_numpy(rng.normal(size=(40, 4, 64))).float().to(device)
+    out = torch.full_like(q, 3.0)
+    for starts in ([0, 30, 10, 40], [40, 0, 40, 0], [0, -5, 40, 39]):
+        dev.attention(0, q, kc.words([0, 1, 2], device), kc.words(starts, device), out=out)
+        assert int(dev.status) == kv.BAD_ROWS
+        dev.status.zero_()
+        assert (out == 3.0).all()
