@@ -11,9 +11,11 @@
  * that is not finite makes the scale NaN, and the page reads as NaN until its
  * first token is written again.
  *
- * One workgroup per (page touched, head, half): no other writes there.  Keys
- * are [token][channel] and go out as they come; values are [channel][token],
- * so theirs turn in LDS and whole dwords of tokens go out. */
+ * One workgroup per (page touched, head, half): no other writes there.  A
+ * thread holds eight times four channels of the page's tokens in registers, as
+ * two groups of four tokens, so the rows are read once.  Keys are
+ * [token][channel] and go out as they come; values are [channel][token]: four
+ * tokens make a dword, and the dwords turn in LDS. */
 #include "q38_kernels.h"
 #include "q38_device.h"
 #include "q38_kv.h"
@@ -22,13 +24,14 @@ namespace q38 {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kMostThreads = 1024, kQuads = 8;
 
 struct KVAppend {
     Q38KVPages cache;     /* data and scales moved to the layer */
     KVRows rows;
     const void *key, *value;
     uint64_t row_stride;
+    uint32_t page_shift, dim_shift;
     bool vector;          /* rows are aligned to four elements */
 };
 
@@ -71,12 +74,23 @@ __device__ __forceinline__ float decode(uint32_t code)
     else return (float)(int8_t)code;
 }
 
-template <bool E4M3, int TYPE>
-__global__ __launch_bounds__(kThreads) void kv_append_kernel(KVAppend a)
+/* bytes of `word` that are codes before `used`, rounded to a scale 1 / shrink times as large */
+template <bool E4M3>
+__device__ __forceinline__ uint32_t follow(uint32_t word, uint32_t used, float shrink)
 {
-    extern __shared__ uint8_t turned[];       /* values: [channel][T + 4] codes */
-    __shared__ uint32_t wave_largest[kThreads / 64];
-    const uint32_t T = a.cache.page_tokens, D = a.cache.head_dim;
+    uint32_t out = word;
+    for (uint32_t e = 0; e < 4; ++e)
+        if (e < used)
+            out = (out & ~(0xffu << (8 * e))) | encode<E4M3>(decode<E4M3>(word >> (8 * e) & 0xffu) * shrink) << (8 * e);
+    return out;
+}
+
+template <bool E4M3, int TYPE>
+__global__ __launch_bounds__(kMostThreads) void kv_append_kernel(KVAppend a)
+{
+    extern __shared__ uint32_t turned[];      /* values: [channel][T / 4 + 1] dwords of four tokens */
+    __shared__ uint32_t wave_largest[kMostThreads / 64];
+    const uint32_t T = a.cache.page_tokens, D = a.cache.head_dim, threads = blockDim.x;
     const uint32_t slot = blockIdx.x, half = blockIdx.y & 1, head = blockIdx.y >> 1;
     const int i = kv_find_sequence(a.rows, slot, 1, T, 2);
     if (i < 0) return;
@@ -86,73 +100,90 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(KVAppend a)
     const uint32_t tokens = kv_tokens(a.cache, sequence);
     /* rows that lie before the sequence's first token are left out */
     const uint32_t rows = min(end - begin, tokens), first = tokens - rows;
-    const uint32_t entry = first / T + (slot - kv_slot_base(begin, i, 1, T, 2));
-    if (!rows || entry * T >= tokens) return;
+    const uint32_t entry = (first >> a.page_shift) + (slot - kv_slot_base(begin, i, 1, T, 2));
+    if (!rows || entry >= a.cache.table_entries || entry * T >= tokens) return;
     const int32_t page = kv_page(a.cache, sequence, entry);
     if (page < 0) {
         if (threadIdx.x == 0) atomicOr(a.cache.status, Q38_KV_BAD_PAGE);
         return;
     }
+    /* the page's new tokens: from .. to - 1 */
     const uint32_t from = max(first, entry * T) - entry * T, to = min(tokens, entry * T + T) - entry * T;
-    const uint32_t count = to - from;
     const void *source = half ? a.value : a.key;
-    /* element of new token 0, channel 0 */
-    const uint64_t origin = (uint64_t)(end - tokens + entry * T + from) * a.row_stride + (uint64_t)head * D;
+    /* element of the page's token 0 (which may lie before the rows), channel 0 */
+    const uint64_t origin = ((uint64_t)end - tokens + entry * T) * a.row_stride + (uint64_t)head * D;
     const uint64_t block = kv_block(a.cache, page, half, head);
     uint8_t *codes = a.cache.data + block * (T * D);
-    const uint32_t quads = D / 4;
+    const float was = from ? a.cache.scales[block] : 0.0f;
 
+    /* item k of a thread: token 4 (item / quads) + k % 4 of channels 4 (item % quads) .. */
+    float x[kQuads][4];
     uint32_t largest = 0;
-    for (uint32_t at = threadIdx.x; at < count * quads; at += kThreads) {
-        float x[4];
-        load4<TYPE>(x, source, origin + (at / quads) * a.row_stride + at % quads * 4, a.vector);
-        for (int e = 0; e < 4; ++e) largest = max(largest, __float_as_uint(x[e]) & 0x7fffffffu);
+#pragma unroll
+    for (int k = 0; k < kQuads; ++k) {
+        const uint32_t item = threadIdx.x + (k / 4) * threads, t = (item >> (a.dim_shift - 2)) * 4 + k % 4;
+        const uint32_t d = (item & (D / 4 - 1)) * 4;
+        if (t >= from && t < to) load4<TYPE>(x[k], source, origin + t * a.row_stride + d, a.vector);
+        else x[k][0] = x[k][1] = x[k][2] = x[k][3] = 0.0f;
     }
+#pragma unroll
+    for (int k = 0; k < kQuads; ++k)
+        for (int e = 0; e < 4; ++e) largest = max(largest, __float_as_uint(x[k][e]) & 0x7fffffffu);
     for (int by = 1; by < 64; by *= 2) largest = max(largest, (uint32_t)__shfl_xor((int)largest, by));
     if ((threadIdx.x & 63) == 0) wave_largest[threadIdx.x >> 6] = largest;
-    __syncthreads();
-    for (int w = 0; w < kThreads / 64; ++w) largest = max(largest, wave_largest[w]);
+    __syncthreads();                                   /* also: every thread has read the old scale */
+    for (uint32_t w = 0; w < threads / 64; ++w) largest = max(largest, wave_largest[w]);
 
     const bool finite = largest < 0x7f800000u;
-    const float was = from ? a.cache.scales[block] : 0.0f;
     float scale = finite ? __uint_as_float((uint32_t)(kv_scale_exponent(largest, E4M3) + 127) << 23) : NAN;
     if (!(was <= scale) && finite) scale = was;        /* the larger, or an older NaN */
-    __syncthreads();                                   /* every thread has read the old scale */
     if (threadIdx.x == 0) a.cache.scales[block] = scale;
+    uint32_t *words = reinterpret_cast<uint32_t *>(codes);
     if (from && scale > was) {
         const float shrink = was / scale;
-        for (uint32_t at = threadIdx.x; at < from * D; at += kThreads) {
-            uint8_t *code = codes + (half ? at / from * T + at % from : at);
-            *code = (uint8_t)encode<E4M3>(decode<E4M3>(*code) * shrink);
+        if (!half) {
+            for (uint32_t at = threadIdx.x; at < from * (D / 4); at += threads) words[at] = follow<E4M3>(words[at], 4, shrink);
+        } else {
+            const uint32_t shift = a.page_shift - 2;
+            for (uint32_t at = threadIdx.x; at < D << shift; at += threads) {
+                const uint32_t t = (at & (T / 4 - 1)) * 4;
+                if (t < from) words[at] = follow<E4M3>(words[at], from - t, shrink);
+            }
+            __syncthreads();                           /* a dword of old codes may hold new ones too */
         }
     }
     const bool usable = scale == scale;
     const float inverse = usable ? 1.0f / scale : 0.0f;
-    const bool turn = half && count >= 4;
-    const uint32_t pitch = T + 4;
-    for (uint32_t at = threadIdx.x; at < count * quads; at += kThreads) {
-        const uint32_t t = at / quads, d = at % quads * 4;
-        float x[4];
-        load4<TYPE>(x, source, origin + t * a.row_stride + d, a.vector);
-        uint32_t code[4];
-        for (int e = 0; e < 4; ++e) code[e] = usable ? encode<E4M3>(x[e] * inverse) : 0u;
-        if (!half)
-            *reinterpret_cast<uint32_t *>(codes + (from + t) * D + d) = code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24;
-        else if (turn)
-            for (int e = 0; e < 4; ++e) turned[(d + e) * pitch + from + t] = (uint8_t)code[e];
-        else
-            for (int e = 0; e < 4; ++e) codes[(d + e) * T + from + t] = (uint8_t)code[e];
+    uint32_t code[kQuads][4];
+#pragma unroll
+    for (int k = 0; k < kQuads; ++k)
+        for (int e = 0; e < 4; ++e) code[k][e] = usable ? encode<E4M3>(x[k][e] * inverse) : 0u;
+    const bool turn = half && to - from >= 4;
+    const uint32_t pitch = T / 4 + 1;
+#pragma unroll
+    for (int k = 0; k < kQuads; ++k) {
+        const uint32_t item = threadIdx.x + (k / 4) * threads, group = item >> (a.dim_shift - 2), t = group * 4 + k % 4;
+        const uint32_t d = (item & (D / 4 - 1)) * 4;
+        if (turn) {
+            /* of the four tokens, channel k % 4 here: 4 x 4 bytes turn in registers */
+            const int b = k & ~3, e = k & 3;
+            if (t - e < to) turned[(d + e) * pitch + group] = code[b][e] | code[b + 1][e] << 8 | code[b + 2][e] << 16 | code[b + 3][e] << 24;
+        } else if (t >= from && t < to) {
+            if (!half) words[(t * D + d) / 4] = code[k][0] | code[k][1] << 8 | code[k][2] << 16 | code[k][3] << 24;
+            else
+                for (int e = 0; e < 4; ++e) codes[(d + e) * T + t] = (uint8_t)code[k][e];
+        }
     }
     if (!turn) return;
     __syncthreads();
-    const uint32_t words = T / 4;
-    for (uint32_t at = threadIdx.x; at < D * words; at += kThreads) {
-        const uint32_t d = at / words, t = at % words * 4;
-        if (t >= from && t + 4 <= to)
-            *reinterpret_cast<uint32_t *>(codes + d * T + t) = *reinterpret_cast<const uint32_t *>(turned + d * pitch + t);
+    for (uint32_t at = threadIdx.x; at < D << (a.page_shift - 2); at += threads) {
+        const uint32_t d = at >> (a.page_shift - 2), group = at & (T / 4 - 1), t = group * 4;
+        if (t >= to || t + 4 <= from) continue;
+        const uint32_t word = turned[d * pitch + group];
+        if (t >= from && t + 4 <= to) words[at] = word;
         else
-            for (uint32_t e = t; e < t + 4; ++e)
-                if (e >= from && e < to) codes[d * T + e] = turned[d * pitch + e];
+            for (uint32_t e = 0; e < 4; ++e)
+                if (t + e >= from && t + e < to) codes[d * T + t + e] = (uint8_t)(word >> (8 * e));
     }
 }
 
@@ -162,8 +193,10 @@ bool launch_typed(const KVAppend &a, uint32_t slots, hipStream_t stream)
     KVAppend call = a;
     void *arguments[] = {&call};
     const uint32_t lds = a.cache.head_dim * (a.cache.page_tokens + 4);
+    /* a page is T D / 4 quads, eight a thread; a smaller page leaves threads of its one wavefront idle */
+    const uint32_t threads = a.cache.page_tokens * a.cache.head_dim / (4 * kQuads);
     return hipLaunchKernel(reinterpret_cast<const void *>(kv_append_kernel<E4M3, TYPE>),
-                           dim3(slots, 2 * a.cache.kv_heads), dim3(kThreads), arguments, lds, stream) == hipSuccess;
+                           dim3(slots, 2 * a.cache.kv_heads), dim3(threads < 64 ? 64 : threads), arguments, lds, stream) == hipSuccess;
 }
 template <bool E4M3>
 bool launch_kind(const KVAppend &a, int type, uint32_t slots, hipStream_t stream)
@@ -178,7 +211,8 @@ bool launch_kind(const KVAppend &a, int type, uint32_t slots, hipStream_t stream
 bool launch_kv_append(const Q38KVPages &cache, uint32_t layer, const void *key, const void *value, int type,
                       uint64_t row_stride, const KVRows &rows, hipStream_t stream)
 {
-    KVAppend a{cache, rows, key, value, row_stride, false};
+    KVAppend a{cache, rows, key, value, row_stride, (uint32_t)__builtin_ctz(cache.page_tokens),
+               (uint32_t)__builtin_ctz(cache.head_dim), false};
     a.cache.data += (uint64_t)layer * cache.pages * kv_page_bytes(cache);
     a.cache.scales += (uint64_t)layer * cache.pages * 2 * cache.kv_heads;
     const uintptr_t step = type == kElementF32 ? 4 : 2;

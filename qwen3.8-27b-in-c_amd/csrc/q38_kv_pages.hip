@@ -161,23 +161,29 @@ __global__ __launch_bounds__(kPlan) void kv_extend_kernel(Q38KVPages c, const in
     if (i < count) c.lengths[id] = (int32_t)after;
 }
 
-/* 16 bytes per thread and turn of page sources[pair] of a layer to page targets[pair] */
-constexpr uint32_t kCopySlice = 256 * 16 * 4;
+/* A slice, 32 bytes per thread, of page `source` of a layer to page `target`.
+ * (A vector type of the compiler's own: an array of uint4 went through LDS.) */
+using kv_bytes16 = uint32_t __attribute__((ext_vector_type(4)));
+constexpr uint32_t kCopySlice = 256 * 16 * 2;
 __device__ __forceinline__ void copy_slice(const Q38KVPages &c, int32_t source, int32_t target, uint32_t layer, uint32_t slice)
 {
     const uint64_t bytes = kv_page_bytes(c), pages = (uint64_t)layer * c.pages;
-    const uint4 *from = reinterpret_cast<const uint4 *>(c.data + (pages + source) * bytes);
-    uint4 *to = reinterpret_cast<uint4 *>(c.data + (pages + target) * bytes);
-    const uint64_t first = (uint64_t)slice * (kCopySlice / 16) + threadIdx.x, end = bytes / 16;
-    uint4 v[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (first + 256 * e < end) v[e] = from[first + 256 * e];
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (first + 256 * e < end) to[first + 256 * e] = v[e];
+    const kv_bytes16 *from = reinterpret_cast<const kv_bytes16 *>(c.data + (pages + source) * bytes);
+    kv_bytes16 *to = reinterpret_cast<kv_bytes16 *>(c.data + (pages + target) * bytes);
+    const uint32_t first = slice * (kCopySlice / 16) + threadIdx.x, second = first + 256, end = (uint32_t)(bytes / 16);
+    float scale = 0.0f;
+    const bool scales = slice == 0 && threadIdx.x < 2 * c.kv_heads;
+    if (scales) scale = c.scales[(pages + source) * 2 * c.kv_heads + threadIdx.x];
+    if (second < end) {
+        const kv_bytes16 v = from[first], w = from[second];
+        to[first] = v;
+        to[second] = w;
+    } else if (first < end) {
+        to[first] = from[first];
+    }
+    if (scales) c.scales[(pages + target) * 2 * c.kv_heads + threadIdx.x] = scale;
     if (slice == 0)
-        for (uint32_t e = threadIdx.x; e < 2 * c.kv_heads; e += 256)
+        for (uint32_t e = 256 + threadIdx.x; e < 2 * c.kv_heads; e += 256)
             c.scales[(pages + target) * 2 * c.kv_heads + e] = c.scales[(pages + source) * 2 * c.kv_heads + e];
 }
 
@@ -295,19 +301,16 @@ __global__ __launch_bounds__(kPlan) void kv_compact_plan_kernel(Q38KVPages c, in
     }
 }
 
-/* the moves, and the tables after them */
+/* the moves, and the tables after them: blockIdx.x is a slice of a layer's
+ * page, blockIdx.y every so-manieth move */
 __global__ __launch_bounds__(256) void kv_compact_kernel(Q38KVPages c, const int32_t *plan, uint32_t slices)
 {
-    const uint32_t moves = (uint32_t)plan[0];
+    const uint32_t moves = (uint32_t)plan[0], slice = blockIdx.x % slices, layer = blockIdx.x / slices;
     const int32_t live = plan[1];
     const int32_t *targets = plan + 2, *sources = targets + c.pages, *place = sources + c.pages;
-    const uint64_t units = (uint64_t)moves * c.layers * slices;
-    for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const uint32_t slice = (uint32_t)(u % slices), k = (uint32_t)(u / slices % moves);
-        copy_slice(c, sources[k], targets[k], (uint32_t)(u / slices / moves), slice);
-    }
-    const uint64_t entries = (uint64_t)c.sequences * c.table_entries;
-    for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < entries; e += (uint64_t)gridDim.x * 256) {
+    for (uint32_t k = blockIdx.y; k < moves; k += gridDim.y) copy_slice(c, sources[k], targets[k], layer, slice);
+    const uint64_t entries = (uint64_t)c.sequences * c.table_entries, blocks = (uint64_t)gridDim.x * gridDim.y;
+    for (uint64_t e = ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x; e < entries; e += blocks * 256) {
         const int32_t page = c.tables[e];
         if (page >= live && (uint32_t)page < c.pages) c.tables[e] = place[page];
     }
@@ -360,8 +363,10 @@ bool launch_kv_truncate(const Q38KVPages &c, const int32_t *sequences, const int
 
 bool launch_kv_compact(const Q38KVPages &c, int32_t *workspace, hipStream_t stream)
 {
+    const uint32_t slices = copy_slices(c), across = slices * c.layers, wanted = across < 8192 ? 8192 / across : 1;
     return launch_kernel(kv_compact_plan_kernel, dim3(1), dim3(kPlan), stream, c, workspace) &&
-           launch_kernel(kv_compact_kernel, dim3(2048), dim3(256), stream, c, (const int32_t *)workspace, copy_slices(c));
+           launch_kernel(kv_compact_kernel, dim3(across, wanted < c.pages ? wanted : c.pages), dim3(256), stream, c,
+                         (const int32_t *)workspace, slices);
 }
 
 }  // namespace q38

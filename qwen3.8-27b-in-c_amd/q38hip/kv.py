@@ -14,7 +14,7 @@ reads.
 """
 import ctypes
 
-from . import _check, _stream, lib
+from . import _check, lib
 
 BAD_SEQUENCE, POOL_FULL, TABLE_FULL, BAD_PAGE, NOT_EMPTY, BAD_ROWS = 1, 2, 4, 8, 16, 32
 KINDS = {"int8": 0, "e4m3": 1}
@@ -57,12 +57,9 @@ def _lib():
     return _BOUND
 
 
-def _element_type(dtype):
+def _element_types():
     import torch
-    try:
-        return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}[dtype]
-    except KeyError:
-        raise ValueError("expected float32, float16 or bfloat16 rows")
+    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 
 
 class KVPages:
@@ -99,6 +96,10 @@ class KVPages:
                              status.data_ptr(), layers, pages, page_tokens, kv_heads, head_dim, self.sequences,
                              self.table_entries, KINDS[kind])
         self._ref = ctypes.byref(self._struct)
+        self._torch, self._int32, self._device, self._types = torch, torch.int32, data.device, _element_types()
+        self._index = data.get_device()
+        self._bytes = {}                       # workspace of an attention call, by its sizes
+        self._pages_workspace = None
 
     @classmethod
     def allocate(cls, layers, pages, page_tokens, kv_heads, head_dim, sequences, table_entries, kind="int8",
@@ -114,19 +115,30 @@ class KVPages:
 
     # ---- checks ----------------------------------------------------------------
 
+    def _stream(self):
+        """torch's current stream of the cache's device"""
+        return self._torch._C._cuda_getCurrentRawStream(self._index)
+
+    def _type(self, dtype):
+        kind = self._types.get(dtype)
+        if kind is None:
+            raise ValueError("expected float32, float16 or bfloat16 rows")
+        return kind
+
     def _words(self, tensor, name, count=None):
         """pointer of an int32 [count] device tensor"""
-        import torch
-        if tensor.dtype != torch.int32 or tensor.dim() != 1 or not tensor.is_contiguous():
+        shape = tensor.shape
+        if tensor.dtype != self._int32 or len(shape) != 1 or not tensor.is_contiguous():
             raise ValueError("%s must be a contiguous int32 vector" % name)
-        if count is not None and tensor.shape[0] != count:
+        if count is not None and shape[0] != count:
             raise ValueError("%s must have %d words" % (name, count))
-        if tensor.device != self.data.device:
+        if tensor.get_device() != self._index:
             raise ValueError("%s must be on the cache's device" % name)
         return tensor.data_ptr()
 
     def _rows(self, sequences, row_starts, total):
-        count = sequences.shape[0] if sequences.dim() == 1 else 0
+        shape = sequences.shape
+        count = shape[0] if len(shape) == 1 else 0
         ids = self._words(sequences, "sequences")
         starts = None if row_starts is None else self._words(row_starts, "row_starts", count + 1)
         if row_starts is None and count and total % count:
@@ -134,8 +146,7 @@ class KVPages:
         return ids, starts, count
 
     def _workspace(self, nbytes):
-        import torch
-        return torch.empty(nbytes, dtype=torch.uint8, device=self.data.device)
+        return self._torch.empty(nbytes, dtype=self._torch.uint8, device=self._device)
 
     def check(self):
         """Synchronises; raises where a call found bad ids or no room, and clears the status."""
@@ -150,85 +161,87 @@ class KVPages:
 
     def reset(self):
         """every page free, every sequence empty"""
-        _check(_lib().q38hip_kv_reset(self._ref, _stream()), "q38hip_kv_reset")
+        _check(_lib().q38hip_kv_reset(self._ref, self._stream()), "q38hip_kv_reset")
 
     def extend(self, sequences, rows):
         """sequences[i] grows by rows[i] tokens; shared last pages are copied first"""
         ids = self._words(sequences, "sequences")
         more = self._words(rows, "rows", sequences.shape[0])
-        work = self._workspace(_lib().q38hip_kv_workspace_bytes(self._ref))
-        _check(_lib().q38hip_kv_extend(self._ref, ids, more, sequences.shape[0], work.data_ptr(), _stream()),
-               "q38hip_kv_extend")
+        if self._pages_workspace is None:      # calls on a cache are in order, so one serves them all
+            self._pages_workspace = self._workspace(_lib().q38hip_kv_workspace_bytes(self._ref))
+        _check(_lib().q38hip_kv_extend(self._ref, ids, more, sequences.shape[0], self._pages_workspace.data_ptr(),
+                                       self._stream()), "q38hip_kv_extend")
 
     def fork(self, parents, children, lengths=None):
         """children[i] (empty) becomes the first lengths[i] tokens (default: all) of parents[i]"""
         count = parents.shape[0]
         _check(_lib().q38hip_kv_fork(self._ref, self._words(parents, "parents"), self._words(children, "children", count),
                                      None if lengths is None else self._words(lengths, "lengths", count), count,
-                                     _stream()), "q38hip_kv_fork")
+                                     self._stream()), "q38hip_kv_fork")
 
     def truncate(self, sequences, lengths):
         """sequences[i] keeps its first lengths[i] tokens; 0 frees it"""
         count = sequences.shape[0]
         _check(_lib().q38hip_kv_truncate(self._ref, self._words(sequences, "sequences"),
-                                         self._words(lengths, "lengths", count), count, _stream()), "q38hip_kv_truncate")
+                                         self._words(lengths, "lengths", count), count, self._stream()), "q38hip_kv_truncate")
 
     def compact(self):
         """The pages in use move to the front of the pool.  Returns an int32
         [2] device tensor: the pages moved and the pages in use."""
-        import torch
         work = self._workspace(_lib().q38hip_kv_workspace_bytes(self._ref))
-        _check(_lib().q38hip_kv_compact(self._ref, work.data_ptr(), _stream()), "q38hip_kv_compact")
-        return work[:8].view(torch.int32)
+        _check(_lib().q38hip_kv_compact(self._ref, work.data_ptr(), self._stream()), "q38hip_kv_compact")
+        return work[:8].view(self._int32)
 
     def copy(self, sources, targets):
         """pages sources[i] to pages targets[i], in all layers"""
         count = sources.shape[0]
         _check(_lib().q38hip_kv_copy(self._ref, self._words(sources, "sources"), self._words(targets, "targets", count),
-                                     count, _stream()), "q38hip_kv_copy")
+                                     count, self._stream()), "q38hip_kv_copy")
 
     # ---- rows --------------------------------------------------------------------
 
     def append(self, layer, key, value, sequences, row_starts=None):
         """The last rows of each sequence into one layer: key and value [rows,
         kv_heads, head_dim] with equal row strides."""
-        shape = (key.shape[0], self.kv_heads, self.head_dim)
-        for tensor in (key, value):
-            if tuple(tensor.shape) != shape or tensor.stride()[1:] != (self.head_dim, 1):
-                raise ValueError("expected keys and values [rows, %d, %d] with contiguous heads" % shape[1:])
-        if key.dtype != value.dtype or key.stride(0) != value.stride(0) and shape[0] > 1:
+        rows, heads, dim = key.shape[0], self.kv_heads, self.head_dim
+        stride = key.stride()
+        if key.shape != (rows, heads, dim) or value.shape != key.shape or stride[1:] != (dim, 1) or \
+                value.stride()[1:] != (dim, 1):
+            raise ValueError("expected keys and values [rows, %d, %d] with contiguous heads" % (heads, dim))
+        if key.dtype != value.dtype or stride[0] != value.stride(0) and rows > 1:
             raise ValueError("keys and values must have one type and row stride")
-        if key.device != self.data.device or value.device != self.data.device:
+        if key.get_device() != self._index or value.get_device() != self._index:
             raise ValueError("keys and values must be on the cache's device")
-        ids, starts, count = self._rows(sequences, row_starts, shape[0])
-        _check(_lib().q38hip_kv_append(self._ref, layer, key.data_ptr(), value.data_ptr(), _element_type(key.dtype),
-                                       key.stride(0), ids, starts, count, shape[0], _stream()), "q38hip_kv_append")
+        ids, starts, count = self._rows(sequences, row_starts, rows)
+        _check(_lib().q38hip_kv_append(self._ref, layer, key.data_ptr(), value.data_ptr(), self._type(key.dtype), stride[0],
+                                       ids, starts, count, rows, self._stream()), "q38hip_kv_append")
 
     def attention(self, layer, query, sequences, row_starts=None, gate=None, scale=None, out=None):
         """Causal attention of each sequence's last rows in one layer: query
         (and gate) [rows, heads, head_dim] with contiguous channels and equal
         strides; the result [rows, heads, head_dim] in the query's type."""
-        import torch
-        if query.dim() != 3 or query.shape[2] != self.head_dim or query.stride(2) != 1:
+        shape, stride, dtype = query.shape, query.stride(), query.dtype
+        if len(shape) != 3 or shape[2] != self.head_dim or stride[2] != 1:
             raise ValueError("expected queries [rows, heads, %d] with contiguous channels" % self.head_dim)
-        rows, heads, dim = query.shape
-        if gate is not None and (gate.shape != query.shape or gate.stride() != query.stride() or
-                                 gate.dtype != query.dtype or gate.device != query.device):
+        rows, heads, dim = shape
+        if query.get_device() != self._index:
+            raise ValueError("queries must be on the cache's device")
+        if gate is not None and (gate.shape != shape or gate.stride() != stride or gate.dtype != dtype or
+                                 gate.get_device() != self._index):
             raise ValueError("the gate must be laid out as the queries")
         if out is None:
-            out = torch.empty((rows, heads, dim), dtype=query.dtype, device=query.device)
-        elif (out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or
-              out.stride()[1:] != (dim, 1)):
+            out = self._torch.empty(shape, dtype=dtype, device=self._device)
+        elif out.shape != shape or out.dtype != dtype or out.get_device() != self._index or out.stride()[1:] != (dim, 1):
             raise ValueError("out must be [rows, heads, head_dim] in the queries' type with contiguous heads")
-        if query.device != self.data.device:
-            raise ValueError("queries must be on the cache's device")
         ids, starts, count = self._rows(sequences, row_starts, rows)
-        kind = _element_type(query.dtype)
-        nbytes = _lib().q38hip_kv_attention_workspace_bytes(self._ref, kind, heads, count, rows)
+        kind, bound = self._type(dtype), _lib()
+        nbytes = self._bytes.get((kind, heads, count, rows))
+        if nbytes is None:
+            nbytes = bound.q38hip_kv_attention_workspace_bytes(self._ref, kind, heads, count, rows)
+            self._bytes[kind, heads, count, rows] = nbytes
         work = self._workspace(nbytes) if nbytes else None
-        _check(_lib().q38hip_kv_attention(self._ref, layer, out.data_ptr(), query.data_ptr(),
-                                          None if gate is None else gate.data_ptr(), kind, heads, query.stride(0),
-                                          query.stride(1), out.stride(0), dim ** -0.5 if scale is None else scale, ids,
-                                          starts, count, rows, None if work is None else work.data_ptr(), _stream()),
-               "q38hip_kv_attention")
+        _check(bound.q38hip_kv_attention(self._ref, layer, out.data_ptr(), query.data_ptr(),
+                                         None if gate is None else gate.data_ptr(), kind, heads, stride[0], stride[1],
+                                         out.stride(0), dim ** -0.5 if scale is None else scale, ids, starts, count, rows,
+                                         None if work is None else work.data_ptr(), self._stream()), "q38hip_kv_attention")
         return out
