@@ -114,22 +114,6 @@ uint64_t plan_kv_attention(KVAttention &call);
 
 namespace q38 {
 
-/* index of the sequence whose slots hold `slot`, by the whole wavefront (-1: none) */
-__device__ __forceinline__ int kv_find_sequence(const KVRows &rows, uint32_t slot, uint32_t per_row, uint32_t unit,
-                                                uint32_t gap)
-{
-    const uint32_t lane = threadIdx.x & 63;
-    int found = -1;
-    for (uint32_t first = 0; first < rows.count; first += 64) {
-        const uint32_t i = first + lane;
-        const bool at = i < rows.count && kv_slot_base(kv_row_start(rows, i), i, per_row, unit, gap) <= slot;
-        const int before = __popcll(__ballot(at));
-        found = (int)first + before - 1;
-        if (before < 64) break;
-    }
-    return found;
-}
-
 /* launchers (q38_kv_append.hip, q38_kv_attention*.hip, q38_kv_pages.hip); false when a launch failed */
 bool launch_kv_append(const Q38KVPages &cache, uint32_t layer, const void *key, const void *value, int type,
                       uint64_t row_stride, const KVRows &rows, hipStream_t stream);

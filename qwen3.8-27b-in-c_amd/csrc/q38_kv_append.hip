@@ -32,33 +32,54 @@ struct KVAppend {
     const void *key, *value;
     uint64_t row_stride;
     uint32_t page_shift, dim_shift;
-    bool vector;          /* rows are aligned to four elements */
 };
 
-template <int TYPE>
-__device__ __forceinline__ void load4(float *x, const void *base, uint64_t at, bool vector)
+/* the sequence whose slots hold `slot` (kv_slot_base of pages), found by the
+ * whole wavefront: 64 sequences at a time, one per lane */
+struct KVFound {
+    int index;                      /* -1: none */
+    uint32_t begin, end;            /* its rows */
+    int32_t sequence;
+};
+__device__ __forceinline__ KVFound find_sequence(const KVRows &rows, uint32_t slot, uint32_t T)
 {
-    if constexpr (TYPE == kElementF32) {
-        const float *p = static_cast<const float *>(base) + at;
-        if (vector) {
-            const float4 v = *reinterpret_cast<const float4 *>(p);
-            x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-        } else {
-            for (int e = 0; e < 4; ++e) x[e] = p[e];
+    const uint32_t lane = threadIdx.x & 63;
+    KVFound found{-1, 0, 0, -1};
+    for (uint32_t first = 0; first < rows.count; first += 64) {
+        const uint32_t i = first + lane;
+        uint32_t begin = 0, end = 0;
+        int32_t sequence = -1;
+        if (i < rows.count) {
+            begin = kv_row_start(rows, i);
+            end = kv_row_start(rows, i + 1);
+            sequence = rows.sequences[i];
         }
-    } else {
-        const uint16_t *p = static_cast<const uint16_t *>(base) + at;
-        uint16_t bits[4];
-        if (vector) {
-            const uint2 v = *reinterpret_cast<const uint2 *>(p);
-            bits[0] = v.x & 0xffff, bits[1] = v.x >> 16, bits[2] = v.y & 0xffff, bits[3] = v.y >> 16;
-        } else {
-            for (int e = 0; e < 4; ++e) bits[e] = p[e];
-        }
-        for (int e = 0; e < 4; ++e)
-            x[e] = TYPE == kElementF16 ? f16_to_f32(bits[e]) : __uint_as_float((uint32_t)bits[e] << 16);
+        const int before = __popcll(__ballot(i < rows.count && kv_slot_base(begin, i, 1, T, 2) <= slot));
+        if (before)
+            found = {(int)first + before - 1, (uint32_t)__builtin_amdgcn_readlane((int)begin, before - 1),
+                     (uint32_t)__builtin_amdgcn_readlane((int)end, before - 1), __builtin_amdgcn_readlane(sequence, before - 1)};
+        if (before < 64) break;
     }
+    return found;
 }
+
+/* four elements at any alignment of their own */
+template <int TYPE>
+struct Raw4 {
+    struct __attribute__((packed, aligned(2))) Words {
+        uint32_t word[TYPE == kElementF32 ? 4 : 2];
+    } bits;
+    __device__ __forceinline__ void load(const void *base, uint64_t at)
+    {
+        bits = *reinterpret_cast<const Words *>(static_cast<const uint8_t *>(base) + at * (TYPE == kElementF32 ? 4 : 2));
+    }
+    __device__ __forceinline__ float element(int e) const
+    {
+        if constexpr (TYPE == kElementF32) return __uint_as_float(bits.word[e]);
+        const uint32_t half = bits.word[e / 2] >> (e % 2 * 16) & 0xffffu;
+        return TYPE == kElementF16 ? f16_to_f32(half) : __uint_as_float(half << 16);
+    }
+};
 
 /* the code of v, |v| <= 127 or 448 */
 template <bool E4M3>
@@ -92,15 +113,14 @@ __global__ __launch_bounds__(kMostThreads) void kv_append_kernel(KVAppend a)
     __shared__ uint32_t wave_largest[kMostThreads / 64];
     const uint32_t T = a.cache.page_tokens, D = a.cache.head_dim, threads = blockDim.x;
     const uint32_t slot = blockIdx.x, half = blockIdx.y & 1, head = blockIdx.y >> 1;
-    const int i = kv_find_sequence(a.rows, slot, 1, T, 2);
-    if (i < 0) return;
-    const uint32_t begin = kv_row_start(a.rows, i), end = kv_row_start(a.rows, i + 1);
-    if (end <= begin) return;
-    const int32_t sequence = a.rows.sequences[i];
+    const KVFound at_rows = find_sequence(a.rows, slot, T);
+    const uint32_t begin = at_rows.begin, end = at_rows.end;
+    if (at_rows.index < 0 || end <= begin) return;
+    const int32_t sequence = at_rows.sequence;
     const uint32_t tokens = kv_tokens(a.cache, sequence);
     /* rows that lie before the sequence's first token are left out */
     const uint32_t rows = min(end - begin, tokens), first = tokens - rows;
-    const uint32_t entry = (first >> a.page_shift) + (slot - kv_slot_base(begin, i, 1, T, 2));
+    const uint32_t entry = (first >> a.page_shift) + (slot - kv_slot_base(begin, at_rows.index, 1, T, 2));
     if (!rows || entry >= a.cache.table_entries || entry * T >= tokens) return;
     const int32_t page = kv_page(a.cache, sequence, entry);
     if (page < 0) {
@@ -117,18 +137,21 @@ __global__ __launch_bounds__(kMostThreads) void kv_append_kernel(KVAppend a)
     const float was = from ? a.cache.scales[block] : 0.0f;
 
     /* item k of a thread: token 4 (item / quads) + k % 4 of channels 4 (item % quads) .. */
-    float x[kQuads][4];
-    uint32_t largest = 0;
+    Raw4<TYPE> raw[kQuads];
 #pragma unroll
     for (int k = 0; k < kQuads; ++k) {
         const uint32_t item = threadIdx.x + (k / 4) * threads, t = (item >> (a.dim_shift - 2)) * 4 + k % 4;
-        const uint32_t d = (item & (D / 4 - 1)) * 4;
-        if (t >= from && t < to) load4<TYPE>(x[k], source, origin + t * a.row_stride + d, a.vector);
-        else x[k][0] = x[k][1] = x[k][2] = x[k][3] = 0.0f;
+        /* a token that is not new stands in for none: the nearest that is */
+        raw[k].load(source, origin + min(max(t, from), to - 1) * a.row_stride + (item & (D / 4 - 1)) * 4);
     }
+    float x[kQuads][4];
+    uint32_t largest = 0;
 #pragma unroll
     for (int k = 0; k < kQuads; ++k)
-        for (int e = 0; e < 4; ++e) largest = max(largest, __float_as_uint(x[k][e]) & 0x7fffffffu);
+        for (int e = 0; e < 4; ++e) {
+            x[k][e] = raw[k].element(e);
+            largest = max(largest, __float_as_uint(x[k][e]) & 0x7fffffffu);
+        }
     for (int by = 1; by < 64; by *= 2) largest = max(largest, (uint32_t)__shfl_xor((int)largest, by));
     if ((threadIdx.x & 63) == 0) wave_largest[threadIdx.x >> 6] = largest;
     __syncthreads();                                   /* also: every thread has read the old scale */
@@ -212,11 +235,9 @@ bool launch_kv_append(const Q38KVPages &cache, uint32_t layer, const void *key, 
                       uint64_t row_stride, const KVRows &rows, hipStream_t stream)
 {
     KVAppend a{cache, rows, key, value, row_stride, (uint32_t)__builtin_ctz(cache.page_tokens),
-               (uint32_t)__builtin_ctz(cache.head_dim), false};
+               (uint32_t)__builtin_ctz(cache.head_dim)};
     a.cache.data += (uint64_t)layer * cache.pages * kv_page_bytes(cache);
     a.cache.scales += (uint64_t)layer * cache.pages * 2 * cache.kv_heads;
-    const uintptr_t step = type == kElementF32 ? 4 : 2;
-    a.vector = row_stride % 4 == 0 && ((uintptr_t)key | (uintptr_t)value) % (4 * step) == 0;
     const uint32_t slots = (uint32_t)kv_slots(rows.total_rows, rows.count, 1, cache.page_tokens, 2);
     return cache.type == Q38_KV_E4M3 ? launch_kind<true>(a, type, slots, stream)
                                      : launch_kind<false>(a, type, slots, stream);

@@ -78,6 +78,8 @@ __global__ __launch_bounds__(kPlan) void kv_extend_kernel(Q38KVPages c, const in
     uint32_t before = 0, after = 0, bad = 0, take = 0;
     int32_t id = -1, tail = -1;
     bool copy = false;
+    /* the scan's first round is on its way while the items are looked at */
+    const uint32_t first_bits = free_bits(c.refs, i * kScanEach, c.pages);
     if (i == 0) trouble = 0;
     if (i < count) {
         id = sequences[i];
@@ -124,7 +126,7 @@ __global__ __launch_bounds__(kPlan) void kv_extend_kernel(Q38KVPages c, const in
     /* the lowest free pages */
     uint32_t have = 0;
     for (uint32_t first = 0; first < c.pages && have < total; first += kPlan * kScanEach) {
-        uint32_t bits = free_bits(c.refs, first + i * kScanEach, c.pages), all;
+        uint32_t bits = first ? free_bits(c.refs, first + i * kScanEach, c.pages) : first_bits, all;
         uint32_t rank = have + block_prefix(__popc(bits), sums, all);
         for (; bits && rank < total; bits &= bits - 1, ++rank) found[rank] = (int32_t)(first + i * kScanEach + __ffs(bits) - 1);
         have += all;
@@ -261,9 +263,13 @@ __global__ __launch_bounds__(kPlan) void kv_compact_plan_kernel(Q38KVPages c, in
     __shared__ uint32_t sums[kPlan / 64];
     int32_t *targets = plan + 2, *sources = targets + c.pages, *place = sources + c.pages;
     const uint32_t i = threadIdx.x;
-    uint32_t free_pages = 0, all;
-    for (uint64_t first = 0; first < c.pages; first += kPlan * kScanEach)
-        if (first + i * kScanEach < c.pages) free_pages += __popc(free_bits(c.refs, (uint32_t)first + i * kScanEach, c.pages));
+    uint32_t free_pages = 0, all, first_bits = 0;
+    for (uint64_t first = 0; first < c.pages; first += kPlan * kScanEach) {
+        const uint64_t mine = first + i * kScanEach;
+        const uint32_t bits = mine < c.pages ? free_bits(c.refs, (uint32_t)mine, c.pages) : 0;
+        if (!first) first_bits = bits;
+        free_pages += __popc(bits);
+    }
     block_prefix(free_pages, sums, all);
     const uint32_t live = c.pages - all;
     __syncthreads();
@@ -274,17 +280,18 @@ __global__ __launch_bounds__(kPlan) void kv_compact_plan_kernel(Q38KVPages c, in
         if (mine < c.pages) {
             const uint32_t inside = (uint32_t)min((uint64_t)kScanEach, c.pages - mine);
             const uint32_t below = mine >= live ? 0 : (uint32_t)min((uint64_t)kScanEach, live - mine);
-            const uint32_t bits = free_bits(c.refs, (uint32_t)mine, c.pages);
+            const uint32_t bits = first ? free_bits(c.refs, (uint32_t)mine, c.pages) : first_bits;
             hole = bits & ((1u << below) - 1);
             mover = ~bits & ((1u << inside) - 1) & ~((1u << below) - 1);
         }
-        uint32_t rank = holes + block_prefix(__popc(hole), sums, all);
-        holes += all;
+        /* both ranks in one sum: a round has 2^14 pages */
+        const uint32_t before = block_prefix((uint32_t)__popc(hole) | (uint32_t)__popc(mover) << 16, sums, all);
+        uint32_t rank = holes + (before & 0xffffu);
         for (; hole; hole &= hole - 1) targets[rank++] = (int32_t)mine + __ffs(hole) - 1;
-        __syncthreads();
-        rank = movers + block_prefix(__popc(mover), sums, all);
-        movers += all;
+        rank = movers + (before >> 16);
         for (; mover; mover &= mover - 1) sources[rank++] = (int32_t)mine + __ffs(mover) - 1;
+        holes += all & 0xffffu;
+        movers += all >> 16;
         __syncthreads();
     }
     __threadfence_block();
