@@ -97,7 +97,8 @@ struct KVAttention {
     void *output;
     float *partial;        /* the workspace (q38_kv_attention.h) */
     uint64_t query_row, query_head, output_row;
-    uint32_t group, page_shift;
+    uint32_t group, group_magic, page_shift;
+    float workgroups_inverse;
     uint32_t columns, slots;               /* columns of a slot, at most that many slots */
     uint32_t workgroups, shift, least;     /* per key/value head; steps of a unit (log2); units of a workgroup at least */
     int type;

@@ -61,6 +61,7 @@ const char *plan_attention(const Q38KVPages *cache, uint32_t type, uint32_t head
     a.rows = {nullptr, nullptr, count, total_rows, total_rows / count};
     a.type = (int)type;
     a.group = heads / cache->kv_heads;
+    if (a.group > 32768) return "more than 32768 query heads to a key/value head";
     bytes = q38::plan_kv_attention(a);
     return nullptr;
 }

@@ -216,22 +216,30 @@ __device__ __forceinline__ void kv_finish4(const KVAttention &a, uint32_t row, u
 
 /* ---- work ---------------------------------------------------------------------- */
 
-/* A slot: up to a.columns columns of one sequence. */
+/* A slot: up to a.columns columns of one sequence, from the rem-th query head
+ * of the group in its row `row` on. */
 struct KVSlot {
     uint32_t index;                              /* among the call's slots */
-    uint32_t first_row, rows, column, columns;   /* columns column .. column + columns - 1 of the sequence's rows x group */
-    int32_t sequence, tokens;                    /* sequence -1 where the id is bad */
-    int32_t seen;                                /* tokens the slot's last row sees */
-    __device__ __forceinline__ int32_t seen_by(uint32_t column_at, uint32_t group) const
+    uint32_t first_row, row, rem, columns;       /* the sequence's first row in the call */
+    int32_t sequence, seen_first, seen;          /* -1 where the id is bad; tokens that row `row`, and the last, sees */
+    /* row of the slot's column c, from `row` on, and its head of the group */
+    __device__ __forceinline__ uint32_t row_of(const KVAttention &a, uint32_t c) const { return kv_divide(rem + c, a.group_magic); }
+    __device__ __forceinline__ uint32_t head_of(const KVAttention &a, uint32_t c) const
     {
-        return tokens - (int32_t)rows + (int32_t)(column_at / group) + 1;
+        return rem + c - row_of(a, c) * a.group;
+    }
+    /* tokens that column c sees, none or fewer for a row before the sequence's first token */
+    __device__ __forceinline__ int32_t seen_by(const KVAttention &a, uint32_t c) const
+    {
+        return seen_first + (int32_t)row_of(a, c);
     }
 };
 
 /* 64 sequences of the call, one per lane, and the prefix sums of their slots
  * and units (kv_slot_units) */
+template <uint32_t COLUMNS>
 struct KVLanes {
-    uint32_t first, count;                       /* of the block; sequences of the call */
+    uint32_t first;                              /* of the block */
     uint32_t begin, end, slots, each;            /* the lane's; units of each slot */
     int32_t id, tokens;
     uint32_t slots_upto, units_upto;             /* inclusive, within the block */
@@ -249,12 +257,17 @@ struct KVLanes {
             begin = kv_row_start(a.rows, i);
             end = kv_row_start(a.rows, i + 1);
             tokens = (int32_t)kv_tokens(a.cache, id);
-            slots = ((end - begin) * a.group + a.columns - 1) / a.columns;
+            slots = ((end - begin) * a.group + COLUMNS - 1) / COLUMNS;
             each = kv_slot_units(kv_steps((uint32_t)tokens), a.shift);
         }
         good = __all(begin <= end);
         slots_upto = slots;
         units_upto = slots * each;
+        if (a.rows.count == 1) {
+            slots_upto = of(slots_upto, 0);
+            units_upto = of(units_upto, 0);
+            return;
+        }
         for (int by = 1; by < 64; by *= 2) {
             const uint32_t s = (uint32_t)__shfl_up((int)slots_upto, by), u = (uint32_t)__shfl_up((int)units_upto, by);
             if (lane >= (uint32_t)by) slots_upto += s, units_upto += u;
@@ -269,8 +282,10 @@ struct KVLanes {
 /* What a workgroup does.  The slots' units, one after another, are cut into
  * equal ranges, one per workgroup (and key/value head); a slot of few units
  * goes whole to the range that it begins in. */
+template <uint32_t COLUMNS>
 struct KVWalk {
-    KVLanes block;
+    using Lanes = KVLanes<COLUMNS>;
+    Lanes block;
     uint32_t block_slots, block_units;           /* of the sequences before the block */
     uint32_t total_slots, total_units, chunk, small, at, end;
 
@@ -281,8 +296,8 @@ struct KVWalk {
         for (uint32_t first = (a.rows.count - 1) / 64 * 64 + 64; first; ) {
             first -= 64;
             block.load(a, first);
-            total_slots += KVLanes::of(block.slots_upto, 63);
-            total_units += KVLanes::of(block.units_upto, 63);
+            total_slots += Lanes::of(block.slots_upto, 63);
+            total_units += Lanes::of(block.units_upto, 63);
             good = good && block.good;
         }
         if (!good) {
@@ -290,7 +305,7 @@ struct KVWalk {
             if (threadIdx.x == 0) atomicOr(a.cache.status, Q38_KV_BAD_ROWS);
             total_slots = total_units = 0;
         }
-        chunk = kv_chunk(total_units, a.workgroups, a.least);
+        chunk = kv_chunk(total_units, a.workgroups, a.workgroups_inverse, a.least);
         small = kv_small(chunk);
         at = min((uint64_t)workgroup * chunk, (uint64_t)total_units);
         end = min((uint64_t)at + chunk, (uint64_t)total_units);
@@ -301,23 +316,25 @@ struct KVWalk {
     {
         const uint32_t from = at;
         while (at < end) {
-            while (at - block_units >= KVLanes::of(block.units_upto, 63)) {
-                block_slots += KVLanes::of(block.slots_upto, 63);
-                block_units += KVLanes::of(block.units_upto, 63);
+            while (at - block_units >= Lanes::of(block.units_upto, 63)) {
+                block_slots += Lanes::of(block.slots_upto, 63);
+                block_units += Lanes::of(block.units_upto, 63);
                 block.load(a, block.first + 64);
             }
             const int i = __popcll(__ballot(block.units_upto <= at - block_units));
-            const uint32_t slots = KVLanes::of(block.slots, i), each = KVLanes::of(block.each, i);
-            const uint32_t base = block_units + KVLanes::of(block.units_upto, i) - slots * each;
+            const uint32_t slots = Lanes::of(block.slots, i), each = Lanes::of(block.each, i);
+            const uint32_t base = block_units + Lanes::of(block.units_upto, i) - slots * each;
             const uint32_t j = slots == 1 ? 0 : (at - base) / each, slot_at = base + j * each;
-            s.first_row = KVLanes::of(block.begin, i);
-            s.rows = KVLanes::of(block.end, i) - s.first_row;
-            s.index = block_slots + KVLanes::of(block.slots_upto, i) - slots + j;
-            s.column = j * a.columns;
-            s.columns = min(a.columns, s.rows * a.group - s.column);
-            s.tokens = (int32_t)KVLanes::of((uint32_t)block.tokens, i);
-            s.sequence = s.tokens > 0 ? (int32_t)KVLanes::of((uint32_t)block.id, i) : -1;
-            s.seen = max(0, s.seen_by(s.column + s.columns - 1, a.group));
+            const uint32_t rows = Lanes::of(block.end, i) - Lanes::of(block.begin, i), column = j * COLUMNS;
+            const int32_t tokens = (int32_t)Lanes::of((uint32_t)block.tokens, i);
+            s.first_row = Lanes::of(block.begin, i);
+            s.index = block_slots + Lanes::of(block.slots_upto, i) - slots + j;
+            s.row = j ? column / a.group : 0;
+            s.rem = column - s.row * a.group;
+            s.columns = min(COLUMNS, rows * a.group - column);
+            s.sequence = tokens > 0 ? (int32_t)Lanes::of((uint32_t)block.id, i) : -1;
+            s.seen_first = tokens - (int32_t)rows + (int32_t)s.row + 1;
+            s.seen = max(0, s.seen_by(a, s.columns - 1));
             at = slot_at + each;
             piece = kv_piece(slot_at, each, kv_steps((uint32_t)s.seen), from, end, small, a.shift);
             if (piece.some) return true;
@@ -330,7 +347,7 @@ struct KVWalk {
  * is the number of slots), then the sums of the pieces, then their (maximum,
  * total). */
 struct KVRecord {
-    uint32_t pieces, first_piece, first_row, column, columns, unused[3];
+    uint32_t pieces, first_piece, row, rem, columns, unused[3];    /* row: of the call */
 };
 __device__ __forceinline__ KVRecord *kv_records(const KVAttention &a) { return reinterpret_cast<KVRecord *>(a.partial); }
 __device__ __forceinline__ float *kv_partial(const KVAttention &a, uint64_t piece, uint32_t head)
@@ -388,10 +405,10 @@ __device__ __forceinline__ uint32_t kv_key_turn(uint32_t n)
 template <int D, bool COLUMNS>
 constexpr int kv_ring_bytes() { return (COLUMNS ? 2 : 4) * 128 * D; }
 constexpr int kKVMetaBytes = 4 * 2 * 256;
-template <int D, int TILE, bool COLUMNS>
+template <int D, bool COLUMNS>
 constexpr int kv_lds_bytes()
 {
-    constexpr int merge = 4 * TILE * (D + 4) * 4;
+    constexpr int merge = 4 * 16 * (D + 4) * 4;
     return (kv_ring_bytes<D, COLUMNS>() > merge ? kv_ring_bytes<D, COLUMNS>() : merge) + kKVMetaBytes;
 }
 
@@ -404,19 +421,22 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
     constexpr int kPitch = D + 4;
     constexpr int kCopies = D / 16;                                /* copies of 1 KiB of a step's keys or values */
     constexpr int kRuns = D / 64;                                  /* of 16-token groups that a lane copies keys of */
-    __shared__ __attribute__((aligned(16))) uint8_t ring[kv_lds_bytes<D, kTile, COLUMNS>()];
-    __shared__ float merge_m[4 * NT * kTile], merge_l[4 * NT * kTile];
+    constexpr uint32_t kColumns = NT * kTile * (COLUMNS ? 4 : 1);
+    constexpr int kTileBytes = 16 * D * 2;                          /* a tile's queries in fp16, as the products take them */
+    __shared__ __attribute__((aligned(16))) uint8_t ring[kv_lds_bytes<D, COLUMNS>()];
+    __shared__ __attribute__((aligned(16))) uint8_t queries[COLUMNS ? 16 : NT * kTileBytes];
+    __shared__ float merge_m[4 * NT * kTile], merge_l[4 * NT * kTile], to_exponent[kColumns];
 
     const uint32_t head = blockIdx.y;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     const uint32_t T = a.cache.page_tokens, low_half = n >= 8 ? 0xffffffffu : 0u;
     uint8_t *mine = ring + (COLUMNS ? 0 : wave * 128 * D);        /* the (first) keys; values 64 D behind */
-    float *meta = reinterpret_cast<float *>(ring + kv_lds_bytes<D, kTile, COLUMNS>() - kKVMetaBytes) + wave * 128;
+    float *meta = reinterpret_cast<float *>(ring + kv_lds_bytes<D, COLUMNS>() - kKVMetaBytes) + wave * 128;
 
     /* LDS places of the lane's reads */
-    uint32_t key_at[kChunks];
+    uint32_t key_at[COLUMNS ? kChunks : 1];
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j) key_at[j] = n * D + (((uint32_t)(4 * j + g) ^ kv_key_turn<D>(n)) & (D / 16 - 1)) * 16;
+    for (int j = 0; COLUMNS && j < kChunks; ++j) key_at[j] = n * D + (((uint32_t)(4 * j + g) ^ kv_key_turn<D>(n)) & (D / 16 - 1)) * 16;
     const uint32_t value_at = 64 * D + n * 64 + (g ^ (n >> 2)) * 16;
     /* what the lane copies.  Keys: copy d = kRuns i + run is rows 16 i + (64 /
      * D..) of the tile: within a run every i is four tokens further on */
@@ -424,36 +444,22 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
     const uint32_t copy_row = lane / kLanesPerRow;                /* + run * kRowsPerCopy = n of the row */
     const uint32_t value_group = (lane & 3) ^ ((lane >> 4) & 3);
 
-    KVWalk walk;
+    KVWalk<kColumns> walk;
     walk.start(a, blockIdx.x);
     if (a.workgroups > 1 && blockIdx.x == 0 && head == 0 && threadIdx.x == 0) kv_records(a)->pieces = walk.total_slots;
     KVSlot s;
     KVPiece piece;
     while (walk.next(a, s, piece)) {
-        /* the wavefront's columns */
-        uint32_t column[NT];
+        /* the wavefront's columns, and least and most that they see: columns are in row order */
+        const uint32_t first_column = COLUMNS ? wave * NT * kTile : 0;
         int32_t seen[NT], seen_least = 0x7fffffff, seen_most = 0;
-        float to_u[NT];
-        kv_half8 q[NT][2 * kChunks];
-        constexpr int kRaw = SPLIT ? 8 : 4;
-        uint32_t raw[NT][2 * kChunks][kRaw];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            column[t] = ((COLUMNS ? wave * NT : 0) + t) * kTile + (SPLIT ? n & 7 : n);
-            const bool held = column[t] < s.columns;
-            const uint32_t at = s.column + (held ? column[t] : 0);
-            seen[t] = held ? s.seen_by(at, a.group) : 0;
-            const uint64_t from = (s.first_row + at / a.group) * a.query_row + (head * a.group + at % a.group) * a.query_head;
-#pragma unroll
-            for (int c = 0; c < 2 * kChunks; ++c) kv_load8<SPLIT>(raw[t][c], a.query, from + (c / 2) * 64 + g * 16 + (c & 1) * 8);
-        }
-        /* least and most over the wavefront's columns: columns are in row order */
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const uint32_t first = ((COLUMNS ? wave * NT : 0) + t) * kTile;
+            const uint32_t first = first_column + t * kTile, c = first + (SPLIT ? n & 7 : n);
+            seen[t] = c < s.columns ? s.seen_by(a, c) : 0;
             if (first < s.columns) {
-                seen_least = min(seen_least, s.seen_by(s.column + first, a.group));
-                seen_most = max(seen_most, s.seen_by(s.column + min(first + kTile, s.columns) - 1, a.group));
+                seen_least = min(seen_least, s.seen_by(a, first));
+                seen_most = max(seen_most, s.seen_by(a, min(first + kTile, s.columns) - 1));
             }
         }
         constexpr uint32_t kStride = COLUMNS ? 1 : 4;
@@ -482,7 +488,7 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                 const uint32_t token = at * kKVStep + 16 * (row >> 2) + (row & 3);
                 const int32_t page = max(__shfl(pages, (int)(4 * turn + (row >> 2))), 0);
                 const uint8_t *from = a.cache.data + kv_block(a.cache, page, 0, head) * (T * D) + (token & (T - 1)) * D + chunk * 16;
-#pragma unroll
+#pragma unroll 1
                 for (int i = first; i < first + count; ++i) kv_copy16(from + 4 * i * D, to + (kRuns * i + run) * 1024);
             }
         };
@@ -490,49 +496,93 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
             const int32_t page = max(__shfl(pages, (int)(4 * turn + value_group)), 0);
             const uint8_t *from = a.cache.data + kv_block(a.cache, page, 1, head) * (T * D) + (first * 16 + (lane >> 2)) * T +
                                   ((at * kKVStep + 16 * value_group) & (T - 1));
-#pragma unroll
+#pragma unroll 4
             for (int c = 0; c < count; ++c) kv_copy16(from + c * 16 * T, to + (first + c) * 1024);
         };
 
-        load_pages(step);
-        if (step < end) {
-            if (COLUMNS) {
+        /* Queries to fp16, scaled to a power of two by the largest of their row: a thread
+         * takes eight channels, a row's threads are neighbours.  Lane (n, g) of the i-th
+         * of a tile's 1 KiB has what it multiplies in the i-th product. */
+        constexpr int kThreads = COLUMNS ? 64 : 256, kEights = D / 8;
+        constexpr int kRows = COLUMNS ? kTile : NT * kTile, kEach = (kRows * kEights + kThreads - 1) / kThreads;
+        uint32_t raw[kEach][SPLIT ? 8 : 4];
+        const uint32_t eight = threadIdx.x % kEights, row_at = (COLUMNS ? lane : threadIdx.x) / kEights;
+        auto load_queries = [&](uint32_t first) {
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                const uint32_t c = first + k * (kThreads / kEights) + row_at, taken = min(c, s.columns - 1);
+                kv_load8<SPLIT>(raw[k], a.query,
+                                (s.first_row + s.row + s.row_of(a, taken)) * a.query_row +
+                                    (head * a.group + s.head_of(a, taken)) * a.query_head + eight * 8);
+            }
+        };
+        auto convert_queries = [&](uint32_t first, uint8_t *to) {
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                const uint32_t at = k * (kThreads / kEights) + row_at, c = first + at;
+                uint32_t largest = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    largest = max(largest, __float_as_uint(kv_element8<SPLIT>(raw[k], e, a.type)) & 0x7fffffffu);
+                /* non-negative floats order as their bits; NaN is above all of them */
+                for (int by = 1; by < kEights; by *= 2) largest = max(largest, (uint32_t)__shfl_xor((int)largest, by));
+                const uint32_t exponent = max(largest >> 23, 30u);
+                /* largest * scale is in 2^13..2^14; columns that are not there are zero */
+                const float scale = c < s.columns ? __uint_as_float((267u - exponent) << 23) : 0.0f;
+                if (kRows * kEights < kThreads && at >= kRows) break;
+                if (eight == 0) to_exponent[c] = a.scale * __uint_as_float((exponent - 13u) << 23);
+                kv_half8 high, low;
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const float v = c < s.columns ? kv_element8<SPLIT>(raw[k], e, a.type) * scale : 0.0f;
+                    const float w = c < s.columns ? kv_element8<SPLIT>(raw[k], e + 1, a.type) * scale : 0.0f;
+                    const kv_half2 a2 = kv_round2<false>(v, w, 0), b2 = kv_round2<SPLIT>(v, w, 0xffffffffu);
+                    high[e] = a2[0], high[e + 1] = a2[1];
+                    low[e] = b2[0], low[e + 1] = b2[1];
+                }
+                kv_half8 *fragment = reinterpret_cast<kv_half8 *>(to + at / kTile * kTileBytes) +
+                                     ((eight >> 3) * 2 + (eight & 1)) * 64 + (eight >> 1 & 3) * 16 + at % kTile;
+                fragment[0] = high;
+                if (SPLIT) fragment[8] = low;
+            }
+        };
+
+        kv_half8 q[COLUMNS ? NT : 1][2 * kChunks];
+        uint8_t *const other = ring + 128 * D;                     /* COLUMNS: free until the first step */
+        if (COLUMNS) {
+            load_pages(step);
+            if (step < end) {
                 copy_keys(step, kv_lds(mine), wave, 1);
                 copy_values(step, kv_lds(mine) + 64 * D, wave * (kCopies / 4), kCopies / 4);
-            } else {
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                uint8_t *to = other + wave * kTileBytes;
+                load_queries(first_column + t * kTile);
+                convert_queries(first_column + t * kTile, to);
+                kv_reads_done();
+#pragma unroll
+                for (int c = 0; c < 2 * kChunks; ++c) q[COLUMNS ? t : 0][c] = reinterpret_cast<const kv_half8 *>(to)[c * 64 + lane];
+                kv_reads_done();
+            }
+        } else {
+            load_queries(0);
+            /* here, so that nothing the compiler waits for is behind the copies */
+#pragma unroll
+            for (int k = 0; k < kEach; ++k)
+#pragma unroll
+                for (int e = 0; e < (SPLIT ? 8 : 4); ++e) asm volatile("" ::"v"(raw[k][e]));
+            load_pages(step);
+            if (step < end) {
                 copy_keys(step, kv_lds(mine), 0, 4);
                 copy_values(step, kv_lds(mine) + 64 * D, 0, kCopies);
             }
+            convert_queries(0, queries);
+            kv_barrier();
         }
+        float to_u[NT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            uint32_t largest = 0;
-            const bool held = column[t] < s.columns;
-#pragma unroll
-            for (int c = 0; c < 2 * kChunks; ++c)
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    largest = max(largest, __float_as_uint(kv_element8<SPLIT>(raw[t][c], e, a.type)) & 0x7fffffffu);
-            /* non-negative floats order as their bits; NaN is above all of them */
-            {
-                auto r = __builtin_amdgcn_permlane16_swap(largest, largest, false, false);
-                largest = max(r[0], r[1]);
-                r = __builtin_amdgcn_permlane32_swap(largest, largest, false, false);
-                largest = max(r[0], r[1]);
-            }
-            if (!held) largest = 0;
-            const uint32_t exponent = max(largest >> 23, 30u);
-            const float scale = held ? __uint_as_float((267u - exponent) << 23) : 0.0f;   /* largest * scale in 2^13..2^14 */
-            to_u[t] = a.scale * __uint_as_float((exponent - 13u) << 23);
-#pragma unroll
-            for (int c = 0; c < 2 * kChunks; ++c)
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    const kv_half2 pair = kv_round2<SPLIT>(kv_element8<SPLIT>(raw[t][c], e, a.type) * scale,
-                                                           kv_element8<SPLIT>(raw[t][c], e + 1, a.type) * scale, low_half);
-                    q[t][c][e] = pair[0], q[t][c][e + 1] = pair[1];
-                }
-        }
+        for (int t = 0; t < NT; ++t) to_u[t] = to_exponent[first_column + t * kTile + (SPLIT ? n & 7 : n)];
 
         kv_float4 o[NT][kChannels];
         float m[NT], l[NT];
@@ -569,7 +619,7 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int t = 0; t < NT; ++t) score[t][i] = {0.0f, 0.0f, 0.0f, 0.0f};
-                {
+                if constexpr (COLUMNS) {
                     /* pieces in the order (j, i), read two ahead; the fences keep the
                      * compiler from reading all of them first, for which there are no registers */
                     uint4 raw_codes[3];
@@ -592,6 +642,30 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                             score[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(high, q[t][2 * j + 1], score[t][i], 0, 0, 0);
                     }
                     __builtin_amdgcn_sched_barrier(0);
+                } else {
+                    /* few steps and all of their time in memory: a short loop, with the queries in LDS */
+                    const kv_half8 *mine_q = reinterpret_cast<const kv_half8 *>(queries) + lane;
+#pragma unroll 1
+                    for (int j = 0; j < kChunks; ++j) {
+                        const uint8_t *keys = codes + n * D + (((uint32_t)(4 * j + g) ^ kv_key_turn<D>(n)) & (D / 16 - 1)) * 16;
+                        kv_half8 q0[NT], q1[NT];
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            q0[t] = mine_q[(t * 2 * kChunks + 2 * j) * 64];
+                            q1[t] = mine_q[(t * 2 * kChunks + 2 * j + 1) * 64];
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint4 k = *reinterpret_cast<const uint4 *>(keys + i * 16 * D);
+                            const kv_half8 low = kv_decode8<E4M3>(k.x, k.y), high = kv_decode8<E4M3>(k.z, k.w);
+#pragma unroll
+                            for (int t = 0; t < NT; ++t)
+                                score[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(low, q0[t], score[t][i], 0, 0, 0);
+#pragma unroll
+                            for (int t = 0; t < NT; ++t)
+                                score[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(high, q1[t], score[t][i], 0, 0, 0);
+                        }
+                    }
                 }
                 if (!COLUMNS && more) {
                     kv_reads_done();
@@ -623,8 +697,9 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                     }
 #pragma unroll
                     for (int e = 0; e < 16; ++e) most = fmaxf(most, u[e]);
-                    const uint64_t passed = __ballot(most > kKVWeightExponent + kKVMaximumSlack);
+                    const bool passed = __any(most > kKVWeightExponent + kKVMaximumSlack);
                     float keep = 1.0f;
+                    uint64_t scaled = 0;
                     if (passed) {
                         /* a maximum was passed by that much (m = -inf: the first tokens): sums follow the new one */
                         most = -INFINITY;
@@ -638,6 +713,7 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                         const float now = fmaxf(m[t], most);
                         const float by = m[t] == now ? 0.0f : m[t] - now;
                         keep = exp2f(by);
+                        scaled = __ballot(by != 0.0f && by != -INFINITY);
                         m[t] = now;
                         l[t] = kv_lower(l[t], by);
                         if (!kAccumulators)
@@ -648,7 +724,7 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                         for (int e = 0; e < 16; ++e) u[e] += offset;
                     }
 #pragma unroll
-                    for (int c = 0; kAccumulators && c < kChannels; c += 2) kv_scale(o[t][c], o[t][c + 1], keep, passed);
+                    for (int c = 0; kAccumulators && c < kChannels; c += 2) kv_scale(o[t][c], o[t][c + 1], keep, scaled);
                     float sum = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
@@ -729,7 +805,7 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
         float *partial = kv_partial(a, index, head), *stats = kv_stats(a, index, head);
         if (a.workgroups > 1 && head == 0 && piece.first_piece && threadIdx.x == 0)
             kv_records(a)[1 + s.index] = {piece.whole ? 1 : kv_pieces(piece.units, walk.chunk, walk.at, piece.each),
-                                          (uint32_t)index, s.first_row, s.column, s.columns, {0, 0, 0}};
+                                          (uint32_t)index, s.first_row + s.row, s.rem, s.columns, {0, 0, 0}};
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             l[t] = kv_other_rows(l[t], false);
@@ -748,21 +824,9 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 if (tile_at != t) continue;
-                float keep = 1.0f;
-                if (!COLUMNS) {
-                    float top = -INFINITY;
-                    for (int w = 0; w < 4; ++w) top = fmaxf(top, merge_m[(w * NT + t) * kTile + (SPLIT ? n & 7 : n)]);
-                    keep = m[t] == top ? (m[t] == -INFINITY ? 0.0f : 1.0f) : exp2f(m[t] - top);
-                }
 #pragma unroll
-                for (int c = 0; c < kChannels; ++c) {
-                    kv_float4 sum = o[t][c];
-                    if (SPLIT)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) sum[e] += kv_partner(sum[e]);
-                    if (!SPLIT || n < 8)
-                        *reinterpret_cast<kv_float4 *>(&merge_o[(wave * kTile + n) * kPitch + c * 16 + 4 * g]) = sum * keep;
-                }
+                for (int c = 0; c < kChannels; ++c)
+                    *reinterpret_cast<kv_float4 *>(&merge_o[(wave * 16 + n) * kPitch + c * 16 + 4 * g]) = o[t][c];
             }
             if (COLUMNS) kv_reads_done();           /* the wavefront's own rows; the writes too */
             else __syncthreads();
@@ -772,22 +836,28 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                 if (of >= s.columns) break;
                 float top = -INFINITY, total = 0.0f;
                 kv_float4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+                auto row = [&](uint32_t w) {
+                    const float *from = &merge_o[(w * 16 + c) * kPitch + d];
+                    const kv_float4 v = *reinterpret_cast<const kv_float4 *>(from);
+                    return SPLIT ? v + *reinterpret_cast<const kv_float4 *>(from + 8 * kPitch) : v;
+                };
                 if (COLUMNS) {
                     top = merge_m[of];
                     total = merge_l[of];
-                    sum = *reinterpret_cast<const kv_float4 *>(&merge_o[(wave * kTile + c) * kPitch + d]);
+                    sum = row(wave);
                 } else {
                     for (int w = 0; w < 4; ++w) top = fmaxf(top, merge_m[w * NT * kTile + of]);
+#pragma unroll 1
                     for (int w = 0; w < 4; ++w) {
                         const float mw = merge_m[w * NT * kTile + of];
                         if (mw == -INFINITY) continue;
-                        total += kv_lower(merge_l[w * NT * kTile + of], mw - top);
-                        sum += *reinterpret_cast<const kv_float4 *>(&merge_o[(w * kTile + c) * kPitch + d]);
+                        const float by = mw == top ? 0.0f : mw - top;
+                        total += kv_lower(merge_l[w * NT * kTile + of], by);
+                        sum += row(w) * exp2f(by);
                     }
                 }
                 if (piece.whole) {
-                    const uint32_t col = s.column + of;
-                    kv_finish4(a, s.first_row + col / a.group, head * a.group + col % a.group, d, sum, total);
+                    kv_finish4(a, s.first_row + s.row + s.row_of(a, of), head * a.group + s.head_of(a, of), d, sum, total);
                 } else {
                     *reinterpret_cast<kv_float4 *>(partial + of * D + d) = sum;
                     if (d == 0) {

@@ -55,8 +55,8 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KVAttention a)
         if (group) return;
         for (uint32_t k = 1; k < groups; ++k) sum += sums[threadIdx.x + k * quads];
     }
-    const uint32_t column = r.column + c;
-    kv_finish4(a, r.first_row + column / a.group, head * a.group + column % a.group, d, sum, total);
+    const uint32_t row = kv_divide(r.rem + c, a.group_magic);
+    kv_finish4(a, r.row + row, head * a.group + r.rem + c - row * a.group, d, sum, total);
 }
 
 }  // namespace
@@ -73,10 +73,12 @@ uint64_t plan_kv_attention(KVAttention &a)
     a.least = a.shift ? 1 : shape.columns ? 8 : 4;
     /* as many workgroups as run at once: by LDS where wavefronts have their own
      * tokens (64 D bytes of keys and of values each), else by registers */
-    const uint32_t on_a_unit = shape.columns ? kv_waves(D, shape.tiles, true) : 256 / D;
+    const uint32_t on_a_unit = !shape.columns ? (D == 64 && shape.tiles == 2 ? 2 : 256 / D) : kv_waves(D, shape.tiles, true);
     const uint64_t units = (uint64_t)a.slots * kv_slot_units(most, a.shift), wanted = 256 * on_a_unit / heads;
     const uint64_t useful = (units + a.least - 1) / a.least;
     a.workgroups = (uint32_t)(wanted < 1 ? 1 : wanted < useful ? wanted : useful);
+    a.workgroups_inverse = 1.0f / (float)a.workgroups;
+    a.group_magic = kv_magic(a.group);
     if (a.workgroups == 1) return 0;
     return (a.slots + 1) * sizeof(KVRecord) +
            ((uint64_t)a.workgroups + a.slots) * heads * a.columns * (D + 2) * sizeof(float);

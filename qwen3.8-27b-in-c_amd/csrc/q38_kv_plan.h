@@ -12,17 +12,27 @@ constexpr int kKVStep = 64;               /* tokens of a step */
  * about as long as that many steps */
 constexpr uint32_t kKVSlotOverhead = 2;
 
+/* n / d of n d < 2^32, d < 2^16, from kv_magic(d) */
+inline uint32_t kv_magic(uint32_t d) { return d == 1 ? 0 : (uint32_t)(0xffffffffu / d + 1); }
+Q38_HD uint32_t kv_divide(uint32_t n, uint32_t magic)
+{
+    return magic ? (uint32_t)((uint64_t)n * magic >> 32) : n;
+}
+
 Q38_HD uint32_t kv_steps(uint32_t tokens) { return (tokens + kKVStep - 1) / kKVStep; }
 /* units of a slot of a sequence with that many steps, 2^shift steps each */
 Q38_HD uint32_t kv_slot_units(uint32_t steps, uint32_t shift)
 {
     return ((steps + (1u << shift) - 1) >> shift) + kKVSlotOverhead;
 }
-/* units of a workgroup's range, and of a slot that is never cut */
-Q38_HD uint32_t kv_chunk(uint32_t units, uint32_t workgroups, uint32_t least)
+/* units of a workgroup's range, ceil(units / workgroups) or `least`: units and
+ * workgroups are below 2^31 and 2^16, the quotient by the inverse is one off at most */
+Q38_HD uint32_t kv_chunk(uint32_t units, uint32_t workgroups, float workgroups_inverse, uint32_t least)
 {
-    const uint32_t each = units / workgroups + (units % workgroups ? 1 : 0);
-    return each > least ? each : least;
+    if (units <= least * (uint64_t)workgroups) return least;
+    uint32_t each = (uint32_t)((float)units * workgroups_inverse);
+    while ((uint64_t)each * workgroups < units) each += each >> 22 ? each >> 22 : 1;
+    return each;
 }
 Q38_HD uint32_t kv_small(uint32_t chunk) { return chunk / 4; }
 
@@ -53,7 +63,7 @@ Q38_HD uint32_t kv_pieces(uint32_t units, uint32_t chunk, uint32_t behind, uint3
 /* Column tiles (of 8 fp32 or 16 other columns): up to kv_token_tiles in a
  * workgroup whose wavefronts share the tokens, else one or two in each
  * wavefront. */
-constexpr int kv_token_tiles(int head_dim) { return head_dim == 128 ? 2 : 3; }
+constexpr int kv_token_tiles(int head_dim) { return head_dim == 256 ? 3 : 2; }
 /* wavefronts that share a SIMD's registers: one has 512, of two each 256 */
 constexpr int kv_waves(int head_dim, int tiles, bool columns)
 {
