@@ -492,10 +492,14 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                 for (int i = first; i < first + count; ++i) kv_copy16(from + 4 * i * D, to + (kRuns * i + run) * 1024);
             }
         };
-        auto copy_values = [&](uint32_t at, uint32_t to, int first, int count) {
+        /* where the lane's 16 bytes of value copy 0 of a step come from; copy c is 16 channels on */
+        auto value_from = [&](uint32_t at) {
             const int32_t page = max(__shfl(pages, (int)(4 * turn + value_group)), 0);
-            const uint8_t *from = a.cache.data + kv_block(a.cache, page, 1, head) * (T * D) + (first * 16 + (lane >> 2)) * T +
-                                  ((at * kKVStep + 16 * value_group) & (T - 1));
+            return a.cache.data + kv_block(a.cache, page, 1, head) * (T * D) + (lane >> 2) * T +
+                   ((at * kKVStep + 16 * value_group) & (T - 1));
+        };
+        auto copy_values = [&](uint32_t at, uint32_t to, int first, int count) {
+            const uint8_t *from = value_from(at) + first * 16 * T;
 #pragma unroll 4
             for (int c = 0; c < count; ++c) kv_copy16(from + c * 16 * T, to + (first + c) * 1024);
         };
@@ -643,9 +647,9 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 } else {
-                    /* few steps and all of their time in memory: a short loop, with the queries in LDS */
+                    /* queries in LDS: their registers hold the sums */
                     const kv_half8 *mine_q = reinterpret_cast<const kv_half8 *>(queries) + lane;
-#pragma unroll 1
+#pragma unroll
                     for (int j = 0; j < kChunks; ++j) {
                         const uint8_t *keys = codes + n * D + (((uint32_t)(4 * j + g) ^ kv_key_turn<D>(n)) & (D / 16 - 1)) * 16;
                         kv_half8 q0[NT], q1[NT];
@@ -771,6 +775,8 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                         }
                 }
                 {
+                    /* the next step's channels follow those that were read */
+                    const uint8_t *from = !COLUMNS && more ? value_from(step + kStride) : nullptr;
                     uint4 raw_codes[3];
 #pragma unroll
                     for (int c = 0; c < 2; ++c) raw_codes[c] = *reinterpret_cast<const uint4 *>(codes + value_at + c * 1024);
@@ -787,12 +793,13 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
 #pragma unroll
                         for (int t = 0; t < NT; ++t)
                             o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(high, weight[t][1], o[t][c], 0, 0, 0);
+                        if (!COLUMNS && more && c % 4 == 3) {
+                            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                            for (int e = c - 3; e <= c; ++e) kv_copy16(from + e * 16 * T, kv_lds(mine) + 64 * D + e * 1024);
+                        }
                     }
                     __builtin_amdgcn_sched_barrier(0);
-                }
-                if (!COLUMNS && more) {
-                    kv_reads_done();
-                    copy_values(step + kStride, kv_lds(mine) + 64 * D, 0, kCopies);
                 }
             }
             if (COLUMNS) tile ^= 128 * D;

@@ -8,55 +8,90 @@ namespace q38 {
 namespace {
 
 /* One output of a column's four channels is sum 2^(m_p - top) O_p over its
- * pieces, in an order that the sizes alone decide.  FEW (prompt chunks: many
+ * pieces, in an order that the sizes alone decide.  Few (prompt chunks: many
  * columns of two or three pieces): a thread takes all pieces of four channels.
- * Else a workgroup takes one column, and its 1024 / D groups of threads take
- * every so-manieth piece. */
-template <bool FEW>
-__global__ __launch_bounds__(256) void kv_join_kernel(KVAttention a)
+ * Else a workgroup takes one column after another, and its 4 THREADS / D
+ * groups of threads take every so-manieth piece, so that all are read at once:
+ * 1024 threads where there may be many (one sequence in 64 pieces: 6 us, 10 with
+ * 256), else 256 (480 slots of a few pieces: 5 us, 16 with 1024). */
+__device__ __forceinline__ void finish_column(const KVAttention &a, const KVRecord &r, uint32_t head, uint32_t c, uint32_t d,
+                                              kv_float4 sum, float total)
 {
-    __shared__ kv_float4 sums[FEW ? 1 : 256];
-    const uint32_t slot = blockIdx.x, head = blockIdx.y, D = a.cache.head_dim, quads = D / 4, groups = 256 / quads;
+    const uint32_t row = kv_divide(r.rem + c, a.group_magic);
+    kv_finish4(a, r.row + row, head * a.group + r.rem + c - row * a.group, d, sum, total);
+}
+
+__global__ __launch_bounds__(256) void kv_join_few_kernel(KVAttention a)
+{
+    const uint32_t slot = blockIdx.x, head = blockIdx.y, D = a.cache.head_dim, quads = D / 4;
+    const uint32_t c = blockIdx.z * (256 / quads) + threadIdx.x / quads, d = threadIdx.x % quads * 4;
     const KVRecord r = kv_records(a)[1 + slot];
-    if (slot >= kv_records(a)->pieces || r.pieces < 2) return;
-    const uint32_t group = threadIdx.x / quads, d = threadIdx.x % quads * 4;
-    const uint32_t c = FEW ? blockIdx.z * groups + group : blockIdx.z;
-    if (c >= r.columns) return;
+    if (slot >= kv_records(a)->pieces || r.pieces < 2 || c >= r.columns) return;
     const float *stats = kv_stats(a, r.first_piece, head) + 2 * c, *partial = kv_partial(a, r.first_piece, head) + c * D + d;
     const uint64_t stats_step = (uint64_t)a.cache.kv_heads * a.columns * 2, step = (uint64_t)a.cache.kv_heads * a.columns * D;
     float top = -INFINITY, total = 0.0f;
-    if (FEW) {
-        for (uint32_t p = 0; p < r.pieces; ++p) top = fmaxf(top, stats[p * stats_step]);
-        for (uint32_t p = 0; p < r.pieces; ++p) {
-            const float m = stats[p * stats_step];
-            if (m != -INFINITY) total += kv_lower(stats[p * stats_step + 1], m - top);
-        }
-    } else {
-        /* the same in every wavefront */
-        const uint32_t lane = threadIdx.x & 63;
-        for (uint32_t p = lane; p < r.pieces; p += 64) top = fmaxf(top, stats[p * stats_step]);
-        for (int by = 1; by < 64; by *= 2) top = fmaxf(top, __shfl_xor(top, by));
-        for (uint32_t p = lane; p < r.pieces; p += 64) {
-            const float m = stats[p * stats_step];
-            if (m != -INFINITY) total += kv_lower(stats[p * stats_step + 1], m - top);
-        }
-        for (int by = 1; by < 64; by *= 2) total += __shfl_xor(total, by);
-    }
     kv_float4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (uint32_t p = FEW ? 0 : group; p < r.pieces; p += FEW ? 1 : groups) {
+    for (uint32_t p = 0; p < r.pieces; ++p) top = fmaxf(top, stats[p * stats_step]);
+    for (uint32_t p = 0; p < r.pieces; ++p) {
         const float m = stats[p * stats_step];
-        const float keep = m == -INFINITY ? 0.0f : exp2f(m - top);
-        sum += *reinterpret_cast<const kv_float4 *>(partial + p * step) * keep;
+        if (m == -INFINITY) continue;
+        const float by = m == top ? 0.0f : m - top;
+        total += kv_lower(stats[p * stats_step + 1], by);
+        sum += *reinterpret_cast<const kv_float4 *>(partial + p * step) * exp2f(by);
     }
-    if (!FEW) {
+    finish_column(a, r, head, c, d, sum, total);
+}
+
+template <uint32_t THREADS>
+__global__ __launch_bounds__(THREADS) void kv_join_kernel(KVAttention a)
+{
+    __shared__ kv_float4 sums[THREADS];
+    const uint32_t slot = blockIdx.x, head = blockIdx.y, D = a.cache.head_dim, quads = D / 4;
+    const uint32_t groups = THREADS / quads, group = threadIdx.x / quads, d = threadIdx.x % quads * 4, lane = threadIdx.x & 63;
+    const KVRecord r = kv_records(a)[1 + slot];
+    if (slot >= kv_records(a)->pieces || r.pieces < 2) return;
+    const uint64_t stats_step = (uint64_t)a.cache.kv_heads * a.columns * 2, step = (uint64_t)a.cache.kv_heads * a.columns * D;
+    for (uint32_t c = blockIdx.z; c < r.columns; c += gridDim.z) {
+        const float *stats = kv_stats(a, r.first_piece, head) + 2 * c;
+        const float *partial = kv_partial(a, r.first_piece, head) + c * D + d;
+        /* the group's first pieces are on their way while the maxima are looked at */
+        constexpr uint32_t kAhead = 4;
+        kv_float4 first[kAhead];
+        float first_m[kAhead];
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; ++k) {
+            const uint32_t p = group + k * groups;
+            first[k] = {0.0f, 0.0f, 0.0f, 0.0f};
+            first_m[k] = -INFINITY;
+            if (p >= r.pieces) continue;
+            first[k] = *reinterpret_cast<const kv_float4 *>(partial + p * step);
+            first_m[k] = stats[p * stats_step];
+        }
+        /* maximum and total, the same in every wavefront */
+        const float mine_m = lane < r.pieces ? stats[lane * stats_step] : -INFINITY;
+        const float mine_l = lane < r.pieces ? stats[lane * stats_step + 1] : 0.0f;
+        float top = mine_m;
+        for (uint32_t p = lane + 64; p < r.pieces; p += 64) top = fmaxf(top, stats[p * stats_step]);
+        for (int by = 1; by < 64; by *= 2) top = fmaxf(top, __shfl_xor(top, by));
+        auto lowered = [&](float m, float l) { return m == -INFINITY ? 0.0f : kv_lower(l, m == top ? 0.0f : m - top); };
+        float total = lowered(mine_m, mine_l);
+        for (uint32_t p = lane + 64; p < r.pieces; p += 64) total += lowered(stats[p * stats_step], stats[p * stats_step + 1]);
+        for (int by = 1; by < 64; by *= 2) total += __shfl_xor(total, by);
+        kv_float4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        auto add = [&](float m, kv_float4 o) {
+            if (m != -INFINITY) sum += o * exp2f(m == top ? 0.0f : m - top);
+        };
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; ++k) add(first_m[k], first[k]);
+        for (uint32_t p = group + kAhead * groups; p < r.pieces; p += groups)
+            add(stats[p * stats_step], *reinterpret_cast<const kv_float4 *>(partial + p * step));
         sums[threadIdx.x] = sum;
-        __syncthreads();
-        if (group) return;
-        for (uint32_t k = 1; k < groups; ++k) sum += sums[threadIdx.x + k * quads];
+        for (uint32_t half = groups / 2; half; half /= 2) {
+            __syncthreads();
+            if (group < half) sums[threadIdx.x] = sum = sum + sums[threadIdx.x + half * quads];
+        }
+        if (!group) finish_column(a, r, head, c, d, sum, total);
     }
-    const uint32_t row = kv_divide(r.rem + c, a.group_magic);
-    kv_finish4(a, r.row + row, head * a.group + r.rem + c - row * a.group, d, sum, total);
 }
 
 }  // namespace
@@ -97,10 +132,16 @@ bool launch_kv_attention(const KVAttention &a, hipStream_t stream)
                   : D == 128 ? launch_kv_attention_width<128>(a, stream) : launch_kv_attention_width<256>(a, stream)))
         return false;
     if (a.workgroups == 1) return true;
-    const bool few = kv_shape(a).columns;
-    const uint32_t together = few ? 1024 / D : 1;
-    return launch_kernel(few ? kv_join_kernel<true> : kv_join_kernel<false>,
-                         dim3(a.slots, a.cache.kv_heads, (a.columns + together - 1) / together), dim3(256), stream, a);
+    if (kv_shape(a).columns) {
+        const uint32_t together = 1024 / D;
+        return launch_kernel(kv_join_few_kernel, dim3(a.slots, a.cache.kv_heads, (a.columns + together - 1) / together), dim3(256),
+                             stream, a);
+    }
+    /* as many columns at once as a sequence has on average: workgroups without any cost a launch too */
+    const uint64_t columns = ((uint64_t)a.rows.total_rows * a.group + a.rows.count - 1) / a.rows.count;
+    const dim3 grid(a.slots, a.cache.kv_heads, columns < a.columns ? (uint32_t)columns : a.columns);
+    return a.workgroups >= 8 * a.slots ? launch_kernel(kv_join_kernel<1024>, grid, dim3(1024), stream, a)
+                                       : launch_kernel(kv_join_kernel<256>, grid, dim3(256), stream, a);
 }
 
 }  // namespace q38
