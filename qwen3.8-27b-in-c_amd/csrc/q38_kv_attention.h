@@ -105,27 +105,45 @@ __device__ __forceinline__ kv_half8 kv_decode8(uint32_t lo, uint32_t hi)
     return r.all;
 }
 
+/* sums += A B for sums in accumulation registers, in place: the builtin lets
+ * the compiler give the result other registers, and it moved all sums about once
+ * a step.  What it cannot see it cannot guard, so the wait states are here: two
+ * between a vector instruction that writes A or B, or the product that wrote the
+ * sums, and this one. */
+__device__ __forceinline__ void kv_accumulate(kv_float4 &sums, kv_half8 a, kv_half8 b)
+{
+    asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(sums) : "v"(a), "v"(b));
+}
+
 /* sums times keep where `some` (uniform).  The branch is within the assembly, so
  * that the sums are one value on both ways and stay in their accumulation
  * registers; 18 wait states cover a matrix product that may still write them. */
-__device__ __forceinline__ void kv_scale(kv_float4 &x, kv_float4 &y, float keep, uint64_t some)
+__device__ __forceinline__ void kv_scale(kv_float4 (&x)[4], float keep, uint64_t some)
 {
-    float a = x[0], b = x[1], c = x[2], d = x[3], e = y[0], f = y[1], g = y[2], h = y[3], t;
-    asm volatile("s_cmp_eq_u64 %10, 0\n\ts_cbranch_scc1 1f\n\ts_nop 15\n\ts_nop 3\n\t"
-                 "v_accvgpr_read_b32 %8, %0\n\tv_mul_f32 %8, %8, %9\n\tv_accvgpr_write_b32 %0, %8\n\t"
-                 "v_accvgpr_read_b32 %8, %1\n\tv_mul_f32 %8, %8, %9\n\tv_accvgpr_write_b32 %1, %8\n\t"
-                 "v_accvgpr_read_b32 %8, %2\n\tv_mul_f32 %8, %8, %9\n\tv_accvgpr_write_b32 %2, %8\n\t"
-                 "v_accvgpr_read_b32 %8, %3\n\tv_mul_f32 %8, %8, %9\n\tv_accvgpr_write_b32 %3, %8\n\t"
-                 "v_accvgpr_read_b32 %8, %4\n\tv_mul_f32 %8, %8, %9\n\tv_accvgpr_write_b32 %4, %8\n\t"
-                 "v_accvgpr_read_b32 %8, %5\n\tv_mul_f32 %8, %8, %9\n\tv_accvgpr_write_b32 %5, %8\n\t"
-                 "v_accvgpr_read_b32 %8, %6\n\tv_mul_f32 %8, %8, %9\n\tv_accvgpr_write_b32 %6, %8\n\t"
-                 "v_accvgpr_read_b32 %8, %7\n\tv_mul_f32 %8, %8, %9\n\tv_accvgpr_write_b32 %7, %8\n\t"
+    float v[16], t;
+    for (int e = 0; e < 16; ++e) v[e] = x[e / 4][e % 4];
+    asm volatile("s_cmp_eq_u64 %18, 0\n\ts_cbranch_scc1 1f\n\ts_nop 15\n\ts_nop 3\n\t"
+                 "v_accvgpr_read_b32 %16, %0\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %0, %16\n\t"
+                 "v_accvgpr_read_b32 %16, %1\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %1, %16\n\t"
+                 "v_accvgpr_read_b32 %16, %2\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %2, %16\n\t"
+                 "v_accvgpr_read_b32 %16, %3\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %3, %16\n\t"
+                 "v_accvgpr_read_b32 %16, %4\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %4, %16\n\t"
+                 "v_accvgpr_read_b32 %16, %5\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %5, %16\n\t"
+                 "v_accvgpr_read_b32 %16, %6\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %6, %16\n\t"
+                 "v_accvgpr_read_b32 %16, %7\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %7, %16\n\t"
+                 "v_accvgpr_read_b32 %16, %8\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %8, %16\n\t"
+                 "v_accvgpr_read_b32 %16, %9\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %9, %16\n\t"
+                 "v_accvgpr_read_b32 %16, %10\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %10, %16\n\t"
+                 "v_accvgpr_read_b32 %16, %11\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %11, %16\n\t"
+                 "v_accvgpr_read_b32 %16, %12\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %12, %16\n\t"
+                 "v_accvgpr_read_b32 %16, %13\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %13, %16\n\t"
+                 "v_accvgpr_read_b32 %16, %14\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %14, %16\n\t"
+                 "v_accvgpr_read_b32 %16, %15\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %15, %16\n\t"
                  "s_nop 3\n1:"
-                 : "+a"(a), "+a"(b), "+a"(c), "+a"(d), "+a"(e), "+a"(f), "+a"(g), "+a"(h), "=&v"(t)
+                 : "+a"(v[0]), "+a"(v[1]), "+a"(v[2]), "+a"(v[3]), "+a"(v[4]), "+a"(v[5]), "+a"(v[6]), "+a"(v[7]), "+a"(v[8]), "+a"(v[9]), "+a"(v[10]), "+a"(v[11]), "+a"(v[12]), "+a"(v[13]), "+a"(v[14]), "+a"(v[15]), "=&v"(t)
                  : "v"(keep), "s"(some)
                  : "scc");
-    x = {a, b, c, d};
-    y = {e, f, g, h};
+    for (int e = 0; e < 16; ++e) x[e / 4][e % 4] = v[e];
 }
 
 /* 16, 8 and 4 bytes at any alignment of the element */
@@ -397,19 +415,29 @@ __device__ __forceinline__ uint32_t kv_key_turn(uint32_t n)
     return D == 256 ? n : D == 128 ? n >> 1 : n >> 2;
 }
 
+/* the same of a row of fp16 keys */
+template <int D>
+__device__ __forceinline__ uint32_t kv_wide_turn(uint32_t n)
+{
+    return D == 64 ? n >> 1 : n;
+}
+
 /* One workgroup of four wavefronts per (range of work, key/value head).
  * COLUMNS false: the wavefronts take steps of the tokens in turn, over the
- * same NT tiles of columns, each with its own step in LDS, and are joined at
- * the end.  COLUMNS true (prompt chunks): every wavefront has NT column tiles
- * of its own over all steps, which all four read from one pair of buffers. */
-template <int D, bool COLUMNS>
-constexpr int kv_ring_bytes() { return (COLUMNS ? 2 : 4) * 128 * D; }
+ * same NT tiles of columns, each with its own step's codes in LDS, and are
+ * joined at the end.  COLUMNS true (prompt chunks): every wavefront has NT
+ * column tiles of its own over all steps.  The products are the bound there, so
+ * a step is decoded once for all four: through registers, a step ahead, into one
+ * of two tiles of fp16, 2 D bytes a key and 128 a channel.  Its 16-byte pieces
+ * of eight are turned by the row like those of the codes. */
+template <int D>
+constexpr int kv_ring_bytes() { return 512 * D; }
 constexpr int kKVMetaBytes = 4 * 2 * 256;
-template <int D, bool COLUMNS>
+template <int D>
 constexpr int kv_lds_bytes()
 {
     constexpr int merge = 4 * 16 * (D + 4) * 4;
-    return (kv_ring_bytes<D, COLUMNS>() > merge ? kv_ring_bytes<D, COLUMNS>() : merge) + kKVMetaBytes;
+    return (kv_ring_bytes<D>() > merge ? kv_ring_bytes<D>() : merge) + kKVMetaBytes;
 }
 
 template <bool E4M3, int D, int NT, bool SPLIT, bool COLUMNS>
@@ -423,7 +451,7 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
     constexpr int kRuns = D / 64;                                  /* of 16-token groups that a lane copies keys of */
     constexpr uint32_t kColumns = NT * kTile * (COLUMNS ? 4 : 1);
     constexpr int kTileBytes = 16 * D * 2;                          /* a tile's queries in fp16, as the products take them */
-    __shared__ __attribute__((aligned(16))) uint8_t ring[kv_lds_bytes<D, COLUMNS>()];
+    __shared__ __attribute__((aligned(16))) uint8_t ring[kv_lds_bytes<D>()];
     __shared__ __attribute__((aligned(16))) uint8_t queries[COLUMNS ? 16 : NT * kTileBytes];
     __shared__ float merge_m[4 * NT * kTile], merge_l[4 * NT * kTile], to_exponent[kColumns];
 
@@ -431,12 +459,11 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     const uint32_t T = a.cache.page_tokens, low_half = n >= 8 ? 0xffffffffu : 0u;
     uint8_t *mine = ring + (COLUMNS ? 0 : wave * 128 * D);        /* the (first) keys; values 64 D behind */
-    float *meta = reinterpret_cast<float *>(ring + kv_lds_bytes<D, COLUMNS>() - kKVMetaBytes) + wave * 128;
+    float *meta = reinterpret_cast<float *>(ring + kv_lds_bytes<D>() - kKVMetaBytes) + wave * 128;
 
-    /* LDS places of the lane's reads */
-    uint32_t key_at[COLUMNS ? kChunks : 1];
-#pragma unroll
-    for (int j = 0; COLUMNS && j < kChunks; ++j) key_at[j] = n * D + (((uint32_t)(4 * j + g) ^ kv_key_turn<D>(n)) & (D / 16 - 1)) * 16;
+    /* LDS places of the lane's reads; COLUMNS: of eight channels, of eight tokens */
+    const uint32_t wide_key_at = n * 2 * D + ((2 * g) ^ kv_wide_turn<D>(n)) * 16;
+    const uint32_t wide_value_at = 128 * D + n * 128 + ((2 * g) ^ (n >> 1)) * 16;
     const uint32_t value_at = 64 * D + n * 64 + (g ^ (n >> 2)) * 16;
     /* what the lane copies.  Keys: copy d = kRuns i + run is rows 16 i + (64 /
      * D..) of the tile: within a run every i is four tokens further on */
@@ -504,6 +531,52 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
             for (int c = 0; c < count; ++c) kv_copy16(from + c * 16 * T, to + (first + c) * 1024);
         };
 
+        /* COLUMNS: the thread's part of a step, 16 codes at a time: to registers, and from there decoded to LDS */
+        constexpr int kPieces = D / 64;
+        using kv_codes16 = uint32_t __attribute__((ext_vector_type(4)));
+        kv_codes16 raw_codes[COLUMNS ? 2 * kPieces : 1];
+        int32_t value_good = 16;
+        const uint32_t stage_piece = threadIdx.x % (D / 16);
+        auto stage_token = [&](int k) { return threadIdx.x / (D / 16) + k * (4096 / D); };
+        auto load_codes = [&](uint32_t at) {
+#pragma unroll
+            for (int k = 0; k < kPieces; ++k) {
+                const uint32_t token = stage_token(k);
+                const int32_t page = max(__shfl(pages, (int)(4 * turn + (token >> 4))), 0);
+                raw_codes[COLUMNS ? k : 0] = *reinterpret_cast<const kv_codes16 *>(
+                    a.cache.data + kv_block(a.cache, page, 0, head) * (T * D) + ((at * kKVStep + token) & (T - 1)) * D + stage_piece * 16);
+            }
+            const uint32_t token = at * kKVStep + 16 * (threadIdx.x & 3);
+            const int32_t page = __shfl(pages, (int)(4 * turn + (threadIdx.x & 3)));
+            value_good = page < 0 ? 0 : min(16, max(0, s.seen - (int32_t)token));
+            const uint8_t *from = a.cache.data + kv_block(a.cache, max(page, 0), 1, head) * (T * D) + (threadIdx.x >> 2) * T + (token & (T - 1));
+#pragma unroll
+            for (int k = 0; k < kPieces; ++k) raw_codes[COLUMNS ? kPieces + k : 0] = *reinterpret_cast<const kv_codes16 *>(from + k * 64 * T);
+        };
+        auto write_codes = [&](int k, uint8_t *to) {
+            kv_codes16 v = raw_codes[COLUMNS ? k : 0];
+            if (k < kPieces) {
+                const uint32_t token = stage_token(k), row = (token >> 4) * 4 + (token & 3);     /* n of the key row */
+                to += ((token >> 2 & 3) * 16 + row) * 2 * D;
+                const uint32_t turned = kv_wide_turn<D>(row);
+                *reinterpret_cast<kv_half8 *>(to + ((2 * stage_piece) ^ turned) * 16) = kv_decode8<E4M3>(v.x, v.y);
+                *reinterpret_cast<kv_half8 *>(to + ((2 * stage_piece + 1) ^ turned) * 16) = kv_decode8<E4M3>(v.z, v.w);
+            } else {
+                if (E4M3 && __any(value_good < 16)) {
+                    /* codes of tokens that no column of the slot sees may be any bytes, NaN among them */
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const int left = value_good - 4 * b;
+                        v[b] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+                    }
+                }
+                const uint32_t channel = (threadIdx.x >> 2) + (k - kPieces) * 64, u = 2 * (threadIdx.x & 3), turned = (channel & 15) >> 1;
+                to += 128 * D + channel * 128;
+                *reinterpret_cast<kv_half8 *>(to + (u ^ turned) * 16) = kv_decode8<E4M3>(v.x, v.y);
+                *reinterpret_cast<kv_half8 *>(to + ((u + 1) ^ turned) * 16) = kv_decode8<E4M3>(v.z, v.w);
+            }
+        };
+
         /* Queries to fp16, scaled to a power of two by the largest of their row: a thread
          * takes eight channels, a row's threads are neighbours.  Lane (n, g) of the i-th
          * of a tile's 1 KiB has what it multiplies in the i-th product. */
@@ -552,16 +625,12 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
         };
 
         kv_half8 q[COLUMNS ? NT : 1][2 * kChunks];
-        uint8_t *const other = ring + 128 * D;                     /* COLUMNS: free until the first step */
         if (COLUMNS) {
             load_pages(step);
-            if (step < end) {
-                copy_keys(step, kv_lds(mine), wave, 1);
-                copy_values(step, kv_lds(mine) + 64 * D, wave * (kCopies / 4), kCopies / 4);
-            }
+            if (step < end) load_codes(step);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                uint8_t *to = other + wave * kTileBytes;
+                uint8_t *to = ring + 256 * D + wave * kTileBytes;   /* the second tile */
                 load_queries(first_column + t * kTile);
                 convert_queries(first_column + t * kTile, to);
                 kv_reads_done();
@@ -569,6 +638,10 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                 for (int c = 0; c < 2 * kChunks; ++c) q[COLUMNS ? t : 0][c] = reinterpret_cast<const kv_half8 *>(to)[c * 64 + lane];
                 kv_reads_done();
             }
+            if (step < end)
+#pragma unroll
+                for (int k = 0; k < 2 * kPieces; ++k) write_codes(k, ring);
+            kv_barrier();
         } else {
             load_queries(0);
             /* here, so that nothing the compiler waits for is behind the copies */
@@ -598,12 +671,16 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
             for (int c = 0; c < kChannels; ++c) o[t][c] = {0.0f, 0.0f, 0.0f, 0.0f};
         }
 
+        auto accumulate = [](kv_float4 &sums, kv_half8 x, kv_half8 y) {
+            if constexpr (kAccumulators) kv_accumulate(sums, x, y);
+            else sums = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, sums, 0, 0, 0);
+        };
+
         /* one step's columns: keys and values of `tile` */
         uint32_t tile = 0;
         while (step < end) {
             const bool more = step + kStride < end;
-            kv_wait<COLUMNS ? 0 : kCopies>();                     /* the keys are there */
-            if (COLUMNS) kv_barrier();
+            if (!COLUMNS) kv_wait<kCopies>();                     /* the keys are there */
             const int32_t page = __shfl(pages, (int)(4 * turn + g));
             float key_scale = meta[4 * turn + g], value_scale = meta[64 + 4 * turn + g];
             if (page < 0) key_scale = value_scale = 1.0f;
@@ -612,10 +689,9 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                 kv_reads_done();
                 ++turn;
                 if (refresh) load_pages(step + kStride);
-                const uint32_t to = kv_lds(mine) + (tile ^ (128 * D));
-                copy_keys(step + kStride, to, wave, 1);
-                copy_values(step + kStride, to + 64 * D, wave * (kCopies / 4), kCopies / 4);
+                load_codes(step + kStride);
             }
+            uint8_t *const next_tile = ring + (tile ^ (256 * D));
             const uint8_t *codes = mine + tile;
             if (!COLUMNS || step < own_end) {
                 kv_float4 score[NT][4];
@@ -624,26 +700,25 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
 #pragma unroll
                     for (int t = 0; t < NT; ++t) score[t][i] = {0.0f, 0.0f, 0.0f, 0.0f};
                 if constexpr (COLUMNS) {
-                    /* pieces in the order (j, i), read two ahead; the fences keep the
-                     * compiler from reading all of them first, for which there are no registers */
-                    uint4 raw_codes[3];
+                    /* 1 KiB fragments in the order (c, i), read ahead; the fences keep the compiler
+                     * from reading all of them first, for which there are no registers */
+                    constexpr int kAhead = 4, kFragments = 8 * kChunks;
+                    kv_half8 fragment[kAhead + 1];
+                    auto read = [&](int f) {
+                        const int i = f % 4, c = f / 4;
+                        return *reinterpret_cast<const kv_half8 *>(codes + (wide_key_at ^ (uint32_t)((8 * (c / 2) + (c & 1)) * 16)) +
+                                                                   i * 32 * D);
+                    };
 #pragma unroll
-                    for (int p = 0; p < 2; ++p)
-                        raw_codes[p] = *reinterpret_cast<const uint4 *>(codes + key_at[p / 4] + p % 4 * 16 * D);
+                    for (int f = 0; f < kAhead; ++f) fragment[f] = read(f);
 #pragma unroll
-                    for (int p = 0; p < 4 * kChunks; ++p) {
-                        const int i = p % 4, j = p / 4, ahead = p + 2;
+                    for (int f = 0; f < kFragments; ++f) {
                         __builtin_amdgcn_sched_barrier(0);
-                        if (ahead < 4 * kChunks)
-                            raw_codes[ahead % 3] = *reinterpret_cast<const uint4 *>(codes + key_at[ahead / 4] + ahead % 4 * 16 * D);
-                        const uint4 k = raw_codes[p % 3];
-                        const kv_half8 low = kv_decode8<E4M3>(k.x, k.y), high = kv_decode8<E4M3>(k.z, k.w);
+                        if (f + kAhead < kFragments) fragment[(f + kAhead) % (kAhead + 1)] = read(f + kAhead);
 #pragma unroll
                         for (int t = 0; t < NT; ++t)
-                            score[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(low, q[t][2 * j], score[t][i], 0, 0, 0);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t)
-                            score[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(high, q[t][2 * j + 1], score[t][i], 0, 0, 0);
+                            score[t][f % 4] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fragment[f % (kAhead + 1)], q[t][f / 4],
+                                                                                     score[t][f % 4], 0, 0, 0);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 } else {
@@ -728,7 +803,8 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                         for (int e = 0; e < 16; ++e) u[e] += offset;
                     }
 #pragma unroll
-                    for (int c = 0; kAccumulators && c < kChannels; c += 2) kv_scale(o[t][c], o[t][c + 1], keep, scaled);
+                    for (int c = 0; kAccumulators && c < kChannels; c += 4)
+                        kv_scale(*reinterpret_cast<kv_float4(*)[4]>(&o[t][c]), keep, scaled);
                     float sum = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
@@ -756,9 +832,9 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                     if (more) kv_wait<kCopies>();                 /* the values are there; the next keys may not be */
                     else kv_wait<0>();
                 }
-                if (E4M3 && !whole) {
+                if (E4M3 && !COLUMNS && !whole) {
                     /* codes of tokens that no column of the slot sees may be any bytes, NaN among
-                     * them: made zero (the wavefronts that share the tile write the same) */
+                     * them: made zero */
                     const int32_t good = page < 0 ? 0 : min(16, max(0, s.seen - (int32_t)token));
                     if (__any(good < 16))
 #pragma unroll 1
@@ -774,7 +850,26 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                             *at = make_uint4(word[0], word[1], word[2], word[3]);
                         }
                 }
-                {
+                if constexpr (COLUMNS) {
+                    constexpr int kAhead = 4, kFragments = 2 * kChannels;
+                    kv_half8 fragment[kAhead + 1];
+                    auto read = [&](int f) {
+                        return *reinterpret_cast<const kv_half8 *>(codes + (wide_value_at ^ (uint32_t)(f % 2 * 16)) + f / 2 * 2048);
+                    };
+#pragma unroll
+                    for (int f = 0; f < kAhead; ++f) fragment[f] = read(f);
+#pragma unroll
+                    for (int f = 0; f < kFragments; ++f) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (f + kAhead < kFragments) fragment[(f + kAhead) % (kAhead + 1)] = read(f + kAhead);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+                            accumulate(o[t][f / 2], fragment[f % (kAhead + 1)], weight[t][f % 2]);
+                        /* the next step's codes, in the products' shadow */
+                        if (f % 4 == 3 && more) write_codes(f / 4, next_tile);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                } else {
                     /* the next step's channels follow those that were read */
                     const uint8_t *from = !COLUMNS && more ? value_from(step + kStride) : nullptr;
                     uint4 raw_codes[3];
@@ -789,10 +884,10 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                         const kv_half8 low = kv_decode8<E4M3>(v.x, v.y), high = kv_decode8<E4M3>(v.z, v.w);
 #pragma unroll
                         for (int t = 0; t < NT; ++t)
-                            o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(low, weight[t][0], o[t][c], 0, 0, 0);
+                            accumulate(o[t][c], low, weight[t][0]);
 #pragma unroll
                         for (int t = 0; t < NT; ++t)
-                            o[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(high, weight[t][1], o[t][c], 0, 0, 0);
+                            accumulate(o[t][c], high, weight[t][1]);
                         if (!COLUMNS && more && c % 4 == 3) {
                             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -802,11 +897,24 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            if (COLUMNS) tile ^= 128 * D;
+            if (COLUMNS) {
+                if (more && step >= own_end)
+#pragma unroll
+                    for (int k = 0; k < 2 * kPieces; ++k) write_codes(k, next_tile);
+                kv_barrier();
+                tile ^= 256 * D;
+            }
             step += kStride;
         }
 
         kv_wait<0>();                               /* nothing is on its way to LDS */
+        if (kAccumulators) {
+            asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int c = 0; c < kChannels; ++c) asm volatile("" : "+a"(o[t][c]));    /* read after the products, not before */
+        }
 
         const uint64_t index = (uint64_t)blockIdx.x + s.index;
         float *partial = kv_partial(a, index, head), *stats = kv_stats(a, index, head);

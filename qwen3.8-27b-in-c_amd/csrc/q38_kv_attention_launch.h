@@ -13,7 +13,7 @@ bool launch_kv_attention_typed(const KVAttention &a, hipStream_t stream)
     const dim3 grid(a.workgroups, a.cache.kv_heads), block(256);
     const KVShape shape = kv_shape(a);
     if (shape.columns)
-        return launch_kernel(shape.tiles == 1 ? kv_attention_kernel<E4M3, D, 1, SPLIT, true> : kv_attention_kernel<E4M3, D, 2, SPLIT, true>,
+        return launch_kernel(shape.tiles == 1 ? kv_attention_kernel<E4M3, D, 1, SPLIT, true> : kv_attention_kernel<E4M3, D, kv_most_tiles(D), SPLIT, true>,
                              grid, block, stream, a);
     if constexpr (kv_token_tiles(D) == 3)
         if (shape.tiles == 3) return launch_kernel(kv_attention_kernel<E4M3, D, 3, SPLIT, false>, grid, block, stream, a);

@@ -64,11 +64,13 @@ Q38_HD uint32_t kv_pieces(uint32_t units, uint32_t chunk, uint32_t behind, uint3
  * workgroup whose wavefronts share the tokens, else one or two in each
  * wavefront. */
 constexpr int kv_token_tiles(int head_dim) { return head_dim == 256 ? 3 : 2; }
+/* tiles of a wavefront of its own columns, where there are many */
+#ifndef KVT
+#define KVT 2
+#endif
+constexpr int kv_most_tiles(int head_dim) { return KVT; }
 /* wavefronts that share a SIMD's registers: one has 512, of two each 256 */
-constexpr int kv_waves(int head_dim, int tiles, bool columns)
-{
-    return head_dim == 256 && (!columns || tiles == 2) ? 1 : 2;
-}
+constexpr int kv_waves(int head_dim, int tiles, bool columns) { return head_dim == 256 ? 1 : 2; }
 
 struct KVShape {
     int tiles;
@@ -81,7 +83,7 @@ inline KVShape kv_shape(const KVAttention &a)
     const uint64_t columns = ((uint64_t)a.rows.total_rows * a.group + a.rows.count - 1) / a.rows.count;
     const uint64_t shared = (columns + tile - 1) / tile;
     if (shared <= (uint64_t)kv_token_tiles(a.cache.head_dim)) return {(int)shared, false};
-    return {columns <= 16 * tile ? 1 : 2, true};
+    return {columns <= 16 * tile ? 1 : kv_most_tiles(a.cache.head_dim), true};
 }
 
 }  // namespace q38
