@@ -55,6 +55,20 @@ __device__ __forceinline__ float kv_other_rows(float v, bool maximum)
     auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return maximum ? fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1])) : __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
+/* largest of 8, 16 or 32 neighbouring lanes: within quads, eights and rows of 16 by row operations */
+template <int LANES>
+__device__ __forceinline__ uint32_t kv_largest(uint32_t v)
+{
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));      /* lane ^ 1 */
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));      /* lane ^ 2 */
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, false));     /* 7 - lane of eight */
+    if (LANES >= 16) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, false));    /* 15 - lane */
+    if (LANES == 32) {
+        auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = max(r[0], r[1]);
+    }
+    return v;
+}
 /* l 2^d, d <= 0: a total counts pages without their value scales, so it can be
  * as large as 2^d is small, and 2^d alone may leave fp32 */
 __device__ __forceinline__ float kv_lower(float l, float d)
@@ -157,10 +171,12 @@ struct __attribute__((packed, aligned(4))) KVFloats4 {
     float v[4];
 };
 
-__device__ __forceinline__ float kv_half(uint32_t bits, int type)
+/* fp16 where `f16` is -1, bf16 where it is 0: no branch for each element */
+__device__ __forceinline__ float kv_half(uint32_t bits, uint32_t f16)
 {
-    return type == kElementF16 ? f16_to_f32(bits) : __uint_as_float(bits << 16);
+    return __uint_as_float((__float_as_uint(f16_to_f32(bits)) & f16) | (bits << 16 & ~f16));
 }
+__device__ __forceinline__ uint32_t kv_f16(const KVAttention &a) { return a.type == kElementF16 ? 0xffffffffu : 0u; }
 
 /* elements at .. at + 7 as stored: fp32 eight words, 16-bit types four */
 template <bool F32>
@@ -176,33 +192,34 @@ __device__ __forceinline__ void kv_load8(uint32_t *raw, const void *base, uint64
     }
 }
 template <bool F32>
-__device__ __forceinline__ float kv_element8(const uint32_t *raw, int e, int type)
+__device__ __forceinline__ float kv_element8(const uint32_t *raw, int e, uint32_t f16)
 {
     if constexpr (F32) return __uint_as_float(raw[e]);
-    else return kv_half(e & 1 ? raw[e / 2] >> 16 : raw[e / 2] & 0xffffu, type);
+    else return kv_half(e & 1 ? raw[e / 2] >> 16 : raw[e / 2] & 0xffffu, f16);
 }
 
 /* elements at .. at + 3 */
-__device__ __forceinline__ kv_float4 kv_load4(const void *base, uint64_t at, int type)
+__device__ __forceinline__ kv_float4 kv_load4(const void *base, uint64_t at, const KVAttention &a)
 {
-    if (type == kElementF32) {
+    if (a.type == kElementF32) {
         const KVFloats4 v = *reinterpret_cast<const KVFloats4 *>(static_cast<const float *>(base) + at);
         return {v.v[0], v.v[1], v.v[2], v.v[3]};
     }
     const KVBytes8 v = *reinterpret_cast<const KVBytes8 *>(static_cast<const uint16_t *>(base) + at);
-    return {kv_half(v.word[0] & 0xffffu, type), kv_half(v.word[0] >> 16, type), kv_half(v.word[1] & 0xffffu, type),
-            kv_half(v.word[1] >> 16, type)};
+    const uint32_t f16 = kv_f16(a);
+    return {kv_half(v.word[0] & 0xffffu, f16), kv_half(v.word[0] >> 16, f16), kv_half(v.word[1] & 0xffffu, f16),
+            kv_half(v.word[1] >> 16, f16)};
 }
 /* four consecutive outputs, rounded once */
-__device__ __forceinline__ void kv_store4(void *base, uint64_t at, int type, const kv_float4 v)
+__device__ __forceinline__ void kv_store4(void *base, uint64_t at, const KVAttention &a, const kv_float4 v)
 {
-    if (type == kElementF32) {
+    if (a.type == kElementF32) {
         *reinterpret_cast<KVFloats4 *>(static_cast<float *>(base) + at) = {{v[0], v[1], v[2], v[3]}};
     } else {
+        const uint32_t f16 = kv_f16(a);
         uint32_t bits[4];
         for (int e = 0; e < 4; ++e)
-            bits[e] = type == kElementF16 ? __builtin_bit_cast(uint16_t, (_Float16)v[e])
-                                          : __builtin_bit_cast(uint16_t, (__bf16)v[e]);
+            bits[e] = (__builtin_bit_cast(uint16_t, (_Float16)v[e]) & f16) | (__builtin_bit_cast(uint16_t, (__bf16)v[e]) & ~f16);
         *reinterpret_cast<KVBytes8 *>(static_cast<uint16_t *>(base) + at) = {{bits[0] | bits[1] << 16, bits[2] | bits[3] << 16}};
     }
 }
@@ -226,10 +243,10 @@ __device__ __forceinline__ void kv_finish4(const KVAttention &a, uint32_t row, u
 {
     o *= l == 0.0f ? 0.0f : 1.0f / l;
     if (a.gate) {
-        const kv_float4 gate = kv_load4(a.gate, row * a.query_row + head * a.query_head + d, a.type);
+        const kv_float4 gate = kv_load4(a.gate, row * a.query_row + head * a.query_head + d, a);
         for (int e = 0; e < 4; ++e) o[e] *= kv_sigmoid(gate[e]);
     }
-    kv_store4(a.output, row * a.output_row + (uint64_t)head * a.cache.head_dim + d, a.type, o);
+    kv_store4(a.output, row * a.output_row + (uint64_t)head * a.cache.head_dim + d, a, o);
 }
 
 /* ---- work ---------------------------------------------------------------------- */
@@ -457,7 +474,7 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
 
     const uint32_t head = blockIdx.y;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-    const uint32_t T = a.cache.page_tokens, low_half = n >= 8 ? 0xffffffffu : 0u;
+    const uint32_t T = a.cache.page_tokens, low_half = n >= 8 ? 0xffffffffu : 0u, f16 = kv_f16(a);
     uint8_t *mine = ring + (COLUMNS ? 0 : wave * 128 * D);        /* the (first) keys; values 64 D behind */
     float *meta = reinterpret_cast<float *>(ring + kv_lds_bytes<D>() - kKVMetaBytes) + wave * 128;
 
@@ -538,16 +555,23 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
         int32_t value_good = 16;
         const uint32_t stage_piece = threadIdx.x % (D / 16);
         auto stage_token = [&](int k) { return threadIdx.x / (D / 16) + k * (4096 / D); };
+        int32_t stage_page[COLUMNS ? kPieces + 1 : 1];
+        /* the pages first, some time before their codes: they come from other lanes */
+        auto find_codes = [&] {
+#pragma unroll
+            for (int k = 0; k < kPieces; ++k) stage_page[COLUMNS ? k : 0] = __shfl(pages, (int)(4 * turn + (stage_token(k) >> 4)));
+            stage_page[COLUMNS ? kPieces : 0] = __shfl(pages, (int)(4 * turn + (threadIdx.x & 3)));
+        };
         auto load_codes = [&](uint32_t at) {
 #pragma unroll
             for (int k = 0; k < kPieces; ++k) {
                 const uint32_t token = stage_token(k);
-                const int32_t page = max(__shfl(pages, (int)(4 * turn + (token >> 4))), 0);
+                const int32_t page = max(stage_page[COLUMNS ? k : 0], 0);
                 raw_codes[COLUMNS ? k : 0] = *reinterpret_cast<const kv_codes16 *>(
                     a.cache.data + kv_block(a.cache, page, 0, head) * (T * D) + ((at * kKVStep + token) & (T - 1)) * D + stage_piece * 16);
             }
             const uint32_t token = at * kKVStep + 16 * (threadIdx.x & 3);
-            const int32_t page = __shfl(pages, (int)(4 * turn + (threadIdx.x & 3)));
+            const int32_t page = stage_page[COLUMNS ? kPieces : 0];
             value_good = page < 0 ? 0 : min(16, max(0, s.seen - (int32_t)token));
             const uint8_t *from = a.cache.data + kv_block(a.cache, max(page, 0), 1, head) * (T * D) + (threadIdx.x >> 2) * T + (token & (T - 1));
 #pragma unroll
@@ -600,9 +624,9 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                 uint32_t largest = 0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    largest = max(largest, __float_as_uint(kv_element8<SPLIT>(raw[k], e, a.type)) & 0x7fffffffu);
+                    largest = max(largest, __float_as_uint(kv_element8<SPLIT>(raw[k], e, f16)) & 0x7fffffffu);
                 /* non-negative floats order as their bits; NaN is above all of them */
-                for (int by = 1; by < kEights; by *= 2) largest = max(largest, (uint32_t)__shfl_xor((int)largest, by));
+                largest = kv_largest<kEights>(largest);
                 const uint32_t exponent = max(largest >> 23, 30u);
                 /* largest * scale is in 2^13..2^14; columns that are not there are zero */
                 const float scale = c < s.columns ? __uint_as_float((267u - exponent) << 23) : 0.0f;
@@ -611,8 +635,8 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                 kv_half8 high, low;
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
-                    const float v = c < s.columns ? kv_element8<SPLIT>(raw[k], e, a.type) * scale : 0.0f;
-                    const float w = c < s.columns ? kv_element8<SPLIT>(raw[k], e + 1, a.type) * scale : 0.0f;
+                    const float v = c < s.columns ? kv_element8<SPLIT>(raw[k], e, f16) * scale : 0.0f;
+                    const float w = c < s.columns ? kv_element8<SPLIT>(raw[k], e + 1, f16) * scale : 0.0f;
                     const kv_half2 a2 = kv_round2<false>(v, w, 0), b2 = kv_round2<SPLIT>(v, w, 0xffffffffu);
                     high[e] = a2[0], high[e + 1] = a2[1];
                     low[e] = b2[0], low[e + 1] = b2[1];
@@ -627,7 +651,10 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
         kv_half8 q[COLUMNS ? NT : 1][2 * kChunks];
         if (COLUMNS) {
             load_pages(step);
-            if (step < end) load_codes(step);
+            if (step < end) {
+                find_codes();
+                load_codes(step);
+            }
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 uint8_t *to = ring + 256 * D + wave * kTileBytes;   /* the second tile */
@@ -683,13 +710,16 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
             if (!COLUMNS) kv_wait<kCopies>();                     /* the keys are there */
             const int32_t page = __shfl(pages, (int)(4 * turn + g));
             float key_scale = meta[4 * turn + g], value_scale = meta[64 + 4 * turn + g];
-            if (page < 0) key_scale = value_scale = 1.0f;
             const bool refresh = turn == 15;
             if (COLUMNS && more) {
-                kv_reads_done();
-                ++turn;
-                if (refresh) load_pages(step + kStride);
-                load_codes(step + kStride);
+                if (refresh) {
+                    kv_reads_done();
+                    load_pages(step + kStride);
+                } else {
+                    ++turn;
+                }
+                find_codes();
+                if (step >= own_end) load_codes(step + kStride);
             }
             uint8_t *const next_tile = ring + (tile ^ (256 * D));
             const uint8_t *codes = mine + tile;
@@ -719,6 +749,7 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                         for (int t = 0; t < NT; ++t)
                             score[t][f % 4] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fragment[f % (kAhead + 1)], q[t][f / 4],
                                                                                      score[t][f % 4], 0, 0, 0);
+                        if (f == kFragments / 4 && more) load_codes(step + kStride);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 } else {
@@ -753,6 +784,7 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                     copy_keys(step + kStride, kv_lds(mine), 0, 4);
                 }
 
+                if (page < 0) key_scale = value_scale = 1.0f;
                 const uint32_t token = step * kKVStep + 16 * g;
                 const uint32_t scale_bits = __float_as_uint(value_scale);
                 const float value_log = value_scale == value_scale ? (float)((int)(scale_bits >> 23) - 127) : value_scale;
@@ -853,8 +885,12 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                 if constexpr (COLUMNS) {
                     constexpr int kAhead = 4, kFragments = 2 * kChannels;
                     kv_half8 fragment[kAhead + 1];
+                    /* four channel tiles' first halves, then their second ones: a product waits for the
+                     * one before it on the same sums */
+                    auto tile_of = [](int f) { return f / 8 * 4 + f % 4; };
                     auto read = [&](int f) {
-                        return *reinterpret_cast<const kv_half8 *>(codes + (wide_value_at ^ (uint32_t)(f % 2 * 16)) + f / 2 * 2048);
+                        return *reinterpret_cast<const kv_half8 *>(codes + (wide_value_at ^ (uint32_t)(f / 4 % 2 * 16)) +
+                                                                   tile_of(f) * 2048);
                     };
 #pragma unroll
                     for (int f = 0; f < kAhead; ++f) fragment[f] = read(f);
@@ -864,7 +900,7 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                         if (f + kAhead < kFragments) fragment[(f + kAhead) % (kAhead + 1)] = read(f + kAhead);
 #pragma unroll
                         for (int t = 0; t < NT; ++t)
-                            accumulate(o[t][f / 2], fragment[f % (kAhead + 1)], weight[t][f % 2]);
+                            accumulate(o[t][tile_of(f)], fragment[f % (kAhead + 1)], weight[t][f / 4 % 2]);
                         /* the next step's codes, in the products' shadow */
                         if (f % 4 == 3 && more) write_codes(f / 4, next_tile);
                     }
@@ -872,26 +908,34 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                 } else {
                     /* the next step's channels follow those that were read */
                     const uint8_t *from = !COLUMNS && more ? value_from(step + kStride) : nullptr;
-                    uint4 raw_codes[3];
+                    uint4 next[2];
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) raw_codes[c] = *reinterpret_cast<const uint4 *>(codes + value_at + c * 1024);
+                    for (int c = 0; c < 2; ++c) next[c] = *reinterpret_cast<const uint4 *>(codes + value_at + c * 1024);
 #pragma unroll
-                    for (int c = 0; c < kChannels; ++c) {
+                    for (int c = 0; c < kChannels; c += 2) {
                         __builtin_amdgcn_sched_barrier(0);
+                        const uint4 v = next[0], w = next[1];
                         if (c + 2 < kChannels)
-                            raw_codes[(c + 2) % 3] = *reinterpret_cast<const uint4 *>(codes + value_at + (c + 2) * 1024);
-                        const uint4 v = raw_codes[c % 3];
-                        const kv_half8 low = kv_decode8<E4M3>(v.x, v.y), high = kv_decode8<E4M3>(v.z, v.w);
 #pragma unroll
-                        for (int t = 0; t < NT; ++t)
-                            accumulate(o[t][c], low, weight[t][0]);
+                            for (int e = 0; e < 2; ++e)
+                                next[e] = *reinterpret_cast<const uint4 *>(codes + value_at + (c + 2 + e) * 1024);
+                        /* first halves, then second ones: a product waits for the one before it on the same sums */
+                        const kv_half8 v0 = kv_decode8<E4M3>(v.x, v.y), w0 = kv_decode8<E4M3>(w.x, w.y);
 #pragma unroll
-                        for (int t = 0; t < NT; ++t)
-                            accumulate(o[t][c], high, weight[t][1]);
-                        if (!COLUMNS && more && c % 4 == 3) {
+                        for (int t = 0; t < NT; ++t) {
+                            accumulate(o[t][c], v0, weight[t][0]);
+                            accumulate(o[t][c + 1], w0, weight[t][0]);
+                        }
+                        const kv_half8 v1 = kv_decode8<E4M3>(v.z, v.w), w1 = kv_decode8<E4M3>(w.z, w.w);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            accumulate(o[t][c], v1, weight[t][1]);
+                            accumulate(o[t][c + 1], w1, weight[t][1]);
+                        }
+                        if (!COLUMNS && more && c % 4 == 2) {
                             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                            for (int e = c - 3; e <= c; ++e) kv_copy16(from + e * 16 * T, kv_lds(mine) + 64 * D + e * 1024);
+                            for (int e = c - 2; e < c + 2; ++e) kv_copy16(from + e * 16 * T, kv_lds(mine) + 64 * D + e * 1024);
                         }
                     }
                     __builtin_amdgcn_sched_barrier(0);
