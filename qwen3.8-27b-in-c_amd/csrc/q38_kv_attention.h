@@ -129,35 +129,21 @@ __device__ __forceinline__ void kv_accumulate(kv_float4 &sums, kv_half8 a, kv_ha
     asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(sums) : "v"(a), "v"(b));
 }
 
-/* sums times keep where `some` (uniform).  The branch is within the assembly, so
- * that the sums are one value on both ways and stay in their accumulation
- * registers; 18 wait states cover a matrix product that may still write them. */
-__device__ __forceinline__ void kv_scale(kv_float4 (&x)[4], float keep, uint64_t some)
+/* Sums in accumulation registers times keep, by way of 16 bytes of LDS per
+ * lane: vector instructions take no accumulation registers, and four of them
+ * have no names of their own here.  Seldom done.  The 20 wait states cover a
+ * product that may still write the sums. */
+__device__ __forceinline__ void kv_scale(kv_float4 &sums, float keep, uint32_t lane_lds)
 {
-    float v[16], t;
-    for (int e = 0; e < 16; ++e) v[e] = x[e / 4][e % 4];
-    asm volatile("s_cmp_eq_u64 %18, 0\n\ts_cbranch_scc1 1f\n\ts_nop 15\n\ts_nop 3\n\t"
-                 "v_accvgpr_read_b32 %16, %0\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %0, %16\n\t"
-                 "v_accvgpr_read_b32 %16, %1\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %1, %16\n\t"
-                 "v_accvgpr_read_b32 %16, %2\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %2, %16\n\t"
-                 "v_accvgpr_read_b32 %16, %3\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %3, %16\n\t"
-                 "v_accvgpr_read_b32 %16, %4\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %4, %16\n\t"
-                 "v_accvgpr_read_b32 %16, %5\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %5, %16\n\t"
-                 "v_accvgpr_read_b32 %16, %6\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %6, %16\n\t"
-                 "v_accvgpr_read_b32 %16, %7\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %7, %16\n\t"
-                 "v_accvgpr_read_b32 %16, %8\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %8, %16\n\t"
-                 "v_accvgpr_read_b32 %16, %9\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %9, %16\n\t"
-                 "v_accvgpr_read_b32 %16, %10\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %10, %16\n\t"
-                 "v_accvgpr_read_b32 %16, %11\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %11, %16\n\t"
-                 "v_accvgpr_read_b32 %16, %12\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %12, %16\n\t"
-                 "v_accvgpr_read_b32 %16, %13\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %13, %16\n\t"
-                 "v_accvgpr_read_b32 %16, %14\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %14, %16\n\t"
-                 "v_accvgpr_read_b32 %16, %15\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %15, %16\n\t"
-                 "s_nop 3\n1:"
-                 : "+a"(v[0]), "+a"(v[1]), "+a"(v[2]), "+a"(v[3]), "+a"(v[4]), "+a"(v[5]), "+a"(v[6]), "+a"(v[7]), "+a"(v[8]), "+a"(v[9]), "+a"(v[10]), "+a"(v[11]), "+a"(v[12]), "+a"(v[13]), "+a"(v[14]), "+a"(v[15]), "=&v"(t)
-                 : "v"(keep), "s"(some)
-                 : "scc");
-    for (int e = 0; e < 16; ++e) x[e / 4][e % 4] = v[e];
+    float a, b, c, d;
+    asm volatile("s_nop 15\n\ts_nop 3\n\tds_write_b128 %6, %0\n\t"
+                 "ds_read_b32 %1, %6\n\tds_read_b32 %2, %6 offset:4\n\tds_read_b32 %3, %6 offset:8\n\tds_read_b32 %4, %6 offset:12\n\t"
+                 "s_waitcnt lgkmcnt(0)\n\tv_mul_f32 %1, %1, %5\n\tv_mul_f32 %2, %2, %5\n\tv_mul_f32 %3, %3, %5\n\tv_mul_f32 %4, %4, %5\n\t"
+                 "ds_write_b32 %6, %1\n\tds_write_b32 %6, %2 offset:4\n\tds_write_b32 %6, %3 offset:8\n\tds_write_b32 %6, %4 offset:12\n\t"
+                 "ds_read_b128 %0, %6\n\ts_waitcnt lgkmcnt(0)"
+                 : "+a"(sums), "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d)
+                 : "v"(keep), "v"(lane_lds)
+                 : "memory");
 }
 
 /* 16, 8 and 4 bytes at any alignment of the element */
@@ -449,34 +435,36 @@ __device__ __forceinline__ uint32_t kv_wide_turn(uint32_t n)
  * of eight are turned by the row like those of the codes. */
 template <int D>
 constexpr int kv_ring_bytes() { return 512 * D; }
-constexpr int kKVMetaBytes = 4 * 2 * 256;
-template <int D>
+template <int D, int WAVES>
 constexpr int kv_lds_bytes()
 {
-    constexpr int merge = 4 * 16 * (D + 4) * 4;
-    return (kv_ring_bytes<D>() > merge ? kv_ring_bytes<D>() : merge) + kKVMetaBytes;
+    constexpr int merge = WAVES * 16 * (D + 4) * 4;
+    return kv_ring_bytes<D>() > merge ? kv_ring_bytes<D>() : merge;
 }
 
 template <bool E4M3, int D, int NT, bool SPLIT, bool COLUMNS>
-__global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_kernel(KVAttention a)
+__global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, NT, COLUMNS)) void kv_attention_kernel(KVAttention a)
 {
-    constexpr int kTile = SPLIT ? 8 : 16;
+    constexpr int kTile = SPLIT ? 8 : 16, kWaves = kv_workgroup_waves(D, COLUMNS);
     constexpr bool kAccumulators = kv_waves(D, NT, COLUMNS) == 1;  /* more registers than VGPRs: sums in AGPRs */
     constexpr int kChunks = D / 64, kChannels = D / 16;
     constexpr int kPitch = D + 4;
     constexpr int kCopies = D / 16;                                /* copies of 1 KiB of a step's keys or values */
     constexpr int kRuns = D / 64;                                  /* of 16-token groups that a lane copies keys of */
-    constexpr uint32_t kColumns = NT * kTile * (COLUMNS ? 4 : 1);
+    constexpr uint32_t kColumns = NT * kTile * (COLUMNS ? kWaves : 1);
     constexpr int kTileBytes = 16 * D * 2;                          /* a tile's queries in fp16, as the products take them */
-    __shared__ __attribute__((aligned(16))) uint8_t ring[kv_lds_bytes<D>()];
+    __shared__ __attribute__((aligned(16))) uint8_t ring[kv_lds_bytes<D, kWaves>()];
+    __shared__ float metas[kWaves * 128];                           /* scales: of 16 steps, keys then values, each wavefront's */
     __shared__ __attribute__((aligned(16))) uint8_t queries[COLUMNS ? 16 : NT * kTileBytes];
-    __shared__ float merge_m[4 * NT * kTile], merge_l[4 * NT * kTile], to_exponent[kColumns];
+    __shared__ kv_float4 bounces[kAccumulators ? 256 : 1];
+    kv_float4 *bounce = bounces + (kAccumulators ? threadIdx.x : 0);
+    __shared__ float merge_m[kWaves * NT * kTile], merge_l[kWaves * NT * kTile], to_exponent[kColumns];
 
     const uint32_t head = blockIdx.y;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     const uint32_t T = a.cache.page_tokens, low_half = n >= 8 ? 0xffffffffu : 0u, f16 = kv_f16(a);
     uint8_t *mine = ring + (COLUMNS ? 0 : wave * 128 * D);        /* the (first) keys; values 64 D behind */
-    float *meta = reinterpret_cast<float *>(ring + kv_lds_bytes<D>() - kKVMetaBytes) + wave * 128;
+    float *meta = metas + wave * 128;
 
     /* LDS places of the lane's reads; COLUMNS: of eight channels, of eight tokens */
     const uint32_t wide_key_at = n * 2 * D + ((2 * g) ^ kv_wide_turn<D>(n)) * 16;
@@ -549,62 +537,66 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
         };
 
         /* COLUMNS: the thread's part of a step, 16 codes at a time: to registers, and from there decoded to LDS */
-        constexpr int kPieces = D / 64;
+        constexpr int kPieces = COLUMNS ? D * 4 / (64 * kWaves) : 1;
         using kv_codes16 = uint32_t __attribute__((ext_vector_type(4)));
         kv_codes16 raw_codes[COLUMNS ? 2 * kPieces : 1];
         int32_t value_good = 16;
-        const uint32_t stage_piece = threadIdx.x % (D / 16);
-        auto stage_token = [&](int k) { return threadIdx.x / (D / 16) + k * (4096 / D); };
-        int32_t stage_page[COLUMNS ? kPieces + 1 : 1];
-        /* the pages first, some time before their codes: they come from other lanes */
-        auto find_codes = [&] {
-#pragma unroll
-            for (int k = 0; k < kPieces; ++k) stage_page[COLUMNS ? k : 0] = __shfl(pages, (int)(4 * turn + (stage_token(k) >> 4)));
-            stage_page[COLUMNS ? kPieces : 0] = __shfl(pages, (int)(4 * turn + (threadIdx.x & 3)));
-        };
+        bool value_partial = false;
+        /* Pieces of 16 codes of a key that the thread takes, of token stage_token + kStageTokens k:
+         * 16 lanes write two rows or more, whose turns differ, so their two halves use all banks */
+        const uint32_t stage_piece = D == 256 ? (threadIdx.x & 7) + (threadIdx.x >> 1 & 8) : threadIdx.x % (D / 16);
+        const uint32_t stage_token = D == 256 ? (threadIdx.x >> 5) * 2 + (threadIdx.x >> 3 & 1) : threadIdx.x / (D / 16);
+        const uint32_t stage_group = wave * 64 / D;            /* its 16-token group, the wavefront's */
+        constexpr int kStageTokens = 1024 * kWaves / D;
+        int32_t value_page = -1;
+        /* the page of the thread's values comes from another lane: asked for some time before its use */
+        auto find_codes = [&] { value_page = __shfl(pages, (int)(4 * turn + (threadIdx.x & 3))); };
         auto load_codes = [&](uint32_t at) {
 #pragma unroll
             for (int k = 0; k < kPieces; ++k) {
-                const uint32_t token = stage_token(k);
-                const int32_t page = max(stage_page[COLUMNS ? k : 0], 0);
-                raw_codes[COLUMNS ? k : 0] = *reinterpret_cast<const kv_codes16 *>(
-                    a.cache.data + kv_block(a.cache, page, 0, head) * (T * D) + ((at * kKVStep + token) & (T - 1)) * D + stage_piece * 16);
+                const uint32_t group = stage_group + k * kStageTokens / 16;
+                const int32_t page = max(__builtin_amdgcn_readlane(pages, (int)(4 * turn + group)), 0);
+                const uint8_t *keys = a.cache.data + kv_block(a.cache, page, 0, head) * (T * D) + ((at * kKVStep + group * 16) & (T - 1)) * D;
+                raw_codes[COLUMNS ? k : 0] =
+                    *reinterpret_cast<const kv_codes16 *>(keys + (stage_token + k * kStageTokens - group * 16) * D + stage_piece * 16);
             }
             const uint32_t token = at * kKVStep + 16 * (threadIdx.x & 3);
-            const int32_t page = stage_page[COLUMNS ? kPieces : 0];
-            value_good = page < 0 ? 0 : min(16, max(0, s.seen - (int32_t)token));
-            const uint8_t *from = a.cache.data + kv_block(a.cache, max(page, 0), 1, head) * (T * D) + (threadIdx.x >> 2) * T + (token & (T - 1));
+            value_good = value_page < 0 ? 0 : min(16, max(0, s.seen - (int32_t)token));
+            value_partial = E4M3 && __any(value_good < 16);
+            const uint8_t *from =
+                a.cache.data + kv_block(a.cache, max(value_page, 0), 1, head) * (T * D) + (threadIdx.x >> 2) * T + (token & (T - 1));
 #pragma unroll
-            for (int k = 0; k < kPieces; ++k) raw_codes[COLUMNS ? kPieces + k : 0] = *reinterpret_cast<const kv_codes16 *>(from + k * 64 * T);
+            for (int k = 0; k < kPieces; ++k) raw_codes[COLUMNS ? kPieces + k : 0] = *reinterpret_cast<const kv_codes16 *>(from + k * 16 * kWaves * T);
         };
-        auto write_codes = [&](int k, uint8_t *to) {
+        /* half 0 or 1 of the k-th piece, eight codes, to its tile */
+        auto write_codes = [&](int k, int part, uint8_t *to) {
             kv_codes16 v = raw_codes[COLUMNS ? k : 0];
             if (k < kPieces) {
-                const uint32_t token = stage_token(k), row = (token >> 4) * 4 + (token & 3);     /* n of the key row */
-                to += ((token >> 2 & 3) * 16 + row) * 2 * D;
-                const uint32_t turned = kv_wide_turn<D>(row);
-                *reinterpret_cast<kv_half8 *>(to + ((2 * stage_piece) ^ turned) * 16) = kv_decode8<E4M3>(v.x, v.y);
-                *reinterpret_cast<kv_half8 *>(to + ((2 * stage_piece + 1) ^ turned) * 16) = kv_decode8<E4M3>(v.z, v.w);
+                const uint32_t token = stage_token + k * kStageTokens, row = (token >> 4) * 4 + (token & 3);     /* n of the key row */
+                to += ((token >> 2 & 3) * 16 + row) * 2 * D + ((2 * stage_piece + part) ^ kv_wide_turn<D>(row)) * 16;
             } else {
-                if (E4M3 && __any(value_good < 16)) {
+                if (E4M3 && value_partial) {
                     /* codes of tokens that no column of the slot sees may be any bytes, NaN among them */
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) {
+                    for (int b = 2 * part; b < 2 * part + 2; ++b) {
                         const int left = value_good - 4 * b;
                         v[b] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
                     }
                 }
-                const uint32_t channel = (threadIdx.x >> 2) + (k - kPieces) * 64, u = 2 * (threadIdx.x & 3), turned = (channel & 15) >> 1;
-                to += 128 * D + channel * 128;
-                *reinterpret_cast<kv_half8 *>(to + (u ^ turned) * 16) = kv_decode8<E4M3>(v.x, v.y);
-                *reinterpret_cast<kv_half8 *>(to + ((u + 1) ^ turned) * 16) = kv_decode8<E4M3>(v.z, v.w);
+                const uint32_t channel = (threadIdx.x >> 2) + (k - kPieces) * 16 * kWaves;
+                to += 128 * D + channel * 128 + ((2 * (threadIdx.x & 3) + part) ^ ((channel & 15) >> 1)) * 16;
             }
+            *reinterpret_cast<kv_half8 *>(to) = kv_decode8<E4M3>(v[2 * part], v[2 * part + 1]);
+        };
+        auto write_all = [&](uint8_t *to) {
+#pragma unroll
+            for (int k = 0; k < 4 * kPieces; ++k) write_codes(k / 2, k % 2, to);
         };
 
         /* Queries to fp16, scaled to a power of two by the largest of their row: a thread
          * takes eight channels, a row's threads are neighbours.  Lane (n, g) of the i-th
          * of a tile's 1 KiB has what it multiplies in the i-th product. */
-        constexpr int kThreads = COLUMNS ? 64 : 256, kEights = D / 8;
+        constexpr int kThreads = COLUMNS ? 64 : 64 * kWaves, kEights = D / 8;
         constexpr int kRows = COLUMNS ? kTile : NT * kTile, kEach = (kRows * kEights + kThreads - 1) / kThreads;
         uint32_t raw[kEach][SPLIT ? 8 : 4];
         const uint32_t eight = threadIdx.x % kEights, row_at = (COLUMNS ? lane : threadIdx.x) / kEights;
@@ -665,9 +657,7 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                 for (int c = 0; c < 2 * kChunks; ++c) q[COLUMNS ? t : 0][c] = reinterpret_cast<const kv_half8 *>(to)[c * 64 + lane];
                 kv_reads_done();
             }
-            if (step < end)
-#pragma unroll
-                for (int k = 0; k < 2 * kPieces; ++k) write_codes(k, ring);
+            if (step < end) write_all(ring);
             kv_barrier();
         } else {
             load_queries(0);
@@ -732,7 +722,7 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                 if constexpr (COLUMNS) {
                     /* 1 KiB fragments in the order (c, i), read ahead; the fences keep the compiler
                      * from reading all of them first, for which there are no registers */
-                    constexpr int kAhead = 4, kFragments = 8 * kChunks;
+                    constexpr int kAhead = 6, kFragments = 8 * kChunks;
                     kv_half8 fragment[kAhead + 1];
                     auto read = [&](int f) {
                         const int i = f % 4, c = f / 4;
@@ -834,9 +824,9 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
 #pragma unroll
                         for (int e = 0; e < 16; ++e) u[e] += offset;
                     }
+                    if (kAccumulators && scaled)
 #pragma unroll
-                    for (int c = 0; kAccumulators && c < kChannels; c += 4)
-                        kv_scale(*reinterpret_cast<kv_float4(*)[4]>(&o[t][c]), keep, scaled);
+                        for (int c = 0; c < kChannels; ++c) kv_scale(o[t][c], keep, kv_lds(bounce));
                     float sum = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
@@ -883,7 +873,7 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                         }
                 }
                 if constexpr (COLUMNS) {
-                    constexpr int kAhead = 4, kFragments = 2 * kChannels;
+                    constexpr int kAhead = 6, kFragments = 2 * kChannels;
                     kv_half8 fragment[kAhead + 1];
                     /* four channel tiles' first halves, then their second ones: a product waits for the
                      * one before it on the same sums */
@@ -901,8 +891,9 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
 #pragma unroll
                         for (int t = 0; t < NT; ++t)
                             accumulate(o[t][tile_of(f)], fragment[f % (kAhead + 1)], weight[t][f / 4 % 2]);
-                        /* the next step's codes, in the products' shadow */
-                        if (f % 4 == 3 && more) write_codes(f / 4, next_tile);
+                        /* the next step's codes, in the products' shadow (what is there without one goes unread) */
+                        constexpr int kEvery = kFragments / (4 * kPieces);
+                        if (f % kEvery == kEvery - 1) write_codes(f / kEvery / 2, f / kEvery % 2, next_tile);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 } else {
@@ -942,9 +933,7 @@ __global__ __launch_bounds__(256, kv_waves(D, NT, COLUMNS)) void kv_attention_ke
                 }
             }
             if (COLUMNS) {
-                if (more && step >= own_end)
-#pragma unroll
-                    for (int k = 0; k < 2 * kPieces; ++k) write_codes(k, next_tile);
+                if (more && step >= own_end) write_all(next_tile);
                 kv_barrier();
                 tile ^= 256 * D;
             }

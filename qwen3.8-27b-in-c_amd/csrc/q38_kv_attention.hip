@@ -100,7 +100,7 @@ uint64_t plan_kv_attention(KVAttention &a)
 {
     const KVShape shape = kv_shape(a);
     const uint32_t tile = a.type == kElementF32 ? 8 : 16, D = a.cache.head_dim, heads = a.cache.kv_heads;
-    a.columns = tile * shape.tiles * (shape.columns ? 4 : 1);
+    a.columns = tile * shape.tiles * (shape.columns ? kv_workgroup_waves(D, true) : 1);
     a.slots = (uint32_t)kv_slots(a.rows.total_rows, a.rows.count, a.group, a.columns, 1);
     const uint32_t most = kv_steps(a.cache.table_entries * a.cache.page_tokens);
     a.shift = 0;
@@ -108,7 +108,7 @@ uint64_t plan_kv_attention(KVAttention &a)
     a.least = a.shift ? 1 : shape.columns ? 8 : 4;
     /* as many workgroups as run at once: by LDS where wavefronts have their own
      * tokens (64 D bytes of keys and of values each), else by registers */
-    const uint32_t on_a_unit = !shape.columns ? (D == 64 && shape.tiles == 2 ? 2 : 256 / D) : kv_waves(D, shape.tiles, true);
+    const uint32_t on_a_unit = !shape.columns ? (D == 64 && shape.tiles == 2 ? 2 : 256 / D) : D == 64 ? 2 : 1;
     const uint64_t units = (uint64_t)a.slots * kv_slot_units(most, a.shift), wanted = 256 * on_a_unit / heads;
     const uint64_t useful = (units + a.least - 1) / a.least;
     a.workgroups = (uint32_t)(wanted < 1 ? 1 : wanted < useful ? wanted : useful);

@@ -10,8 +10,8 @@ namespace q38 {
 template <bool E4M3, int D, bool SPLIT>
 bool launch_kv_attention_typed(const KVAttention &a, hipStream_t stream)
 {
-    const dim3 grid(a.workgroups, a.cache.kv_heads), block(256);
     const KVShape shape = kv_shape(a);
+    const dim3 grid(a.workgroups, a.cache.kv_heads), block(64 * kv_workgroup_waves(D, shape.columns));
     if (shape.columns)
         return launch_kernel(shape.tiles == 1 ? kv_attention_kernel<E4M3, D, 1, SPLIT, true> : kv_attention_kernel<E4M3, D, kv_most_tiles(D), SPLIT, true>,
                              grid, block, stream, a);

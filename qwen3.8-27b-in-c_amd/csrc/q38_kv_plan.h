@@ -64,13 +64,16 @@ Q38_HD uint32_t kv_pieces(uint32_t units, uint32_t chunk, uint32_t behind, uint3
  * workgroup whose wavefronts share the tokens, else one or two in each
  * wavefront. */
 constexpr int kv_token_tiles(int head_dim) { return head_dim == 256 ? 3 : 2; }
-/* tiles of a wavefront of its own columns, where there are many */
+/* Tiles of a wavefront of its own columns, where there are many, and wavefronts
+ * of a workgroup: one wavefront alone on a SIMD issues an instruction every four
+ * cycles at most, so two share it, with 256 registers each. */
 #ifndef KVT
-#define KVT 2
+#define KVT (head_dim == 256 ? 1 : 2)
 #endif
 constexpr int kv_most_tiles(int head_dim) { return KVT; }
+constexpr int kv_workgroup_waves(int head_dim, bool columns) { return columns && head_dim > 64 ? 8 : 4; }
 /* wavefronts that share a SIMD's registers: one has 512, of two each 256 */
-constexpr int kv_waves(int head_dim, int tiles, bool columns) { return head_dim == 256 ? 1 : 2; }
+constexpr int kv_waves(int head_dim, int tiles, bool columns) { return head_dim == 256 && !columns ? 1 : 2; }
 
 struct KVShape {
     int tiles;
