@@ -408,21 +408,27 @@ __device__ __forceinline__ void kv_barrier()
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-/* The 64 tokens of a step as D * 64 bytes of keys and as many of values.
- * Key row r = 16 i + n (token 16 (n / 4) + 4 i + n % 4) holds its 16-byte
- * pieces p at p ^ kv_key_turn(n); value row (channel) its four at p ^ (n / 4),
+/* Places in LDS.  A read of 16 bytes by all lanes is served 16 lanes at a time,
+ * of each 32 the lanes 0..3, 12..15, 20..27, then the others; the turns below put
+ * the 16 pieces that are read together, two columns (g) of eight rows, at places
+ * of their own modulo 256 bytes.
+ *
+ * Codes of a step's 64 tokens, D * 64 bytes of keys and as many of values: key
+ * row r = 16 i + n (token 16 (n / 4) + 4 i + n % 4) holds its 16-byte pieces p
+ * at p ^ kv_key_turn(n); a value row (channel) its four at p ^ kv_value_turn(n),
  * n the channel's low four bits. */
 template <int D>
 __device__ __forceinline__ uint32_t kv_key_turn(uint32_t n)
 {
-    return D == 256 ? n : D == 128 ? n >> 1 : n >> 2;
+    return D == 256 ? n : D == 128 ? n >> 1 : ((n >> 2) + 1) & 3;
 }
-
-/* the same of a row of fp16 keys */
+__device__ __forceinline__ uint32_t kv_value_turn(uint32_t n) { return ((n >> 2) + 1) & 3; }
+/* the same of rows of fp16 keys (2 D bytes) and values (128 bytes) */
+__device__ __forceinline__ uint32_t kv_wide_value_turn(uint32_t n) { return ((n >> 1) + 2) & 7; }
 template <int D>
 __device__ __forceinline__ uint32_t kv_wide_turn(uint32_t n)
 {
-    return D == 64 ? n >> 1 : n;
+    return D == 64 ? kv_wide_value_turn(n) : n;
 }
 
 /* One workgroup of four wavefronts per (range of work, key/value head).
@@ -468,13 +474,13 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, NT
 
     /* LDS places of the lane's reads; COLUMNS: of eight channels, of eight tokens */
     const uint32_t wide_key_at = n * 2 * D + ((2 * g) ^ kv_wide_turn<D>(n)) * 16;
-    const uint32_t wide_value_at = 128 * D + n * 128 + ((2 * g) ^ (n >> 1)) * 16;
-    const uint32_t value_at = 64 * D + n * 64 + (g ^ (n >> 2)) * 16;
+    const uint32_t wide_value_at = 128 * D + n * 128 + ((2 * g) ^ kv_wide_value_turn(n)) * 16;
+    const uint32_t value_at = 64 * D + n * 64 + (g ^ kv_value_turn(n)) * 16;
     /* what the lane copies.  Keys: copy d = kRuns i + run is rows 16 i + (64 /
      * D..) of the tile: within a run every i is four tokens further on */
     constexpr int kLanesPerRow = D / 16, kRowsPerCopy = 64 / kLanesPerRow;
     const uint32_t copy_row = lane / kLanesPerRow;                /* + run * kRowsPerCopy = n of the row */
-    const uint32_t value_group = (lane & 3) ^ ((lane >> 4) & 3);
+    const uint32_t value_group = (lane & 3) ^ kv_value_turn(lane >> 2);
 
     KVWalk<kColumns> walk;
     walk.start(a, blockIdx.x);
@@ -584,7 +590,7 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, NT
                     }
                 }
                 const uint32_t channel = (threadIdx.x >> 2) + (k - kPieces) * 16 * kWaves;
-                to += 128 * D + channel * 128 + ((2 * (threadIdx.x & 3) + part) ^ ((channel & 15) >> 1)) * 16;
+                to += 128 * D + channel * 128 + ((2 * (threadIdx.x & 3) + part) ^ kv_wide_value_turn(channel & 15)) * 16;
             }
             *reinterpret_cast<kv_half8 *>(to) = kv_decode8<E4M3>(v[2 * part], v[2 * part + 1]);
         };
