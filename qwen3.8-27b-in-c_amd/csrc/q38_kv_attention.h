@@ -73,7 +73,7 @@ __device__ __forceinline__ uint32_t kv_largest(uint32_t v)
  * as large as 2^d is small, and 2^d alone may leave fp32 */
 __device__ __forceinline__ float kv_lower(float l, float d)
 {
-    const float half = exp2f(0.5f * d);
+    const float half = __builtin_amdgcn_exp2f(0.5f * d);
     return l * half * half;
 }
 /* lane n ^ 8 of the same 16 lanes (row rotation by 8) */
@@ -223,15 +223,19 @@ __device__ __forceinline__ float kv_sigmoid(float x)
     return fmaf(inverse, fmaf(-d, inverse, 1.0f), inverse);
 }
 
-/* out[row][head][d .. d + 3] = O / l, times sigmoid(gate); 0 where the row saw nothing */
+__device__ __forceinline__ kv_float4 kv_gate4(const KVAttention &a, uint32_t row, uint32_t head, uint32_t d)
+{
+    if (!a.gate) return {0.0f, 0.0f, 0.0f, 0.0f};
+    return kv_load4(a.gate, row * a.query_row + head * a.query_head + d, a);
+}
+/* out[row][head][d .. d + 3] = O / l, times sigmoid(gate); 0 where the row saw
+ * nothing.  The gate was asked for by kv_gate4 some time before. */
 __device__ __forceinline__ void kv_finish4(const KVAttention &a, uint32_t row, uint32_t head, uint32_t d, kv_float4 o,
-                                           float l)
+                                           float l, kv_float4 gate)
 {
     o *= l == 0.0f ? 0.0f : 1.0f / l;
-    if (a.gate) {
-        const kv_float4 gate = kv_load4(a.gate, row * a.query_row + head * a.query_head + d, a);
+    if (a.gate)
         for (int e = 0; e < 4; ++e) o[e] *= kv_sigmoid(gate[e]);
-    }
     kv_store4(a.output, row * a.output_row + (uint64_t)head * a.cache.head_dim + d, a, o);
 }
 
@@ -345,12 +349,21 @@ struct KVWalk {
             const int i = __popcll(__ballot(block.units_upto <= at - block_units));
             const uint32_t slots = Lanes::of(block.slots, i), each = Lanes::of(block.each, i);
             const uint32_t base = block_units + Lanes::of(block.units_upto, i) - slots * each;
-            const uint32_t j = slots == 1 ? 0 : (at - base) / each, slot_at = base + j * each;
+            uint32_t j = 0;
+            if (slots != 1) {
+                asm volatile("");              /* a division that is skipped, not one whose result is not taken */
+                j = (at - base) / each;
+            }
+            const uint32_t slot_at = base + j * each;
             const uint32_t rows = Lanes::of(block.end, i) - Lanes::of(block.begin, i), column = j * COLUMNS;
             const int32_t tokens = (int32_t)Lanes::of((uint32_t)block.tokens, i);
             s.first_row = Lanes::of(block.begin, i);
             s.index = block_slots + Lanes::of(block.slots_upto, i) - slots + j;
-            s.row = j ? column / a.group : 0;
+            s.row = 0;
+            if (j) {
+                asm volatile("");
+                s.row = column / a.group;
+            }
             s.rem = column - s.row * a.group;
             s.columns = min(COLUMNS, rows * a.group - column);
             s.sequence = tokens > 0 ? (int32_t)Lanes::of((uint32_t)block.id, i) : -1;
@@ -982,12 +995,23 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, NT
                 for (int c = 0; c < kChannels; ++c)
                     *reinterpret_cast<kv_float4 *>(&merge_o[(wave * 16 + n) * kPitch + c * 16 + 4 * g]) = o[t][c];
             }
+            const uint32_t first = COLUMNS ? (wave * NT + tile_at) * kTile : tile_at * kTile;
+            constexpr uint32_t kItems = kTile * (D / 4), kItemStep = COLUMNS ? 64 : 256;
+            /* gates are asked for an item ahead */
+            auto gate_of = [&](uint32_t at) -> kv_float4 {
+                const uint32_t of = first + at / (D / 4);
+                if (!piece.whole || at >= kItems || of >= s.columns) return {0.0f, 0.0f, 0.0f, 0.0f};
+                return kv_gate4(a, s.first_row + s.row + s.row_of(a, of), head * a.group + s.head_of(a, of), at % (D / 4) * 4);
+            };
+            uint32_t at = COLUMNS ? lane : threadIdx.x;
+            kv_float4 gate = gate_of(at);
             if (COLUMNS) kv_reads_done();           /* the wavefront's own rows; the writes too */
             else __syncthreads();
-            const uint32_t first = COLUMNS ? (wave * NT + tile_at) * kTile : tile_at * kTile;
-            for (uint32_t at = COLUMNS ? lane : threadIdx.x; at < kTile * (D / 4); at += COLUMNS ? 64 : 256) {
+#pragma unroll 1
+            for (; at < kItems; at += kItemStep) {
                 const uint32_t c = at / (D / 4), d = at % (D / 4) * 4, of = first + c;
                 if (of >= s.columns) break;
+                const kv_float4 next_gate = gate_of(at + kItemStep);
                 float top = -INFINITY, total = 0.0f;
                 kv_float4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
                 auto row = [&](uint32_t w) {
@@ -1000,18 +1024,25 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, NT
                     total = merge_l[of];
                     sum = row(wave);
                 } else {
-                    for (int w = 0; w < 4; ++w) top = fmaxf(top, merge_m[w * NT * kTile + of]);
-#pragma unroll 1
+                    float part_m[4], part_l[4];
+                    kv_float4 part[4];
+#pragma unroll
                     for (int w = 0; w < 4; ++w) {
-                        const float mw = merge_m[w * NT * kTile + of];
-                        if (mw == -INFINITY) continue;
-                        const float by = mw == top ? 0.0f : mw - top;
-                        total += kv_lower(merge_l[w * NT * kTile + of], by);
-                        sum += row(w) * exp2f(by);
+                        part_m[w] = merge_m[w * NT * kTile + of];
+                        part_l[w] = merge_l[w * NT * kTile + of];
+                        part[w] = row(w);
+                        top = fmaxf(top, part_m[w]);
+                    }
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        /* (a wavefront without any token has sums of zero) */
+                        const float by = part_m[w] == top ? 0.0f : part_m[w] - top;
+                        total += kv_lower(part_l[w], by);
+                        sum += part[w] * __builtin_amdgcn_exp2f(by);
                     }
                 }
                 if (piece.whole) {
-                    kv_finish4(a, s.first_row + s.row + s.row_of(a, of), head * a.group + s.head_of(a, of), d, sum, total);
+                    kv_finish4(a, s.first_row + s.row + s.row_of(a, of), head * a.group + s.head_of(a, of), d, sum, total, gate);
                 } else {
                     *reinterpret_cast<kv_float4 *>(partial + of * D + d) = sum;
                     if (d == 0) {
@@ -1019,6 +1050,7 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, NT
                         stats[2 * of + 1] = total;
                     }
                 }
+                gate = next_gate;
             }
             if (!COLUMNS) __syncthreads();
         }

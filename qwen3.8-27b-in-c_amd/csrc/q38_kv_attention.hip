@@ -14,12 +14,15 @@ namespace {
  * groups of threads take every so-manieth piece, so that all are read at once:
  * 1024 threads where there may be many (one sequence in 64 pieces: 6 us, 10 with
  * 256), else 256 (480 slots of a few pieces: 5 us, 16 with 1024). */
-__device__ __forceinline__ void finish_column(const KVAttention &a, const KVRecord &r, uint32_t head, uint32_t c, uint32_t d,
-                                              kv_float4 sum, float total)
-{
-    const uint32_t row = kv_divide(r.rem + c, a.group_magic);
-    kv_finish4(a, r.row + row, head * a.group + r.rem + c - row * a.group, d, sum, total);
-}
+struct Column {
+    uint32_t row, head;
+    __device__ __forceinline__ Column(const KVAttention &a, const KVRecord &r, uint32_t kv_head, uint32_t c)
+    {
+        const uint32_t at = kv_divide(r.rem + c, a.group_magic);
+        row = r.row + at;
+        head = kv_head * a.group + r.rem + c - at * a.group;
+    }
+};
 
 __global__ __launch_bounds__(256) void kv_join_few_kernel(KVAttention a)
 {
@@ -29,6 +32,8 @@ __global__ __launch_bounds__(256) void kv_join_few_kernel(KVAttention a)
     if (slot >= kv_records(a)->pieces || r.pieces < 2 || c >= r.columns) return;
     const float *stats = kv_stats(a, r.first_piece, head) + 2 * c, *partial = kv_partial(a, r.first_piece, head) + c * D + d;
     const uint64_t stats_step = (uint64_t)a.cache.kv_heads * a.columns * 2, step = (uint64_t)a.cache.kv_heads * a.columns * D;
+    const Column column(a, r, head, c);
+    const kv_float4 gate = kv_gate4(a, column.row, column.head, d);
     float top = -INFINITY, total = 0.0f;
     kv_float4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t p = 0; p < r.pieces; ++p) top = fmaxf(top, stats[p * stats_step]);
@@ -39,7 +44,7 @@ __global__ __launch_bounds__(256) void kv_join_few_kernel(KVAttention a)
         total += kv_lower(stats[p * stats_step + 1], by);
         sum += *reinterpret_cast<const kv_float4 *>(partial + p * step) * exp2f(by);
     }
-    finish_column(a, r, head, c, d, sum, total);
+    kv_finish4(a, column.row, column.head, d, sum, total, gate);
 }
 
 template <uint32_t THREADS>
@@ -54,6 +59,9 @@ __global__ __launch_bounds__(THREADS) void kv_join_kernel(KVAttention a)
     for (uint32_t c = blockIdx.z; c < r.columns; c += gridDim.z) {
         const float *stats = kv_stats(a, r.first_piece, head) + 2 * c;
         const float *partial = kv_partial(a, r.first_piece, head) + c * D + d;
+        const Column column(a, r, head, c);
+        kv_float4 gate = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (!group) gate = kv_gate4(a, column.row, column.head, d);
         /* the group's first pieces are on their way while the maxima are looked at */
         constexpr uint32_t kAhead = 4;
         kv_float4 first[kAhead];
@@ -90,7 +98,7 @@ __global__ __launch_bounds__(THREADS) void kv_join_kernel(KVAttention a)
             __syncthreads();
             if (group < half) sums[threadIdx.x] = sum = sum + sums[threadIdx.x + half * quads];
         }
-        if (!group) finish_column(a, r, head, c, d, sum, total);
+        if (!group) kv_finish4(a, column.row, column.head, d, sum, total, gate);
     }
 }
 

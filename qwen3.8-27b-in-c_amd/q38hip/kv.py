@@ -99,7 +99,7 @@ class KVPages:
         self._torch, self._int32, self._device, self._types = torch, torch.int32, data.device, _element_types()
         self._index = data.get_device()
         self._bytes = {}                       # workspace of an attention call, by its sizes
-        self._pages_workspace = None
+        self._pages_workspace, self._words_needed = None, 0
 
     @classmethod
     def allocate(cls, layers, pages, page_tokens, kv_heads, head_dim, sequences, table_entries, kind="int8",
@@ -148,6 +148,12 @@ class KVPages:
     def _workspace(self, nbytes):
         return self._torch.empty(nbytes, dtype=self._torch.uint8, device=self._device)
 
+    def _pages_words(self):
+        """32-bit words of the workspace of extend and compact"""
+        if not self._words_needed:
+            self._words_needed = _lib().q38hip_kv_workspace_bytes(self._ref) // 4
+        return self._words_needed
+
     def check(self):
         """Synchronises; raises where a call found bad ids or no room, and clears the status."""
         bits = int(self.status.item())
@@ -168,7 +174,7 @@ class KVPages:
         ids = self._words(sequences, "sequences")
         more = self._words(rows, "rows", sequences.shape[0])
         if self._pages_workspace is None:      # calls on a cache are in order, so one serves them all
-            self._pages_workspace = self._workspace(_lib().q38hip_kv_workspace_bytes(self._ref))
+            self._pages_workspace = self._workspace(4 * self._pages_words())
         _check(_lib().q38hip_kv_extend(self._ref, ids, more, sequences.shape[0], self._pages_workspace.data_ptr(),
                                        self._stream()), "q38hip_kv_extend")
 
@@ -188,9 +194,9 @@ class KVPages:
     def compact(self):
         """The pages in use move to the front of the pool.  Returns an int32
         [2] device tensor: the pages moved and the pages in use."""
-        work = self._workspace(_lib().q38hip_kv_workspace_bytes(self._ref))
+        work = self._torch.empty(self._pages_words(), dtype=self._int32, device=self._device)
         _check(_lib().q38hip_kv_compact(self._ref, work.data_ptr(), self._stream()), "q38hip_kv_compact")
-        return work[:8].view(self._int32)
+        return work[:2]
 
     def copy(self, sources, targets):
         """pages sources[i] to pages targets[i], in all layers"""
