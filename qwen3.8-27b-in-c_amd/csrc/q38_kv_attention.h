@@ -659,6 +659,16 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, NT
             }
         };
 
+        /* The outputs' gates are asked for an item ahead, or here where a thread has two items at most */
+        constexpr uint32_t kItems = kTile * (D / 4), kItemStep = COLUMNS ? 64 : 256, kEarlyGates = (kItems + 255) / 256;
+        constexpr bool kEarly = !COLUMNS && NT == 1 && kEarlyGates <= 2;
+        auto gate_of = [&](uint32_t first, uint32_t at) -> kv_float4 {
+            const uint32_t of = first + at / (D / 4);
+            if (!piece.whole || at >= kItems || of >= s.columns) return {0.0f, 0.0f, 0.0f, 0.0f};
+            return kv_gate4(a, s.first_row + s.row + s.row_of(a, of), head * a.group + s.head_of(a, of), at % (D / 4) * 4);
+        };
+        kv_float4 early_gate[kEarly ? kEarlyGates : 1];
+
         kv_half8 q[COLUMNS ? NT : 1][2 * kChunks];
         if (COLUMNS) {
             load_pages(step);
@@ -680,6 +690,9 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, NT
             kv_barrier();
         } else {
             load_queries(0);
+            if (kEarly)
+#pragma unroll
+                for (uint32_t e = 0; e < kEarlyGates; ++e) early_gate[e] = gate_of(0, threadIdx.x + e * 256);
             /* here, so that nothing the compiler waits for is behind the copies */
 #pragma unroll
             for (int k = 0; k < kEach; ++k)
@@ -996,22 +1009,14 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, NT
                     *reinterpret_cast<kv_float4 *>(&merge_o[(wave * 16 + n) * kPitch + c * 16 + 4 * g]) = o[t][c];
             }
             const uint32_t first = COLUMNS ? (wave * NT + tile_at) * kTile : tile_at * kTile;
-            constexpr uint32_t kItems = kTile * (D / 4), kItemStep = COLUMNS ? 64 : 256;
-            /* gates are asked for an item ahead */
-            auto gate_of = [&](uint32_t at) -> kv_float4 {
-                const uint32_t of = first + at / (D / 4);
-                if (!piece.whole || at >= kItems || of >= s.columns) return {0.0f, 0.0f, 0.0f, 0.0f};
-                return kv_gate4(a, s.first_row + s.row + s.row_of(a, of), head * a.group + s.head_of(a, of), at % (D / 4) * 4);
-            };
             uint32_t at = COLUMNS ? lane : threadIdx.x;
-            kv_float4 gate = gate_of(at);
+            kv_float4 gate = kEarly ? early_gate[0] : gate_of(first, at);
             if (COLUMNS) kv_reads_done();           /* the wavefront's own rows; the writes too */
             else __syncthreads();
-#pragma unroll 1
             for (; at < kItems; at += kItemStep) {
                 const uint32_t c = at / (D / 4), d = at % (D / 4) * 4, of = first + c;
                 if (of >= s.columns) break;
-                const kv_float4 next_gate = gate_of(at + kItemStep);
+                const kv_float4 next_gate = kEarly ? early_gate[1 % kEarlyGates] : gate_of(first, at + kItemStep);
                 float top = -INFINITY, total = 0.0f;
                 kv_float4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
                 auto row = [&](uint32_t w) {
