@@ -9,8 +9,8 @@ namespace q38 {
 
 constexpr int kKVStep = 64;               /* tokens of a step */
 /* units of a slot beside those of its steps: queries, joining and output take
- * about as long as that many steps */
-constexpr uint32_t kKVSlotOverhead = 2;
+ * about as long as eight steps */
+constexpr uint32_t kKVSlotOverhead = 8;
 
 /* n / d of n d < 2^32, d < 2^16, from kv_magic(d) */
 inline uint32_t kv_magic(uint32_t d) { return d == 1 ? 0 : (uint32_t)(0xffffffffu / d + 1); }
@@ -34,7 +34,10 @@ Q38_HD uint32_t kv_chunk(uint32_t units, uint32_t workgroups, float workgroups_i
     while ((uint64_t)each * workgroups < units) each += each >> 22 ? each >> 22 : 1;
     return each;
 }
-Q38_HD uint32_t kv_small(uint32_t chunk) { return chunk / 4; }
+Q38_HD uint32_t kv_small(uint32_t chunk)
+{
+    return chunk / 4 > kKVSlotOverhead + 4 ? chunk / 4 : kKVSlotOverhead + 4;
+}
 
 /* What a range of units begin .. end - 1 holds of the slot whose `each` units
  * (of `steps` steps) begin at `slot` < end: steps first .. last - 1.  A slot of
