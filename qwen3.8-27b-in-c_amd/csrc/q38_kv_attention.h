@@ -641,7 +641,7 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, NT
                 const uint32_t exponent = max(largest >> 23, 30u);
                 /* largest * scale is in 2^13..2^14; columns that are not there are zero */
                 const float scale = c < s.columns ? __uint_as_float((267u - exponent) << 23) : 0.0f;
-                if (kRows * kEights < kThreads && at >= kRows) break;
+                if (kRows * kEights % kThreads && at >= kRows) break;
                 if (eight == 0) to_exponent[c] = a.scale * __uint_as_float((exponent - 13u) << 23);
                 kv_half8 high, low;
 #pragma unroll

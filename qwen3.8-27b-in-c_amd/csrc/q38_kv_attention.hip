@@ -116,7 +116,7 @@ uint64_t plan_kv_attention(KVAttention &a)
     a.least = a.shift ? 1 : shape.columns ? 8 : 4;
     /* as many workgroups as run at once: by LDS where wavefronts have their own
      * tokens (64 D bytes of keys and of values each), else by registers */
-    const uint32_t on_a_unit = !shape.columns ? (D == 64 && shape.tiles == 2 ? 2 : 256 / D) : D == 64 ? 2 : 1;
+    const uint32_t on_a_unit = !shape.columns ? (D == 64 && shape.tiles > 1 ? 2 : 256 / D) : D == 64 ? 4 - shape.tiles : 1;
     const uint64_t units = (uint64_t)a.slots * kv_slot_units(most, a.shift), wanted = 256 * on_a_unit / heads;
     const uint64_t useful = (units + a.least - 1) / a.least;
     a.workgroups = (uint32_t)(wanted < 1 ? 1 : wanted < useful ? wanted : useful);

@@ -66,7 +66,7 @@ Q38_HD uint32_t kv_pieces(uint32_t units, uint32_t chunk, uint32_t behind, uint3
 /* Column tiles (of 8 fp32 or 16 other columns): up to kv_token_tiles in a
  * workgroup whose wavefronts share the tokens, else one or two in each
  * wavefront. */
-constexpr int kv_token_tiles(int head_dim) { return head_dim == 256 ? 3 : 2; }
+constexpr int kv_token_tiles(int head_dim) { return head_dim == 128 ? 2 : 3; }
 /* Tiles of a wavefront of its own columns, where there are many, and wavefronts
  * of a workgroup: one wavefront alone on a SIMD issues an instruction every four
  * cycles at most, so two share it, with 256 registers each. */
