@@ -193,3 +193,49 @@ def test_row_offsets_that_decrease(device):
         assert int(dev.status) == kv.BAD_ROWS
         dev.status.zero_()
         assert (out == 3.0).all()
+
+
+@pytest.mark.parametrize("dim,dtype,kind", [(64, F16, "int8"), (128, F32, "e4m3"), (256, BF16, "int8")])
+def test_many_sequences_of_all_lengths(device, dim, dtype, kind):
+    """more sequences than a wavefront has lanes, some without tokens or rows, long ones cut between workgroups"""
+    rng = np.random.default_rng(dim)
+    lengths = [int(n) for n in np.exp(rng.uniform(0, np.log(1500), size=150))]
+    lengths[3] = lengths[149] = 0
+    rows = [int(r) for r in rng.integers(0, 4, size=150)]
+    rows[0], rows[149] = 2, 1
+    cache, starts, q, gate = _case(rng, 2, 1, dim, 32, kind, dtype, lengths, rows, device)
+    order = [int(i) for i in rng.permutation(150)]
+    got = cache.to(device).attention(0, q, kc.words(order, device), kc.words(starts, device), gate=gate)
+    want, mass, size = cache.attention(0, q.double().cpu().numpy(), order, starts, dim ** -0.5, gate.double().cpu().numpy())
+    _compare(got, want, mass, size, dtype, max(lengths))
+
+
+@pytest.mark.parametrize("dim,dtype,kind,heads", [(64, F32, "e4m3", 1), (64, BF16, "int8", 6), (128, F16, "e4m3", 3),
+                                                  (128, F32, "int8", 1), (256, BF16, "e4m3", 2), (256, F32, "int8", 1)])
+def test_prompts_that_are_cut(device, dim, dtype, kind, heads):
+    """columns of several workgroups' wavefronts, cut along the tokens and joined"""
+    rng = np.random.default_rng(dim + heads)
+    lengths, rows = [2100, 333], [150, 333]
+    cache, starts, q, gate = _case(rng, heads, 1, dim, 64, kind, dtype, lengths, rows, device)
+    got = cache.to(device).attention(0, q, kc.words([0, 1], device), kc.words(starts, device), gate=gate)
+    want, mass, size = cache.attention(0, q.double().cpu().numpy(), [0, 1], starts, dim ** -0.5, gate.double().cpu().numpy())
+    _compare(got, want, mass, size, dtype, max(lengths))
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows,heads,dtype", [(1, 2, F32), (2, 6, F32), (4, 6, F32), (3, 12, BF16), (60, 3, F16), (60, 3, F32)])
+def test_maxima_that_rise(device, dim, rows, heads, dtype):
+    """every page's scores pass those before it by more than the sums allow: they are rescaled again and again"""
+    rng = np.random.default_rng(rows)
+    cache = kc.filled(rng, [500], "int8", 16, 1, dim)
+    direction = rng.normal(size=dim)
+    for entry in range(cache.pages(500)):
+        page = cache.tables[0, entry]
+        x = direction * (0.5 + entry) / dim * 12 + rng.normal(size=(16, dim)) * 0.01
+        scale = kc.scale_of(np.abs(x).max(), "int8")
+        cache.scales[0, page, 0, 0] = scale
+        cache.half(0, page, 0, 0)[:] = kc.encode(x / scale, "int8")
+    q = torch.from_numpy(direction + rng.normal(size=(rows, heads, dim)) * 0.05).to(dtype).to(device)
+    got = cache.to(device).attention(0, q, kc.words([0], device), scale=1.0)
+    want, mass, size = cache.attention(0, q.double().cpu().numpy(), [0], [0, rows], 1.0)
+    _compare(got, want, mass, size, dtype, 500)

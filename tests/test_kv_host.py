@@ -205,3 +205,83 @@ def test_model_of_the_codes(kind):
     want = torch.from_numpy(middle).float()
     want = want.round() if kind == "int8" else want.to(torch.float8_e4m3fn).float()
     assert np.array_equal(got, want.double().numpy())
+
+
+WORK_CHECK = r"""
+#include <cstdio>
+#include <cstdlib>
+#include <vector>
+#include "q38_kv_plan.h"
+using namespace q38;
+#define CHECK(x) do { if (!(x)) { std::printf("line %d: %s\n", __LINE__, #x); return 1; } } while (0)
+static uint32_t state = 54321;
+static uint32_t draw(uint32_t n) { state = state * 1664525u + 1013904223u; return (state >> 8) % n; }
+struct Slot { uint32_t at, each, steps; };
+int main()
+{
+    /* divisions by a group */
+    for (uint32_t d = 1; d <= 32768; d = d < 70 ? d + 1 : d * 2 - d / 3)
+        for (uint32_t n = 0; n < d + 256; n += 1 + n / 300) CHECK(kv_divide(n, kv_magic(d)) == n / d);
+    /* ranges: workgroups of them hold all units, and one less would not */
+    for (int trial = 0; trial < 200000; ++trial) {
+        const uint32_t units = draw(2) ? draw(100000) : (draw(1 << 24) << 7) + draw(128), groups = 1 + draw(1024), least = 1 + draw(8);
+        const uint32_t chunk = kv_chunk(units, groups, 1.0f / (float)groups, least);
+        CHECK(chunk >= least && (uint64_t)chunk * groups >= units);
+        CHECK(chunk == least || chunk <= units / groups * (1 + 1e-6) + 2);
+    }
+    /* every step of every slot is in one piece, its pieces are counted, and each has a place of its own */
+    for (int trial = 0; trial < 4000; ++trial) {
+        const uint32_t shift = trial % 5 ? 0 : draw(4), groups = 1 + draw(40), least = shift ? 1 : 4;
+        std::vector<Slot> slots;
+        uint32_t total = 0;
+        for (uint32_t n = 1 + draw(30); n; --n) {
+            const uint32_t most = draw(3) ? draw(20) : draw(600), each = kv_slot_units(most, shift);
+            for (uint32_t k = 1 + draw(3); k; --k) {              /* slots of one sequence: the last rows see all steps */
+                slots.push_back({total, each, most - (most ? draw(most < 3 ? most : 3) : 0)});
+                total += each;
+            }
+        }
+        const uint32_t chunk = kv_chunk(total, groups, 1.0f / (float)groups, least), small = kv_small(chunk);
+        std::vector<uint32_t> reached(slots.size(), 0), pieces(slots.size(), 0), firsts(slots.size(), 0);
+        std::vector<char> used(groups + slots.size(), 0);
+        for (uint32_t w = 0; w < groups; ++w) {
+            const uint64_t begin = (uint64_t)w * chunk, end64 = begin + chunk;
+            if (begin >= total) break;
+            const uint32_t end = end64 < total ? (uint32_t)end64 : total;
+            for (uint32_t k = 0; k < slots.size(); ++k) {
+                const Slot &s = slots[k];
+                if (s.at >= end || s.at + s.each <= begin) continue;
+                const KVPiece p = kv_piece(s.at, s.each, s.steps, (uint32_t)begin, end, small, shift);
+                if (!p.some) continue;
+                CHECK(p.first == reached[k] && p.last >= p.first && p.last <= s.steps);
+                reached[k] = p.last;
+                ++pieces[k];
+                CHECK(p.first_piece == (pieces[k] == 1));
+                if (p.first_piece) firsts[k] = p.whole ? 1 : kv_pieces(p.units, chunk, s.at + s.each, s.each);
+                CHECK(!p.whole || p.last == s.steps);
+                CHECK(w + k < used.size() && !used[w + k]);
+                used[w + k] = 1;
+            }
+        }
+        for (uint32_t k = 0; k < slots.size(); ++k) CHECK(reached[k] == slots[k].steps && pieces[k] >= 1 && pieces[k] == firsts[k]);
+    }
+    std::puts("ok");
+    return 0;
+}
+"""
+
+
+def test_work_split(tmp_path):
+    """how the tokens of a paged attention call are cut between workgroups (csrc/q38_kv_plan.h)"""
+    source, program = tmp_path / "kv_work.cpp", tmp_path / "kv_work"
+    source.write_text(WORK_CHECK)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror",
+                    "-I", os.path.join(ROOT, "include"), "-I", os.path.join(ROOT, "qwen3.8-27b-in-c_amd", "csrc"), str(source),
+                    "-o", str(program)], check=True)
+    assert subprocess.run([str(program)], capture_output=True, text=True, timeout=120).stdout == "ok\n"
+
+
+def test_too_many_query_heads_are_refused():
+    cache = ctypes.byref(_cache(kv_heads=1))
+    assert kv._lib().q38hip_kv_attention_workspace_bytes(cache, 0, 32769, 1, 1) == 0
+    assert "32768" in q38hip.last_error()
