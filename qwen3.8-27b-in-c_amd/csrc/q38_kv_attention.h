@@ -17,10 +17,21 @@
  * are both its slice of the second product and 16 consecutive bytes of a value
  * channel.
  *
- * Codes go from memory straight into LDS (global_load_lds, 1 KiB each, whole
- * rows of keys or values, so requests are contiguous and no register waits for
- * them), in 16-byte pieces whose place in a row is exclusive-ored with the row
- * so that the 16 lanes that read one piece of 16 rows use all banks.
+ * Few columns (decode, verify): memory is the bound.  Codes go straight into
+ * LDS (global_load_lds, 1 KiB each, whole rows of keys or values, so requests
+ * are contiguous and no register waits for them); a wavefront asks for its next
+ * keys when it has read the present ones, and for its next values channel by
+ * channel.  48 sequences of up to 16384 tokens (32 heads, 8 of keys, 128 wide,
+ * 339 MB): 65 us, 5.2 TB/s, what a large copy reaches here.  Four rows at 131075
+ * tokens (24 heads, 4 of keys, 256 wide, 268 MB): 67 us, 4.0 TB/s; 9 us pass
+ * before the first step's codes are there, 7 in the merge at the end.
+ *
+ * Many columns (prompts): the products are the bound.  512 rows behind 7679
+ * tokens (24 heads, 4 of keys, 256 wide, 100 GFLOP): 147 us, 680 TFLOP/s; of
+ * its cycles the matrix unit is busy in a third, LDS in over half.
+ *
+ * Short calls are instruction fetch: 37 tokens take 11 us, of which memory is
+ * three; what runs once is kept short.
  *
  * 8-bit codes are exact in fp16, and so is a 16-bit query once its row is
  * scaled by a power of two to a maximum of 2^13..2^14 (but for what lies 2^37
@@ -444,14 +455,13 @@ __device__ __forceinline__ uint32_t kv_wide_turn(uint32_t n)
     return D == 64 ? kv_wide_value_turn(n) : n;
 }
 
-/* One workgroup of four wavefronts per (range of work, key/value head).
- * COLUMNS false: the wavefronts take steps of the tokens in turn, over the
- * same NT tiles of columns, each with its own step's codes in LDS, and are
- * joined at the end.  COLUMNS true (prompt chunks): every wavefront has NT
- * column tiles of its own over all steps.  The products are the bound there, so
- * a step is decoded once for all four: through registers, a step ahead, into one
- * of two tiles of fp16, 2 D bytes a key and 128 a channel.  Its 16-byte pieces
- * of eight are turned by the row like those of the codes. */
+/* One workgroup per (range of work, key/value head).
+ * COLUMNS false: four wavefronts take steps of the tokens in turn, over the same
+ * NT tiles of columns, each with its own step's codes in LDS, and are joined at
+ * the end.  COLUMNS true: every wavefront has NT column tiles of its own over
+ * all steps; a step is decoded once for all of them, through registers, a step
+ * ahead, into one of two tiles of fp16, 2 D bytes a key and 128 a channel, whose
+ * 16-byte pieces of eight are turned by the row like those of the codes. */
 template <int D>
 constexpr int kv_ring_bytes() { return 512 * D; }
 template <int D, int WAVES>
@@ -462,10 +472,10 @@ constexpr int kv_lds_bytes()
 }
 
 template <bool E4M3, int D, int NT, bool SPLIT, bool COLUMNS>
-__global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, NT, COLUMNS)) void kv_attention_kernel(KVAttention a)
+__global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, COLUMNS)) void kv_attention_kernel(KVAttention a)
 {
     constexpr int kTile = SPLIT ? 8 : 16, kWaves = kv_workgroup_waves(D, COLUMNS);
-    constexpr bool kAccumulators = kv_waves(D, NT, COLUMNS) == 1;  /* more registers than VGPRs: sums in AGPRs */
+    constexpr bool kAccumulators = kv_waves(D, COLUMNS) == 1;  /* more registers than VGPRs: sums in AGPRs */
     constexpr int kChunks = D / 64, kChannels = D / 16;
     constexpr int kPitch = D + 4;
     constexpr int kCopies = D / 16;                                /* copies of 1 KiB of a step's keys or values */

@@ -34,15 +34,33 @@ __global__ __launch_bounds__(256) void kv_join_few_kernel(KVAttention a)
     const uint64_t stats_step = (uint64_t)a.cache.kv_heads * a.columns * 2, step = (uint64_t)a.cache.kv_heads * a.columns * D;
     const Column column(a, r, head, c);
     const kv_float4 gate = kv_gate4(a, column.row, column.head, d);
+    /* four pieces at once */
     float top = -INFINITY, total = 0.0f;
     kv_float4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t p = 0; p < r.pieces; ++p) top = fmaxf(top, stats[p * stats_step]);
-    for (uint32_t p = 0; p < r.pieces; ++p) {
-        const float m = stats[p * stats_step];
-        if (m == -INFINITY) continue;
-        const float by = m == top ? 0.0f : m - top;
-        total += kv_lower(stats[p * stats_step + 1], by);
-        sum += *reinterpret_cast<const kv_float4 *>(partial + p * step) * exp2f(by);
+    for (uint32_t first = 0; first < r.pieces; first += 4) {
+        kv_float4 part[4];
+        float part_m[4], part_l[4], largest = top;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            part[k] = {0.0f, 0.0f, 0.0f, 0.0f};
+            part_m[k] = -INFINITY;
+            part_l[k] = 0.0f;
+            if (first + k >= r.pieces) continue;
+            part[k] = *reinterpret_cast<const kv_float4 *>(partial + (first + k) * step);
+            part_m[k] = stats[(first + k) * stats_step];
+            part_l[k] = stats[(first + k) * stats_step + 1];
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) largest = fmaxf(largest, part_m[k]);
+        auto less = [&](float m) { return m == largest ? 0.0f : m - largest; };    /* (-inf: nothing was seen) */
+        total = kv_lower(total, less(top));
+        sum *= exp2f(less(top));
+        top = largest;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            total += kv_lower(part_l[k], less(part_m[k]));
+            sum += part[k] * exp2f(less(part_m[k]));
+        }
     }
     kv_finish4(a, column.row, column.head, d, sum, total, gate);
 }

@@ -64,19 +64,19 @@ Q38_HD uint32_t kv_pieces(uint32_t units, uint32_t chunk, uint32_t behind, uint3
 }
 
 /* Column tiles (of 8 fp32 or 16 other columns): up to kv_token_tiles in a
- * workgroup whose wavefronts share the tokens, else one or two in each
- * wavefront. */
+ * workgroup whose wavefronts share the tokens (128-wide heads: a third tile's
+ * registers would leave one wavefront to a SIMD), else one or kv_most_tiles in
+ * each wavefront. */
 constexpr int kv_token_tiles(int head_dim) { return head_dim == 128 ? 2 : 3; }
-/* Tiles of a wavefront of its own columns, where there are many, and wavefronts
- * of a workgroup: one wavefront alone on a SIMD issues an instruction every four
- * cycles at most, so two share it, with 256 registers each. */
-#ifndef KVT
-#define KVT (head_dim == 256 ? 1 : 2)
-#endif
-constexpr int kv_most_tiles(int head_dim) { return KVT; }
+constexpr int kv_most_tiles(int head_dim) { return head_dim == 256 ? 1 : 2; }
+/* Wavefronts of a workgroup.  One alone on a SIMD issues an instruction every
+ * four cycles at most, so where the products are the bound two share it: 512
+ * columns of 256-wide heads over 8191 tokens took 195 us with four wavefronts of
+ * two tiles, 175 with eight of one. */
 constexpr int kv_workgroup_waves(int head_dim, bool columns) { return columns && head_dim > 64 ? 8 : 4; }
-/* wavefronts that share a SIMD's registers: one has 512, of two each 256 */
-constexpr int kv_waves(int head_dim, int tiles, bool columns) { return head_dim == 256 && !columns ? 1 : 2; }
+/* Wavefronts that share a SIMD's registers: one has 512, of two each 256.  256-wide
+ * heads over shared tokens fill the LDS with one workgroup. */
+constexpr int kv_waves(int head_dim, bool columns) { return head_dim == 256 && !columns ? 1 : 2; }
 
 struct KVShape {
     int tiles;
@@ -89,6 +89,8 @@ inline KVShape kv_shape(const KVAttention &a)
     const uint64_t columns = ((uint64_t)a.rows.total_rows * a.group + a.rows.count - 1) / a.rows.count;
     const uint64_t shared = (columns + tile - 1) / tile;
     if (shared <= (uint64_t)kv_token_tiles(a.cache.head_dim)) return {(int)shared, false};
+    /* few columns: two tiles a wavefront would leave most wavefronts none (prompts of up to 300
+     * rows at 16 heads of 64: 43 us with two, 36 with one) */
     return {columns <= 16 * tile ? 1 : kv_most_tiles(a.cache.head_dim), true};
 }
 
