@@ -101,6 +101,7 @@ struct KVAttention {
     float workgroups_inverse;
     uint32_t columns, slots;               /* columns of a slot, at most that many slots */
     uint32_t workgroups, shift, least;     /* per key/value head; steps of a unit (log2); units of a workgroup at least */
+    bool cut;                              /* slots may be, and what is cut is joined */
     int type;
     float scale;           /* softmax scale times log2(e) */
 };

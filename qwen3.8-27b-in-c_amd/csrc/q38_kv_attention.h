@@ -362,8 +362,10 @@ struct KVWalk {
             const uint32_t base = block_units + Lanes::of(block.units_upto, i) - slots * each;
             uint32_t j = 0;
             if (slots != 1) {
-                asm volatile("");              /* a division that is skipped, not one whose result is not taken */
-                j = (at - base) / each;
+                /* (opaque: a division that is skipped, not one that is begun ahead of the branch) */
+                uint32_t by = each;
+                asm volatile("" : "+v"(by));
+                j = __builtin_amdgcn_readfirstlane((at - base) / by);
             }
             const uint32_t slot_at = base + j * each;
             const uint32_t rows = Lanes::of(block.end, i) - Lanes::of(block.begin, i), column = j * COLUMNS;
@@ -372,8 +374,9 @@ struct KVWalk {
             s.index = block_slots + Lanes::of(block.slots_upto, i) - slots + j;
             s.row = 0;
             if (j) {
-                asm volatile("");
-                s.row = column / a.group;
+                uint32_t group = a.group;
+                asm volatile("" : "+v"(group));
+                s.row = __builtin_amdgcn_readfirstlane(column / group);
             }
             s.rem = column - s.row * a.group;
             s.columns = min(COLUMNS, rows * a.group - column);
@@ -507,7 +510,7 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, CO
 
     KVWalk<kColumns> walk;
     walk.start(a, blockIdx.x);
-    if (a.workgroups > 1 && blockIdx.x == 0 && head == 0 && threadIdx.x == 0) kv_records(a)->pieces = walk.total_slots;
+    if (a.cut && blockIdx.x == 0 && head == 0 && threadIdx.x == 0) kv_records(a)->pieces = walk.total_slots;
     KVSlot s;
     KVPiece piece;
     while (walk.next(a, s, piece)) {
@@ -993,9 +996,12 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, CO
 
         const uint64_t index = (uint64_t)blockIdx.x + s.index;
         float *partial = kv_partial(a, index, head), *stats = kv_stats(a, index, head);
-        if (a.workgroups > 1 && head == 0 && piece.first_piece && threadIdx.x == 0)
-            kv_records(a)[1 + s.index] = {piece.whole ? 1 : kv_pieces(piece.units, walk.chunk, walk.at, piece.each),
+        if (a.cut && head == 0 && piece.first_piece && threadIdx.x == 0) {
+            uint32_t chunk = walk.chunk;
+            asm volatile("" : "+v"(chunk));
+            kv_records(a)[1 + s.index] = {piece.whole ? 1 : kv_pieces(piece.units, chunk, walk.at, piece.each),
                                           (uint32_t)index, s.first_row + s.row, s.rem, s.columns, {0, 0, 0}};
+        }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             l[t] = kv_other_rows(l[t], false);

@@ -138,9 +138,12 @@ uint64_t plan_kv_attention(KVAttention &a)
     const uint64_t units = (uint64_t)a.slots * kv_slot_units(most, a.shift), wanted = 256 * on_a_unit / heads;
     const uint64_t useful = (units + a.least - 1) / a.least;
     a.workgroups = (uint32_t)(wanted < 1 ? 1 : wanted < useful ? wanted : useful);
+    if (a.slots == 1 && kv_slot_units(most, a.shift) <= kv_small(0)) a.workgroups = 1;
     a.workgroups_inverse = 1.0f / (float)a.workgroups;
     a.group_magic = kv_magic(a.group);
-    if (a.workgroups == 1) return 0;
+    /* a table that holds short sequences only: no slot is ever cut, nothing is joined */
+    a.cut = a.workgroups > 1 && kv_slot_units(most, a.shift) > kv_small(0);
+    if (!a.cut) return 0;
     return (a.slots + 1) * sizeof(KVRecord) +
            ((uint64_t)a.workgroups + a.slots) * heads * a.columns * (D + 2) * sizeof(float);
 }
@@ -157,7 +160,7 @@ bool launch_kv_attention(const KVAttention &a, hipStream_t stream)
     if (!(D == 64 ? launch_kv_attention_width<64>(a, stream)
                   : D == 128 ? launch_kv_attention_width<128>(a, stream) : launch_kv_attention_width<256>(a, stream)))
         return false;
-    if (a.workgroups == 1) return true;
+    if (!a.cut) return true;
     if (kv_shape(a).columns) {
         const uint32_t together = 1024 / D;
         return launch_kernel(kv_join_few_kernel, dim3(a.slots, a.cache.kv_heads, (a.columns + together - 1) / together), dim3(256),
