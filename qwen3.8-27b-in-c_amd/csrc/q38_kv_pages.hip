@@ -11,9 +11,11 @@ namespace q38 {
 namespace {
 
 constexpr int kPlan = 1024;               /* threads of the one planning workgroup */
+constexpr uint32_t kNear = 2048;           /* new pages of an extension that stay in LDS */
 constexpr uint32_t kScanEach = 16;        /* pages per thread of one round of its scans */
 
-__device__ __forceinline__ uint32_t pages_of(uint32_t tokens, uint32_t T) { return (tokens + T - 1) / T; }
+/* T is a power of two */
+__device__ __forceinline__ uint32_t pages_of(uint32_t tokens, uint32_t T) { return (tokens + T - 1) >> (__ffs(T) - 1); }
 
 /* exclusive prefix sum over the workgroup of kPlan threads, and the total;
  * the caller's barrier separates two uses of `sums` */
@@ -72,7 +74,8 @@ __global__ __launch_bounds__(kPlan) void kv_extend_kernel(Q38KVPages c, const in
 {
     __shared__ uint32_t sums[kPlan / 64];
     __shared__ int32_t ids[kPlan], tails[kPlan];
-    __shared__ uint32_t offsets[kPlan + 1];
+    __shared__ uint32_t offsets[kPlan + 1], lasts[kPlan];    /* first of the item's pages; table entries behind it */
+    __shared__ int32_t near[kNear];                          /* the first pages found */
     __shared__ uint32_t trouble;
     const uint32_t i = threadIdx.x, T = c.page_tokens;
     uint32_t before = 0, after = 0, bad = 0, take = 0;
@@ -91,8 +94,8 @@ __global__ __launch_bounds__(kPlan) void kv_extend_kernel(Q38KVPages c, const in
             const uint64_t last = (uint64_t)before + (uint32_t)more;
             if (last > (uint64_t)c.table_entries * T) bad = Q38_KV_TABLE_FULL;
             else after = (uint32_t)last;
-            if (!bad && more && before % T) {
-                tail = kv_page(c, id, before / T);
+            if (!bad && more && (before & (T - 1))) {
+                tail = kv_page(c, id, before >> (__ffs(T) - 1));
                 if (tail < 0) bad = Q38_KV_BAD_PAGE;
             }
         }
@@ -113,6 +116,7 @@ __global__ __launch_bounds__(kPlan) void kv_extend_kernel(Q38KVPages c, const in
     uint32_t total;
     const uint32_t offset = block_prefix(i < count ? take : 0, sums, total);
     offsets[i] = offset;
+    lasts[i] = pages_of(after, T);
     if (i == 0) offsets[kPlan] = total;
     if (i < count) {
         pairs[i] = -1;
@@ -128,7 +132,11 @@ __global__ __launch_bounds__(kPlan) void kv_extend_kernel(Q38KVPages c, const in
     for (uint32_t first = 0; first < c.pages && have < total; first += kPlan * kScanEach) {
         uint32_t bits = first ? free_bits(c.refs, first + i * kScanEach, c.pages) : first_bits, all;
         uint32_t rank = have + block_prefix(__popc(bits), sums, all);
-        for (; bits && rank < total; bits &= bits - 1, ++rank) found[rank] = (int32_t)(first + i * kScanEach + __ffs(bits) - 1);
+        for (; bits && rank < total; bits &= bits - 1, ++rank) {
+            const int32_t page = (int32_t)(first + i * kScanEach + __ffs(bits) - 1);
+            if (rank < kNear) near[rank] = page;
+            else found[rank] = page;
+        }
         have += all;
         __syncthreads();
     }
@@ -140,7 +148,7 @@ __global__ __launch_bounds__(kPlan) void kv_extend_kernel(Q38KVPages c, const in
     __syncthreads();
     if (i < count && copy) {
         pairs[i] = tail;
-        pairs[count + i] = found[offset];
+        pairs[count + i] = offset < kNear ? near[offset] : found[offset];
         atomicSub(&c.refs[tail], 1);
     }
     for (uint32_t k = i; k < total; k += kPlan) {
@@ -151,12 +159,10 @@ __global__ __launch_bounds__(kPlan) void kv_extend_kernel(Q38KVPages c, const in
             if (offsets[mid] <= k) low = mid;
             else high = mid;
         }
-        const int32_t page = found[k], of = ids[low];
-        const uint32_t held = kv_tokens(c, of);
+        const int32_t page = k < kNear ? near[k] : found[k];
         /* entries go up from the tail's where it is copied, else from the first new one */
         const uint32_t own = offsets[low + 1] - offsets[low];
-        const uint32_t last = pages_of(held + (uint32_t)rows[low], T);
-        c.tables[(uint64_t)of * c.table_entries + (last - own + (k - offsets[low]))] = page;
+        c.tables[(uint64_t)ids[low] * c.table_entries + (lasts[low] - own + (k - offsets[low]))] = page;
         c.refs[page] = 1;
     }
     __syncthreads();

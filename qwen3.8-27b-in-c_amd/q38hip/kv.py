@@ -244,6 +244,8 @@ class KVPages:
         nbytes = self._bytes.get((kind, heads, count, rows))
         if nbytes is None:
             nbytes = bound.q38hip_kv_attention_workspace_bytes(self._ref, kind, heads, count, rows)
+            if len(self._bytes) >= 4096:
+                self._bytes.clear()
             self._bytes[kind, heads, count, rows] = nbytes
         work = self._workspace(nbytes) if nbytes else None
         _check(bound.q38hip_kv_attention(self._ref, layer, out.data_ptr(), query.data_ptr(),
