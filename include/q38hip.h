@@ -346,7 +346,7 @@ int q38hip_kv_copy(const Q38KVPages *cache, const int32_t *sources, const int32_
  * row_starts[i + 1] - 1 of total_rows (device words, non-decreasing), or
  * total_rows / count rows each where row_starts is NULL.  They are the last
  * rows of the sequence's tokens: row t of r stands at position
- * length - r + t.  type is the GGML id of the rows: F32 0, F16 1, BF16 30. */
+ * length - r + t.  Rows that no sequence owns are neither read nor written.  type is the GGML id of the rows: F32 0, F16 1, BF16 30. */
 
 /* Quantises the rows' keys and values ([kv_heads][head_dim], rows row_stride
  * elements apart) into the pages of one layer.  Per page, head and half: with

@@ -393,7 +393,7 @@ struct KVWalk {
 
 /* Workspace of a call whose slots may be cut: one KVRecord per slot (record 0
  * is the number of slots), then the sums of the pieces, then their (maximum,
- * total). */
+ * total).  A workgroup has two pieces of cut slots at most, kv_place. */
 struct KVRecord {
     uint32_t pieces, first_piece, row, rem, columns, unused[3];    /* row: of the call */
 };
@@ -404,7 +404,7 @@ __device__ __forceinline__ float *kv_partial(const KVAttention &a, uint64_t piec
 }
 __device__ __forceinline__ float *kv_stats(const KVAttention &a, uint64_t piece, uint32_t head)
 {
-    return kv_partial(a, (uint64_t)a.workgroups + a.slots, 0) + (piece * a.cache.kv_heads + head) * a.columns * 2;
+    return kv_partial(a, 2ull * a.workgroups, 0) + (piece * a.cache.kv_heads + head) * a.columns * 2;
 }
 
 /* ---- codes to LDS -------------------------------------------------------------- */
@@ -994,13 +994,13 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, CO
                 for (int c = 0; c < kChannels; ++c) asm volatile("" : "+a"(o[t][c]));    /* read after the products, not before */
         }
 
-        const uint64_t index = (uint64_t)blockIdx.x + s.index;
+        const uint32_t index = kv_place(blockIdx.x, piece.first_piece);
         float *partial = kv_partial(a, index, head), *stats = kv_stats(a, index, head);
         if (a.cut && head == 0 && piece.first_piece && threadIdx.x == 0) {
             uint32_t chunk = walk.chunk;
             asm volatile("" : "+v"(chunk));
             kv_records(a)[1 + s.index] = {piece.whole ? 1 : kv_pieces(piece.units, chunk, walk.at, piece.each),
-                                          (uint32_t)index, s.first_row + s.row, s.rem, s.columns, {0, 0, 0}};
+                                          index, s.first_row + s.row, s.rem, s.columns, {0, 0, 0}};
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {

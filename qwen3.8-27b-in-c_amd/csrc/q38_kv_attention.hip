@@ -46,9 +46,10 @@ __global__ __launch_bounds__(256) void kv_join_few_kernel(KVAttention a)
             part_m[k] = -INFINITY;
             part_l[k] = 0.0f;
             if (first + k >= r.pieces) continue;
-            part[k] = *reinterpret_cast<const kv_float4 *>(partial + (first + k) * step);
-            part_m[k] = stats[(first + k) * stats_step];
-            part_l[k] = stats[(first + k) * stats_step + 1];
+            const uint32_t at = kv_place_step(first + k);
+            part[k] = *reinterpret_cast<const kv_float4 *>(partial + at * step);
+            part_m[k] = stats[at * stats_step];
+            part_l[k] = stats[at * stats_step + 1];
         }
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) largest = fmaxf(largest, part_m[k]);
@@ -86,22 +87,23 @@ __global__ __launch_bounds__(THREADS) void kv_join_kernel(KVAttention a)
         float first_m[kAhead];
 #pragma unroll
         for (uint32_t k = 0; k < kAhead; ++k) {
-            const uint32_t p = group + k * groups;
+            const uint32_t p = group + k * groups, at = kv_place_step(p);
             first[k] = {0.0f, 0.0f, 0.0f, 0.0f};
             first_m[k] = -INFINITY;
             if (p >= r.pieces) continue;
-            first[k] = *reinterpret_cast<const kv_float4 *>(partial + p * step);
-            first_m[k] = stats[p * stats_step];
+            first[k] = *reinterpret_cast<const kv_float4 *>(partial + at * step);
+            first_m[k] = stats[at * stats_step];
         }
         /* maximum and total, the same in every wavefront */
-        const float mine_m = lane < r.pieces ? stats[lane * stats_step] : -INFINITY;
-        const float mine_l = lane < r.pieces ? stats[lane * stats_step + 1] : 0.0f;
+        auto stat = [&](uint32_t p) { return stats + kv_place_step(p) * stats_step; };
+        const float mine_m = lane < r.pieces ? stat(lane)[0] : -INFINITY;
+        const float mine_l = lane < r.pieces ? stat(lane)[1] : 0.0f;
         float top = mine_m;
-        for (uint32_t p = lane + 64; p < r.pieces; p += 64) top = fmaxf(top, stats[p * stats_step]);
+        for (uint32_t p = lane + 64; p < r.pieces; p += 64) top = fmaxf(top, stat(p)[0]);
         for (int by = 1; by < 64; by *= 2) top = fmaxf(top, __shfl_xor(top, by));
         auto lowered = [&](float m, float l) { return m == -INFINITY ? 0.0f : kv_lower(l, m == top ? 0.0f : m - top); };
         float total = lowered(mine_m, mine_l);
-        for (uint32_t p = lane + 64; p < r.pieces; p += 64) total += lowered(stats[p * stats_step], stats[p * stats_step + 1]);
+        for (uint32_t p = lane + 64; p < r.pieces; p += 64) total += lowered(stat(p)[0], stat(p)[1]);
         for (int by = 1; by < 64; by *= 2) total += __shfl_xor(total, by);
         kv_float4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
         auto add = [&](float m, kv_float4 o) {
@@ -110,7 +112,7 @@ __global__ __launch_bounds__(THREADS) void kv_join_kernel(KVAttention a)
 #pragma unroll
         for (uint32_t k = 0; k < kAhead; ++k) add(first_m[k], first[k]);
         for (uint32_t p = group + kAhead * groups; p < r.pieces; p += groups)
-            add(stats[p * stats_step], *reinterpret_cast<const kv_float4 *>(partial + p * step));
+            add(stat(p)[0], *reinterpret_cast<const kv_float4 *>(partial + kv_place_step(p) * step));
         sums[threadIdx.x] = sum;
         for (uint32_t half = groups / 2; half; half /= 2) {
             __syncthreads();
@@ -145,7 +147,7 @@ uint64_t plan_kv_attention(KVAttention &a)
     a.cut = a.workgroups > 1 && kv_slot_units(most, a.shift) > kv_small(0);
     if (!a.cut) return 0;
     return (a.slots + 1) * sizeof(KVRecord) +
-           ((uint64_t)a.workgroups + a.slots) * heads * a.columns * (D + 2) * sizeof(float);
+           2ull * a.workgroups * heads * a.columns * (D + 2) * sizeof(float);
 }
 
 template <int D>

@@ -63,6 +63,12 @@ Q38_HD uint32_t kv_pieces(uint32_t units, uint32_t chunk, uint32_t behind, uint3
     return (slot + units - 1) / chunk - slot / chunk + 1;
 }
 
+/* Place of a workgroup's piece of a cut slot: its range begins in one such slot
+ * at most and ends in one.  The p-th piece of a slot is kv_place_step(p) places
+ * behind the first, as the ranges follow each other. */
+Q38_HD uint32_t kv_place(uint32_t workgroup, bool first_piece) { return 2 * workgroup + (first_piece ? 1 : 0); }
+Q38_HD uint32_t kv_place_step(uint32_t p) { return p ? 2 * p - 1 : 0; }
+
 /* Column tiles (of 8 fp32 or 16 other columns): up to kv_token_tiles in a
  * workgroup whose wavefronts share the tokens (128-wide heads: a third tile's
  * registers would leave one wavefront to a SIMD), else one or kv_most_tiles in

@@ -225,7 +225,8 @@ class KVPages:
     def attention(self, layer, query, sequences, row_starts=None, gate=None, scale=None, out=None):
         """Causal attention of each sequence's last rows in one layer: query
         (and gate) [rows, heads, head_dim] with contiguous channels and equal
-        strides; the result [rows, heads, head_dim] in the query's type."""
+        strides; the result [rows, heads, head_dim] in the query's type.
+        Rows that row_starts leaves out are not written."""
         shape, stride, dtype = query.shape, query.stride(), query.dtype
         if len(shape) != 3 or shape[2] != self.head_dim or stride[2] != 1:
             raise ValueError("expected queries [rows, heads, %d] with contiguous channels" % self.head_dim)

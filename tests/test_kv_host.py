@@ -243,7 +243,8 @@ int main()
         }
         const uint32_t chunk = kv_chunk(total, groups, 1.0f / (float)groups, least), small = kv_small(chunk);
         std::vector<uint32_t> reached(slots.size(), 0), pieces(slots.size(), 0), firsts(slots.size(), 0);
-        std::vector<char> used(groups + slots.size(), 0);
+        std::vector<uint32_t> places(slots.size(), 0);
+        std::vector<char> used(2 * groups, 0);
         for (uint32_t w = 0; w < groups; ++w) {
             const uint64_t begin = (uint64_t)w * chunk, end64 = begin + chunk;
             if (begin >= total) break;
@@ -259,8 +260,12 @@ int main()
                 CHECK(p.first_piece == (pieces[k] == 1));
                 if (p.first_piece) firsts[k] = p.whole ? 1 : kv_pieces(p.units, chunk, s.at + s.each, s.each);
                 CHECK(!p.whole || p.last == s.steps);
-                CHECK(w + k < used.size() && !used[w + k]);
-                used[w + k] = 1;
+                if (p.whole) continue;
+                const uint32_t place = kv_place(w, p.first_piece);
+                CHECK(place < used.size() && !used[place]);
+                used[place] = 1;
+                if (p.first_piece) places[k] = place;
+                CHECK(place == places[k] + kv_place_step(pieces[k] - 1));
             }
         }
         for (uint32_t k = 0; k < slots.size(); ++k) CHECK(reached[k] == slots[k].steps && pieces[k] >= 1 && pieces[k] == firsts[k]);
@@ -285,3 +290,12 @@ def test_too_many_query_heads_are_refused():
     cache = ctypes.byref(_cache(kv_heads=1))
     assert kv._lib().q38hip_kv_attention_workspace_bytes(cache, 0, 32769, 1, 1) == 0
     assert "32768" in q38hip.last_error()
+
+
+def test_workspace_follows_the_workgroups():
+    """only slots that are cut need room, and they are no more than the workgroups, however long the prompt"""
+    cache = ctypes.byref(_cache(kv_heads=4, head_dim=256, page_tokens=64, table_entries=1024, pages=2048))
+    sizes = [kv._lib().q38hip_kv_attention_workspace_bytes(cache, 30, 24, 1, rows) for rows in (1, 512, 4096, 32768)]
+    assert 0 < sizes[0] < sizes[1] and max(sizes) < 80e6 and sizes[3] - sizes[2] < 1e6
+    short = ctypes.byref(_cache(kv_heads=4, head_dim=256, page_tokens=16, table_entries=8, pages=64))
+    assert kv._lib().q38hip_kv_attention_workspace_bytes(short, 0, 24, 2, 2) == 0
