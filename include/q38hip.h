@@ -323,7 +323,8 @@ int q38hip_kv_extend(const Q38KVPages *cache, const int32_t *sequences, const in
 
 /* Sequence children[i], which has to be empty, becomes the first lengths[i]
  * tokens of parents[i] (all of them where lengths is NULL) and shares their
- * pages.  Children are distinct and none is a parent in the same call. */
+ * pages.  Children (count <= 65536) are distinct and none is a parent in the
+ * same call. */
 int q38hip_kv_fork(const Q38KVPages *cache, const int32_t *parents, const int32_t *children, const int32_t *lengths,
                    uint32_t count, void *stream);
 

@@ -8,6 +8,7 @@ namespace {
 using q38::abi_fail;
 
 constexpr uint32_t kMaxExtend = 1024;
+constexpr uint32_t kMaxFork = 65536;      /* every pair looks at all children */
 constexpr uint32_t kMaxGridYZ = 65535;
 
 bool power_of_two_in(uint32_t v, uint32_t low, uint32_t high) { return v >= low && v <= high && (v & (v - 1)) == 0; }
@@ -25,6 +26,8 @@ const char *cache_fault(const Q38KVPages *c)
         (uint64_t)c->table_entries * c->page_tokens > 0x7fffffffull ||
         (uint64_t)c->sequences * c->table_entries > 0xffffffffull)
         return "cache of more than 2^31 pages, sequences or tokens";
+    /* launches of a workgroup per 8 KiB of a page stay below 2^32 threads */
+    if (q38::kv_page_bytes(*c) * c->layers > 1ull << 36) return "a page of more than 2^36 bytes in all layers";
     if (reinterpret_cast<uintptr_t>(c->data) & 15) return "cache data must be 16-byte aligned";
     return nullptr;
 }
@@ -99,7 +102,8 @@ extern "C" int q38hip_kv_fork(const Q38KVPages *cache, const int32_t *parents, c
                               const int32_t *lengths, uint32_t count, void *stream)
 {
     if (const char *fault = cache_fault(cache)) return abi_fail(fault);
-    if (!parents || !children || !count || count > (1u << 24)) return abi_fail("bad fork arguments");
+    if (!parents || !children || !count) return abi_fail("bad fork arguments");
+    if (count > kMaxFork) return abi_fail("more than 65536 sequences in one fork");
     return q38::launch_kv_fork(*cache, parents, children, lengths, count, static_cast<hipStream_t>(stream))
                ? 1
                : abi_fail("cache fork kernel failed");

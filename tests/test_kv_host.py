@@ -30,7 +30,8 @@ def _cache(**change):
 BAD_CACHES = [dict(data=0), dict(status=0), dict(layers=0), dict(pages=0), dict(kv_heads=0), dict(sequences=0),
               dict(table_entries=0), dict(page_tokens=8), dict(page_tokens=48), dict(page_tokens=256), dict(head_dim=32),
               dict(head_dim=96), dict(head_dim=512), dict(type=2), dict(pages=0x80000000), dict(table_entries=0x10000000),
-              dict(kv_heads=40000), dict(layers=70000), dict(sequences=0x80000000)]
+              dict(kv_heads=40000), dict(layers=70000), dict(sequences=0x80000000),
+              dict(kv_heads=32767, layers=65535, page_tokens=128, head_dim=256)]
 
 
 @pytest.mark.parametrize("change", BAD_CACHES, ids=str)
@@ -74,6 +75,16 @@ def test_bad_arguments_are_refused():
     assert not lib.q38hip_kv_truncate(cache, p, None, 1, None)
     assert not lib.q38hip_kv_compact(cache, None, None)
     assert not lib.q38hip_kv_copy(cache, p, p, 0, None)
+
+
+def test_launches_that_a_grid_cannot_hold_are_refused():
+    lib, p = kv._lib(), 4096
+    assert not lib.q38hip_kv_fork(ctypes.byref(_cache()), p, p, None, 65537, None)
+    assert "65536" in q38hip.last_error()
+    page = dict(kv_heads=32767, page_tokens=128, head_dim=256)          # 2 GiB less 64 KiB
+    assert lib.q38hip_kv_workspace_bytes(ctypes.byref(_cache(layers=32, **page)))
+    assert not lib.q38hip_kv_workspace_bytes(ctypes.byref(_cache(layers=33, **page)))
+    assert "all layers" in q38hip.last_error()
 
 
 def test_python_checks():
