@@ -544,7 +544,7 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, CO
             kv_copy4(scales, kv_lds(meta));
             kv_copy4(scales + a.cache.kv_heads, kv_lds(meta + 64));
         };
-        auto copy_keys = [&](uint32_t at, uint32_t to, int first, int count) {
+        auto copy_keys = [&](uint32_t at, uint32_t to) {
 #pragma unroll
             for (int run = 0; run < kRuns; ++run) {
                 const uint32_t row = run * kRowsPerCopy + copy_row;            /* n */
@@ -553,7 +553,7 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, CO
                 const int32_t page = max(__shfl(pages, (int)(4 * turn + (row >> 2))), 0);
                 const uint8_t *from = a.cache.data + kv_block(a.cache, page, 0, head) * (T * D) + (token & (T - 1)) * D + chunk * 16;
 #pragma unroll 1
-                for (int i = first; i < first + count; ++i) kv_copy16(from + 4 * i * D, to + (kRuns * i + run) * 1024);
+                for (int i = 0; i < 4; ++i) kv_copy16(from + 4 * i * D, to + (kRuns * i + run) * 1024);
             }
         };
         /* where the lane's 16 bytes of value copy 0 of a step come from; copy c is 16 channels on */
@@ -562,10 +562,10 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, CO
             return a.cache.data + kv_block(a.cache, page, 1, head) * (T * D) + (lane >> 2) * T +
                    ((at * kKVStep + 16 * value_group) & (T - 1));
         };
-        auto copy_values = [&](uint32_t at, uint32_t to, int first, int count) {
-            const uint8_t *from = value_from(at) + first * 16 * T;
+        auto copy_values = [&](uint32_t at, uint32_t to) {
+            const uint8_t *from = value_from(at);
 #pragma unroll 4
-            for (int c = 0; c < count; ++c) kv_copy16(from + c * 16 * T, to + (first + c) * 1024);
+            for (int c = 0; c < kCopies; ++c) kv_copy16(from + c * 16 * T, to + c * 1024);
         };
 
         /* COLUMNS: the thread's part of a step, 16 codes at a time: to registers, and from there decoded to LDS */
@@ -713,8 +713,8 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, CO
                 for (int e = 0; e < (SPLIT ? 8 : 4); ++e) asm volatile("" ::"v"(raw[k][e]));
             load_pages(step);
             if (step < end) {
-                copy_keys(step, kv_lds(mine), 0, 4);
-                copy_values(step, kv_lds(mine) + 64 * D, 0, kCopies);
+                copy_keys(step, kv_lds(mine));
+                copy_values(step, kv_lds(mine) + 64 * D);
             }
             convert_queries(0, queries);
             kv_barrier();
@@ -816,7 +816,7 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, CO
                     kv_reads_done();
                     ++turn;
                     if (refresh) load_pages(step + kStride);
-                    copy_keys(step + kStride, kv_lds(mine), 0, 4);
+                    copy_keys(step + kStride, kv_lds(mine));
                 }
 
                 if (page < 0) key_scale = value_scale = 1.0f;
