@@ -119,6 +119,9 @@ __global__ __launch_bounds__(THREADS) void kv_join_kernel(KVAttention a)
             if (group < half) sums[threadIdx.x] = sum = sum + sums[threadIdx.x + half * quads];
         }
         if (!group) kv_finish4(a, column.row, column.head, d, sum, total, gate);
+        /* the last step's `sums` are read before the next column's are written (256-wide heads:
+         * the two groups of that step are two wavefronts) */
+        if (c + gridDim.z < r.columns) __syncthreads();
     }
 }
 

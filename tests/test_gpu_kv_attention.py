@@ -239,3 +239,18 @@ def test_maxima_that_rise(device, dim, rows, heads, dtype):
     got = cache.to(device).attention(0, q, kc.words([0], device), scale=1.0)
     want, mass, size = cache.attention(0, q.double().cpu().numpy(), [0], [0, rows], 1.0)
     _compare(got, want, mass, size, dtype, 500)
+
+
+@pytest.mark.parametrize("dtype,kind,lengths,rows", [(F32, "int8", [5000, 3000], [4, 1]),
+                                                     (BF16, "e4m3", [900 + 37 * i for i in range(24)], [1, 2, 1] * 8)])
+def test_more_columns_than_workgroups_that_join(device, dtype, kind, lengths, rows):
+    """ragged rows of 256-wide heads that are cut: a workgroup joins one column after another"""
+    rng = np.random.default_rng(len(lengths))
+    cache, starts, q, gate = _case(rng, 24, 4, 256, 64, kind, dtype, lengths, rows, device)
+    dev, ids, ends = cache.to(device), kc.words(range(len(lengths)), device), kc.words(starts, device)
+    first = dev.attention(0, q, ids, ends, gate=gate)
+    want, mass, size = cache.attention(0, q.double().cpu().numpy(), range(len(lengths)), starts, 256 ** -0.5,
+                                       gate.double().cpu().numpy())
+    _compare(first, want, mass, size, dtype, max(lengths))
+    for _ in range(20):
+        assert torch.equal(dev.attention(0, q, ids, ends, gate=gate), first)
