@@ -488,10 +488,11 @@ __device__ __forceinline__ uint32_t lds_address(const void *p)
  * 1 KiB is contiguous).  Issued from inline assembly so that the compiler's
  * wait-count pass does not treat it as an LDS store: it would otherwise drain
  * every outstanding copy before each later LDS read.  Callers place the
- * s_waitcnt themselves. */
+ * s_waitcnt themselves; the s_nop is the wait state that a load to LDS needs
+ * behind a scalar write of the M0 that it reads. */
 __device__ __forceinline__ void lds_dma16(const void *gaddr, uint32_t lds_base)
 {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off"
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
                  :: "v"(gaddr), "s"(lds_base) : "memory", "m0");
 }
 

@@ -331,15 +331,16 @@ __device__ __forceinline__ uint32_t dot4_lds_address(const void *p)
 
 /* 16 bytes per lane from gaddr to LDS at m0 + 16 * lane, or 4 bytes to
  * m0 + 4 * lane.  Inline assembly keeps the compiler's wait-count pass
- * from draining these copies before unrelated LDS accesses; callers wait. */
+ * from draining these copies before unrelated LDS accesses; callers wait.
+ * The s_nop is the wait state between the write of M0 and the load that reads it. */
 __device__ __forceinline__ void dot4_copy16(const void *gaddr, uint32_t m0)
 {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gaddr), "s"(m0) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gaddr), "s"(m0) : "memory", "m0");
 }
 
 __device__ __forceinline__ void dot4_copy4(const void *gaddr, uint32_t m0)
 {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(gaddr), "s"(m0) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(gaddr), "s"(m0) : "memory", "m0");
 }
 
 template <int N>

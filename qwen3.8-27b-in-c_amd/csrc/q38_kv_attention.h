@@ -414,14 +414,15 @@ __device__ __forceinline__ uint32_t kv_lds(const void *p)
     return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
 }
 /* 16 (4) bytes per lane to LDS at `to` + 16 (4) lane.  Inline assembly keeps
- * the compiler's wait counts out of it: callers wait. */
+ * the compiler's wait counts out of it: callers wait.  So is the wait state
+ * that a load to LDS needs behind a scalar write of the M0 that it reads. */
 __device__ __forceinline__ void kv_copy16(const void *from, uint32_t to)
 {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory", "m0");
 }
 __device__ __forceinline__ void kv_copy4(const void *from, uint32_t to)
 {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(to) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(to) : "memory", "m0");
 }
 template <int N>
 __device__ __forceinline__ void kv_wait()

@@ -70,15 +70,16 @@ __device__ __forceinline__ uint32_t lds_addr(const void *p)
  * bytes per lane, written by the load unit straight into LDS (lane i's bytes
  * land at dst + 16 i, dst + 1024 + 16 i and dst + 2048 + 4 i).  Inline
  * assembly, so the compiler's wait-count pass does not see LDS stores and
- * drain them before every LDS read; the caller waits with wait_vmcnt.  Out of
- * range bytes (past the resource) read as zero. */
+ * drain them before every LDS read; the caller waits with wait_vmcnt.  The
+ * s_nop is the wait state between the write of M0 and the load that reads it.
+ * Out of range bytes (past the resource) read as zero. */
 __device__ __forceinline__ void dma_tile_block(__amdgpu_buffer_rsrc_t rsrc, int soff, uint32_t dst, int lane)
 {
-    asm volatile("s_mov_b32 m0, %1\n\tbuffer_load_dwordx4 %0, %2, %3 offen lds"
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, %3 offen lds"
                  :: "v"(lane * 16), "s"(dst), "s"(rsrc), "s"(soff) : "memory", "m0");
-    asm volatile("s_mov_b32 m0, %1\n\tbuffer_load_dwordx4 %0, %2, %3 offen lds"
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, %3 offen lds"
                  :: "v"(1024 + lane * 16), "s"(dst + 1024), "s"(rsrc), "s"(soff) : "memory", "m0");
-    asm volatile("s_mov_b32 m0, %1\n\tbuffer_load_dword %0, %2, %3 offen lds"
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %0, %2, %3 offen lds"
                  :: "v"(2048 + lane * 4), "s"(dst + 2048), "s"(rsrc), "s"(soff) : "memory", "m0");
 }
 constexpr int kDmaOps = 3;   /* vector-memory operations per tile-block */

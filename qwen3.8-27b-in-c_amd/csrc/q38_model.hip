@@ -1013,7 +1013,8 @@ __device__ __forceinline__ void mix_barrier() { asm volatile("s_barrier" ::: "me
  * the end are never read).  Probability load: lane i takes position
  * 32c + i, at slot + 8192 + 4 i; that resource ends at position n.  Inline
  * assembly, so the compiler's wait-count pass does not treat the loads as
- * LDS stores. */
+ * LDS stores; the s_nop is the wait state between the write of M0 and the load
+ * that reads it. */
 __device__ __forceinline__ void mix_load_chunk(__amdgpu_buffer_rsrc_t vr, __amdgpu_buffer_rsrc_t pr,
                                                const uint32_t (&v_lane)[kMixVOps], uint32_t p_lane, int c, int last,
                                                uint32_t slot)
@@ -1021,9 +1022,9 @@ __device__ __forceinline__ void mix_load_chunk(__amdgpu_buffer_rsrc_t vr, __amdg
     const uint32_t chunk_off = (uint32_t)(c < last ? c : last) * (kMixChunk * 4);
 #pragma unroll
     for (int j = 0; j < kMixVOps; ++j)
-        asm volatile("s_mov_b32 m0, %1\n\tbuffer_load_dwordx4 %0, %2, %3 offen lds"
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, %3 offen lds"
                      :: "v"(v_lane[j]), "s"(slot + 1024 * j), "s"(vr), "s"(chunk_off) : "memory", "m0");
-    asm volatile("s_mov_b32 m0, %1\n\tbuffer_load_dword %0, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %0, %2, 0 offen lds"
                  :: "v"(p_lane + (uint32_t)c * (kMixChunk * 4)), "s"(slot + kMixChunk * 256), "s"(pr)
                  : "memory", "m0");
 }

@@ -2,7 +2,9 @@
 (csrc/q38_kv.h) compiled for the CPU: work slots of ragged batches, bad ids and
 pages, scale exponents."""
 import ctypes
+import glob
 import os
+import re
 import subprocess
 
 import numpy as np
@@ -310,3 +312,17 @@ def test_workspace_follows_the_workgroups():
     assert 0 < sizes[0] < sizes[1] and max(sizes) < 80e6 and sizes[3] - sizes[2] < 1e6
     short = ctypes.byref(_cache(kv_heads=4, head_dim=256, page_tokens=16, table_entries=8, pages=64))
     assert kv._lib().q38hip_kv_attention_workspace_bytes(short, 0, 24, 2, 2) == 0
+
+
+def test_loads_to_lds_wait_for_their_base():
+    """a load to LDS that reads M0 needs a wait state behind the scalar write of M0; the compiler adds none inside
+    inline assembly"""
+    found = 0
+    for path in glob.glob(os.path.join(ROOT, "qwen3.8-27b-in-c_amd", "csrc", "*.h*")):
+        for block in re.findall(r'asm volatile\(((?:\s*"(?:[^"\\]|\\.)*")+)', open(path).read()):
+            lines = [line.strip() for line in "".join(re.findall(r'"((?:[^"\\]|\\.)*)"', block)).replace("\\t", " ").split("\\n")]
+            for at, line in enumerate(lines):
+                if re.match(r"s_\w+ m0\b", line):
+                    found += 1
+                    assert lines[at + 1].startswith("s_nop"), (path, lines)
+    assert found
