@@ -293,7 +293,7 @@ enum {
     Q38_KV_TABLE_FULL = 4,     /* extend: longer than a table holds; nothing was done */
     Q38_KV_BAD_PAGE = 8,       /* a page outside the pool */
     Q38_KV_NOT_EMPTY = 16,     /* fork: the child holds tokens; that pair was left out */
-    Q38_KV_BAD_ROWS = 32       /* attention: row_starts that decrease; nothing was done */
+    Q38_KV_BAD_ROWS = 32       /* append, attention: row_starts that decrease; nothing was done */
 };
 typedef struct {
     uint8_t *data;

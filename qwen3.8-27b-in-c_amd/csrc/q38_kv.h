@@ -58,6 +58,26 @@ Q38_HD uint32_t kv_tokens(const Q38KVPages &cache, int32_t seq)
     return n <= 0 ? 0u : (uint32_t)n < most ? (uint32_t)n : most;
 }
 
+/* What slot `slot` holds of an append: with the rows begin .. end - 1 of a
+ * sequence of `tokens` tokens, whose slots (of pages) begin at `base`, tokens
+ * from .. to - 1 of its table entry `entry`; token t is row end - tokens +
+ * entry * T + t.  Rows before the sequence's first token are left out.  Where
+ * row offsets decrease, a sequence may be found for a slot before its own. */
+struct KVPageRows {
+    bool some;
+    uint32_t entry, from, to;
+};
+Q38_HD KVPageRows kv_page_rows(uint32_t begin, uint32_t end, uint32_t tokens, uint32_t slot, uint32_t base,
+                               uint32_t page_shift, uint32_t table_entries)
+{
+    if (end <= begin || !tokens || slot < base) return {false, 0, 0, 0};
+    const uint32_t T = 1u << page_shift, rows = end - begin < tokens ? end - begin : tokens, first = tokens - rows;
+    const uint32_t entry = (first >> page_shift) + (slot - base);
+    if (entry >= table_entries || entry * T >= tokens) return {false, 0, 0, 0};
+    const uint32_t at = entry * T;
+    return {true, entry, (first > at ? first : at) - at, (tokens - at < T ? tokens - at : T)};
+}
+
 /* page of table entry `entry` of sequence `seq` (< sequences), or -1 where the
  * entry lies outside the table or names no page of the pool */
 Q38_HD int32_t kv_page(const Q38KVPages &cache, uint32_t seq, uint32_t entry)

@@ -63,6 +63,15 @@ __device__ __forceinline__ KVFound find_sequence(const KVRows &rows, uint32_t sl
     return found;
 }
 
+/* row offsets that decrease, among those that the thread looks at */
+__device__ __forceinline__ bool rows_decrease(const KVRows &rows)
+{
+    bool bad = false;
+    if (rows.row_starts)
+        for (uint32_t i = threadIdx.x; i < rows.count; i += blockDim.x) bad |= kv_row_start(rows, i) > kv_row_start(rows, i + 1);
+    return bad;
+}
+
 /* four elements at any alignment of their own */
 template <int TYPE>
 struct Raw4 {
@@ -113,22 +122,23 @@ __global__ __launch_bounds__(kMostThreads) void kv_append_kernel(KVAppend a)
     __shared__ uint32_t wave_largest[kMostThreads / 64];
     const uint32_t T = a.cache.page_tokens, D = a.cache.head_dim, threads = blockDim.x;
     const uint32_t slot = blockIdx.x, half = blockIdx.y & 1, head = blockIdx.y >> 1;
+    /* the last slot is seldom any sequence's: a workgroup that has time to report bad offsets */
+    if (slot == gridDim.x - 1 && blockIdx.y == 0 && rows_decrease(a.rows)) atomicOr(a.cache.status, Q38_KV_BAD_ROWS);
     const KVFound at_rows = find_sequence(a.rows, slot, T);
     const uint32_t begin = at_rows.begin, end = at_rows.end;
     if (at_rows.index < 0 || end <= begin) return;
     const int32_t sequence = at_rows.sequence;
     const uint32_t tokens = kv_tokens(a.cache, sequence);
-    /* rows that lie before the sequence's first token are left out */
-    const uint32_t rows = min(end - begin, tokens), first = tokens - rows;
-    const uint32_t entry = (first >> a.page_shift) + (slot - kv_slot_base(begin, at_rows.index, 1, T, 2));
-    if (!rows || entry >= a.cache.table_entries || entry * T >= tokens) return;
+    /* the page's new tokens: from .. to - 1 */
+    const KVPageRows part = kv_page_rows(begin, end, tokens, slot, kv_slot_base(begin, at_rows.index, 1, T, 2), a.page_shift,
+                                         a.cache.table_entries);
+    if (!part.some) return;
+    const uint32_t entry = part.entry, from = part.from, to = part.to;
     const int32_t page = kv_page(a.cache, sequence, entry);
     if (page < 0) {
         if (threadIdx.x == 0) atomicOr(a.cache.status, Q38_KV_BAD_PAGE);
         return;
     }
-    /* the page's new tokens: from .. to - 1 */
-    const uint32_t from = max(first, entry * T) - entry * T, to = min(tokens, entry * T + T) - entry * T;
     const void *source = half ? a.value : a.key;
     /* element of the page's token 0 (which may lie before the rows), channel 0 */
     const uint64_t origin = ((uint64_t)end - tokens + entry * T) * a.row_stride + (uint64_t)head * D;
@@ -144,6 +154,7 @@ __global__ __launch_bounds__(kMostThreads) void kv_append_kernel(KVAppend a)
         /* a token that is not new stands in for none: the nearest that is */
         raw[k].load(source, origin + min(max(t, from), to - 1) * a.row_stride + (item & (D / 4 - 1)) * 4);
     }
+    const bool decrease = rows_decrease(a.rows);       /* here: under way with the rows */
     float x[kQuads][4];
     uint32_t largest = 0;
 #pragma unroll
@@ -153,9 +164,11 @@ __global__ __launch_bounds__(kMostThreads) void kv_append_kernel(KVAppend a)
             largest = max(largest, __float_as_uint(x[k][e]) & 0x7fffffffu);
         }
     for (int by = 1; by < 64; by *= 2) largest = max(largest, (uint32_t)__shfl_xor((int)largest, by));
+    if (__any(decrease)) largest = 0xffffffffu;       /* above all values: the call does nothing */
     if ((threadIdx.x & 63) == 0) wave_largest[threadIdx.x >> 6] = largest;
     __syncthreads();                                   /* also: every thread has read the old scale */
     for (uint32_t w = 0; w < threads / 64; ++w) largest = max(largest, wave_largest[w]);
+    if (largest == 0xffffffffu) return;
 
     const bool finite = largest < 0x7f800000u;
     float scale = finite ? __uint_as_float((uint32_t)(kv_scale_exponent(largest, E4M3) + 127) << 23) : NAN;

@@ -134,6 +134,24 @@ def test_append_outside_the_cache(device):
     assert int(dev.status) == kv.BAD_PAGE
 
 
+@pytest.mark.parametrize("count", [5, 150])
+def test_append_row_offsets_that_decrease(device, count):
+    """nothing is written, and the status says so"""
+    from q38hip import kv
+    rng = np.random.default_rng(7)
+    cache = kc.filled(rng, [600] * count, "int8", 16, 1, 64, garbage=False)
+    dev = cache.to(device)
+    x = _rows(rng, 1300, 1, 64, F32, device, 1000.0)
+    up = [1250 + i % 3 for i in range(count - 5)]
+    for starts in ([0, 1000, 1200, 10, 1300] + sorted(up) + [1300], [1300, 0] * (count // 2) + [1300] * (1 + count % 2),
+                   [0, -5] + [40] * (count - 2) + [39]):
+        assert len(starts) == count + 1
+        dev.append(0, x, x, kc.words(range(count), device), kc.words(starts, device))
+        assert int(dev.status) == kv.BAD_ROWS
+        dev.status.zero_()
+        cache.same(dev)
+
+
 # ---- pages ---------------------------------------------------------------------
 
 

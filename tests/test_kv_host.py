@@ -148,6 +148,38 @@ int main()
         CHECK(kv_slot_base(total, count, per_row, unit, 1) <= kv_slots(total, count, per_row, unit, 1));
         CHECK(kv_slot_base(total, count, 1, T, 2) <= kv_slots(total, count, 1, T, 2));
     }
+    /* a slot of an append holds each of a sequence's pages once, and with offsets that decrease it still
+     * stays within a page and within its sequence's rows */
+    for (int trial = 0; trial < 20000; ++trial) {
+        const uint32_t count = 1 + draw(12), shift = 4 + draw(4), T = 1u << shift, entries = 1 + draw(200);
+        const bool rising = trial % 2;
+        std::vector<int32_t> starts(1, rising ? 0 : draw(100)), ids(count, 0);
+        std::vector<uint32_t> tokens;
+        for (uint32_t i = 0; i < count; ++i) {
+            starts.push_back(rising ? starts.back() + draw(200) : draw(2) ? draw(4000) : starts.back() + draw(300));
+            tokens.push_back(draw(4) ? draw(entries * T + 1) : draw(3));
+        }
+        const uint32_t total = rising ? starts.back() : 4000;
+        if (!total) continue;
+        const KVRows rows{ids.data(), starts.data(), count, total, 0};
+        std::vector<uint32_t> written(count, 0);
+        for (uint32_t slot = 0; slot < kv_slots(total, count, 1, T, 2); ++slot) {
+            uint32_t before = 0;           /* as many bases as lie at or before the slot: the sequence, if they rise */
+            for (uint32_t i = 0; i < count; ++i) before += kv_slot_base(kv_row_start(rows, i), i, 1, T, 2) <= slot;
+            if (!before) continue;
+            const uint32_t i = before - 1, b = kv_row_start(rows, i), e = kv_row_start(rows, i + 1);
+            const KVPageRows p = kv_page_rows(b, e, tokens[i], slot, kv_slot_base(b, i, 1, T, 2), shift, entries);
+            if (!p.some) continue;
+            CHECK(p.entry < entries && p.from < p.to && p.to <= T && p.entry * T + p.to <= tokens[i]);
+            const uint32_t row = e - tokens[i] + p.entry * T;
+            CHECK((int32_t)(row + p.from) >= (int32_t)b && row + p.to <= e);
+            written[i] += p.to - p.from;
+        }
+        for (uint32_t i = 0; rising && i < count; ++i) {
+            const uint32_t n = starts[i + 1] - starts[i];
+            CHECK(written[i] == (n < tokens[i] ? n : tokens[i]));
+        }
+    }
     /* offsets that are not: never past the rows */
     int32_t odd[4] = {-7, 3, 1 << 30, 2}, id = 0;
     const KVRows rows{&id, odd, 3, 10, 3};
