@@ -221,17 +221,21 @@ __device__ __forceinline__ void kv_store4(void *base, uint64_t at, const KVAtten
     }
 }
 
-/* 1 / (1 + e^-x) within 2^-22 of itself: x log2(e) in two parts, so the error
- * does not grow with x */
+/* 1 / (1 + e^-x) within 2^-21 of itself, or, where it is subnormal, 2^-149.
+ * With E = e^-|x| it is 1 / (1 + E), for negative x E / (1 + E): nothing
+ * overflows.  E = 2^(n + f), n whole, with log2(e) in two parts, so f's error
+ * does not grow with x; E is 0 in fp32 from |x| = 104 on, so x ends at 128 (a NaN
+ * stays one). */
 __device__ __forceinline__ float kv_sigmoid(float x)
 {
     constexpr float kHigh = 1.44269502f, kLow = 1.92596299e-8f;
-    float t = -x * kHigh;
-    const float rest = fmaf(-x, kHigh, -t) - x * kLow;
-    if (t > 126.0f) t = 126.0f;
-    const float e = __builtin_amdgcn_exp2f(t), d = 1.0f + fmaf(e, rest * 0.693147182f, e);
-    const float inverse = __builtin_amdgcn_rcpf(d);
-    return fmaf(inverse, fmaf(-d, inverse, 1.0f), inverse);
+    float a = fabsf(x);
+    if (a > 128.0f) a = 128.0f;
+    const float n = __builtin_rintf(-a * kHigh);
+    const float f = fmaf(-a, kLow, fmaf(-a, kHigh, -n));
+    const float e = ldexpf(__builtin_amdgcn_exp2f(f), (int)n), d = 1.0f + e;
+    const float first = __builtin_amdgcn_rcpf(d), inverse = fmaf(first, fmaf(-d, first, 1.0f), first);
+    return x < 0.0f ? e * inverse : inverse;
 }
 
 __device__ __forceinline__ kv_float4 kv_gate4(const KVAttention &a, uint32_t row, uint32_t head, uint32_t d)

@@ -254,3 +254,28 @@ def test_more_columns_than_workgroups_that_join(device, dtype, kind, lengths, ro
     _compare(first, want, mass, size, dtype, max(lengths))
     for _ in range(20):
         assert torch.equal(dev.attention(0, q, ids, ends, gate=gate), first)
+
+
+GATES = [0.0, 20.0, -20.0, 87.0, -87.0, 90.0, -90.0, 100.0, -100.0, 104.0, -104.0, 1e4, -1e4, 5e4, -5e4, 1e9, -1e9, 1e30, -1e30, 3e38,
+         -3e38, float("inf"), float("-inf"), float("nan")]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dim,heads,length,rows", [(256, 6, 20, 1), (128, 4, 6000, 2), (256, 6, 2000, 40)])
+def test_gates_of_all_sizes(device, dtype, dim, heads, length, rows):
+    """whole slots, cut ones and prompts; sigmoids that are subnormal in fp32 keep the bits that those have"""
+    rng = np.random.default_rng(dim + rows)
+    cache, starts, q, _ = _case(rng, heads, 1, dim, 64, "int8", dtype, [length], [rows], device)
+    at = torch.arange(rows)[:, None, None] + torch.arange(heads)[:, None] + torch.arange(dim)
+    gate = torch.tensor(GATES, dtype=torch.float64)[at % len(GATES)].to(dtype)
+    got = cache.to(device).attention(0, q, kc.words([0], device), gate=gate.to(device)).double().cpu().numpy()
+    with np.errstate(over="ignore"):
+        want, mass, size = cache.attention(0, q.double().cpu().numpy(), [0], starts, dim ** -0.5, gate.double().numpy())
+    number = ~np.isnan(gate.double().numpy())
+    assert np.array_equal(np.isnan(got), ~number)
+    # the smallest steps: of the sigmoid (times the sum's size), and of the output
+    value = cache.attention(0, q.double().cpu().numpy(), [0], starts, dim ** -0.5)[0]
+    least = {F32: 2.0 ** -150, BF16: 2.0 ** -134, F16: 0.0}[dtype]
+    bound = kc.tolerance(want, mass, size, dtype, length) - (1e-30 if dtype != F16 else 0) + 2.0 ** -149 * (1 + np.abs(value)) + least
+    far = np.abs(got - want)[number] / bound[number]
+    assert far.max() <= 1, "worst %g of its bound" % far.max()
