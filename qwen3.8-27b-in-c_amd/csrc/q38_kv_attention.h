@@ -134,20 +134,22 @@ __device__ __forceinline__ kv_half8 kv_decode8(uint32_t lo, uint32_t hi)
  * the compiler give the result other registers, and it moved all sums about once
  * a step.  What it cannot see it cannot guard, so the wait states are here: two
  * between a vector instruction that writes A or B, or the product that wrote the
- * sums, and this one. */
-__device__ __forceinline__ void kv_accumulate(kv_float4 &sums, kv_half8 a, kv_half8 b)
+ * sums, and this one; eight behind the last one of a step, before anything else
+ * may touch its sums.  (A product takes three with its own, so those before it
+ * are done by then.)  The compiler may copy the sums anywhere behind it. */
+__device__ __forceinline__ void kv_accumulate(kv_float4 &sums, kv_half8 a, kv_half8 b, bool last)
 {
-    asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(sums) : "v"(a), "v"(b));
+    if (last) asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_f16 %0, %1, %2, %0\n\ts_nop 7" : "+a"(sums) : "v"(a), "v"(b));
+    else asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(sums) : "v"(a), "v"(b));
 }
 
 /* Sums in accumulation registers times keep, by way of 16 bytes of LDS per
  * lane: vector instructions take no accumulation registers, and four of them
- * have no names of their own here.  Seldom done.  The 20 wait states cover a
- * product that may still write the sums. */
+ * have no names of their own here.  Seldom done, and no product is under way. */
 __device__ __forceinline__ void kv_scale(kv_float4 &sums, float keep, uint32_t lane_lds)
 {
     float a, b, c, d;
-    asm volatile("s_nop 15\n\ts_nop 3\n\tds_write_b128 %6, %0\n\t"
+    asm volatile("ds_write_b128 %6, %0\n\t"
                  "ds_read_b32 %1, %6\n\tds_read_b32 %2, %6 offset:4\n\tds_read_b32 %3, %6 offset:8\n\tds_read_b32 %4, %6 offset:12\n\t"
                  "s_waitcnt lgkmcnt(0)\n\tv_mul_f32 %1, %1, %5\n\tv_mul_f32 %2, %2, %5\n\tv_mul_f32 %3, %3, %5\n\tv_mul_f32 %4, %4, %5\n\t"
                  "ds_write_b32 %6, %1\n\tds_write_b32 %6, %2 offset:4\n\tds_write_b32 %6, %3 offset:8\n\tds_write_b32 %6, %4 offset:12\n\t"
@@ -738,8 +740,8 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, CO
             for (int c = 0; c < kChannels; ++c) o[t][c] = {0.0f, 0.0f, 0.0f, 0.0f};
         }
 
-        auto accumulate = [](kv_float4 &sums, kv_half8 x, kv_half8 y) {
-            if constexpr (kAccumulators) kv_accumulate(sums, x, y);
+        auto accumulate = [](kv_float4 &sums, kv_half8 x, kv_half8 y, bool last) {
+            if constexpr (kAccumulators) kv_accumulate(sums, x, y, last);
             else sums = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, sums, 0, 0, 0);
         };
 
@@ -940,7 +942,7 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, CO
                         if (f + kAhead < kFragments) fragment[(f + kAhead) % (kAhead + 1)] = read(f + kAhead);
 #pragma unroll
                         for (int t = 0; t < NT; ++t)
-                            accumulate(o[t][tile_of(f)], fragment[f % (kAhead + 1)], weight[t][f / 4 % 2]);
+                            accumulate(o[t][tile_of(f)], fragment[f % (kAhead + 1)], weight[t][f / 4 % 2], false);
                         /* the next step's codes, in the products' shadow (what is there without one goes unread) */
                         constexpr int kEvery = kFragments / (4 * kPieces);
                         if (f % kEvery == kEvery - 1) write_codes(f / kEvery / 2, f / kEvery % 2, next_tile);
@@ -964,14 +966,14 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, CO
                         const kv_half8 v0 = kv_decode8<E4M3>(v.x, v.y), w0 = kv_decode8<E4M3>(w.x, w.y);
 #pragma unroll
                         for (int t = 0; t < NT; ++t) {
-                            accumulate(o[t][c], v0, weight[t][0]);
-                            accumulate(o[t][c + 1], w0, weight[t][0]);
+                            accumulate(o[t][c], v0, weight[t][0], false);
+                            accumulate(o[t][c + 1], w0, weight[t][0], false);
                         }
                         const kv_half8 v1 = kv_decode8<E4M3>(v.z, v.w), w1 = kv_decode8<E4M3>(w.z, w.w);
 #pragma unroll
                         for (int t = 0; t < NT; ++t) {
-                            accumulate(o[t][c], v1, weight[t][1]);
-                            accumulate(o[t][c + 1], w1, weight[t][1]);
+                            accumulate(o[t][c], v1, weight[t][1], false);
+                            accumulate(o[t][c + 1], w1, weight[t][1], c + 2 == kChannels && t == NT - 1);
                         }
                         if (!COLUMNS && more && c % 4 == 2) {
                             __builtin_amdgcn_sched_barrier(0);
@@ -991,13 +993,6 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, CO
         }
 
         kv_wait<0>();                               /* nothing is on its way to LDS */
-        if (kAccumulators) {
-            asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int c = 0; c < kChannels; ++c) asm volatile("" : "+a"(o[t][c]));    /* read after the products, not before */
-        }
 
         const uint32_t index = kv_place(blockIdx.x, piece.first_piece);
         float *partial = kv_partial(a, index, head), *stats = kv_stats(a, index, head);

@@ -358,3 +358,67 @@ def test_loads_to_lds_wait_for_their_base():
                     found += 1
                     assert lines[at + 1].startswith("s_nop"), (path, lines)
     assert found
+
+
+def _assembly(tmp_path, name):
+    """the device assembly of one of csrc's files, with the flags that it is built with"""
+    package = os.path.join(ROOT, "qwen3.8-27b-in-c_amd")
+    lines = subprocess.run(["make", "-n", "-B", "-C", package], capture_output=True, text=True, check=True).stdout.splitlines()
+    command = next(line for line in lines if line.endswith("/" + name + ".o") and " -c " in line).split()
+    command[command.index("-c")] = "-S"
+    command[command.index("-o") + 1] = str(tmp_path / (name + ".s"))
+    subprocess.run(command + ["--offload-device-only"], check=True, capture_output=True)
+    return (tmp_path / (name + ".s")).read_text()
+
+
+def _registers(text):
+    found = set()
+    for kind, first, last, single, number in re.findall(r"\b([va])\[(\d+):(\d+)\]|\b([va])(\d+)\b", text):
+        found |= {(kind, n) for n in range(int(first), int(last) + 1)} if kind else {(single, int(number))}
+    return found
+
+
+def _touched_too_soon(body, states):
+    """vector instructions that touch the registers of a product in inline assembly, which the compiler does not see,
+    fewer than `states` wait states behind it, over all branches; and the number of such products"""
+    code, labels, inside = [], {}, False
+    for line in body.split("\n"):
+        inside = "#ASMSTART" in line or inside and "#ASMEND" not in line
+        text = line.split(";")[0].strip()
+        if text.endswith(":"):
+            labels[text[:-1]] = len(code)
+        elif text and not text.startswith("."):
+            code.append((text, inside))
+    products = [at for at, (text, own) in enumerate(code) if own and text.startswith("v_mfma")]
+    bad = []
+    for product in products:
+        written, ways, known = _registers(code[product][0].split(",")[0]), [(product + 1, 0)], set()
+        while ways:
+            at, waited = ways.pop()
+            while at < len(code) and waited < states and (at, waited) not in known:
+                known.add((at, waited))
+                text, own = code[at]
+                what = text.split()[0]
+                if what == "s_nop":
+                    waited += int(text.split()[1])
+                if what.startswith(("v_", "ds_", "global_", "scratch_")) and not (own and what.startswith("v_mfma")) and \
+                        _registers(text) & written:
+                    bad.append((code[product][0], text, waited))
+                    break
+                if what.startswith("s_cbranch"):
+                    ways.append((labels[text.split()[1]], waited + 1))
+                at, waited = labels[text.split()[1]] if what == "s_branch" else at + 1, waited + 1
+    return bad, len(products)
+
+
+def test_sums_are_left_alone_until_they_are_written(tmp_path):
+    """256-wide attention multiplies into accumulation registers by inline assembly: whatever the compiler does with
+    them comes eight wait states behind the product, as it does behind the compiler's own"""
+    text = _assembly(tmp_path, "q38_kv_attention256")
+    kernels = re.findall(r"^(_ZN3q38\w*kv_attention_kernel\w*):(.*?)^\.Lfunc_end", text, re.S | re.M)
+    products = 0
+    for name, body in kernels:
+        bad, count = _touched_too_soon(body, 8)
+        assert not bad, (name, bad[:3])
+        products += count
+    assert len(kernels) == 16 and products
