@@ -285,7 +285,9 @@ int q38hip_attention_rows(float *attention, Q38Q8KBlock *attention_q8k, const fl
  * page_tokens is 16, 32, 64 or 128, head_dim 64, 128 or 256, table_entries *
  * page_tokens below 2^31.  A page serves all layers.  All ids are 32-bit words
  * in device memory.  Ids and pages outside the cache are never followed: they
- * set a status bit, and what they stand for holds no tokens. */
+ * set a status bit, and what they stand for holds no tokens.  (Append alone
+ * leaves the rows of a bad id out without a bit: the extend call before it and
+ * the attention call behind it report the id.) */
 enum { Q38_KV_INT8 = 0, Q38_KV_E4M3 = 1 };
 enum {
     Q38_KV_BAD_SEQUENCE = 1,   /* an id outside the cache, or twice in one call */

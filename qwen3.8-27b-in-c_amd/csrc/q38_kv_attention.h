@@ -285,7 +285,7 @@ struct KVLanes {
     uint32_t begin, end, slots, each;            /* the lane's; units of each slot */
     int32_t id, tokens;
     uint32_t slots_upto, units_upto;             /* inclusive, within the block */
-    bool good;                                   /* the block's row offsets do not decrease */
+    uint32_t trouble;                            /* Q38_KV_*: row offsets that decrease, bad ids that own rows */
 
     __device__ __forceinline__ void load(const KVAttention &a, uint32_t at)
     {
@@ -302,7 +302,8 @@ struct KVLanes {
             slots = ((end - begin) * a.group + COLUMNS - 1) / COLUMNS;
             each = kv_slot_units(kv_steps((uint32_t)tokens), a.shift);
         }
-        good = __all(begin <= end);
+        trouble = (__any(begin > end) ? Q38_KV_BAD_ROWS : 0) |
+                  (__any(begin < end && (uint32_t)id >= a.cache.sequences) ? Q38_KV_BAD_SEQUENCE : 0);
         slots_upto = slots;
         units_upto = slots * each;
         if (a.rows.count == 1) {
@@ -334,18 +335,18 @@ struct KVWalk {
     __device__ __forceinline__ void start(const KVAttention &a, uint32_t workgroup)
     {
         total_slots = total_units = block_slots = block_units = 0;
-        bool good = true;
+        uint32_t trouble = 0;
         for (uint32_t first = (a.rows.count - 1) / 64 * 64 + 64; first; ) {
             first -= 64;
             block.load(a, first);
             total_slots += Lanes::of(block.slots_upto, 63);
             total_units += Lanes::of(block.units_upto, 63);
-            good = good && block.good;
+            trouble |= block.trouble;
         }
-        if (!good) {
-            /* the sums mean nothing, and the workspace need not hold the slots */
-            if (threadIdx.x == 0) atomicOr(a.cache.status, Q38_KV_BAD_ROWS);
-            total_slots = total_units = 0;
+        if (trouble) {
+            if (threadIdx.x == 0) atomicOr(a.cache.status, (int32_t)trouble);
+            /* with bad offsets the sums mean nothing, and the workspace need not hold the slots */
+            if (trouble & Q38_KV_BAD_ROWS) total_slots = total_units = 0;
         }
         chunk = kv_chunk(total_units, a.workgroups, a.workgroups_inverse, a.least);
         small = kv_small(chunk);
@@ -544,8 +545,11 @@ __global__ __launch_bounds__(64 * kv_workgroup_waves(D, COLUMNS), kv_waves(D, CO
         auto load_pages = [&](uint32_t first) {
             const uint32_t at = first + (lane >> 2) * kStride, token = at * kKVStep + 16 * (lane & 3);
             pages = -1;
-            if (at < end && s.sequence >= 0 && token < (uint32_t)s.seen)
+            if (at < end && s.sequence >= 0 && token < (uint32_t)s.seen) {
                 pages = kv_page(a.cache, s.sequence, token >> a.page_shift);
+                /* (anywhere in the loop or before it this costs four rows at 131k tokens 3 us of 68) */
+                if (pages < 0) atomicOr(a.cache.status, Q38_KV_BAD_PAGE);
+            }
             turn = 0;
             const float *scales = a.cache.scales + kv_block(a.cache, max(pages, 0), 0, head);
             kv_copy4(scales, kv_lds(meta));

@@ -279,3 +279,26 @@ def test_gates_of_all_sizes(device, dtype, dim, heads, length, rows):
     bound = kc.tolerance(want, mass, size, dtype, length) - (1e-30 if dtype != F16 else 0) + 2.0 ** -149 * (1 + np.abs(value)) + least
     far = np.abs(got - want)[number] / bound[number]
     assert far.max() <= 1, "worst %g of its bound" % far.max()
+
+
+def test_status_of_ids_and_pages(device):
+    """bad ids that own rows, and bad pages that a row sees, are reported"""
+    from q38hip import kv
+    rng = np.random.default_rng(12)
+    cache = kc.filled(rng, [48, 48, 700], "int8", 16, 1, 64)
+    q = torch.from_numpy(rng.normal(size=(40, 2, 64))).float().to(device)
+    for rows in (1, 40):
+        for bad in (99, -1, 5):
+            dev = cache.to(device)
+            dev.attention(0, q[:rows], kc.words([0, bad, 2], device), kc.words([0, 0, 0, rows], device))
+            assert int(dev.status) == 0                     # an id without rows
+            dev.attention(0, q[:rows], kc.words([0, 2, bad], device), kc.words([0, 0, 0, rows], device))
+            assert int(dev.status) == kv.BAD_SEQUENCE
+        for sequence, entry, page in ((1, 0, -1), (1, 2, 1 << 20), (2, 43, -7)):
+            dev = cache.to(device)
+            dev.tables[0, 3] = 1 << 20                      # behind the sequence's tokens
+            dev.attention(0, q[:rows], kc.words([0], device))
+            assert int(dev.status) == 0
+            dev.tables[sequence, entry] = page
+            dev.attention(0, q[:rows], kc.words([sequence], device))
+            assert int(dev.status) == kv.BAD_PAGE
