@@ -235,7 +235,7 @@ __global__ __launch_bounds__(256) void kv_fork_kernel(Q38KVPages c, const int32_
     }
     const uint32_t held = kv_tokens(c, parent);
     const uint32_t tokens = lengths ? (uint32_t)min((int64_t)held, max((int64_t)0, (int64_t)lengths[blockIdx.x])) : held;
-    if (!tokens) return;
+    /* (for no tokens too: the child must be empty then as well) */
     if (threadIdx.x == 0) taken = atomicCAS(&c.lengths[child], 0, (int32_t)tokens) != 0;
     __syncthreads();
     if (taken) {

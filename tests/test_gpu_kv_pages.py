@@ -272,6 +272,25 @@ def test_status_bits(device):
     cache.same(dev)
 
 
+def test_fork_of_nothing(device):
+    """a child that holds tokens is reported and left as it is where there is nothing to take, too"""
+    from q38hip import kv
+    cache = kc.Cache(1, 6, 16, 1, 64, 4, 3, "int8")
+    dev = cache.to(device)
+    w = lambda *v: kc.words(v, device)  # noqa: E731
+    assert cache.extend([0, 1], [30, 16])
+    dev.extend(w(0, 1), w(30, 16))
+    for call, bits in ((lambda: dev.fork(w(2), w(3)), 0),                          # an empty parent, an empty child
+                       (lambda: dev.fork(w(0), w(2), w(0)), 0),
+                       (lambda: dev.fork(w(2), w(0)), kv.NOT_EMPTY),
+                       (lambda: dev.fork(w(0), w(1), w(0)), kv.NOT_EMPTY),
+                       (lambda: dev.fork(w(0), w(1), w(-9)), kv.NOT_EMPTY)):
+        call()
+        assert int(dev.status) == bits
+        dev.status.zero_()
+        cache.same(dev)
+
+
 def test_copy_and_reset(device):
     cache = kc.Cache(2, 8, 32, 2, 128, 3, 2, "e4m3")
     _noise(np.random.default_rng(2), cache)
