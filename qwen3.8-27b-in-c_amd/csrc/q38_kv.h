@@ -49,6 +49,17 @@ Q38_HD uint64_t kv_slots(uint64_t total_rows, uint64_t count, uint64_t per_row, 
     return total_rows * per_row / unit + gap * count;
 }
 
+/* a launch has fewer than 2^32 threads along each direction of its grid */
+inline bool kv_launch_holds(uint64_t workgroups, uint32_t threads) { return workgroups * threads <= 0xffffffffull; }
+
+/* of an append: threads of a workgroup (a page is T D / 4 quads, eight a thread; a
+ * smaller page leaves threads of its one wavefront idle) */
+inline uint32_t kv_append_threads(const Q38KVPages &cache)
+{
+    const uint32_t threads = cache.page_tokens * cache.head_dim / 32;
+    return threads < 64 ? 64 : threads;
+}
+
 /* tokens of sequence `seq` that the table can hold; 0 for an id outside the cache */
 Q38_HD uint32_t kv_tokens(const Q38KVPages &cache, int32_t seq)
 {
@@ -119,7 +130,8 @@ struct KVAttention {
     uint64_t query_row, query_head, output_row;
     uint32_t group, group_magic, page_shift;
     float workgroups_inverse;
-    uint32_t columns, slots;               /* columns of a slot, at most that many slots */
+    uint32_t columns;                      /* of a slot */
+    uint32_t slots;                        /* at most that many */
     uint32_t workgroups, shift, least;     /* per key/value head; steps of a unit (log2); units of a workgroup at least */
     bool cut;                              /* slots may be, and what is cut is joined */
     int type;

@@ -24,8 +24,8 @@ const char *cache_fault(const Q38KVPages *c)
     if (c->layers > kMaxGridYZ || c->kv_heads > kMaxGridYZ / 2) return "too many layers or heads";
     if (c->pages > 0x7fffffffu - (1u << 14) || c->sequences > 0x7fffffffu ||
         (uint64_t)c->table_entries * c->page_tokens > 0x7fffffffull ||
-        (uint64_t)c->sequences * c->table_entries > 0xffffffffull)
-        return "cache of more than 2^31 pages, sequences or tokens";
+        !q38::kv_launch_holds(((uint64_t)c->sequences * c->table_entries + 255) / 256, 256))
+        return "cache of more than 2^31 pages, sequences or tokens, or 2^32 - 256 table entries";
     /* launches of a workgroup per 8 KiB of a page stay below 2^32 threads */
     if (q38::kv_page_bytes(*c) * c->layers > 1ull << 36) return "a page of more than 2^36 bytes in all layers";
     if (reinterpret_cast<uintptr_t>(c->data) & 15) return "cache data must be 16-byte aligned";
@@ -66,6 +66,8 @@ const char *plan_attention(const Q38KVPages *cache, uint32_t type, uint32_t head
     a.group = heads / cache->kv_heads;
     if (a.group > 32768) return "more than 32768 query heads to a key/value head";
     bytes = q38::plan_kv_attention(a);
+    /* the join of slots that may be cut: 256 threads for each (1024 where they are few) */
+    if (a.cut && !q38::kv_launch_holds(a.slots, 256)) return "more rows or sequences than a launch of attention's join holds";
     return nullptr;
 }
 
@@ -113,7 +115,8 @@ extern "C" int q38hip_kv_truncate(const Q38KVPages *cache, const int32_t *sequen
                                   uint32_t count, void *stream)
 {
     if (const char *fault = cache_fault(cache)) return abi_fail(fault);
-    if (!sequences || !lengths || !count || count > (1u << 24)) return abi_fail("bad truncate arguments");
+    if (!sequences || !lengths || !count) return abi_fail("bad truncate arguments");
+    if (!q38::kv_launch_holds(count, 256)) return abi_fail("more than 2^24 - 1 sequences in one truncation");
     return q38::launch_kv_truncate(*cache, sequences, lengths, count, static_cast<hipStream_t>(stream))
                ? 1
                : abi_fail("cache truncate kernel failed");
@@ -148,6 +151,8 @@ extern "C" int q38hip_kv_append(const Q38KVPages *cache, uint32_t layer, const v
     if (!element_type(type)) return abi_fail("rows must be F32, F16 or BF16");
     if (layer >= cache->layers) return abi_fail("layer beyond the cache");
     if (total_rows > 1 && row_stride < (uint64_t)cache->kv_heads * cache->head_dim) return abi_fail("row stride too small");
+    if (!q38::kv_launch_holds(q38::kv_slots(total_rows, count, 1, cache->page_tokens, 2), q38::kv_append_threads(*cache)))
+        return abi_fail("more rows or sequences than a launch of append holds");
     return q38::launch_kv_append(*cache, layer, key, value, (int)type, row_stride,
                                  rows_of(sequences, row_starts, count, total_rows), static_cast<hipStream_t>(stream))
                ? 1

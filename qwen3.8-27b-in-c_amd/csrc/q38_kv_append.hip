@@ -229,10 +229,9 @@ bool launch_typed(const KVAppend &a, uint32_t slots, hipStream_t stream)
     KVAppend call = a;
     void *arguments[] = {&call};
     const uint32_t lds = a.cache.head_dim * (a.cache.page_tokens + 4);
-    /* a page is T D / 4 quads, eight a thread; a smaller page leaves threads of its one wavefront idle */
-    const uint32_t threads = a.cache.page_tokens * a.cache.head_dim / (4 * kQuads);
+    static_assert(kQuads == 8, "kv_append_threads");
     return hipLaunchKernel(reinterpret_cast<const void *>(kv_append_kernel<E4M3, TYPE>),
-                           dim3(slots, 2 * a.cache.kv_heads), dim3(threads < 64 ? 64 : threads), arguments, lds, stream) == hipSuccess;
+                           dim3(slots, 2 * a.cache.kv_heads), dim3(kv_append_threads(a.cache)), arguments, lds, stream) == hipSuccess;
 }
 template <bool E4M3>
 bool launch_kind(const KVAppend &a, int type, uint32_t slots, hipStream_t stream)

@@ -422,3 +422,31 @@ def test_sums_are_left_alone_until_they_are_written(tmp_path):
         assert not bad, (name, bad[:3])
         products += count
     assert len(kernels) == 16 and products
+
+
+def test_calls_of_more_threads_than_a_launch_are_refused():
+    """2^32 threads or more along the grid: refused on the host, before anything is enqueued"""
+    lib, p = kv._lib(), 4096
+
+    def refused(ok, *words):
+        assert not ok and "failed" not in q38hip.last_error(), q38hip.last_error()
+        for word in words:
+            assert word in q38hip.last_error(), q38hip.last_error()
+
+    # append: rows / page_tokens + 2 sequences workgroups of page_tokens * head_dim / 32 threads
+    wide = ctypes.byref(_cache(page_tokens=128, head_dim=256, kv_heads=1))
+    refused(lib.q38hip_kv_append(wide, 0, p, p, 0, 256, p, p, 1 << 21, 1 << 21, None), "append", "sequences")
+    refused(lib.q38hip_kv_append(wide, 0, p, p, 0, 256, p, p, 1 << 24, 1 << 24, None), "append", "sequences")
+    refused(lib.q38hip_kv_append(ctypes.byref(_cache(kv_heads=1, page_tokens=128)), 0, p, p, 0, 64, p, None, 1 << 24, 1 << 24, None),
+            "append", "sequences")
+    refused(lib.q38hip_kv_truncate(ctypes.byref(_cache()), p, p, 1 << 24, None), "2^24")
+    # attention: the join of slots that may be cut has a workgroup of 256 threads for each of them
+    long = ctypes.byref(_cache(kv_heads=1, table_entries=1 << 16))
+    for count, total in ((1 << 24, 1 << 24), ((1 << 24) - 1, 1 << 24)):
+        refused(lib.q38hip_kv_attention_workspace_bytes(long, 0, 8, count, total), "attention", "sequences")
+        refused(lib.q38hip_kv_attention(long, 0, p, p, None, 0, 8, 512, 64, 512, 1.0, p, p, count, total, p, None), "attention")
+    assert lib.q38hip_kv_attention_workspace_bytes(long, 0, 1, 1 << 20, 1 << 20)
+    # reset: a thread for each table entry
+    most = dict(sequences=1 << 14, table_entries=1 << 18)
+    refused(lib.q38hip_kv_reset(ctypes.byref(_cache(**most)), None), "table")
+    refused(lib.q38hip_kv_reset(ctypes.byref(_cache(sequences=0xffffffff // 255, table_entries=255)), None), "table")
