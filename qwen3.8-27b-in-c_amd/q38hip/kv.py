@@ -1,8 +1,8 @@
 """Paged 8-bit key/value cache (section 3 of include/q38hip.h).
 
 KVPages wraps the device tensors of a cache; its methods enqueue on torch's
-current stream, check shapes and types on the host and read nothing back.
-Ids, lengths and row offsets are int32 device tensors; what the device finds
+current stream of their device, check shapes and types on the host and read
+nothing back.  Ids, lengths and row offsets are int32 device tensors; what the device finds
 wrong in them goes to the cache's status word (bits below), which check()
 reads.
 
@@ -55,6 +55,21 @@ def _lib():
             function.restype, function.argtypes = result, arguments
         _BOUND = bound
     return _BOUND
+
+
+class _Elsewhere:
+    """the library's functions, called with a device that is not the current one"""
+
+    def __init__(self, device):
+        self._device = device
+
+    def __getattr__(self, name):
+        function = getattr(_lib(), name)
+
+        def call(*arguments):
+            with self._device:
+                return function(*arguments)
+        return call
 
 
 def _element_types():
@@ -119,6 +134,12 @@ class KVPages:
         """torch's current stream of the cache's device"""
         return self._torch._C._cuda_getCurrentRawStream(self._index)
 
+    def _calls(self):
+        """the library's functions.  They launch on the current device, which has to be the cache's: the handle of a
+        default stream is the same on all devices."""
+        torch = self._torch
+        return _lib() if torch._C._cuda_getDevice() == self._index else _Elsewhere(torch.cuda.device(self._index))
+
     def _type(self, dtype):
         kind = self._types.get(dtype)
         if kind is None:
@@ -167,7 +188,7 @@ class KVPages:
 
     def reset(self):
         """every page free, every sequence empty"""
-        _check(_lib().q38hip_kv_reset(self._ref, self._stream()), "q38hip_kv_reset")
+        _check(self._calls().q38hip_kv_reset(self._ref, self._stream()), "q38hip_kv_reset")
 
     def extend(self, sequences, rows):
         """sequences[i] grows by rows[i] tokens; shared last pages are copied first"""
@@ -175,34 +196,34 @@ class KVPages:
         more = self._words(rows, "rows", sequences.shape[0])
         if self._pages_workspace is None:      # calls on a cache are in order, so one serves them all
             self._pages_workspace = self._workspace(4 * self._pages_words())
-        _check(_lib().q38hip_kv_extend(self._ref, ids, more, sequences.shape[0], self._pages_workspace.data_ptr(),
-                                       self._stream()), "q38hip_kv_extend")
+        _check(self._calls().q38hip_kv_extend(self._ref, ids, more, sequences.shape[0], self._pages_workspace.data_ptr(),
+                                              self._stream()), "q38hip_kv_extend")
 
     def fork(self, parents, children, lengths=None):
         """children[i] (empty) becomes the first lengths[i] tokens (default: all) of parents[i]"""
         count = parents.shape[0]
-        _check(_lib().q38hip_kv_fork(self._ref, self._words(parents, "parents"), self._words(children, "children", count),
-                                     None if lengths is None else self._words(lengths, "lengths", count), count,
-                                     self._stream()), "q38hip_kv_fork")
+        taken, given = self._words(parents, "parents"), self._words(children, "children", count)
+        keep = None if lengths is None else self._words(lengths, "lengths", count)
+        _check(self._calls().q38hip_kv_fork(self._ref, taken, given, keep, count, self._stream()), "q38hip_kv_fork")
 
     def truncate(self, sequences, lengths):
         """sequences[i] keeps its first lengths[i] tokens; 0 frees it"""
         count = sequences.shape[0]
-        _check(_lib().q38hip_kv_truncate(self._ref, self._words(sequences, "sequences"),
-                                         self._words(lengths, "lengths", count), count, self._stream()), "q38hip_kv_truncate")
+        ids, keep = self._words(sequences, "sequences"), self._words(lengths, "lengths", count)
+        _check(self._calls().q38hip_kv_truncate(self._ref, ids, keep, count, self._stream()), "q38hip_kv_truncate")
 
     def compact(self):
         """The pages in use move to the front of the pool.  Returns an int32
         [2] device tensor: the pages moved and the pages in use."""
         work = self._torch.empty(self._pages_words(), dtype=self._int32, device=self._device)
-        _check(_lib().q38hip_kv_compact(self._ref, work.data_ptr(), self._stream()), "q38hip_kv_compact")
+        _check(self._calls().q38hip_kv_compact(self._ref, work.data_ptr(), self._stream()), "q38hip_kv_compact")
         return work[:2]
 
     def copy(self, sources, targets):
         """pages sources[i] to pages targets[i], in all layers"""
         count = sources.shape[0]
-        _check(_lib().q38hip_kv_copy(self._ref, self._words(sources, "sources"), self._words(targets, "targets", count),
-                                     count, self._stream()), "q38hip_kv_copy")
+        taken, given = self._words(sources, "sources"), self._words(targets, "targets", count)
+        _check(self._calls().q38hip_kv_copy(self._ref, taken, given, count, self._stream()), "q38hip_kv_copy")
 
     # ---- rows --------------------------------------------------------------------
 
@@ -219,8 +240,9 @@ class KVPages:
         if key.get_device() != self._index or value.get_device() != self._index:
             raise ValueError("keys and values must be on the cache's device")
         ids, starts, count = self._rows(sequences, row_starts, rows)
-        _check(_lib().q38hip_kv_append(self._ref, layer, key.data_ptr(), value.data_ptr(), self._type(key.dtype), stride[0],
-                                       ids, starts, count, rows, self._stream()), "q38hip_kv_append")
+        kind = self._type(key.dtype)
+        _check(self._calls().q38hip_kv_append(self._ref, layer, key.data_ptr(), value.data_ptr(), kind, stride[0], ids, starts,
+                                              count, rows, self._stream()), "q38hip_kv_append")
 
     def attention(self, layer, query, sequences, row_starts=None, gate=None, scale=None, out=None):
         """Causal attention of each sequence's last rows in one layer: query
@@ -241,7 +263,7 @@ class KVPages:
         elif out.shape != shape or out.dtype != dtype or out.get_device() != self._index or out.stride()[1:] != (dim, 1):
             raise ValueError("out must be [rows, heads, head_dim] in the queries' type with contiguous heads")
         ids, starts, count = self._rows(sequences, row_starts, rows)
-        kind, bound = self._type(dtype), _lib()
+        kind, bound = self._type(dtype), self._calls()
         nbytes = self._bytes.get((kind, heads, count, rows))
         if nbytes is None:
             nbytes = bound.q38hip_kv_attention_workspace_bytes(self._ref, kind, heads, count, rows)

@@ -450,3 +450,55 @@ def test_calls_of_more_threads_than_a_launch_are_refused():
     most = dict(sequences=1 << 14, table_entries=1 << 18)
     refused(lib.q38hip_kv_reset(ctypes.byref(_cache(**most)), None), "table")
     refused(lib.q38hip_kv_reset(ctypes.byref(_cache(sequences=0xffffffff // 255, table_entries=255)), None), "table")
+
+
+def test_calls_are_made_on_the_device_of_the_cache(monkeypatch):
+    """a default stream's handle names no device: whatever device is current, a call is made with the cache's"""
+    plain = kc.Cache(1, 4, 16, 2, 64, 2, 2, "int8").to("cpu")            # (its device index is -1)
+    ids, more, row, heads = kc.words([0], "cpu"), kc.words([1], "cpu"), torch.zeros(1, 2, 64), torch.zeros(1, 4, 64)
+    current, calls = [3], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            current.append(self.index)
+
+        def __exit__(self, *what):
+            current.pop()
+
+    class Library:
+        def __getattr__(self, name):
+            if name.endswith("workspace_bytes"):
+                return lambda *arguments: 64
+            return lambda *arguments: calls.append((name, current[-1], arguments[-1])) or 1
+
+    class Torch:
+        empty = staticmethod(torch.empty)
+        uint8 = torch.uint8
+
+        class _C:
+            _cuda_getDevice = staticmethod(lambda: current[-1])
+            _cuda_getCurrentRawStream = staticmethod(lambda index: 1000 + index)
+
+        class cuda:
+            device = Device
+
+    monkeypatch.setattr(kv, "_lib", Library)
+    plain._torch = Torch
+    for now in (3, -1):
+        current[:] = [now]
+        calls.clear()
+        plain.reset()
+        plain.extend(ids, more)
+        plain.fork(ids, ids)
+        plain.truncate(ids, ids)
+        plain.compact()
+        plain.copy(ids, ids)
+        plain.append(0, row, row, ids)
+        plain.attention(0, heads, ids, gate=heads)
+        assert [name[len("q38hip_kv_"):] for name, _, _ in calls] == ["reset", "extend", "fork", "truncate", "compact", "copy",
+                                                                      "append", "attention"]
+        assert all(device == -1 and stream == 999 for _, device, stream in calls), calls
+        assert current == [now]
