@@ -267,8 +267,9 @@ int q38hip_attention_rows(float *attention, Q38Q8KBlock *attention_q8k, const fl
  * belongs to one sequence): keys and values of many sequences as 8-bit codes
  * in pages that sequences can share.  Everything lives in device memory that
  * the caller owns and describes by a Q38KVPages; the calls enqueue on
- * `stream`, allocate nothing, read nothing back and can be captured into a
- * HIP graph.  Calls on one cache have to be ordered (one stream, or events).
+ * `stream` (of the current device, the cache's), allocate nothing, read nothing
+ * back and can be captured into a HIP graph.  Calls on one cache have to be
+ * ordered (one stream, or events).
  *
  *   data    [layers][pages][2][kv_heads][page_tokens * head_dim] codes, 16-byte
  *           aligned: keys (half 0) are [token][channel], values (half 1)
@@ -290,7 +291,7 @@ int q38hip_attention_rows(float *attention, Q38Q8KBlock *attention_q8k, const fl
  * the attention call behind it report the id.) */
 enum { Q38_KV_INT8 = 0, Q38_KV_E4M3 = 1 };
 enum {
-    Q38_KV_BAD_SEQUENCE = 1,   /* an id outside the cache, or twice in one call */
+    Q38_KV_BAD_SEQUENCE = 1,   /* an id outside the cache; extend: twice in a call, or fewer than 0 rows; fork: a child as parent */
     Q38_KV_POOL_FULL = 2,      /* extend: fewer free pages than asked for; nothing was done */
     Q38_KV_TABLE_FULL = 4,     /* extend: longer than a table holds; nothing was done */
     Q38_KV_BAD_PAGE = 8,       /* a page outside the pool */
@@ -349,7 +350,9 @@ int q38hip_kv_copy(const Q38KVPages *cache, const int32_t *sources, const int32_
  * row_starts[i + 1] - 1 of total_rows (device words, non-decreasing), or
  * total_rows / count rows each where row_starts is NULL.  They are the last
  * rows of the sequence's tokens: row t of r stands at position
- * length - r + t.  Rows that no sequence owns are neither read nor written.  type is the GGML id of the rows: F32 0, F16 1, BF16 30. */
+ * length - r + t.  Rows that no sequence owns are neither read nor written.
+ * type is the GGML id of the rows: F32 0, F16 1, BF16 30.  What a launch cannot
+ * hold is refused: from about 2^21 sequences to an append on, 2^24 to the others. */
 
 /* Quantises the rows' keys and values ([kv_heads][head_dim], rows row_stride
  * elements apart) into the pages of one layer.  Per page, head and half: with
@@ -357,7 +360,9 @@ int q38hip_kv_copy(const Q38KVPages *cache, const int32_t *sources, const int32_
  * <= M 2^k (M = 127 or 448), the scale becomes 2^k where the page holds no
  * older token, else the larger of 2^k and what it was, and older codes are
  * rounded to a scale that grew; new codes are value / scale, rounded to
- * nearest, ties to even.  A value that is not finite makes the scale NaN. */
+ * nearest, ties to even.  A value that is not finite makes the scale NaN.  The
+ * sequences of a call are distinct, and the pages that their rows fall into
+ * theirs alone, as extend leaves them. */
 int q38hip_kv_append(const Q38KVPages *cache, uint32_t layer, const void *key, const void *value, uint32_t type,
                      uint64_t row_stride, const int32_t *sequences, const int32_t *row_starts, uint32_t count,
                      uint32_t total_rows, void *stream);
@@ -368,8 +373,11 @@ int q38hip_kv_append(const Q38KVPages *cache, uint32_t layer, const void *key, c
  * that sees nothing.  Query head h reads key/value head h / (heads /
  * kv_heads).  Head h of a row begins at row * query_row_stride + h *
  * query_head_stride elements of query and of gate; output rows are
- * output_row_stride elements apart, heads head_dim.  Sums and softmax are in
- * fp32; fp32 rows keep 22 bits of queries and weights in the products.
+ * output_row_stride elements apart, heads head_dim.  Sums, maxima and totals are
+ * in fp32.  In the products queries of fp32 rows keep 22 bits, and a weight times
+ * its page's value scale 11 (16-bit rows) or 22 (fp32 rows), or 2^-31 of the
+ * largest where that is more: a page whose values count that little is left out,
+ * in channels too where the pages that count hold zeros.
  * q38hip_kv_attention_workspace_bytes: device memory for the call (16-byte
  * aligned; 0: none needed, or a bad call). */
 uint64_t q38hip_kv_attention_workspace_bytes(const Q38KVPages *cache, uint32_t type, uint32_t heads, uint32_t count,
