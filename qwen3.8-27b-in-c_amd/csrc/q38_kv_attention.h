@@ -22,12 +22,12 @@
  * are contiguous and no register waits for them); a wavefront asks for its next
  * keys when it has read the present ones, and for its next values channel by
  * channel.  48 sequences of up to 16384 tokens (32 heads, 8 of keys, 128 wide,
- * 339 MB): 65 us, 5.2 TB/s, what a large copy reaches here.  Four rows at 131075
- * tokens (24 heads, 4 of keys, 256 wide, 268 MB): 67 us, 4.0 TB/s; 9 us pass
+ * 339 MB): 63 us, 5.3 TB/s, what a large copy reaches here.  Four rows at 131075
+ * tokens (24 heads, 4 of keys, 256 wide, 268 MB): 71 us, 3.8 TB/s; 9 us pass
  * before the first step's codes are there, 7 in the merge at the end.
  *
  * Many columns (prompts): the products are the bound.  512 rows behind 7679
- * tokens (24 heads, 4 of keys, 256 wide, 100 GFLOP): 147 us, 680 TFLOP/s; of
+ * tokens (24 heads, 4 of keys, 256 wide, 100 GFLOP): 146 us, 680 TFLOP/s; of
  * its cycles the matrix unit is busy in a third, LDS in over half.
  *
  * Short calls are instruction fetch: 37 tokens take 11 us, of which memory is
