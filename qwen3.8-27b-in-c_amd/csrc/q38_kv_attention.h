@@ -40,10 +40,10 @@
  * 22 bits together.  16-bit calls keep the fp16 weight alone, for half the
  * products: its error, up to 2^-11 of the weight, is an eighth of a bf16 output's
  * own rounding and as large as an fp16 output's for one token, less over many
- * (512 rows behind 7679 tokens, bf16: 1.67e-3 off the 64-bit result instead of
- * 1.66e-3; prompts of up to 300 tokens, fp16: 2.5e-4 instead of 2.1e-4).  The
- * largest weight is 2^6 or more, fp16's least step 2^-24: what lies 2^20 below the
- * largest loses bits, what lies 2^31 below is nothing. */
+ * (off the 64-bit result, root of the mean square: 512 rows behind 7679 tokens,
+ * bf16, 1.7e-3 as with fp32 weights; prompts of up to 300 tokens, fp16, 2.5e-4
+ * instead of 2.1e-4).  The largest weight is 2^6 or more, fp16's least step 2^-24:
+ * what lies 2^20 below the largest loses bits, what lies 2^31 below is nothing. */
 #pragma once
 
 #include "q38_device.h"
