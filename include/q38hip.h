@@ -1,6 +1,7 @@
 /* libq38hip: MI355X (gfx950) kernels for the Qwen3.8 decode hot path.
  *
- * C ABI only: plain pointers and sizes.  Two families of entry points:
+ * C ABI only: plain pointers and sizes.  Two families of entry points, and
+ * two library extensions (sections 3 and 4):
  *
  *  1. Drop-in replacements for the reference kernel ABI
  *     (include/qwen38/qwen38_quant.h:20-49 of shyringo/qwen3.8-27b-in-c):
@@ -386,6 +387,93 @@ int q38hip_kv_attention(const Q38KVPages *cache, uint32_t layer, void *output, c
                         uint32_t type, uint32_t heads, uint64_t query_row_stride, uint64_t query_head_stride,
                         uint64_t output_row_stride, float scale, const int32_t *sequences, const int32_t *row_starts,
                         uint32_t count, uint32_t total_rows, void *workspace, void *stream);
+
+/* ---- 4. operators of a decoder layer --------------------------------------
+ *
+ * Library extension (no counterpart in the reference, whose engine does these
+ * in fp32, in its own order, for one model): for programs that bring their own
+ * model to the paged cache.  Every pointer is a device pointer; the calls
+ * enqueue on `stream` (of the current device, which holds the tensors),
+ * allocate nothing, read nothing back, keep nothing from one call to the next
+ * and can be captured into a HIP graph.  Calls do not share memory that the
+ * caller does not share between them.
+ *
+ * type is the GGML id of elements: F32 0, F16 1, BF16 30.  Sums, means and
+ * totals are in fp32 or more; a result is rounded once, to its type, ties to
+ * even.  Strides are in elements; elements of a row (of a head) are contiguous.
+ * Any alignment of elements is taken; 16-byte aligned rows are faster.
+ * Outputs overlap no inputs except where said, and no output's rows overlap.
+ *
+ * Rows in 8 bits: codes [rows][width], e4m3 (OCP float8), and scales
+ * [rows][pitch] with one byte e for each 128 neighbours of a row (the last
+ * ones of a row may be fewer): a code c stands for c * 2^(e - 127).  pitch is
+ * the number of blocks rounded up to a multiple of 4; bytes behind the last
+ * block are 0.  With a the block's largest magnitude, e - 127 is the least k >=
+ * -100 with a <= 448 * 2^k, so dividing by the scale is exact and a code is one
+ * rounding.  A block that holds a value that is not finite has scale 255 (NaN) and codes
+ * 0x7f (NaN). */
+
+/* bytes between the scales of two rows of `width` elements; 0 for width 0 or above 2^24 */
+uint32_t q38hip_e4m3_scale_pitch(uint64_t width);
+
+/* Rows into 8 bits: x, or x * silu(gate) where gate is not NULL (gate / (1 +
+ * e^-gate), the middle of a SwiGLU).  width and rows up to 2^24. */
+int q38hip_quantize_e4m3(uint8_t *codes, uint8_t *scales, const void *x, uint64_t x_row_stride, const void *gate,
+                         uint64_t gate_row_stride, uint32_t type, uint64_t width, uint32_t rows, void *stream);
+
+/* Root-mean-square norm of rows: t = x, or x + addend rounded to `type` and
+ * stored in total where addend is not NULL; y = t / sqrt(mean(t^2) + eps) *
+ * (weight + weight_offset).  y goes to output, in `type`, where that is not
+ * NULL, and to codes and scales where those are not NULL; one of them at least.
+ * weight has `width` elements of weight_type.  total may be x or addend itself
+ * (same pointer and stride), output x or addend, total not output. */
+int q38hip_rms_norm(void *output, uint64_t output_row_stride, uint8_t *codes, uint8_t *scales, void *total,
+                    uint64_t total_row_stride, const void *x, uint64_t x_row_stride, const void *addend,
+                    uint64_t addend_row_stride, uint32_t type, const void *weight, uint32_t weight_type,
+                    float weight_offset, float eps, uint64_t width, uint32_t rows, void *stream);
+
+/* Rows in 8 bits times a matrix in e4m3: output[t][r] = sum over blocks b of
+ * 2^(scales[t][b] - 127) * weight_scales[r / 128][b] * (the block's products of
+ * codes[t] and weight[r]), for t < batch_size, r < rows.  weight is
+ * [rows][input_length] codes, weight_scales [ceil(rows / 128)][blocks] floats;
+ * input_length is a multiple of 16, codes and weight 16-byte aligned, scales 4.
+ * output is of `type`, rows output_row_stride elements apart.
+ * q38hip_gemm_e4m3_workspace_bytes: device memory for the call, 16-byte aligned
+ * (0: none needed, or a bad call). */
+uint64_t q38hip_gemm_e4m3_workspace_bytes(uint32_t batch_size, uint64_t input_length, uint32_t rows);
+int q38hip_gemm_e4m3(void *output, uint32_t type, uint64_t output_row_stride, const uint8_t *codes,
+                     const uint8_t *scales, uint32_t batch_size, uint64_t input_length, const uint8_t *weight,
+                     const float *weight_scales, uint32_t rows, void *workspace, void *stream);
+
+/* Rotary positions: in each head of each row, pair i of `pairs` is turned by
+ * positions[row] * frequencies[i] radians and multiplied by magnitude: (a, b)
+ * becomes magnitude * (a cos - b sin, b cos + a sin).  The pair is channels
+ * 2i and 2i + 1 where interleaved is not 0, else i and i + pairs; channels from
+ * 2 * pairs on are copied.  Angles are formed in fp64, so far positions keep
+ * the accuracy of near ones.  output may be x itself (same pointer and strides).
+ * 2 * pairs <= head_dim <= 1024, heads * head_dim <= 2^20. */
+int q38hip_rotary(void *output, uint64_t output_row_stride, uint64_t output_head_stride, const void *x,
+                  uint64_t x_row_stride, uint64_t x_head_stride, uint32_t type, uint32_t rows, uint32_t heads,
+                  uint32_t head_dim, const int32_t *positions, const float *frequencies, uint32_t pairs,
+                  int interleaved, float magnitude, void *stream);
+
+/* Causal attention of whole prompts, packed: sequence i of count owns rows
+ * row_starts[i] .. row_starts[i + 1] - 1 of total_rows (device words,
+ * non-decreasing).  output[row][head] = sum softmax(scale q.k) v over the rows
+ * of its sequence up to itself, times sigmoid(gate) where gate is not NULL.
+ * What other sequences and later rows hold, NaN included, has no part in it.
+ * Rows that no sequence owns are not written.  Where row_starts decrease, what
+ * is written to rows of the output is unspecified.  Query head h reads
+ * key/value head h / (heads / kv_heads).  Head h of a row begins at row *
+ * query_row_stride + h * query_head_stride elements of query and of gate;
+ * rows of key, value and output are their strides apart, heads head_dim, which
+ * is 64, 128 or 256.  In the second product the weights of 16-bit rows have 8
+ * (BF16) or 11 (F16) bits; their total sums what is multiplied. */
+int q38hip_prompt_attention(void *output, uint64_t output_row_stride, const void *query, const void *gate,
+                            uint64_t query_row_stride, uint64_t query_head_stride, const void *key,
+                            uint64_t key_row_stride, const void *value, uint64_t value_row_stride, uint32_t type,
+                            uint32_t heads, uint32_t kv_heads, uint32_t head_dim, float scale,
+                            const int32_t *row_starts, uint32_t count, uint32_t total_rows, void *stream);
 
 /* Last argument error of the calling thread ("" when none). */
 const char *q38hip_last_error(void);

@@ -1,0 +1,88 @@
+/* Operators of a decoder layer (section 4 of include/q38hip.h): what their
+ * kernels, launchers and checks share. */
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "q38hip.h"
+
+namespace q38 {
+
+/* GGML type ids of elements */
+constexpr int kLayerF32 = 0, kLayerF16 = 1, kLayerBF16 = 30;
+
+/* elements that share a scale */
+constexpr uint32_t kE4M3Block = 128;
+
+#define Q38_LAYER_HD __host__ __device__ __forceinline__
+
+Q38_LAYER_HD constexpr uint32_t layer_up(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
+
+/* a launch has fewer than 2^32 threads along a direction of its grid */
+inline bool layer_launch_holds(uint64_t workgroups, uint32_t threads) { return workgroups * threads <= 0xffffffffull; }
+
+/* workgroups of 256 threads to a row that goes into 8 bits, eight elements a thread */
+inline uint32_t quantize_parts(uint64_t width) { return (uint32_t)((width + 2047) / 2048); }
+/* threads to a row that is normalised */
+inline uint32_t norm_threads(uint64_t width) { return width > 8192 ? 1024 : 256; }
+
+inline uint32_t e4m3_blocks(uint64_t width) { return (uint32_t)((width + kE4M3Block - 1) / kE4M3Block); }
+inline uint32_t e4m3_pitch(uint64_t width) { return (e4m3_blocks(width) + 3) / 4 * 4; }
+
+struct QuantizeRows {
+    uint8_t *codes, *scales;
+    const void *x, *gate;
+    uint64_t x_row, gate_row;
+    uint32_t width, pitch, rows;
+};
+
+struct NormRows {
+    void *output, *total;
+    uint8_t *codes, *scales;
+    const void *x, *addend, *weight;
+    uint64_t output_row, total_row, x_row, addend_row;
+    uint32_t width, pitch, rows;
+    int weight_type;
+    float offset, eps;
+};
+
+struct Rotary {
+    void *output;
+    const void *x;
+    uint64_t output_row, output_head, x_row, x_head;
+    uint32_t rows, heads, head_dim, pairs;
+    const int32_t *positions;
+    const float *frequencies;
+    float magnitude;
+    bool interleaved;
+};
+
+struct ProductE4M3 {
+    void *output;
+    uint64_t output_row;
+    const uint8_t *codes, *scales, *weight;
+    const float *weight_scales;
+    float *partial;
+    uint32_t tokens, inputs, outputs, blocks, pitch;
+    int type;
+};
+
+struct PromptAttention {
+    void *output;
+    const void *query, *gate, *key, *value;
+    uint64_t output_row, query_row, query_head, key_row, value_row;
+    const int32_t *row_starts;
+    uint32_t count, rows, heads, kv_heads, head_dim;
+    float scale;           /* softmax scale times log2(e) */
+    int type;
+};
+
+bool launch_quantize_e4m3(const QuantizeRows &a, int type, hipStream_t stream);
+bool launch_rms_norm(const NormRows &a, int type, hipStream_t stream);
+bool launch_rotary(const Rotary &a, int type, hipStream_t stream);
+uint64_t product_e4m3_workspace_bytes(uint32_t tokens, uint64_t inputs, uint32_t outputs);
+bool launch_product_e4m3(const ProductE4M3 &a, hipStream_t stream);
+bool launch_prompt_attention(const PromptAttention &a, hipStream_t stream);
+
+}  // namespace q38

@@ -1,0 +1,280 @@
+"""Operators of a decoder layer (section 4 of include/q38hip.h), for programs
+that bring their own model: norm, projections in 8 bits, rotary positions and
+the attention of packed prompts.
+
+Functions check shapes and types on the host, enqueue on torch's current stream
+of their tensors' device and read nothing back.  Rows in 8 bits are a pair
+(codes, scales): float8_e4m3fn [rows, width] and float8_e8m0fnu [rows, blocks of
+128 rounded up to a multiple of 4].
+
+    y, x = layer.rms_norm(x, weight, addend=attended, e4m3=True)     # x + addend, and its norm in 8 bits
+    both = layer.product(y, gate_up, gate_up_scales)                 # bfloat16 [rows, 2 * hidden]
+    z = layer.quantize(both[:, hidden:], gate=both[:, :hidden])      # SwiGLU, in 8 bits
+    q = layer.rotary(q, positions, frequencies)                      # [rows, heads, head_dim]
+    out = layer.attention(q, k, v, row_starts)                       # causal, within each prompt
+"""
+import ctypes
+import math
+from collections import namedtuple
+
+import torch
+
+from . import _check, lib
+
+EXPORTS = ("q38hip_e4m3_scale_pitch", "q38hip_quantize_e4m3", "q38hip_rms_norm", "q38hip_gemm_e4m3_workspace_bytes",
+           "q38hip_gemm_e4m3", "q38hip_rotary", "q38hip_prompt_attention")
+BLOCK = 128
+
+E4M3Rows = namedtuple("E4M3Rows", "codes scales")
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+_BOUND = None
+
+
+def _lib():
+    """the library, with the argument types of this module's functions"""
+    global _BOUND
+    if _BOUND is None:
+        bound = lib()
+        vp, u32, u64, f32, i32 = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_float, ctypes.c_int
+        for name, result, arguments in (
+                ("e4m3_scale_pitch", u32, [u64]),
+                ("quantize_e4m3", i32, [vp, vp, vp, u64, vp, u64, u32, u64, u32, vp]),
+                ("rms_norm", i32, [vp, u64, vp, vp, vp, u64, vp, u64, vp, u64, u32, vp, u32, f32, f32, u64, u32, vp]),
+                ("gemm_e4m3_workspace_bytes", u64, [u32, u64, u32]),
+                ("gemm_e4m3", i32, [vp, u32, u64, vp, vp, u32, u64, vp, vp, u32, vp, vp]),
+                ("rotary", i32, [vp, u64, u64, vp, u64, u64, u32, u32, u32, u32, vp, vp, u32, i32, f32, vp]),
+                ("prompt_attention", i32, [vp, u64, vp, vp, u64, u64, vp, u64, vp, u64, u32, u32, u32, u32, f32, vp, u32,
+                                           u32, vp])):
+            function = getattr(bound, "q38hip_" + name)
+            function.restype, function.argtypes = result, arguments
+        _BOUND = bound
+    return _BOUND
+
+
+def _call(name, index, *arguments):
+    """enqueues on torch's current stream of device `index`.  The library launches on the current device, which has to be
+    that one: the handle of a default stream is the same on all devices."""
+    function = getattr(_BOUND or _lib(), name)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        ok = function(*arguments, stream)
+    else:
+        with torch.cuda.device(index):
+            ok = function(*arguments, stream)
+    if not ok:
+        _check(ok, name)
+
+
+def _type(tensor, name):
+    kind = _TYPES.get(tensor.dtype)
+    if kind is None:
+        raise ValueError("%s must be float32, float16 or bfloat16" % name)
+    return kind
+
+
+def _device(tensor, name):
+    index = tensor.get_device()
+    if index < 0:
+        raise ValueError("%s must be on a GPU" % name)
+    return index
+
+
+def _alike(tensor, name, x, index):
+    """row stride of a tensor of x's shape, type and device with contiguous rows"""
+    if tensor.shape != x.shape or tensor.dtype != x.dtype or tensor.get_device() != index or _broken(tensor):
+        raise ValueError("%s must be rows of the same shape, type and device, each contiguous" % name)
+    return tensor.stride(0)
+
+
+def _broken(tensor):
+    return tensor.dim() != 2 or tensor.stride(1) != 1 and tensor.shape[1] > 1
+
+
+def _rows(x, name="x"):
+    if _broken(x):
+        raise ValueError("%s must be [rows, width] with contiguous rows" % name)
+    return x.shape
+
+
+def scale_pitch(width):
+    """scale bytes of a row of `width` elements"""
+    return -(-width // (4 * BLOCK)) * 4
+
+
+def _e4m3(rows, width, device, into):
+    if into is None:
+        return E4M3Rows(torch.empty((rows, width), dtype=torch.float8_e4m3fn, device=device),
+                        torch.empty((rows, scale_pitch(width)), dtype=torch.float8_e8m0fnu, device=device))
+    _check_e4m3(into, rows, width, device.index)
+    return E4M3Rows(*into)
+
+
+def _check_e4m3(rows8, rows, width, index):
+    codes, scales = rows8
+    if codes.dtype != torch.float8_e4m3fn or codes.shape != (rows, width) or not codes.is_contiguous() or \
+            scales.dtype != torch.float8_e8m0fnu or scales.shape != (rows, scale_pitch(width)) or not scales.is_contiguous():
+        raise ValueError("rows in 8 bits must be contiguous float8_e4m3fn [%d, %d] and float8_e8m0fnu [%d, %d]"
+                         % (rows, width, rows, scale_pitch(width)))
+    if codes.get_device() != index or scales.get_device() != index:
+        raise ValueError("rows in 8 bits must be on the device of the other tensors")
+
+
+def quantize(x, gate=None, out=None):
+    """x [rows, width], or x * silu(gate), in 8 bits; gate has x's shape and type, and a row stride of its own."""
+    rows, width = _rows(x)
+    kind, index = _type(x, "x"), _device(x, "x")
+    gate_row = 0 if gate is None else _alike(gate, "gate", x, index)
+    out = _e4m3(rows, width, x.device, out)
+    _call("q38hip_quantize_e4m3", index, out.codes.data_ptr(), out.scales.data_ptr(), x.data_ptr(), x.stride(0),
+          None if gate is None else gate.data_ptr(), gate_row, kind, width, rows)
+    return out
+
+
+def rms_norm(x, weight, eps=1e-6, addend=None, offset=0.0, e4m3=False, out=None, total=None):
+    """The root-mean-square norm of x [rows, width], or of x + addend, times weight + offset: in x's type, or in 8 bits
+    where e4m3 is true.  With an addend the result is (norm, sum); total takes the sum, and may be x or addend."""
+    rows, width = _rows(x)
+    kind, index = _type(x, "x"), _device(x, "x")
+    if weight.shape != (width,) or width > 1 and weight.stride(0) != 1 or weight.get_device() != index:
+        raise ValueError("weight must be a contiguous vector of %d elements on x's device" % width)
+    weight_kind = _type(weight, "weight")
+    addend_row = total_row = 0
+    if addend is not None:
+        addend_row = _alike(addend, "addend", x, index)
+        if total is None:
+            total = torch.empty((rows, width), dtype=x.dtype, device=x.device)
+        total_row = _alike(total, "total", x, index)
+    elif total is not None:
+        raise ValueError("total needs an addend")
+    if e4m3:
+        out = _e4m3(rows, width, x.device, out)
+        to, to_row, codes, scales = None, 0, out.codes.data_ptr(), out.scales.data_ptr()
+    else:
+        if out is None:
+            out = torch.empty((rows, width), dtype=x.dtype, device=x.device)
+        to_row = _alike(out, "out", x, index)
+        to, codes, scales = out.data_ptr(), None, None
+    _call("q38hip_rms_norm", index, to, to_row, codes, scales, None if addend is None else total.data_ptr(), total_row,
+          x.data_ptr(), x.stride(0), None if addend is None else addend.data_ptr(), addend_row, kind, weight.data_ptr(),
+          weight_kind, offset, eps, width, rows)
+    return out if addend is None else (out, total)
+
+
+_WORKSPACES = {}
+
+
+def product(rows8, weight, weight_scales, dtype=torch.bfloat16, out=None):
+    """Rows in 8 bits [rows, inputs] times weight [outputs, inputs] (float8_e4m3fn) with weight_scales [ceil(outputs /
+    128), ceil(inputs / 128)] (float32): [rows, outputs] of dtype."""
+    codes, scales = rows8
+    if codes.dim() != 2 or weight.dim() != 2 or codes.shape[1] != weight.shape[1]:
+        raise ValueError("expected codes [rows, inputs] and weight [outputs, inputs]")
+    rows, inputs = codes.shape
+    outputs, index = weight.shape[0], _device(weight, "weight")
+    _check_e4m3(rows8, rows, inputs, index)
+    if weight.dtype != torch.float8_e4m3fn or not weight.is_contiguous():
+        raise ValueError("weight must be contiguous float8_e4m3fn")
+    if weight_scales.dtype != torch.float32 or weight_scales.shape != (-(-outputs // BLOCK), -(-inputs // BLOCK)) or \
+            not weight_scales.is_contiguous() or weight_scales.get_device() != index:
+        raise ValueError("weight_scales must be contiguous float32 [%d, %d] on the weight's device"
+                         % (-(-outputs // BLOCK), -(-inputs // BLOCK)))
+    if out is None:
+        out = torch.empty((rows, outputs), dtype=dtype, device=weight.device)
+    elif out.shape != (rows, outputs) or out.get_device() != index or _broken(out):
+        raise ValueError("out must be [%d, %d] with contiguous rows" % (rows, outputs))
+    kind, sizes = _type(out, "out"), (rows, inputs, outputs)
+    nbytes = _WORKSPACES.get(sizes)
+    if nbytes is None:
+        nbytes = _lib().q38hip_gemm_e4m3_workspace_bytes(*sizes)
+        if len(_WORKSPACES) >= 4096:
+            _WORKSPACES.clear()
+        _WORKSPACES[sizes] = nbytes
+    work = torch.empty(nbytes, dtype=torch.uint8, device=weight.device) if nbytes else None
+    _call("q38hip_gemm_e4m3", index, out.data_ptr(), kind, out.stride(0), codes.data_ptr(), scales.data_ptr(), rows, inputs,
+          weight.data_ptr(), weight_scales.data_ptr(), outputs, None if work is None else work.data_ptr())
+    return out
+
+
+def rotary_frequencies(turned, base=10000.0, factor=1.0, original=None, fast=32.0, slow=1.0, device=None):
+    """Frequencies of the turned / 2 pairs (float32) and the magnitude for rotary(): base^(-2i / turned).  With a factor
+    above 1 for longer contexts: divided by it for all pairs where `original` is None; else, with `original` the context
+    that the model was trained on, pairs that turn at least `fast` times within it stay, those that turn at most `slow`
+    times are divided, those between are blended linearly in the pair's index, and the magnitude is 0.1 ln(factor) + 1."""
+    if turned < 2 or turned % 2 or not base > 1 or not factor >= 1 or (original is not None and not original > 0):
+        raise ValueError("expected an even number of channels, a base above 1 and a factor of at least 1")
+    pairs = torch.arange(turned // 2, dtype=torch.float64)
+    plain, magnitude = base ** (-2 * pairs / turned), 1.0
+    frequencies = plain / factor
+    if original is not None and factor > 1:
+        # pair i turns original * base^(-2i / turned) / (2 pi) times
+        at = lambda turns: turned * math.log(original / (2 * math.pi * turns)) / (2 * math.log(base))  # noqa: E731
+        low, high = max(math.floor(at(fast)), 0), min(math.ceil(at(slow)), turned - 1)
+        part = ((pairs - low) / max(high - low, 0.001)).clamp(0, 1)
+        frequencies = plain * (1 - part) + frequencies * part
+        magnitude = 0.1 * math.log(factor) + 1
+    return frequencies.float().to(device), magnitude
+
+
+def _heads(x, name):
+    if x.dim() != 3 or x.stride(2) != 1 and x.shape[2] > 1:
+        raise ValueError("%s must be [rows, heads, head_dim] with contiguous heads" % name)
+    return x.shape
+
+
+def _words(tensor, name, index):
+    if tensor.dtype != torch.int32 or tensor.dim() != 1 or not tensor.is_contiguous() or tensor.get_device() != index:
+        raise ValueError("%s must be a contiguous int32 vector on the device of the rows" % name)
+    return tensor.shape[0]
+
+
+def rotary(x, positions, frequencies, interleaved=False, magnitude=1.0, out=None):
+    """Turns the first 2 * len(frequencies) channels of each head of x [rows, heads, head_dim] by positions[row] *
+    frequencies[pair]; out may be x."""
+    rows, heads, dim = _heads(x, "x")
+    kind, index = _type(x, "x"), _device(x, "x")
+    if _words(positions, "positions", index) != rows:
+        raise ValueError("positions must have %d words" % rows)
+    if frequencies.dtype != torch.float32 or frequencies.dim() != 1 or not frequencies.is_contiguous() or \
+            frequencies.get_device() != index:
+        raise ValueError("frequencies must be a contiguous float32 vector on x's device")
+    if out is None:
+        out = torch.empty((rows, heads, dim), dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype or out.get_device() != index:
+        raise ValueError("out must be laid out as x")
+    else:
+        _heads(out, "out")
+    _call("q38hip_rotary", index, out.data_ptr(), out.stride(0), out.stride(1), x.data_ptr(), x.stride(0), x.stride(1), kind,
+          rows, heads, dim, positions.data_ptr(), frequencies.data_ptr(), frequencies.shape[0], 1 if interleaved else 0,
+          magnitude)
+    return out
+
+
+def attention(query, key, value, row_starts, gate=None, scale=None, out=None):
+    """Causal attention of packed prompts: sequence i owns rows row_starts[i] .. row_starts[i + 1] - 1 (int32, on the
+    device).  query (and gate, laid out alike) [rows, heads, head_dim], key and value [rows, kv_heads, head_dim] with heads
+    next to each other; the result is [rows, heads, head_dim] in their type.  Rows that no sequence owns are not written."""
+    rows, heads, dim = _heads(query, "query")
+    kind, index = _type(query, "query"), _device(query, "query")
+    if key.dim() != 3 or key.shape[0] != rows or key.shape[2] != dim or value.shape != key.shape or \
+            key.dtype != query.dtype or value.dtype != query.dtype:
+        raise ValueError("key and value must be [%d, kv_heads, %d] in the queries' type" % (rows, dim))
+    for tensor in (key, value):
+        if tensor.get_device() != index or tensor.stride(2) != 1 or tensor.shape[1] > 1 and tensor.stride(1) != dim:
+            raise ValueError("key and value must be on the queries' device, with heads next to each other")
+    if gate is not None and (gate.shape != query.shape or gate.stride() != query.stride() or gate.dtype != query.dtype or
+                             gate.get_device() != index):
+        raise ValueError("the gate must be laid out as the queries")
+    count = _words(row_starts, "row_starts", index) - 1
+    if out is None:
+        out = torch.empty((rows, heads, dim), dtype=query.dtype, device=query.device)
+    elif out.shape != query.shape or out.dtype != query.dtype or out.get_device() != index or out.stride(2) != 1 or \
+            heads > 1 and out.stride(1) != dim:
+        raise ValueError("out must be [rows, heads, head_dim] in the queries' type, with heads next to each other")
+    if count < 1:
+        raise ValueError("row_starts must have an offset for each sequence and one behind the last")
+    _call("q38hip_prompt_attention", index, out.data_ptr(), out.stride(0), query.data_ptr(),
+          None if gate is None else gate.data_ptr(), query.stride(0), query.stride(1), key.data_ptr(), key.stride(0),
+          value.data_ptr(), value.stride(0), kind, heads, key.shape[1], dim, dim ** -0.5 if scale is None else scale,
+          row_starts.data_ptr(), count, rows)
+    return out

@@ -1,0 +1,133 @@
+"""What a decoder layer's operators refuse on the host (section 4 of
+include/q38hip.h, q38hip/layer.py), and the frequencies of rotary positions."""
+import ctypes
+import math
+import os
+
+import numpy as np
+import pytest
+import torch
+
+import q38hip
+from q38hip import layer
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+P = 4096            # an aligned address that no refused call follows
+BIG = (1 << 24) + 16
+
+
+def test_exports():
+    declared = open(os.path.join(ROOT, "include", "q38hip.h")).read()
+    for name in layer.EXPORTS:
+        assert name + "(" in declared and hasattr(q38hip.lib(), name)
+
+
+def _refused(name, good, changes):
+    """a call of the C function with each change of its arguments is refused, with a message"""
+    function = getattr(layer._lib(), name)
+    for change in changes:
+        arguments = dict(good, **change)
+        assert set(arguments) == set(good), change
+        assert function(*arguments.values()) == 0 and q38hip.last_error(), change
+
+
+def test_pitch():
+    lib = layer._lib()
+    for width in (1, 127, 128, 129, 512, 513, 5120, 17408, 1 << 24):
+        assert lib.q38hip_e4m3_scale_pitch(width) == layer.scale_pitch(width) == -(-width // 512) * 4
+    assert lib.q38hip_e4m3_scale_pitch(0) == 0 and lib.q38hip_e4m3_scale_pitch((1 << 24) + 1) == 0
+
+
+def test_quantize_refuses():
+    good = dict(codes=P, scales=P, x=P, x_row=128, gate=None, gate_row=0, type=0, width=128, rows=2, stream=None)
+    _refused("q38hip_quantize_e4m3", good, [
+        dict(codes=None), dict(scales=None), dict(x=None), dict(type=2), dict(width=0), dict(rows=0), dict(width=BIG, x_row=BIG),
+        dict(rows=BIG), dict(x_row=127), dict(gate=P, gate_row=127), dict(x=P + 2), dict(x=P + 1, type=1), dict(gate=P + 2, gate_row=128),
+        dict(rows=1 << 23, width=1 << 18, x_row=1 << 18), dict(rows=1 << 24, width=4096, x_row=4096)])
+
+
+def test_norm_refuses():
+    good = dict(output=P, output_row=256, codes=None, scales=None, total=None, total_row=0, x=2 * P, x_row=256, addend=None,
+                addend_row=0, type=30, weight=3 * P, weight_type=0, offset=0.0, eps=1e-6, width=256, rows=3, stream=None)
+    added = dict(addend=4 * P, addend_row=256, total=5 * P, total_row=256)
+    _refused("q38hip_rms_norm", good, [
+        dict(output=None), dict(codes=P), dict(scales=P), dict(addend=P, addend_row=256), dict(total=P, total_row=256), dict(x=None),
+        dict(weight=None), dict(type=3), dict(weight_type=12), dict(width=0), dict(rows=0), dict(rows=BIG), dict(width=BIG),
+        dict(x_row=255), dict(output_row=255), dict(added, addend_row=255), dict(added, total_row=200),
+        dict(added, total=P), dict(added, total=2 * P, total_row=512), dict(added, total=4 * P, total_row=512),
+        dict(output=2 * P, output_row=512), dict(added, output=4 * P, output_row=512), dict(eps=-1.0), dict(eps=math.nan),
+        dict(eps=math.inf), dict(offset=math.nan), dict(x=2 * P + 1), dict(weight=3 * P + 2), dict(output=P + 1),
+        dict(added, addend=4 * P + 1), dict(added, total=5 * P + 1), dict(rows=1 << 23, width=16384, x_row=16384, output_row=16384)])
+
+
+def test_product_refuses():
+    good = dict(output=P, type=30, output_row=256, codes=P, scales=P, tokens=2, inputs=128, weight=P, weight_scales=P, rows=256,
+                workspace=None, stream=None)
+    _refused("q38hip_gemm_e4m3", good, [
+        dict(output=None), dict(type=8), dict(output_row=255), dict(codes=None), dict(scales=None), dict(weight=None),
+        dict(weight_scales=None), dict(tokens=0), dict(inputs=0), dict(rows=0), dict(inputs=120), dict(inputs=129), dict(tokens=BIG),
+        dict(inputs=BIG), dict(rows=BIG, output_row=BIG), dict(tokens=1 << 20, rows=1 << 20, output_row=1 << 20), dict(codes=P + 8),
+        dict(weight=P + 4), dict(scales=P + 2), dict(weight_scales=P + 2), dict(output=P + 1), dict(workspace=P + 8)])
+    lib = layer._lib()
+    for sizes in ((0, 128, 16), (1, 0, 16), (1, 128, 0), (1, 100, 16), (BIG, 128, 16)):
+        assert lib.q38hip_gemm_e4m3_workspace_bytes(*sizes) == 0 and q38hip.last_error()
+
+
+def test_rotary_refuses():
+    good = dict(output=P, output_row=512, output_head=128, x=2 * P, x_row=512, x_head=128, type=1, rows=3, heads=4, dim=128,
+                positions=P, frequencies=P, pairs=32, interleaved=0, magnitude=1.0, stream=None)
+    _refused("q38hip_rotary", good, [
+        dict(output=None), dict(x=None), dict(positions=None), dict(frequencies=None), dict(type=7), dict(rows=0), dict(heads=0),
+        dict(dim=0), dict(pairs=0), dict(pairs=65), dict(dim=2048, x_head=2048, output_head=2048), dict(heads=1 << 14), dict(rows=BIG),
+        dict(x_head=127), dict(output_head=127), dict(x_row=100), dict(output_row=100), dict(x=P + 1), dict(output=P + 1),
+        dict(positions=P + 2), dict(frequencies=P + 1), dict(output=2 * P, output_row=1024), dict(output=2 * P, output_head=256),
+        dict(magnitude=math.inf), dict(rows=1 << 24)])
+
+
+def test_attention_refuses():
+    good = dict(output=P, output_row=512, query=P, gate=None, query_row=512, query_head=128, key=P, key_row=256, value=P,
+                value_row=256, type=30, heads=4, kv_heads=2, dim=128, scale=1.0, starts=P, count=1, rows=8, stream=None)
+    _refused("q38hip_prompt_attention", good, [
+        dict(output=None), dict(query=None), dict(key=None), dict(value=None), dict(starts=None), dict(type=2), dict(dim=96),
+        dict(dim=512), dict(heads=0), dict(kv_heads=0), dict(heads=3), dict(count=0), dict(rows=0), dict(count=BIG), dict(rows=BIG),
+        dict(heads=1 << 20, kv_heads=2, rows=1 << 12, output_row=1 << 30), dict(query_head=127), dict(query_row=127), dict(key_row=255),
+        dict(value_row=255), dict(output_row=511), dict(output=P + 1), dict(gate=P + 1), dict(key=P + 1), dict(starts=P + 2),
+        dict(scale=math.nan)])
+
+
+def test_python_refuses():
+    x = torch.zeros(3, 256)
+    half, weight = x.half(), torch.ones(256)
+    rows8 = (torch.zeros(3, 256, dtype=torch.float8_e4m3fn), torch.zeros(3, 4, dtype=torch.float8_e8m0fnu))
+    heads, words = torch.zeros(3, 4, 64), torch.zeros(3, dtype=torch.int32)
+    for call in (lambda: layer.quantize(x), lambda: layer.quantize(x.int()), lambda: layer.quantize(x[0]),
+                 lambda: layer.quantize(x.t()), lambda: layer.rms_norm(x, weight), lambda: layer.rms_norm(x.t(), weight),
+                 lambda: layer.product(rows8, rows8[0], torch.ones(1, 2)),
+                 lambda: layer.product(rows8, rows8[0][:, :128], torch.ones(1, 1)),
+                 lambda: layer.rotary(heads, words, torch.ones(8)), lambda: layer.rotary(heads[0], words, torch.ones(8)),
+                 lambda: layer.attention(heads, heads, heads, words), lambda: layer.attention(heads[0], heads, heads, words),
+                 lambda: layer.attention(heads.int(), heads, heads, words),
+                 lambda: layer.rotary_frequencies(0), lambda: layer.rotary_frequencies(7), lambda: layer.rotary_frequencies(8, 1.0),
+                 lambda: layer.rotary_frequencies(8, factor=0.5), lambda: layer.rotary_frequencies(8, factor=2, original=0)):
+        with pytest.raises(ValueError):
+            call()
+    assert half.dtype == torch.float16
+
+
+def test_frequencies():
+    plain, magnitude = layer.rotary_frequencies(64, 1e6)
+    assert magnitude == 1.0 and plain.dtype == torch.float32
+    want = 1e6 ** (-np.arange(0, 64, 2) / 64)
+    assert np.array_equal(plain.numpy(), want.astype(np.float32))
+    slower, magnitude = layer.rotary_frequencies(64, 1e6, factor=4)
+    assert magnitude == 1.0 and np.array_equal(slower.numpy(), (want / 4).astype(np.float32))
+    original = 32768
+    mixed, magnitude = layer.rotary_frequencies(64, 1e6, factor=4, original=original)
+    assert magnitude == pytest.approx(0.1 * math.log(4) + 1)
+    turns = original * want / (2 * np.pi)
+    share = mixed.numpy() / want
+    assert (share[turns >= 64] == 1).all() or np.allclose(share[turns >= 64], 1, rtol=2.0 ** -23)
+    assert np.allclose(share[turns <= 0.5], 0.25, rtol=2.0 ** -23)
+    assert (np.diff(share) <= 2.0 ** -22).all() and share.min() >= 0.25 * (1 - 2.0 ** -23)
+    same, magnitude = layer.rotary_frequencies(64, 1e6, factor=1.0, original=original)
+    assert magnitude == 1.0 and torch.equal(same, plain)
