@@ -173,9 +173,13 @@ extern "C" int q38hip_prompt_attention(void *output, uint64_t output_row_stride,
         !element_aligned(key, type) || !element_aligned(value, type) || !aligned(row_starts, 4))
         return abi_fail("rows must be aligned to their elements");
     if (!std::isfinite(scale)) return abi_fail("scale must be finite");
+    /* weights are equal where the scale is 0 (and where it is so small); a product with
+     * -infinity must not become NaN there */
+    const float factor = scale * 1.44269504088896340736f;
     const q38::PromptAttention a = {output, query, gate, key, value, output_row_stride, query_row_stride,
                                     query_head_stride, key_row_stride, value_row_stride, row_starts, count, total_rows,
-                                    heads, kv_heads, head_dim, scale * 1.44269504088896340736f, (int)type};
+                                    heads, kv_heads, head_dim, std::fabs(factor) < 0x1p-126f ? 0x1p-126f : factor,
+                                    (int)type};
     return q38::launch_prompt_attention(a, static_cast<hipStream_t>(stream)) ? 1
                                                                              : abi_fail("prompt attention kernel failed");
 }
