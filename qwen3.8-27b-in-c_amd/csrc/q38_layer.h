@@ -66,7 +66,34 @@ struct ProductE4M3 {
     float *partial;
     uint32_t tokens, inputs, outputs, blocks, pitch;
     int type;
+    bool wide;             /* four outputs of a row can be stored at once */
 };
+
+/* How a product is cut: tiles of so many matrix rows by tokens, and parts of the
+ * inputs whose sums are joined by a second launch. */
+enum { kProductFew = 0, kProductTile64, kProductTile128, kProductTile256 };
+struct ProductPlan {
+    int tile;
+    uint32_t splits;
+};
+inline ProductPlan plan_product(uint32_t tokens, uint32_t inputs, uint32_t outputs)
+{
+#ifdef Q38_PLAN
+    return {Q38_PLAN};
+#endif
+    if (tokens <= 16) return {kProductFew, 1};
+    const uint32_t blocks = e4m3_blocks(inputs);
+    const auto fill = [&](uint64_t tiles, uint32_t wanted) {
+        uint64_t splits = tiles >= wanted ? 1 : wanted / tiles;
+        if (splits > blocks / 4) splits = blocks / 4;
+        return splits > 1 ? (uint32_t)splits : 1u;
+    };
+    if (tokens <= 64) return {kProductTile64, fill(layer_up(outputs, 128), 512)};
+    const uint64_t small = (uint64_t)layer_up(outputs, 128) * layer_up(tokens, 128);
+    const uint64_t large = (uint64_t)layer_up(outputs, 256) * layer_up(tokens, 256);
+    if (tokens <= 128 || large < 192) return {kProductTile128, fill(small, 512)};
+    return {kProductTile256, 1};
+}
 
 struct PromptAttention {
     void *output;

@@ -124,9 +124,199 @@ __global__ void __launch_bounds__(kWaves * 64) few_kernel(ProductE4M3 a)
     }
 }
 
+/* ---- tiles --------------------------------------------------------------------- */
+
+#define Q38_LDS __attribute__((address_space(3)))
+
+/* 16 bytes per lane from base + offset to LDS at `to` + 16 lane, without registers;
+ * the compiler does not count it, so the kernel waits itself (tile_barrier) */
+__device__ __forceinline__ void copy_to_lds(const uint8_t *base, uint32_t offset, uint32_t to)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ void tile_barrier()
+{
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+/* A workgroup of GN x GM wavefronts, each with WN x WM tiles of 16 matrix rows by
+ * 16 tokens. */
+template <int N, int M, int GN, int GM>
+struct ProductTile {
+    static constexpr int WN = N, WM = M, kWavesN = GN, kWavesM = GM, kThreads = GN * GM * 64;
+    static constexpr int kRows = N * 16 * GN, kTokens = M * 16 * GM;
+    static constexpr int kStage = (kRows + kTokens) * (int)kE4M3Block;   /* bytes of a block of inputs */
+};
+
+/* Rows of 128 bytes in LDS; the eight 16-byte pieces of row r are turned by r / 2: the
+ * 16 lanes that a 16-byte read serves together (of each 32 the lanes 0..3, 12..15,
+ * 20..27, then the others) find places of their own modulo 256 bytes. */
+__device__ __forceinline__ uint32_t piece_turn(uint32_t row) { return row >> 1 & 7; }
+
+/* The whole product where `splits` is 1, else of a part of the inputs, into
+ * a.partial[split][token][row].  Blocks of inputs go through two stages of LDS: one
+ * is read while the next is on its way. */
+template <typename T, typename Tile>
+__global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a, uint32_t splits)
+{
+    constexpr int WN = Tile::WN, WM = Tile::WM, kWaveCount = Tile::kThreads / 64;
+    constexpr int kRowParts = Tile::kRows / 8 / kWaveCount, kTokenParts = Tile::kTokens / 8 / kWaveCount;
+    static_assert(kRowParts * 8 * kWaveCount == Tile::kRows && kTokenParts * 8 * kWaveCount == Tile::kTokens, "whole copies");
+    __shared__ __align__(1024) uint8_t stages[2][Tile::kStage];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t tiles_n = layer_up(a.outputs, Tile::kRows), tiles_m = layer_up(a.tokens, Tile::kTokens);
+
+    /* Workgroups go round the eight dies; each die gets a run of neighbouring tiles, four token
+     * tiles high, so that its cache serves their rows to several of them. */
+    constexpr uint32_t kDies = 8, kHigh = 4;
+    const uint32_t die = blockIdx.x % kDies, share = gridDim.x / kDies, more = gridDim.x % kDies;
+    uint32_t place = die * share + min(die, more) + blockIdx.x / kDies;
+    const uint32_t split = place / (tiles_n * tiles_m);
+    place -= split * tiles_n * tiles_m;
+    const uint32_t band = place / (kHigh * tiles_n), high = min(kHigh, tiles_m - band * kHigh);
+    place -= band * kHigh * tiles_n;
+    const uint32_t row0 = place / high * Tile::kRows, token0 = (band * kHigh + place % high) * Tile::kTokens;
+    const uint32_t first = (uint64_t)a.blocks * split / splits, end = (uint64_t)a.blocks * (split + 1) / splits;
+
+    /* what this lane copies: 8 rows of 128 bytes at a time */
+    const uint8_t *matrix = a.weight + (uint64_t)row0 * a.inputs, *codes = a.codes + (uint64_t)token0 * a.inputs;
+    uint32_t offset[kRowParts + kTokenParts];
+#pragma unroll
+    for (int i = 0; i < kRowParts + kTokenParts; ++i) {
+        const bool token = i >= kRowParts;
+        const uint32_t r = ((token ? i - kRowParts : i) * kWaveCount + wave) * 8 + lane / 8;
+        const uint32_t last = (token ? a.tokens - token0 : a.outputs - row0) - 1;
+        offset[i] = min(r, last) * a.inputs + ((lane & 7) ^ piece_turn(r)) * 16;
+    }
+    const uint32_t stages_at = (uint32_t)(uintptr_t)(Q38_LDS const void *)stages;
+    const auto load = [&](uint32_t block, uint32_t stage) {
+        const uint32_t left = a.inputs - block * kE4M3Block;     /* inputs from here on */
+#pragma unroll
+        for (int i = 0; i < kRowParts + kTokenParts; ++i) {
+            const bool token = i >= kRowParts;
+            uint32_t from = offset[i];
+            if (left < kE4M3Block) {
+                /* behind a row's end its last piece again: no output sums it */
+                const uint32_t r = ((token ? i - kRowParts : i) * kWaveCount + wave) * 8 + lane / 8;
+                const uint32_t at = ((lane & 7) ^ piece_turn(r)) * 16;
+                from -= at > left - 16 ? at - (left - 16) : 0;
+            }
+            copy_to_lds((token ? codes : matrix) + (uint64_t)block * kE4M3Block, from,
+                        stages_at + stage * Tile::kStage + (i * kWaveCount + wave) * 1024);
+        }
+    };
+
+    const uint32_t wave_row = wave / Tile::kWavesM * (WN * 16), wave_token = wave % Tile::kWavesM * (WM * 16);
+    const float *factors = a.weight_scales + (uint64_t)(min(row0 + wave_row, a.outputs - 1) / kE4M3Block) * a.blocks;
+    const uint32_t *scale_words[WM];
+    uint32_t next[WM];
+#pragma unroll
+    for (int m = 0; m < WM; ++m) {
+        const uint64_t token = min(token0 + wave_token + m * 16 + lane % 16, a.tokens - 1);
+        scale_words[m] = reinterpret_cast<const uint32_t *>(a.scales + token * a.pitch);
+        next[m] = scale_words[m][first / 4];
+    }
+    f32x4 sum[WN][WM] = {};
+    load(first, 0);
+    for (uint32_t block = first, stage = 0; block < end; ++block, stage ^= 1) {
+        tile_barrier();
+        uint32_t scale[WM];
+#pragma unroll
+        for (int m = 0; m < WM; ++m) {
+            asm volatile("" : "+v"(next[m]));            /* has come: the compiler does not wait for copies behind it */
+            scale[m] = next[m] >> block % 4 * 8 & 255u;
+        }
+        const float factor = factors[block];
+        if (block + 1 < end) {
+            if (block % 4 == 3) {
+#pragma unroll
+                for (int m = 0; m < WM; ++m) next[m] = scale_words[m][(block + 1) / 4];
+            }
+            load(block + 1, stage ^ 1);
+        }
+        const uint32_t rows_at = stages_at + stage * Tile::kStage, tokens_at = rows_at + Tile::kRows * kE4M3Block;
+        const auto read = [&](uint32_t from, uint32_t row) {
+            const uint32_t r = row + lane % 16, at = from + r * kE4M3Block, g = lane / 16, turn = piece_turn(r);
+            return both(*(Q38_LDS const i32x4 *)(uintptr_t)(at + (g ^ turn) * 16),
+                        *(Q38_LDS const i32x4 *)(uintptr_t)(at + ((4 + g) ^ turn) * 16));
+        };
+        i32x8 token[WM];
+#pragma unroll
+        for (int m = 0; m < WM; ++m) token[m] = read(tokens_at, wave_token + m * 16);
+        const uint32_t left = a.inputs - block * kE4M3Block;
+        if (left < kE4M3Block) {
+            const bool low = lane / 16 * 16 < left, high = lane / 16 * 16 + 64 < left;
+#pragma unroll
+            for (int m = 0; m < WM; ++m)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) token[m][i] = (i < 4 ? low : high) ? token[m][i] : 0;
+        }
+#pragma unroll
+        for (int n = 0; n < WN; ++n) {
+            const i32x8 rows = read(rows_at, wave_row + n * 16);
+#pragma unroll
+            for (int m = 0; m < WM; ++m)
+                sum[n][m] = add_block<std::is_same_v<T, float>>(sum[n][m], rows, token[m], scale[m], factor);
+        }
+    }
+
+#pragma unroll
+    for (int m = 0; m < WM; ++m) {
+        const uint32_t t = token0 + wave_token + m * 16 + lane % 16;
+        if (t >= a.tokens) continue;
+#pragma unroll
+        for (int n = 0; n < WN; ++n) {
+            const uint32_t r = row0 + wave_row + n * 16 + lane / 16 * 4;
+            if (splits > 1) {
+                float *to = a.partial + ((uint64_t)split * a.tokens + t) * a.outputs + r;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (r + i < a.outputs) to[i] = sum[n][m][i];
+            } else if (a.wide && r + 4 <= a.outputs) {
+                T e[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) e[i] = static_cast<T>(sum[n][m][i]);
+                T *to = static_cast<T *>(a.output) + (uint64_t)t * a.output_row + r;
+                if constexpr (sizeof(T) == 2) *reinterpret_cast<layer_u32x2 *>(to) = __builtin_bit_cast(layer_u32x2, e);
+                else *reinterpret_cast<layer_u32x4 *>(to) = __builtin_bit_cast(layer_u32x4, e);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (r + i < a.outputs) store_output<T>(a, t, r + i, sum[n][m][i]);
+            }
+        }
+    }
+}
+
+/* the parts' sums, in their order */
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(ProductE4M3 a, uint32_t splits)
+{
+    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x, all = (uint64_t)a.tokens * a.outputs;
+    if (i >= all) return;
+    float v = 0.0f;
+    for (uint32_t s = 0; s < splits; ++s) v += a.partial[s * all + i];
+    const uint32_t token = i / a.outputs;
+    store_output<T>(a, token, (uint32_t)(i - (uint64_t)token * a.outputs), v);
+}
+
+template <typename T, typename Tile>
+bool tiled(const ProductE4M3 &a, uint32_t splits, hipStream_t stream)
+{
+    const uint64_t workgroups = (uint64_t)layer_up(a.outputs, Tile::kRows) * layer_up(a.tokens, Tile::kTokens) * splits;
+    if (!launch_kernel(tile_kernel<T, Tile>, dim3(workgroups), dim3(Tile::kThreads), stream, a, splits)) return false;
+    if (splits == 1) return true;
+    return launch_kernel(join_kernel<T>, dim3(((uint64_t)a.tokens * a.outputs + 255) / 256), dim3(256), stream, a, splits);
+}
+
 template <typename T>
 bool product(const ProductE4M3 &a, hipStream_t stream)
 {
+    const ProductPlan plan = plan_product(a.tokens, a.inputs, a.outputs);
+    if (plan.tile == kProductTile256) return tiled<T, ProductTile<8, 4, 2, 4>>(a, plan.splits, stream);
+    if (plan.tile == kProductTile128) return tiled<T, ProductTile<4, 4, 2, 2>>(a, plan.splits, stream);
+    if (plan.tile == kProductTile64) return tiled<T, ProductTile<2, 4, 4, 1>>(a, plan.splits, stream);
     const uint32_t tiles = layer_up(a.outputs, 16);
     const int m = a.tokens <= 16 ? 1 : a.tokens <= 32 ? 2 : 4;
     const dim3 grid(tiles, layer_up(a.tokens, 16 * m));
@@ -136,7 +326,11 @@ bool product(const ProductE4M3 &a, hipStream_t stream)
 
 }  // namespace
 
-uint64_t product_e4m3_workspace_bytes(uint32_t, uint64_t, uint32_t) { return 0; }
+uint64_t product_e4m3_workspace_bytes(uint32_t tokens, uint64_t inputs, uint32_t outputs)
+{
+    const ProductPlan plan = plan_product(tokens, (uint32_t)inputs, outputs);
+    return plan.splits > 1 ? (uint64_t)plan.splits * tokens * outputs * 4 : 0;
+}
 
 bool launch_product_e4m3(const ProductE4M3 &a, hipStream_t stream)
 {
