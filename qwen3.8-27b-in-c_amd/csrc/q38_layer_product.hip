@@ -48,26 +48,28 @@ __device__ __forceinline__ bf16x8 decoded(int low, int high, float scale)
                                    2, 3, 4, 5, 6, 7);
 }
 
-/* sum + factor * the products of a block: element r is matrix row 4 (lane / 16) +
- * r, token lane % 16.  `scale` is the token's scale byte. */
-template <bool kExact>
-__device__ __forceinline__ f32x4 add_block(f32x4 sum, i32x8 matrix, i32x8 token, uint32_t scale, float factor)
+/* the products of a block: element r is matrix row 4 (lane / 16) + r, token lane %
+ * 16.  `scale` is the token's scale byte; that of the matrix operand is 1 (127). */
+__device__ __forceinline__ f32x4 block_product(i32x8 matrix, i32x8 token, uint32_t scale)
 {
-    f32x4 p = {};
-    if constexpr (kExact) {
-        const float power = __uint_as_float(scale << 23);
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(decoded(matrix[2 * q], matrix[2 * q + 1], 1.0f),
-                                                        decoded(token[2 * q], token[2 * q + 1], power), p, 0, 0, 0);
-        factor = scale == 255u ? __uint_as_float(0x7fc00000u) : factor;
-    } else {
-        /* the scale of the matrix operand is 1 (127) */
-        p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(matrix, token, p, 0, 0, 0, 127, 0, (int)scale);
-    }
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(matrix, token, f32x4{}, 0, 0, 0, 127, 0, (int)scale);
+}
+__device__ __forceinline__ f32x4 add_scaled(f32x4 sum, f32x4 p, float factor)
+{
 #pragma unroll
     for (int r = 0; r < 4; ++r) sum[r] = fmaf(p[r], factor, sum[r]);
     return sum;
+}
+/* both for fp32 outputs */
+__device__ __forceinline__ f32x4 add_exact(f32x4 sum, i32x8 matrix, i32x8 token, uint32_t scale, float factor)
+{
+    const float power = __uint_as_float(scale << 23);
+    f32x4 p = {};
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(decoded(matrix[2 * q], matrix[2 * q + 1], 1.0f),
+                                                    decoded(token[2 * q], token[2 * q + 1], power), p, 0, 0, 0);
+    return add_scaled(sum, p, scale == 255u ? __uint_as_float(0x7fc00000u) : factor);
 }
 
 template <typename T>
@@ -106,7 +108,9 @@ __global__ void __launch_bounds__(kWaves * 64) few_kernel(ProductE4M3 a)
         const float s = weight_scales[b];
 #pragma unroll
         for (int m = 0; m < M; ++m) {
-            sum[m] = add_block<std::is_same_v<T, float>>(sum[m], w, load(codes[m]), scales[m][b], s);
+            const i32x8 token = load(codes[m]);
+            if constexpr (std::is_same_v<T, float>) sum[m] = add_exact(sum[m], w, token, scales[m][b], s);
+            else sum[m] = add_scaled(sum[m], block_product(w, token, scales[m][b]), s);
         }
     }
 #pragma unroll
@@ -211,6 +215,7 @@ __global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a
     const float *factors = a.weight_scales + (uint64_t)(min(row0 + wave_row, a.outputs - 1) / kE4M3Block) * a.blocks;
     const uint32_t *scale_words[WM];
     uint32_t next[WM];
+    float next_factor = factors[first];
 #pragma unroll
     for (int m = 0; m < WM; ++m) {
         const uint64_t token = min(token0 + wave_token + m * 16 + lane % 16, a.tokens - 1);
@@ -227,8 +232,10 @@ __global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a
             asm volatile("" : "+v"(next[m]));            /* has come: the compiler does not wait for copies behind it */
             scale[m] = next[m] >> block % 4 * 8 & 255u;
         }
-        const float factor = factors[block];
+        asm volatile("" : "+v"(next_factor));
+        const float factor = next_factor;
         if (block + 1 < end) {
+            next_factor = factors[block + 1];
             if (block % 4 == 3) {
 #pragma unroll
                 for (int m = 0; m < WM; ++m) next[m] = scale_words[m][(block + 1) / 4];
@@ -252,12 +259,33 @@ __global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a
 #pragma unroll
                 for (int i = 0; i < 8; ++i) token[m][i] = (i < 4 ? low : high) ? token[m][i] : 0;
         }
+        if constexpr (std::is_same_v<T, float>) {
 #pragma unroll
-        for (int n = 0; n < WN; ++n) {
-            const i32x8 rows = read(rows_at, wave_row + n * 16);
+            for (int n = 0; n < WN; ++n) {
+                const i32x8 rows = read(rows_at, wave_row + n * 16);
 #pragma unroll
-            for (int m = 0; m < WM; ++m)
-                sum[n][m] = add_block<std::is_same_v<T, float>>(sum[n][m], rows, token[m], scale[m], factor);
+                for (int m = 0; m < WM; ++m) sum[n][m] = add_exact(sum[n][m], rows, token[m], scale[m], factor);
+            }
+        } else {
+            /* a product's result takes longer than the next product's start: the sums of one
+             * row of tiles are formed while the next row's products run */
+            i32x8 rows = read(rows_at, wave_row);
+            f32x4 before[WM];
+#pragma unroll
+            for (int n = 0; n <= WN; ++n) {
+                i32x8 following;
+                if (n + 1 < WN) following = read(rows_at, wave_row + (n + 1) * 16);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int m = 0; m < WM; ++m) {
+                    f32x4 now;
+                    if (n < WN) now = block_product(rows, token[m], scale[m]);
+                    if (n > 0) sum[n - 1][m] = add_scaled(sum[n - 1][m], before[m], factor);
+                    before[m] = now;
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                rows = following;
+            }
         }
     }
 
