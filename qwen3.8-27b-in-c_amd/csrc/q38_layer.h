@@ -69,30 +69,33 @@ struct ProductE4M3 {
     bool wide;             /* four outputs of a row can be stored at once */
 };
 
-/* How a product is cut: tiles of so many matrix rows by tokens, and parts of the
- * inputs whose sums are joined by a second launch. */
+/* How a product is cut: tiles of so many matrix rows by tokens; `whole` of them have
+ * a workgroup each, the inputs of the others are cut into `splits` parts whose sums a
+ * second launch joins, from a workspace of `bytes`. */
 enum { kProductFew = 0, kProductTile64, kProductTile128, kProductTile256 };
+constexpr uint32_t kProductRows[] = {16, 128, 128, 256}, kProductTokens[] = {16, 64, 128, 256};
 struct ProductPlan {
-    int tile;
-    uint32_t splits;
+    uint32_t tile, whole, splits;
+    uint64_t bytes;
 };
 inline ProductPlan plan_product(uint32_t tokens, uint32_t inputs, uint32_t outputs)
 {
-#ifdef Q38_PLAN
-    return {Q38_PLAN};
-#endif
-    if (tokens <= 16) return {kProductFew, 1};
     const uint32_t blocks = e4m3_blocks(inputs);
-    const auto fill = [&](uint64_t tiles, uint32_t wanted) {
-        uint64_t splits = tiles >= wanted ? 1 : wanted / tiles;
-        if (splits > blocks / 4) splits = blocks / 4;
-        return splits > 1 ? (uint32_t)splits : 1u;
+    if (tokens <= 16 || inputs < kE4M3Block) return {kProductFew, 0, 1, 0};
+    const auto tiles_of = [&](uint32_t tile) {
+        return (uint64_t)layer_up(outputs, kProductRows[tile]) * layer_up(tokens, kProductTokens[tile]);
     };
-    if (tokens <= 64) return {kProductTile64, fill(layer_up(outputs, 128), 512)};
-    const uint64_t small = (uint64_t)layer_up(outputs, 128) * layer_up(tokens, 128);
-    const uint64_t large = (uint64_t)layer_up(outputs, 256) * layer_up(tokens, 256);
-    if (tokens <= 128 || large < 192) return {kProductTile128, fill(small, 512)};
-    return {kProductTile256, 1};
+    uint32_t tile = tokens <= 64 ? kProductTile64 : tokens <= 128 || tiles_of(kProductTile256) < 192 ? kProductTile128 : kProductTile256;
+#ifdef Q38_TILE
+    tile = Q38_TILE;
+#endif
+    /* workgroups that the card holds at once */
+    const uint32_t slots = tile == kProductTile256 ? 256 : 512;
+    const uint64_t tiles = tiles_of(tile), rest = tiles % slots;
+    uint64_t splits = rest ? slots / rest : 1;
+    if (splits > blocks / 4) splits = blocks / 4;
+    if (splits < 2) return {tile, (uint32_t)tiles, 1, 0};
+    return {tile, (uint32_t)(tiles - rest), (uint32_t)splits, rest * splits * kProductRows[tile] * kProductTokens[tile] * 4};
 }
 
 struct PromptAttention {

@@ -78,6 +78,24 @@ __device__ __forceinline__ void store_output(const ProductE4M3 &a, uint32_t toke
     static_cast<T *>(a.output)[(uint64_t)token * a.output_row + row] = static_cast<T>(v);
 }
 
+/* four neighbouring rows' outputs of a token, as far as there are rows */
+template <typename T>
+__device__ __forceinline__ void store_four(const ProductE4M3 &a, uint32_t token, uint32_t row, f32x4 v)
+{
+    if (a.wide && row + 4 <= a.outputs) {
+        T e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = static_cast<T>(v[i]);
+        T *to = static_cast<T *>(a.output) + (uint64_t)token * a.output_row + row;
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<layer_u32x2 *>(to) = __builtin_bit_cast(layer_u32x2, e);
+        else *reinterpret_cast<layer_u32x4 *>(to) = __builtin_bit_cast(layer_u32x4, e);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (row + i < a.outputs) store_output<T>(a, token, row + i, v[i]);
+    }
+}
+
 /* 16 matrix rows by 16 * M tokens to a workgroup, whose eight wavefronts take
  * every eighth block of inputs and are summed in LDS in their order. */
 template <typename T, int M>
@@ -153,16 +171,36 @@ struct ProductTile {
     static constexpr int kStage = (kRows + kTokens) * (int)kE4M3Block;   /* bytes of a block of inputs */
 };
 
+using Tile256 = ProductTile<8, 4, 2, 4>;
+using Tile128 = ProductTile<4, 4, 2, 2>;
+using Tile64 = ProductTile<2, 4, 4, 1>;
+static_assert(Tile256::kRows == kProductRows[kProductTile256] && Tile256::kTokens == kProductTokens[kProductTile256], "");
+static_assert(Tile128::kRows == kProductRows[kProductTile128] && Tile128::kTokens == kProductTokens[kProductTile128], "");
+static_assert(Tile64::kRows == kProductRows[kProductTile64] && Tile64::kTokens == kProductTokens[kProductTile64], "");
+
 /* Rows of 128 bytes in LDS; the eight 16-byte pieces of row r are turned by r / 2: the
  * 16 lanes that a 16-byte read serves together (of each 32 the lanes 0..3, 12..15,
  * 20..27, then the others) find places of their own modulo 256 bytes. */
 __device__ __forceinline__ uint32_t piece_turn(uint32_t row) { return row >> 1 & 7; }
 
-/* The whole product where `splits` is 1, else of a part of the inputs, into
- * a.partial[split][token][row].  Blocks of inputs go through two stages of LDS: one
- * is read while the next is on its way. */
+/* tile `place`: bands of four tiles of tokens, along the rows */
+struct TilePlace {
+    uint32_t n, m;
+};
+__device__ __forceinline__ TilePlace tile_place(uint32_t place, uint32_t tiles_n, uint32_t tiles_m)
+{
+    constexpr uint32_t kHigh = 4;
+    const uint32_t band = place / (kHigh * tiles_n), high = min(kHigh, tiles_m - band * kHigh);
+    place -= band * kHigh * tiles_n;
+    return {place / high, band * kHigh + place % high};
+}
+
+/* The first plan.whole tiles are formed by a workgroup each; of the others plan.splits
+ * workgroups sum a part of the inputs each (a block at least), into
+ * a.partial[tile][split][token][row].  Blocks of inputs go through two stages of LDS:
+ * one is read while the next is on its way. */
 template <typename T, typename Tile>
-__global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a, uint32_t splits)
+__global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a, ProductPlan plan)
 {
     constexpr int WN = Tile::WN, WM = Tile::WM, kWaveCount = Tile::kThreads / 64;
     constexpr int kRowParts = Tile::kRows / 8 / kWaveCount, kTokenParts = Tile::kTokens / 8 / kWaveCount;
@@ -171,16 +209,16 @@ __global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t tiles_n = layer_up(a.outputs, Tile::kRows), tiles_m = layer_up(a.tokens, Tile::kTokens);
 
-    /* Workgroups go round the eight dies; each die gets a run of neighbouring tiles, four token
-     * tiles high, so that its cache serves their rows to several of them. */
-    constexpr uint32_t kDies = 8, kHigh = 4;
-    const uint32_t die = blockIdx.x % kDies, share = gridDim.x / kDies, more = gridDim.x % kDies;
-    uint32_t place = die * share + min(die, more) + blockIdx.x / kDies;
-    const uint32_t split = place / (tiles_n * tiles_m);
-    place -= split * tiles_n * tiles_m;
-    const uint32_t band = place / (kHigh * tiles_n), high = min(kHigh, tiles_m - band * kHigh);
-    place -= band * kHigh * tiles_n;
-    const uint32_t row0 = place / high * Tile::kRows, token0 = (band * kHigh + place % high) * Tile::kTokens;
+    /* Workgroups go round the eight dies; each die gets a run of neighbouring tiles, so that its
+     * cache serves their rows to several of them. */
+    constexpr uint32_t kDies = 8;
+    const bool whole = blockIdx.x < plan.whole;
+    const uint32_t index = whole ? blockIdx.x : blockIdx.x - plan.whole, all = whole ? plan.whole : gridDim.x - plan.whole;
+    const uint32_t die = index % kDies, share = all / kDies, more = all % kDies;
+    const uint32_t place = die * share + min(die, more) + index / kDies;
+    const uint32_t rest = place / plan.splits, splits = whole ? 1 : plan.splits, split = whole ? 0 : place - rest * splits;
+    const TilePlace tile = tile_place(whole ? place : plan.whole + rest, tiles_n, tiles_m);
+    const uint32_t row0 = tile.n * Tile::kRows, token0 = tile.m * Tile::kTokens;
     const uint32_t first = (uint64_t)a.blocks * split / splits, end = (uint64_t)a.blocks * (split + 1) / splits;
 
     /* what this lane copies: 8 rows of 128 bytes at a time */
@@ -195,20 +233,12 @@ __global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a
     }
     const uint32_t stages_at = (uint32_t)(uintptr_t)(Q38_LDS const void *)stages;
     const auto load = [&](uint32_t block, uint32_t stage) {
-        const uint32_t left = a.inputs - block * kE4M3Block;     /* inputs from here on */
+        /* of a row's end the last 128 codes, so nothing behind it is read */
+        const uint32_t from = min(block * kE4M3Block, a.inputs - kE4M3Block);
 #pragma unroll
-        for (int i = 0; i < kRowParts + kTokenParts; ++i) {
-            const bool token = i >= kRowParts;
-            uint32_t from = offset[i];
-            if (left < kE4M3Block) {
-                /* behind a row's end its last piece again: no output sums it */
-                const uint32_t r = ((token ? i - kRowParts : i) * kWaveCount + wave) * 8 + lane / 8;
-                const uint32_t at = ((lane & 7) ^ piece_turn(r)) * 16;
-                from -= at > left - 16 ? at - (left - 16) : 0;
-            }
-            copy_to_lds((token ? codes : matrix) + (uint64_t)block * kE4M3Block, from,
+        for (int i = 0; i < kRowParts + kTokenParts; ++i)
+            copy_to_lds((i < kRowParts ? matrix : codes) + from, offset[i],
                         stages_at + stage * Tile::kStage + (i * kWaveCount + wave) * 1024);
-        }
     };
 
     const uint32_t wave_row = wave / Tile::kWavesM * (WN * 16), wave_token = wave % Tile::kWavesM * (WM * 16);
@@ -222,6 +252,12 @@ __global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a
         scale_words[m] = reinterpret_cast<const uint32_t *>(a.scales + token * a.pitch);
         next[m] = scale_words[m][first / 4];
     }
+    /* a lane's pieces lane / 16 and 4 + lane / 16 of row lane % 16 of a tile of 16 rows; tiles
+     * are 2 KiB apart, which the reads' own offsets take */
+    const uint32_t piece = (lane / 16 ^ piece_turn(lane % 16)) * 16;
+    uint32_t rows_at = stages_at + (wave_row + lane % 16) * kE4M3Block + piece;
+    uint32_t tokens_at = stages_at + (Tile::kRows + wave_token + lane % 16) * kE4M3Block + piece;
+    asm volatile("" : "+v"(rows_at), "+v"(tokens_at));
     f32x4 sum[WN][WM] = {};
     load(first, 0);
     for (uint32_t block = first, stage = 0; block < end; ++block, stage ^= 1) {
@@ -242,18 +278,19 @@ __global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a
             }
             load(block + 1, stage ^ 1);
         }
-        const uint32_t rows_at = stages_at + stage * Tile::kStage, tokens_at = rows_at + Tile::kRows * kE4M3Block;
-        const auto read = [&](uint32_t from, uint32_t row) {
-            const uint32_t r = row + lane % 16, at = from + r * kE4M3Block, g = lane / 16, turn = piece_turn(r);
-            return both(*(Q38_LDS const i32x4 *)(uintptr_t)(at + (g ^ turn) * 16),
-                        *(Q38_LDS const i32x4 *)(uintptr_t)(at + ((4 + g) ^ turn) * 16));
+        const uint32_t stage_at = stage * Tile::kStage;
+        const uint32_t row_low = rows_at + stage_at, row_high = row_low ^ 64, token_low = tokens_at + stage_at, token_high = token_low ^ 64;
+        const auto read = [](uint32_t low, uint32_t high, int tile) {
+            return both(*(Q38_LDS const i32x4 *)(uintptr_t)(low + tile * 16 * kE4M3Block),
+                        *(Q38_LDS const i32x4 *)(uintptr_t)(high + tile * 16 * kE4M3Block));
         };
         i32x8 token[WM];
 #pragma unroll
-        for (int m = 0; m < WM; ++m) token[m] = read(tokens_at, wave_token + m * 16);
-        const uint32_t left = a.inputs - block * kE4M3Block;
-        if (left < kE4M3Block) {
-            const bool low = lane / 16 * 16 < left, high = lane / 16 * 16 + 64 < left;
+        for (int m = 0; m < WM; ++m) token[m] = read(token_low, token_high, m);
+        if (a.inputs - block * kE4M3Block < kE4M3Block) {
+            /* the stage begins with codes of the block before: they count as 0 */
+            const uint32_t before = (block + 1) * kE4M3Block - a.inputs;
+            const bool low = lane / 16 * 16 >= before, high = lane / 16 * 16 + 64 >= before;
 #pragma unroll
             for (int m = 0; m < WM; ++m)
 #pragma unroll
@@ -262,19 +299,19 @@ __global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a
         if constexpr (std::is_same_v<T, float>) {
 #pragma unroll
             for (int n = 0; n < WN; ++n) {
-                const i32x8 rows = read(rows_at, wave_row + n * 16);
+                const i32x8 rows = read(row_low, row_high, n);
 #pragma unroll
                 for (int m = 0; m < WM; ++m) sum[n][m] = add_exact(sum[n][m], rows, token[m], scale[m], factor);
             }
         } else {
             /* a product's result takes longer than the next product's start: the sums of one
              * row of tiles are formed while the next row's products run */
-            i32x8 rows = read(rows_at, wave_row);
+            i32x8 rows = read(row_low, row_high, 0);
             f32x4 before[WM];
 #pragma unroll
             for (int n = 0; n <= WN; ++n) {
                 i32x8 following;
-                if (n + 1 < WN) following = read(rows_at, wave_row + (n + 1) * 16);
+                if (n + 1 < WN) following = read(row_low, row_high, n + 1);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int m = 0; m < WM; ++m) {
@@ -289,62 +326,57 @@ __global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a
         }
     }
 
+    if (!whole) {
+        float *part = a.partial + (uint64_t)place * (Tile::kRows * Tile::kTokens);
+#pragma unroll
+        for (int m = 0; m < WM; ++m)
+#pragma unroll
+            for (int n = 0; n < WN; ++n)
+                *reinterpret_cast<f32x4 *>(part + (wave_token + m * 16 + lane % 16) * Tile::kRows + wave_row + n * 16 +
+                                           lane / 16 * 4) = sum[n][m];
+        return;
+    }
 #pragma unroll
     for (int m = 0; m < WM; ++m) {
         const uint32_t t = token0 + wave_token + m * 16 + lane % 16;
-        if (t >= a.tokens) continue;
+        if (t < a.tokens) {
 #pragma unroll
-        for (int n = 0; n < WN; ++n) {
-            const uint32_t r = row0 + wave_row + n * 16 + lane / 16 * 4;
-            if (splits > 1) {
-                float *to = a.partial + ((uint64_t)split * a.tokens + t) * a.outputs + r;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (r + i < a.outputs) to[i] = sum[n][m][i];
-            } else if (a.wide && r + 4 <= a.outputs) {
-                T e[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) e[i] = static_cast<T>(sum[n][m][i]);
-                T *to = static_cast<T *>(a.output) + (uint64_t)t * a.output_row + r;
-                if constexpr (sizeof(T) == 2) *reinterpret_cast<layer_u32x2 *>(to) = __builtin_bit_cast(layer_u32x2, e);
-                else *reinterpret_cast<layer_u32x4 *>(to) = __builtin_bit_cast(layer_u32x4, e);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (r + i < a.outputs) store_output<T>(a, t, r + i, sum[n][m][i]);
-            }
+            for (int n = 0; n < WN; ++n) store_four<T>(a, t, row0 + wave_row + n * 16 + lane / 16 * 4, sum[n][m]);
         }
     }
 }
 
-/* the parts' sums, in their order */
-template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(ProductE4M3 a, uint32_t splits)
+/* the sums of the tiles that were cut, parts in their order; a thread takes four rows of a token */
+template <typename T, typename Tile>
+__global__ void __launch_bounds__(256) join_kernel(ProductE4M3 a, ProductPlan plan)
 {
-    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x, all = (uint64_t)a.tokens * a.outputs;
-    if (i >= all) return;
-    float v = 0.0f;
-    for (uint32_t s = 0; s < splits; ++s) v += a.partial[s * all + i];
-    const uint32_t token = i / a.outputs;
-    store_output<T>(a, token, (uint32_t)(i - (uint64_t)token * a.outputs), v);
+    constexpr uint32_t kFours = Tile::kRows * Tile::kTokens / 4, kWorkgroups = kFours / 256;
+    const uint32_t rest = blockIdx.x / kWorkgroups, four = blockIdx.x % kWorkgroups * 256 + threadIdx.x;
+    const TilePlace tile = tile_place(plan.whole + rest, layer_up(a.outputs, Tile::kRows), layer_up(a.tokens, Tile::kTokens));
+    const uint32_t token = tile.m * Tile::kTokens + four / (Tile::kRows / 4), row = tile.n * Tile::kRows + four % (Tile::kRows / 4) * 4;
+    if (token >= a.tokens || row >= a.outputs) return;
+    const f32x4 *part = reinterpret_cast<const f32x4 *>(a.partial) + (uint64_t)rest * plan.splits * kFours + four;
+    f32x4 sum = part[0];
+    for (uint32_t s = 1; s < plan.splits; ++s) sum += part[(uint64_t)s * kFours];
+    store_four<T>(a, token, row, sum);
 }
 
 template <typename T, typename Tile>
-bool tiled(const ProductE4M3 &a, uint32_t splits, hipStream_t stream)
+bool tiled(const ProductE4M3 &a, const ProductPlan &plan, hipStream_t stream)
 {
-    const uint64_t workgroups = (uint64_t)layer_up(a.outputs, Tile::kRows) * layer_up(a.tokens, Tile::kTokens) * splits;
-    if (!launch_kernel(tile_kernel<T, Tile>, dim3(workgroups), dim3(Tile::kThreads), stream, a, splits)) return false;
-    if (splits == 1) return true;
-    return launch_kernel(join_kernel<T>, dim3(((uint64_t)a.tokens * a.outputs + 255) / 256), dim3(256), stream, a, splits);
+    const uint32_t tiles = layer_up(a.outputs, Tile::kRows) * layer_up(a.tokens, Tile::kTokens), rest = tiles - plan.whole;
+    if (!launch_kernel(tile_kernel<T, Tile>, dim3(plan.whole + rest * plan.splits), dim3(Tile::kThreads), stream, a, plan))
+        return false;
+    return !rest || launch_kernel(join_kernel<T, Tile>, dim3(rest * (Tile::kRows * Tile::kTokens / 1024)), dim3(256), stream, a, plan);
 }
 
 template <typename T>
 bool product(const ProductE4M3 &a, hipStream_t stream)
 {
     const ProductPlan plan = plan_product(a.tokens, a.inputs, a.outputs);
-    if (plan.tile == kProductTile256) return tiled<T, ProductTile<8, 4, 2, 4>>(a, plan.splits, stream);
-    if (plan.tile == kProductTile128) return tiled<T, ProductTile<4, 4, 2, 2>>(a, plan.splits, stream);
-    if (plan.tile == kProductTile64) return tiled<T, ProductTile<2, 4, 4, 1>>(a, plan.splits, stream);
+    if (plan.tile == kProductTile256) return tiled<T, Tile256>(a, plan, stream);
+    if (plan.tile == kProductTile128) return tiled<T, Tile128>(a, plan, stream);
+    if (plan.tile == kProductTile64) return tiled<T, Tile64>(a, plan, stream);
     const uint32_t tiles = layer_up(a.outputs, 16);
     const int m = a.tokens <= 16 ? 1 : a.tokens <= 32 ? 2 : 4;
     const dim3 grid(tiles, layer_up(a.tokens, 16 * m));
@@ -356,8 +388,7 @@ bool product(const ProductE4M3 &a, hipStream_t stream)
 
 uint64_t product_e4m3_workspace_bytes(uint32_t tokens, uint64_t inputs, uint32_t outputs)
 {
-    const ProductPlan plan = plan_product(tokens, (uint32_t)inputs, outputs);
-    return plan.splits > 1 ? (uint64_t)plan.splits * tokens * outputs * 4 : 0;
+    return plan_product(tokens, (uint32_t)inputs, outputs).bytes;
 }
 
 bool launch_product_e4m3(const ProductE4M3 &a, hipStream_t stream)
