@@ -72,8 +72,8 @@ struct ProductE4M3 {
 /* How a product is cut: tiles of so many matrix rows by tokens; `whole` of them have
  * a workgroup each, the inputs of the others are cut into `splits` parts whose sums a
  * second launch joins, from a workspace of `bytes`. */
-enum { kProductFew = 0, kProductTile64, kProductTile128, kProductTile256 };
-constexpr uint32_t kProductRows[] = {16, 128, 128, 256}, kProductTokens[] = {16, 64, 128, 256};
+enum { kProductFew = 0, kProductTile16, kProductTile64, kProductTile128, kProductTile256 };
+constexpr uint32_t kProductRows[] = {16, 128, 128, 128, 256}, kProductTokens[] = {16, 16, 64, 128, 256};
 struct ProductPlan {
     uint32_t tile, whole, splits;
     uint64_t bytes;
@@ -81,11 +81,14 @@ struct ProductPlan {
 inline ProductPlan plan_product(uint32_t tokens, uint32_t inputs, uint32_t outputs)
 {
     const uint32_t blocks = e4m3_blocks(inputs);
-    if (tokens <= 16 || inputs < kE4M3Block) return {kProductFew, 0, 1, 0};
+#ifndef Q38_FEW
+#define Q38_FEW 4
+#endif
+    if (tokens <= Q38_FEW || inputs < kE4M3Block) return {kProductFew, 0, 1, 0};
     const auto tiles_of = [&](uint32_t tile) {
         return (uint64_t)layer_up(outputs, kProductRows[tile]) * layer_up(tokens, kProductTokens[tile]);
     };
-    uint32_t tile = tokens <= 64 ? kProductTile64 : tokens <= 128 || tiles_of(kProductTile256) < 192 ? kProductTile128 : kProductTile256;
+    uint32_t tile = tokens <= 16 ? kProductTile16 : tokens <= 64 ? kProductTile64 : tokens <= 128 || tiles_of(kProductTile256) < 192 ? kProductTile128 : kProductTile256;
 #ifdef Q38_TILE
     tile = Q38_TILE;
 #endif

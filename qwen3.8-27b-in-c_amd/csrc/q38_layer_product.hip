@@ -157,26 +157,45 @@ __device__ __forceinline__ void copy_to_lds(const uint8_t *base, uint32_t offset
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to)
                  : "memory", "m0");
 }
+/* the same with 4 bytes per lane */
+__device__ __forceinline__ void copy_words_to_lds(const void *base, uint32_t offset, uint32_t to)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(base), "s"(to)
+                 : "memory", "m0");
+}
+/* all but the last N copies of this wavefront are in LDS and what it read has
+ * returned; then so for all of the workgroup */
+template <int N>
 __device__ __forceinline__ void tile_barrier()
 {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
 /* A workgroup of GN x GM wavefronts, each with WN x WM tiles of 16 matrix rows by
- * 16 tokens. */
-template <int N, int M, int GN, int GM>
+ * 16 tokens; S blocks of inputs in LDS.  A stage holds the codes of the matrix's rows
+ * and of the tokens, a word with the scale bytes of each token and the factors of the
+ * matrix's blocks. */
+template <int N, int M, int GN, int GM, int S>
 struct ProductTile {
-    static constexpr int WN = N, WM = M, kWavesN = GN, kWavesM = GM, kThreads = GN * GM * 64;
+    static constexpr int WN = N, WM = M, kWavesM = GM, kWaveCount = GN * GM, kThreads = kWaveCount * 64, kStages = S;
     static constexpr int kRows = N * 16 * GN, kTokens = M * 16 * GM;
-    static constexpr int kStage = (kRows + kTokens) * (int)kE4M3Block;   /* bytes of a block of inputs */
+    static constexpr int kScalesAt = (kRows + kTokens) * (int)kE4M3Block;
+    static constexpr int kFactorsAt = kScalesAt + (kTokens < 64 ? 64 : kTokens) * 4;
+    static constexpr int kStage = kFactorsAt + 256;
+    /* copies of 1 KiB of a wavefront; the last ones of the tokens may be some wavefronts' only */
+    static constexpr int kRowParts = kRows / 8 / kWaveCount, kTokenParts = (kTokens / 8 + kWaveCount - 1) / kWaveCount;
+    static constexpr int kLeast = kRowParts + kTokens / 8 / kWaveCount;
+    static_assert(kRowParts * kWaveCount * 8 == kRows && kTokens <= 64 * kWaveCount, "copies of a stage");
+    static_assert(WN * 16 <= (int)kE4M3Block && kE4M3Block % (WN * 16) == 0, "a wavefront's rows have one factor");
 };
-
-using Tile256 = ProductTile<8, 4, 2, 4>;
-using Tile128 = ProductTile<4, 4, 2, 2>;
-using Tile64 = ProductTile<2, 4, 4, 1>;
-static_assert(Tile256::kRows == kProductRows[kProductTile256] && Tile256::kTokens == kProductTokens[kProductTile256], "");
-static_assert(Tile128::kRows == kProductRows[kProductTile128] && Tile128::kTokens == kProductTokens[kProductTile128], "");
-static_assert(Tile64::kRows == kProductRows[kProductTile64] && Tile64::kTokens == kProductTokens[kProductTile64], "");
+using Tile256 = ProductTile<8, 4, 2, 4, 2>;
+using Tile128 = ProductTile<4, 4, 2, 2, 2>;
+using Tile64 = ProductTile<2, 4, 4, 1, 3>;
+using Tile16 = ProductTile<2, 1, 4, 1, 4>;
+template <typename Tile>
+constexpr bool tile_is(int tile) { return (int)kProductRows[tile] == Tile::kRows && (int)kProductTokens[tile] == Tile::kTokens; }
+static_assert(tile_is<Tile256>(kProductTile256) && tile_is<Tile128>(kProductTile128) && tile_is<Tile64>(kProductTile64) &&
+                  tile_is<Tile16>(kProductTile16), "the plan's tiles");
 
 /* Rows of 128 bytes in LDS; the eight 16-byte pieces of row r are turned by r / 2: the
  * 16 lanes that a 16-byte read serves together (of each 32 the lanes 0..3, 12..15,
@@ -197,15 +216,14 @@ __device__ __forceinline__ TilePlace tile_place(uint32_t place, uint32_t tiles_n
 
 /* The first plan.whole tiles are formed by a workgroup each; of the others plan.splits
  * workgroups sum a part of the inputs each (a block at least), into
- * a.partial[tile][split][token][row].  Blocks of inputs go through two stages of LDS:
- * one is read while the next is on its way. */
+ * a.partial[tile][split][token][row].  Blocks of inputs go through stages of LDS: one is
+ * read while the next ones are on their way. */
 template <typename T, typename Tile>
 __global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a, ProductPlan plan)
 {
-    constexpr int WN = Tile::WN, WM = Tile::WM, kWaveCount = Tile::kThreads / 64;
-    constexpr int kRowParts = Tile::kRows / 8 / kWaveCount, kTokenParts = Tile::kTokens / 8 / kWaveCount;
-    static_assert(kRowParts * 8 * kWaveCount == Tile::kRows && kTokenParts * 8 * kWaveCount == Tile::kTokens, "whole copies");
-    __shared__ __align__(1024) uint8_t stages[2][Tile::kStage];
+    constexpr int WN = Tile::WN, WM = Tile::WM, kWaveCount = Tile::kWaveCount, kStages = Tile::kStages;
+    constexpr int kRowParts = Tile::kRowParts, kTokenParts = Tile::kTokenParts;
+    __shared__ __align__(1024) uint8_t stages[kStages * Tile::kStage];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t tiles_n = layer_up(a.outputs, Tile::kRows), tiles_m = layer_up(a.tokens, Tile::kTokens);
 
@@ -232,54 +250,55 @@ __global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a
         offset[i] = min(r, last) * a.inputs + ((lane & 7) ^ piece_turn(r)) * 16;
     }
     const uint32_t stages_at = (uint32_t)(uintptr_t)(Q38_LDS const void *)stages;
-    const auto load = [&](uint32_t block, uint32_t stage) {
+    /* wavefront w copies the words of tokens 64 w on, the last one the factors */
+    const bool has_scales = wave * 64 < Tile::kTokens;
+    const uint8_t *scales = a.scales + (uint64_t)token0 * a.pitch;
+    const uint32_t scale_offset = min(wave * 64 + lane, a.tokens - token0 - 1) * a.pitch;
+    const float *factors = a.weight_scales + (uint64_t)(row0 / kE4M3Block) * a.blocks;
+    constexpr uint32_t kFactors = (Tile::kRows + kE4M3Block - 1) / kE4M3Block;
+    const uint32_t factor_offset = min(lane % kFactors, (a.outputs - 1) / kE4M3Block - row0 / kE4M3Block) * a.blocks * 4;
+    const auto load = [&](uint32_t block, uint32_t stage_at) {
+        if (has_scales) copy_words_to_lds(scales + block / 4 * 4, scale_offset, stage_at + Tile::kScalesAt + wave * 256);
+        if (wave == kWaveCount - 1) copy_words_to_lds(factors + block, factor_offset, stage_at + Tile::kFactorsAt);
         /* of a row's end the last 128 codes, so nothing behind it is read */
         const uint32_t from = min(block * kE4M3Block, a.inputs - kE4M3Block);
 #pragma unroll
         for (int i = 0; i < kRowParts + kTokenParts; ++i)
-            copy_to_lds((i < kRowParts ? matrix : codes) + from, offset[i],
-                        stages_at + stage * Tile::kStage + (i * kWaveCount + wave) * 1024);
+            if (i < Tile::kLeast || (i - kRowParts) * kWaveCount + wave < Tile::kTokens / 8)
+                copy_to_lds((i < kRowParts ? matrix : codes) + from, offset[i], stage_at + (i * kWaveCount + wave) * 1024);
     };
 
     const uint32_t wave_row = wave / Tile::kWavesM * (WN * 16), wave_token = wave % Tile::kWavesM * (WM * 16);
-    const float *factors = a.weight_scales + (uint64_t)(min(row0 + wave_row, a.outputs - 1) / kE4M3Block) * a.blocks;
-    const uint32_t *scale_words[WM];
-    uint32_t next[WM];
-    float next_factor = factors[first];
-#pragma unroll
-    for (int m = 0; m < WM; ++m) {
-        const uint64_t token = min(token0 + wave_token + m * 16 + lane % 16, a.tokens - 1);
-        scale_words[m] = reinterpret_cast<const uint32_t *>(a.scales + token * a.pitch);
-        next[m] = scale_words[m][first / 4];
-    }
     /* a lane's pieces lane / 16 and 4 + lane / 16 of row lane % 16 of a tile of 16 rows; tiles
      * are 2 KiB apart, which the reads' own offsets take */
     const uint32_t piece = (lane / 16 ^ piece_turn(lane % 16)) * 16;
-    uint32_t rows_at = stages_at + (wave_row + lane % 16) * kE4M3Block + piece;
-    uint32_t tokens_at = stages_at + (Tile::kRows + wave_token + lane % 16) * kE4M3Block + piece;
+    uint32_t rows_at = (wave_row + lane % 16) * kE4M3Block + piece;
+    uint32_t tokens_at = (Tile::kRows + wave_token + lane % 16) * kE4M3Block + piece;
     asm volatile("" : "+v"(rows_at), "+v"(tokens_at));
     f32x4 sum[WN][WM] = {};
-    load(first, 0);
-    for (uint32_t block = first, stage = 0; block < end; ++block, stage ^= 1) {
-        tile_barrier();
+    const uint32_t stages_end = stages_at + kStages * Tile::kStage;
+    uint32_t stage_at = stages_at, load_at = stages_at, loaded = first;
+    const auto load_next = [&] {
+        load(loaded++, load_at);
+        load_at += Tile::kStage;
+        if (load_at == stages_end) load_at = stages_at;
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i)
+        if (loaded < end) load_next();
+    for (uint32_t block = first; block < end; ++block) {
+        /* where fewer copies follow than the loop leaves open, all are waited for */
+        if (end - block >= kStages - 1) tile_barrier<(kStages - 2) * Tile::kLeast>();
+        else tile_barrier<0>();
+        if (loaded < end) load_next();
         uint32_t scale[WM];
+        const float factor = *(Q38_LDS const float *)(uintptr_t)(stage_at + Tile::kFactorsAt + wave_row / kE4M3Block * 4);
 #pragma unroll
-        for (int m = 0; m < WM; ++m) {
-            asm volatile("" : "+v"(next[m]));            /* has come: the compiler does not wait for copies behind it */
-            scale[m] = next[m] >> block % 4 * 8 & 255u;
-        }
-        asm volatile("" : "+v"(next_factor));
-        const float factor = next_factor;
-        if (block + 1 < end) {
-            next_factor = factors[block + 1];
-            if (block % 4 == 3) {
-#pragma unroll
-                for (int m = 0; m < WM; ++m) next[m] = scale_words[m][(block + 1) / 4];
-            }
-            load(block + 1, stage ^ 1);
-        }
-        const uint32_t stage_at = stage * Tile::kStage;
+        for (int m = 0; m < WM; ++m)
+            scale[m] = *(Q38_LDS const uint8_t *)(uintptr_t)(stage_at + Tile::kScalesAt + (wave_token + m * 16 + lane % 16) * 4 + block % 4);
         const uint32_t row_low = rows_at + stage_at, row_high = row_low ^ 64, token_low = tokens_at + stage_at, token_high = token_low ^ 64;
+        stage_at += Tile::kStage;
+        if (stage_at == stages_end) stage_at = stages_at;
         const auto read = [](uint32_t low, uint32_t high, int tile) {
             return both(*(Q38_LDS const i32x4 *)(uintptr_t)(low + tile * 16 * kE4M3Block),
                         *(Q38_LDS const i32x4 *)(uintptr_t)(high + tile * 16 * kE4M3Block));
@@ -329,11 +348,14 @@ __global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a
     if (!whole) {
         float *part = a.partial + (uint64_t)place * (Tile::kRows * Tile::kTokens);
 #pragma unroll
-        for (int m = 0; m < WM; ++m)
+        for (int m = 0; m < WM; ++m) {
+            const uint32_t t = wave_token + m * 16 + lane % 16;
+            if (token0 + t < a.tokens) {
 #pragma unroll
-            for (int n = 0; n < WN; ++n)
-                *reinterpret_cast<f32x4 *>(part + (wave_token + m * 16 + lane % 16) * Tile::kRows + wave_row + n * 16 +
-                                           lane / 16 * 4) = sum[n][m];
+                for (int n = 0; n < WN; ++n)
+                    *reinterpret_cast<f32x4 *>(part + t * Tile::kRows + wave_row + n * 16 + lane / 16 * 4) = sum[n][m];
+            }
+        }
         return;
     }
 #pragma unroll
@@ -376,6 +398,7 @@ bool product(const ProductE4M3 &a, hipStream_t stream)
     const ProductPlan plan = plan_product(a.tokens, a.inputs, a.outputs);
     if (plan.tile == kProductTile256) return tiled<T, Tile256>(a, plan, stream);
     if (plan.tile == kProductTile128) return tiled<T, Tile128>(a, plan, stream);
+    if (plan.tile == kProductTile16) return tiled<T, Tile16>(a, plan, stream);
     if (plan.tile == kProductTile64) return tiled<T, Tile64>(a, plan, stream);
     const uint32_t tiles = layer_up(a.outputs, 16);
     const int m = a.tokens <= 16 ? 1 : a.tokens <= 32 ? 2 : 4;
