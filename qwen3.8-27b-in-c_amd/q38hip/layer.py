@@ -27,6 +27,8 @@ BLOCK = 128
 
 E4M3Rows = namedtuple("E4M3Rows", "codes scales")
 
+_CODES, _SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
+_device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 _BOUND = None
 
@@ -56,45 +58,35 @@ def _call(name, index, *arguments):
     """enqueues on torch's current stream of device `index`.  The library launches on the current device, which has to be
     that one: the handle of a default stream is the same on all devices."""
     function = getattr(_BOUND or _lib(), name)
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch._C._cuda_getDevice() == index:
-        ok = function(*arguments, stream)
+    if _device() == index:
+        ok = function(*arguments, _stream(index))
     else:
         with torch.cuda.device(index):
-            ok = function(*arguments, stream)
+            ok = function(*arguments, _stream(index))
     if not ok:
         _check(ok, name)
 
 
-def _type(tensor, name):
-    kind = _TYPES.get(tensor.dtype)
+def _rows(x, name):
+    """(rows, width, row stride, element type, device) of rows that are contiguous each.  One look at each property: small
+    calls cost what they cost the host."""
+    shape, stride, index, kind = x.shape, x.stride(), x.get_device(), _TYPES.get(x.dtype)
+    if len(shape) != 2 or stride[1] != 1 and shape[1] > 1:
+        raise ValueError("%s must be [rows, width] with contiguous rows" % name)
     if kind is None:
         raise ValueError("%s must be float32, float16 or bfloat16" % name)
-    return kind
-
-
-def _device(tensor, name):
-    index = tensor.get_device()
     if index < 0:
         raise ValueError("%s must be on a GPU" % name)
-    return index
+    return shape[0], shape[1], stride[0], kind, index
 
 
 def _alike(tensor, name, x, index):
     """row stride of a tensor of x's shape, type and device with contiguous rows"""
-    if tensor.shape != x.shape or tensor.dtype != x.dtype or tensor.get_device() != index or _broken(tensor):
+    stride = tensor.stride()
+    if tensor.shape != x.shape or tensor.dtype != x.dtype or tensor.get_device() != index or \
+            stride[1] != 1 and x.shape[1] > 1:
         raise ValueError("%s must be rows of the same shape, type and device, each contiguous" % name)
-    return tensor.stride(0)
-
-
-def _broken(tensor):
-    return tensor.dim() != 2 or tensor.stride(1) != 1 and tensor.shape[1] > 1
-
-
-def _rows(x, name="x"):
-    if _broken(x):
-        raise ValueError("%s must be [rows, width] with contiguous rows" % name)
-    return x.shape
+    return stride[0]
 
 
 def scale_pitch(width):
@@ -102,18 +94,19 @@ def scale_pitch(width):
     return -(-width // (4 * BLOCK)) * 4
 
 
-def _e4m3(rows, width, device, into):
+def _e4m3(x, rows, width, index, into):
+    """new rows in 8 bits of x's shape, or the caller's"""
     if into is None:
-        return E4M3Rows(torch.empty((rows, width), dtype=torch.float8_e4m3fn, device=device),
-                        torch.empty((rows, scale_pitch(width)), dtype=torch.float8_e8m0fnu, device=device))
-    _check_e4m3(into, rows, width, device.index)
+        return E4M3Rows(torch.empty_like(x, dtype=_CODES, memory_format=torch.contiguous_format),
+                        x.new_empty((rows, scale_pitch(width)), dtype=_SCALES))
+    _check_e4m3(into, rows, width, index)
     return E4M3Rows(*into)
 
 
 def _check_e4m3(rows8, rows, width, index):
     codes, scales = rows8
-    if codes.dtype != torch.float8_e4m3fn or codes.shape != (rows, width) or not codes.is_contiguous() or \
-            scales.dtype != torch.float8_e8m0fnu or scales.shape != (rows, scale_pitch(width)) or not scales.is_contiguous():
+    if codes.dtype != _CODES or codes.shape != (rows, width) or not codes.is_contiguous() or \
+            scales.dtype != _SCALES or scales.shape != (rows, scale_pitch(width)) or not scales.is_contiguous():
         raise ValueError("rows in 8 bits must be contiguous float8_e4m3fn [%d, %d] and float8_e8m0fnu [%d, %d]"
                          % (rows, width, rows, scale_pitch(width)))
     if codes.get_device() != index or scales.get_device() != index:
@@ -122,11 +115,10 @@ def _check_e4m3(rows8, rows, width, index):
 
 def quantize(x, gate=None, out=None):
     """x [rows, width], or x * silu(gate), in 8 bits; gate has x's shape and type, and a row stride of its own."""
-    rows, width = _rows(x)
-    kind, index = _type(x, "x"), _device(x, "x")
+    rows, width, stride, kind, index = _rows(x, "x")
     gate_row = 0 if gate is None else _alike(gate, "gate", x, index)
-    out = _e4m3(rows, width, x.device, out)
-    _call("q38hip_quantize_e4m3", index, out.codes.data_ptr(), out.scales.data_ptr(), x.data_ptr(), x.stride(0),
+    out = _e4m3(x, rows, width, index, out)
+    _call("q38hip_quantize_e4m3", index, out.codes.data_ptr(), out.scales.data_ptr(), x.data_ptr(), stride,
           None if gate is None else gate.data_ptr(), gate_row, kind, width, rows)
     return out
 
@@ -134,30 +126,29 @@ def quantize(x, gate=None, out=None):
 def rms_norm(x, weight, eps=1e-6, addend=None, offset=0.0, e4m3=False, out=None, total=None):
     """The root-mean-square norm of x [rows, width], or of x + addend, times weight + offset: in x's type, or in 8 bits
     where e4m3 is true.  With an addend the result is (norm, sum); total takes the sum, and may be x or addend."""
-    rows, width = _rows(x)
-    kind, index = _type(x, "x"), _device(x, "x")
-    if weight.shape != (width,) or width > 1 and weight.stride(0) != 1 or weight.get_device() != index:
-        raise ValueError("weight must be a contiguous vector of %d elements on x's device" % width)
-    weight_kind = _type(weight, "weight")
-    addend_row = total_row = 0
+    rows, width, stride, kind, index = _rows(x, "x")
+    weight_kind = _TYPES.get(weight.dtype)
+    if weight_kind is None or weight.shape != (width,) or width > 1 and weight.stride(0) != 1 or weight.get_device() != index:
+        raise ValueError("weight must be a contiguous float32, float16 or bfloat16 vector of %d elements on x's device" % width)
     if addend is not None:
-        addend_row = _alike(addend, "addend", x, index)
+        addend_row, added = _alike(addend, "addend", x, index), addend.data_ptr()
         if total is None:
-            total = torch.empty((rows, width), dtype=x.dtype, device=x.device)
-        total_row = _alike(total, "total", x, index)
-    elif total is not None:
+            total = torch.empty_like(x, memory_format=torch.contiguous_format)
+        total_row, sum_at = _alike(total, "total", x, index), total.data_ptr()
+    elif total is None:
+        addend_row = total_row = 0
+        added = sum_at = None
+    else:
         raise ValueError("total needs an addend")
     if e4m3:
-        out = _e4m3(rows, width, x.device, out)
+        out = _e4m3(x, rows, width, index, out)
         to, to_row, codes, scales = None, 0, out.codes.data_ptr(), out.scales.data_ptr()
     else:
         if out is None:
-            out = torch.empty((rows, width), dtype=x.dtype, device=x.device)
-        to_row = _alike(out, "out", x, index)
-        to, codes, scales = out.data_ptr(), None, None
-    _call("q38hip_rms_norm", index, to, to_row, codes, scales, None if addend is None else total.data_ptr(), total_row,
-          x.data_ptr(), x.stride(0), None if addend is None else addend.data_ptr(), addend_row, kind, weight.data_ptr(),
-          weight_kind, offset, eps, width, rows)
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        to_row, to, codes, scales = _alike(out, "out", x, index), out.data_ptr(), None, None
+    _call("q38hip_rms_norm", index, to, to_row, codes, scales, sum_at, total_row, x.data_ptr(), stride, added, addend_row, kind,
+          weight.data_ptr(), weight_kind, offset, eps, width, rows)
     return out if addend is None else (out, total)
 
 
@@ -167,31 +158,35 @@ _WORKSPACES = {}
 def product(rows8, weight, weight_scales, dtype=torch.bfloat16, out=None):
     """Rows in 8 bits [rows, inputs] times weight [outputs, inputs] (float8_e4m3fn) with weight_scales [ceil(outputs /
     128), ceil(inputs / 128)] (float32): [rows, outputs] of dtype."""
-    codes, scales = rows8
-    if codes.dim() != 2 or weight.dim() != 2 or codes.shape[1] != weight.shape[1]:
+    codes = rows8[0]
+    if codes.dim() != 2 or weight.dim() != 2:
         raise ValueError("expected codes [rows, inputs] and weight [outputs, inputs]")
-    rows, inputs = codes.shape
-    outputs, index = weight.shape[0], _device(weight, "weight")
+    (rows, inputs), (outputs, columns), index = codes.shape, weight.shape, weight.get_device()
+    if weight.dtype != _CODES or columns != inputs or not weight.is_contiguous() or index < 0:
+        raise ValueError("weight must be contiguous float8_e4m3fn [outputs, %d] on a GPU" % inputs)
     _check_e4m3(rows8, rows, inputs, index)
-    if weight.dtype != torch.float8_e4m3fn or not weight.is_contiguous():
-        raise ValueError("weight must be contiguous float8_e4m3fn")
     if weight_scales.dtype != torch.float32 or weight_scales.shape != (-(-outputs // BLOCK), -(-inputs // BLOCK)) or \
             not weight_scales.is_contiguous() or weight_scales.get_device() != index:
         raise ValueError("weight_scales must be contiguous float32 [%d, %d] on the weight's device"
                          % (-(-outputs // BLOCK), -(-inputs // BLOCK)))
     if out is None:
-        out = torch.empty((rows, outputs), dtype=dtype, device=weight.device)
-    elif out.shape != (rows, outputs) or out.get_device() != index or _broken(out):
-        raise ValueError("out must be [%d, %d] with contiguous rows" % (rows, outputs))
-    kind, sizes = _type(out, "out"), (rows, inputs, outputs)
+        out = weight.new_empty((rows, outputs), dtype=dtype)
+        stride = outputs
+    else:
+        stride = out.stride()[0] if out.dim() == 2 else 0
+        if out.shape != (rows, outputs) or out.get_device() != index or out.stride(1) != 1 and outputs > 1:
+            raise ValueError("out must be [%d, %d] with contiguous rows on the weight's device" % (rows, outputs))
+    kind, sizes = _TYPES.get(out.dtype), (rows, inputs, outputs)
+    if kind is None:
+        raise ValueError("the result must be float32, float16 or bfloat16")
     nbytes = _WORKSPACES.get(sizes)
     if nbytes is None:
         nbytes = _lib().q38hip_gemm_e4m3_workspace_bytes(*sizes)
         if len(_WORKSPACES) >= 4096:
             _WORKSPACES.clear()
         _WORKSPACES[sizes] = nbytes
-    work = torch.empty(nbytes, dtype=torch.uint8, device=weight.device) if nbytes else None
-    _call("q38hip_gemm_e4m3", index, out.data_ptr(), kind, out.stride(0), codes.data_ptr(), scales.data_ptr(), rows, inputs,
+    work = weight.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
+    _call("q38hip_gemm_e4m3", index, out.data_ptr(), kind, stride, codes.data_ptr(), rows8[1].data_ptr(), rows, inputs,
           weight.data_ptr(), weight_scales.data_ptr(), outputs, None if work is None else work.data_ptr())
     return out
 
@@ -217,9 +212,15 @@ def rotary_frequencies(turned, base=10000.0, factor=1.0, original=None, fast=32.
 
 
 def _heads(x, name):
-    if x.dim() != 3 or x.stride(2) != 1 and x.shape[2] > 1:
+    """(shape, strides, element type, device) of [rows, heads, head_dim] with contiguous heads"""
+    shape, stride, index, kind = x.shape, x.stride(), x.get_device(), _TYPES.get(x.dtype)
+    if len(shape) != 3 or stride[2] != 1 and shape[2] > 1:
         raise ValueError("%s must be [rows, heads, head_dim] with contiguous heads" % name)
-    return x.shape
+    if kind is None:
+        raise ValueError("%s must be float32, float16 or bfloat16" % name)
+    if index < 0:
+        raise ValueError("%s must be on a GPU" % name)
+    return shape, stride, kind, index
 
 
 def _words(tensor, name, index):
@@ -231,50 +232,59 @@ def _words(tensor, name, index):
 def rotary(x, positions, frequencies, interleaved=False, magnitude=1.0, out=None):
     """Turns the first 2 * len(frequencies) channels of each head of x [rows, heads, head_dim] by positions[row] *
     frequencies[pair]; out may be x."""
-    rows, heads, dim = _heads(x, "x")
-    kind, index = _type(x, "x"), _device(x, "x")
+    (rows, heads, dim), stride, kind, index = _heads(x, "x")
     if _words(positions, "positions", index) != rows:
         raise ValueError("positions must have %d words" % rows)
     if frequencies.dtype != torch.float32 or frequencies.dim() != 1 or not frequencies.is_contiguous() or \
             frequencies.get_device() != index:
         raise ValueError("frequencies must be a contiguous float32 vector on x's device")
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.get_device() != index:
-        raise ValueError("out must be laid out as x")
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        to = (heads * dim, dim)
+    elif out is x:
+        to = stride
     else:
-        _heads(out, "out")
-    _call("q38hip_rotary", index, out.data_ptr(), out.stride(0), out.stride(1), x.data_ptr(), x.stride(0), x.stride(1), kind,
-          rows, heads, dim, positions.data_ptr(), frequencies.data_ptr(), frequencies.shape[0], 1 if interleaved else 0,
-          magnitude)
+        shape, to, out_kind, out_index = _heads(out, "out")
+        if shape != x.shape or out_kind != kind or out_index != index:
+            raise ValueError("out must be laid out as x")
+    _call("q38hip_rotary", index, out.data_ptr(), to[0], to[1], x.data_ptr(), stride[0], stride[1], kind, rows, heads, dim,
+          positions.data_ptr(), frequencies.data_ptr(), frequencies.shape[0], 1 if interleaved else 0, magnitude)
     return out
+
+
+def _key_rows(tensor, name, query, rows, dim, index):
+    """row stride of keys or values: heads next to each other"""
+    shape, stride = tensor.shape, tensor.stride()
+    if len(shape) != 3 or shape[0] != rows or shape[2] != dim or tensor.dtype != query.dtype or tensor.get_device() != index or \
+            stride[2] != 1 or stride[1] != dim and shape[1] > 1:
+        raise ValueError("%s must be [%d, kv_heads, %d] of the queries' type and device, with heads next to each other"
+                         % (name, rows, dim))
+    return stride[0]
 
 
 def attention(query, key, value, row_starts, gate=None, scale=None, out=None):
     """Causal attention of packed prompts: sequence i owns rows row_starts[i] .. row_starts[i + 1] - 1 (int32, on the
     device).  query (and gate, laid out alike) [rows, heads, head_dim], key and value [rows, kv_heads, head_dim] with heads
     next to each other; the result is [rows, heads, head_dim] in their type.  Rows that no sequence owns are not written."""
-    rows, heads, dim = _heads(query, "query")
-    kind, index = _type(query, "query"), _device(query, "query")
-    if key.dim() != 3 or key.shape[0] != rows or key.shape[2] != dim or value.shape != key.shape or \
-            key.dtype != query.dtype or value.dtype != query.dtype:
-        raise ValueError("key and value must be [%d, kv_heads, %d] in the queries' type" % (rows, dim))
-    for tensor in (key, value):
-        if tensor.get_device() != index or tensor.stride(2) != 1 or tensor.shape[1] > 1 and tensor.stride(1) != dim:
-            raise ValueError("key and value must be on the queries' device, with heads next to each other")
-    if gate is not None and (gate.shape != query.shape or gate.stride() != query.stride() or gate.dtype != query.dtype or
+    (rows, heads, dim), stride, kind, index = _heads(query, "query")
+    key_row, value_row = _key_rows(key, "key", query, rows, dim, index), _key_rows(value, "value", query, rows, dim, index)
+    if key.shape != value.shape:
+        raise ValueError("keys and values must have one shape")
+    if gate is not None and (gate.shape != query.shape or gate.stride() != stride or gate.dtype != query.dtype or
                              gate.get_device() != index):
         raise ValueError("the gate must be laid out as the queries")
     count = _words(row_starts, "row_starts", index) - 1
-    if out is None:
-        out = torch.empty((rows, heads, dim), dtype=query.dtype, device=query.device)
-    elif out.shape != query.shape or out.dtype != query.dtype or out.get_device() != index or out.stride(2) != 1 or \
-            heads > 1 and out.stride(1) != dim:
-        raise ValueError("out must be [rows, heads, head_dim] in the queries' type, with heads next to each other")
     if count < 1:
         raise ValueError("row_starts must have an offset for each sequence and one behind the last")
-    _call("q38hip_prompt_attention", index, out.data_ptr(), out.stride(0), query.data_ptr(),
-          None if gate is None else gate.data_ptr(), query.stride(0), query.stride(1), key.data_ptr(), key.stride(0),
-          value.data_ptr(), value.stride(0), kind, heads, key.shape[1], dim, dim ** -0.5 if scale is None else scale,
-          row_starts.data_ptr(), count, rows)
+    if out is None:
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+        out_row = heads * dim
+    else:
+        shape, to, out_kind, out_index = _heads(out, "out")
+        if shape != query.shape or out_kind != kind or out_index != index or heads > 1 and to[1] != dim:
+            raise ValueError("out must be [rows, heads, head_dim] in the queries' type, with heads next to each other")
+        out_row = to[0]
+    _call("q38hip_prompt_attention", index, out.data_ptr(), out_row, query.data_ptr(),
+          None if gate is None else gate.data_ptr(), stride[0], stride[1], key.data_ptr(), key_row, value.data_ptr(), value_row,
+          kind, heads, key.shape[1], dim, dim ** -0.5 if scale is None else scale, row_starts.data_ptr(), count, rows)
     return out
