@@ -166,6 +166,12 @@ __device__ __forceinline__ void copy_to_lds(const void *from, uint32_t to)
 {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory", "m0");
 }
+/* the same from base + offset */
+__device__ __forceinline__ void copy_to_lds(const void *base, uint32_t offset, uint32_t to)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to)
+                 : "memory", "m0");
+}
 /* what this wavefront asked for is in LDS and what it read has returned; then so
  * for all of the workgroup */
 __device__ __forceinline__ void tile_barrier()
@@ -204,6 +210,24 @@ __device__ __forceinline__ float halves_sum(float v)
     const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(p[0]) + __uint_as_float(p[1]);
 }
+/* sum and maximum over the wavefront; every lane is active (rows that a broadcast leaves out add 0) */
+__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v)
+{
+    v += dpp_move<0xB1>(0, (int)v);
+    v += dpp_move<0x4E>(0, (int)v);
+    v += dpp_move<0x141>(0, (int)v);
+    v += dpp_move<0x140>(0, (int)v);
+    v += dpp_move<0x142, 0xA>(0, (int)v);
+    v += dpp_move<0x143, 0xC>(0, (int)v);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v)
+{
+    v = row16_max(v);
+    v = max(v, (uint32_t)dpp_move<0x142, 0xA>(0, (int)v));
+    v = max(v, (uint32_t)dpp_move<0x143, 0xC>(0, (int)v));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
 __device__ __forceinline__ int wave_min(int v)
 {
 #pragma unroll
@@ -211,27 +235,28 @@ __device__ __forceinline__ int wave_min(int v)
     return v;
 }
 
-/* Sizes of a workgroup: kWaves wavefronts of 32 * kGroups columns, tiles of kKeys
- * keys.  A column is a row and one of the query heads that share a key/value head,
- * columns of a row next to each other, so all of a tile's columns read the same
- * keys and values. */
+/* Sizes of a workgroup: kWaves wavefronts of 32 columns, tiles of kKeys keys.  A
+ * column is a row and one of the query heads that share a key/value head, columns of a
+ * row next to each other, so all of a tile's columns read the same keys and values. */
 template <typename T, int D>
 struct PromptTile {
-    static constexpr int kGroups = 1;
     static constexpr int kWaves = 4;
-    /* wavefronts of a SIMD, which share 512 registers a lane: two hide each other's
-     * softmax, but the sums and queries of 256-wide heads alone take 192 */
-    static constexpr int kPerUnit = D == 256 ? 1 : 2;
-    static constexpr int kKeys = sizeof(T) == 4 ? 32 : 64;
+    /* Wavefronts of a SIMD, which share 512 registers a lane: two hide each other's softmax
+     * (bf16, 256-wide heads, 8197 tokens: 835 us, one with twice the keys 1187).  The queries and sums
+     * of 256-wide fp32 heads alone fill the registers of one. */
+    static constexpr int kPerUnit = D * sizeof(T) == 1024 ? 1 : 2;
+    static constexpr int kKeys = sizeof(T) == 4 || D == 256 ? 32 : 64;
     static constexpr int kRowBytes = D * (int)sizeof(T);
     static constexpr int kHalf = kKeys * kRowBytes;          /* keys or values of a tile */
-    static constexpr uint32_t kColumns = kWaves * 32 * kGroups;
+    static constexpr uint32_t kColumns = kWaves * 32;
 };
 
 /* Where 16-byte piece `piece` of row `row` lies in its row in LDS.  Keys are read
  * 16 bytes a lane, 16 rows together, so the turn is the row; 16-bit values are read
  * transposed, 64 bytes of four rows together, so the turn is the row modulo 4 in
- * units of 64 bytes.  Values of fp32 are read along their rows: no turn. */
+ * units of 64 bytes.  Values of fp32 are read along their rows: no turn.  All turns
+ * are bits of the row put elsewhere, so the turn of a sum of rows without common bits is
+ * the exclusive-or of their turns. */
 template <int kRowBytes>
 __device__ __forceinline__ uint32_t key_turn(uint32_t row)
 {
@@ -251,78 +276,85 @@ __device__ __forceinline__ uint32_t value_turn(uint32_t row)
  * from that half: the weights go from one product to the other in registers.  So
  * statistics and rescaling are per lane; one exchange between the halves joins a
  * maximum.  The maximum that weights are relative to is raised only where a score
- * exceeds it by more than 2^8: then the sums are rescaled. */
-template <typename T, int D, bool kWhole>
-__global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64), (PromptTile<T, D>::kPerUnit))
+ * exceeds it by more than 2^8: then the sums are rescaled.
+ *
+ * With kParts = 2 the workgroup has twice the wavefronts; the second half of them takes
+ * every other tile of keys for the same columns, and its sums join the first's through LDS. */
+template <typename T, int D, bool kWhole, int kParts>
+__global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (PromptTile<T, D>::kPerUnit))
     prompt_kernel(PromptAttention a)
 {
     using Tile = PromptTile<T, D>;
-    constexpr int NQ = Tile::kGroups, kWaves = Tile::kWaves;
-    constexpr int kRowBytes = Tile::kRowBytes, kKeys = Tile::kKeys, kHalf = Tile::kHalf;
+    constexpr int kWaves = Tile::kWaves, kRowBytes = Tile::kRowBytes, kKeys = Tile::kKeys, kHalf = Tile::kHalf;
     constexpr int kSteps = kRowBytes / 32;                   /* 16 bytes a lane each */
-    __shared__ __align__(1024) uint8_t tiles[2][2][kHalf];
+    constexpr int kTiles = kKeys / 32;
+    /* of each part keys and values, two of each; then the second part's sums and statistics */
+    constexpr int kTilesBytes = kParts * 4 * kHalf, kJoinBytes = kParts > 1 ? (D / 2 + 2) * 256 * kWaves : 0;
+    __shared__ __align__(1024) uint8_t tiles[kTilesBytes > kJoinBytes ? kTilesBytes : kJoinBytes];
     __shared__ int ranges[kWaves][2];
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t lane = threadIdx.x & 63, part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / kWaves;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % kWaves;
     const uint32_t half = lane >> 5, low = lane & 31;
-    const uint32_t group = a.heads / a.kv_heads, columns = a.rows * group;
-    /* later tiles, which see more, first; workgroups of one key/value head eight apart
-     * where they can be, on one die's cache */
-    const uint32_t kv = blockIdx.x % a.kv_heads;
-    const uint32_t first = (gridDim.x / a.kv_heads - 1 - blockIdx.x / a.kv_heads) * Tile::kColumns + wave * (32 * NQ);
-
-    /* the columns' rows and where their sequences begin */
-    uint32_t row[NQ], head[NQ];
-    int start[NQ], owner[NQ];
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-        const uint32_t column = min(first + q * 32 + low, columns - 1);
-        row[q] = column / group;
-        head[q] = kv * group + column - row[q] * group;
-        start[q] = 0;
-        owner[q] = -1;
+    const uint32_t group = a.heads / a.kv_heads, kv = blockIdx.x % a.kv_heads, place = blockIdx.x / a.kv_heads;
+    /* workgroups of one key/value head are eight apart where they can be, on one die's cache */
+    uint32_t first, columns, row0 = 0;       /* this wavefront's first column, of how many from row row0 on */
+    int start = 0, owner = 0;                /* of the column's sequence */
+    if (a.count <= 64) {
+        /* A lane to a sequence.  Tiles that see most first: tile d of any sequence, as many as it
+         * has, before tile d - 1 of any; behind(d) tiles are d or later of theirs. */
+        const uint32_t i = min(lane, a.count - 1);
+        const int begin = min(max(a.row_starts[i], 0), (int)a.rows), end = min(max(a.row_starts[i + 1], begin), (int)a.rows);
+        const uint32_t mine = lane < a.count ? layer_up((uint32_t)(end - begin) * group, Tile::kColumns) : 0;
+        const auto behind = [&](uint32_t d) { return wave_sum_u32(mine > d ? mine - d : 0); };
+        uint32_t low_d = 0, high_d = wave_max_u32(mine), following = 0;
+        if (place >= behind(0)) return;
+        if (a.count == 1) low_d = high_d - 1 - place, following = place;
+        else while (high_d - low_d > 1) {
+            const uint32_t d = (low_d + high_d) / 2, n = behind(d);
+            if (n > place) low_d = d;
+            else high_d = d, following = n;
+        }
+        uint64_t others = __ballot(mine > low_d);
+        for (uint32_t n = place - following; n; --n) others &= others - 1;
+        const uint32_t sequence = __builtin_ctzll(others);
+        row0 = __builtin_amdgcn_readlane(begin, sequence);
+        columns = (__builtin_amdgcn_readlane(end, sequence) - row0) * group;
+        first = low_d * Tile::kColumns + wave * 32;
+        start = row0;
+    } else {
+        columns = a.rows * group;
+        first = (gridDim.x / a.kv_heads - 1 - place) * Tile::kColumns + wave * 32;
     }
-    const int row_first = (int)(min(first, columns - 1) / group), row_last = (int)(min(first + 32 * NQ - 1, columns - 1) / group);
-    uint32_t at = 0;
-    if (a.count > 64) {                                      /* the last sequence at or before the first row */
-        uint32_t end = a.count + 1;
+    const uint32_t column = min(first + low, columns - 1), row = row0 + column / group, head = kv * group + column % group;
+    if (a.count > 64) {
+        const int row_first = (int)(min(first, columns - 1) / group), row_last = (int)(min(first + 31, columns - 1) / group);
+        owner = -1;
+        uint32_t at = 0, end = a.count + 1;                  /* the last sequence at or before the first row */
         while (at < end) {
             const uint32_t mid = (at + end) / 2;
             if (a.row_starts[mid] <= row_first) at = mid + 1;
             else end = mid;
         }
         at = at ? at - 1 : 0;
-    }
-    for (bool more = true; more && at <= a.count; at += 64) {
-        const int begins = at + lane <= a.count ? a.row_starts[at + lane] : INT32_MAX;
-        for (uint32_t i = 0; i < 64; ++i) {
-            const int begin = __builtin_amdgcn_readlane(begins, i);
-            if (begin > row_last) {
-                more = false;
-                break;
+        for (bool more = true; more && at <= a.count; at += 64) {
+            const int begins = at + lane <= a.count ? a.row_starts[at + lane] : INT32_MAX;
+            for (uint32_t i = 0; i < 64; ++i) {
+                const int begin = __builtin_amdgcn_readlane(begins, i);
+                if (begin > row_last) {
+                    more = false;
+                    break;
+                }
+                if (begin <= (int)row) start = begin, owner = (int)(at + i);
             }
-#pragma unroll
-            for (int q = 0; q < NQ; ++q)
-                if (begin <= (int)row[q]) start[q] = begin, owner[q] = (int)(at + i);
         }
+        start = min(max(start, 0), (int)row);
     }
-    int lowest = INT32_MAX, highest = -1, latest = 0, earliest = INT32_MAX;
-    bool owned[NQ];
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-        owned[q] = first + q * 32 + low < columns && owner[q] >= 0 && owner[q] < (int)a.count;
-        start[q] = min(max(start[q], 0), (int)row[q]);
-        if (owned[q]) {
-            lowest = min(lowest, start[q]);
-            latest = max(latest, start[q]);
-            highest = max(highest, (int)row[q]);
-            earliest = min(earliest, (int)row[q]);
-        }
-    }
+    const bool owned = first + low < columns && owner >= 0 && owner < (int)a.count;
     /* the wavefront's keys: some column sees lowest .. highest, all see latest .. earliest */
-    lowest = __builtin_amdgcn_readfirstlane(wave_min(lowest));
-    highest = -__builtin_amdgcn_readfirstlane(wave_min(-highest));
-    latest = -__builtin_amdgcn_readfirstlane(wave_min(-latest));
-    earliest = __builtin_amdgcn_readfirstlane(wave_min(earliest));
+    const int lowest = __builtin_amdgcn_readfirstlane(wave_min(owned ? start : INT32_MAX));
+    const int highest = -__builtin_amdgcn_readfirstlane(wave_min(owned ? -(int)row : 1));
+    const int latest = -__builtin_amdgcn_readfirstlane(wave_min(owned ? -start : 0));
+    const int earliest = __builtin_amdgcn_readfirstlane(wave_min(owned ? (int)row : INT32_MAX));
     if (lane == 0) ranges[wave][0] = lowest, ranges[wave][1] = highest;
     __syncthreads();
     int from = INT32_MAX, to = -1;
@@ -333,227 +365,246 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64), (PromptTile<T
     if (to < 0) return;
 
     /* queries, 16 bytes of each 32, in registers throughout; a negative scale turns their sign */
-    u32x4 query[NQ][kSteps];
-    uint64_t query_at[NQ];
+    constexpr int E = 16 / (int)sizeof(T);
+    u32x4 query[kSteps];
+    const uint64_t query_at = (uint64_t)row * a.query_row + (uint64_t)head * a.query_head;
     const float scale = fabsf(a.scale);
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-        query_at[q] = (uint64_t)row[q] * a.query_row + (uint64_t)head[q] * a.query_head;
-        const T *p = static_cast<const T *>(a.query) + query_at[q];
+    for (int u = 0; u < kSteps; ++u) {
+        const T *p = static_cast<const T *>(a.query) + query_at + (2 * u + half) * E;
+        if constexpr (kWhole) {
+            query[u] = *reinterpret_cast<const u32x4 *>(p);
+        } else {
+            T e[E];
 #pragma unroll
-        for (int u = 0; u < kSteps; ++u) {
-            constexpr int E = 16 / (int)sizeof(T);
-            if constexpr (kWhole) {
-                query[q][u] = *reinterpret_cast<const u32x4 *>(p + (2 * u + half) * E);
-            } else {
-                T e[E];
-#pragma unroll
-                for (int i = 0; i < E; ++i) e[i] = p[(2 * u + half) * E + i];
-                query[q][u] = __builtin_bit_cast(u32x4, e);
-            }
-            if (a.scale < 0) query[q][u] ^= sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+            for (int i = 0; i < E; ++i) e[i] = p[i];
+            query[u] = __builtin_bit_cast(u32x4, e);
         }
+        if (a.scale < 0) query[u] ^= sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
     }
 
     const T *keys = static_cast<const T *>(a.key) + kv * D, *values = static_cast<const T *>(a.value) + kv * D;
-    const uint32_t tiles_at = lds_address(tiles);
-    /* the keys and values from `key` on into a buffer; behind the last that any column
-     * sees, that one again (what lies behind the sequences may be anything) */
-    const auto load = [&](int key, uint32_t buffer) {
-        constexpr int kParts = kHalf / 1024;
-        static_assert(kParts % kWaves == 0, "whole copies of each wavefront");
+    const uint32_t tiles_at = lds_address(tiles) + part * (4 * kHalf);
+    /* The keys or values of rows `key` on into a buffer; behind the last that any column
+     * sees, that one again (what lies behind the sequences may be anything).  A copy is 1 KiB:
+     * kCopyRows rows, the lane's is lane_row of them. */
+    constexpr int kCopyRows = 1024 / kRowBytes, kCopies = kHalf / 1024 / kWaves;
+    static_assert(kCopyRows * kRowBytes == 1024 && kCopies * kWaves * 1024 == kHalf, "whole copies of each wavefront");
+    const uint32_t lane_row = lane * 16 / kRowBytes, lane_piece = lane * 16 % kRowBytes / 16, wave_row = wave * kCopyRows;
+    const uint32_t key_bytes = (uint32_t)a.key_row * sizeof(T), value_bytes = (uint32_t)a.value_row * sizeof(T);
+    const uint32_t key_lane = lane_piece ^ key_turn<kRowBytes>(wave_row + lane_row);
+    const uint32_t value_lane = lane_piece ^ value_turn<T, kRowBytes>(wave_row + lane_row);
+    const auto load = [&](bool value, int key, uint32_t buffer) {
+        const T *base = value ? values : keys;
+        const uint64_t stride = value ? a.value_row : a.key_row;
+        const bool inside = kWhole && key + kKeys - 1 <= to;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const T *base = h ? values : keys;
-            const uint64_t stride = h ? a.value_row : a.key_row;
+        for (int i = 0; i < kCopies; ++i) {
+            const uint32_t r = i * kWaves * kCopyRows;           /* without wave_row and lane_row, whose bits it has not */
+            const uint32_t piece = value ? value_lane ^ value_turn<T, kRowBytes>(r) : key_lane ^ key_turn<kRowBytes>(r);
+            const uint32_t where = tiles_at + (value ? 2 * kHalf : 0) + buffer * kHalf + (i * kWaves + wave) * 1024;
+            if (inside) {
+                copy_to_lds(base + (key + r + wave_row) * stride, lane_row * (value ? value_bytes : key_bytes) + piece * 16, where);
+                continue;
+            }
+            const T *p = base + (uint64_t)min(key + (int)(r + wave_row + lane_row), to) * stride + piece * E;
+            if constexpr (kWhole) {
+                copy_to_lds(p, where);
+            } else {
+                T e[E];
 #pragma unroll
-            for (int i = 0; i < kParts / kWaves; ++i) {
-                const uint32_t place = (i * kWaves + wave) * 1024 + lane * 16;
-                const uint32_t r = place / kRowBytes, piece = place % kRowBytes / 16;
-                const uint32_t turn = h ? value_turn<T, kRowBytes>(r) : key_turn<kRowBytes>(r);
-                const T *p = base + (uint64_t)min(key + (int)r, to) * stride + (piece ^ turn) * (16 / sizeof(T));
-                const uint32_t where = tiles_at + buffer * (2 * kHalf) + h * kHalf + (i * kWaves + wave) * 1024;
-                if constexpr (kWhole) {
-                    copy_to_lds(p, where);
-                } else {
-                    T e[16 / sizeof(T)];
-#pragma unroll
-                    for (int j = 0; j < 16 / (int)sizeof(T); ++j) e[j] = p[j];
-                    *(Q38_LDS u32x4 *)(uintptr_t)(where + lane * 16) = __builtin_bit_cast(u32x4, e);
-                }
+                for (int j = 0; j < E; ++j) e[j] = p[j];
+                *(Q38_LDS u32x4 *)(uintptr_t)(where + lane * 16) = __builtin_bit_cast(u32x4, e);
             }
         }
     };
 
-    f32x16 out[NQ][D / 32] = {};
-    float top[NQ], total[NQ];
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) top[q] = -INFINITY, total[q] = 0.0f;
+    f32x16 out[D / 32] = {};
+    float top = -INFINITY, base = 0.0f, total = 0.0f;
 
-    load(from, 0);
+    /* piece 2 u + half of key row 32 t + low; `lane_at` holds what is the lane's of its place */
+    const uint32_t key_lane_at = low * kRowBytes + (half ^ key_turn<kRowBytes>(low)) * 16;
+    const auto key_piece = [](uint32_t lane_at, int t, int u) {
+        return lds_read<u32x4>((lane_at ^ u % 8 * 32) + t * 32 * kRowBytes + u / 8 * 256);
+    };
+    /* Keys 16 s on of 32 channels from 32 d on, as O^T's product takes them, 16-bit.  A transposed
+     * read: 16 lanes name four rows of 16 neighbours, four lanes a row, and get a column of four
+     * each.  A lane of fp32 reads one value of row 4 half and rows from there. */
+    const uint32_t i16 = lane & 15, value_row = half * 4 + (sizeof(T) == 2 ? i16 / 4 : 0);
+    const uint32_t value_lane_at =
+        value_row * kRowBytes +
+        (sizeof(T) == 2 ? (i16 & 1) * 8 + (((lane >> 4 & 1) * 2 + (i16 & 3) / 2) ^ value_turn<T, kRowBytes>(value_row)) * 16 : low * 4);
+    const auto value_piece = [](uint32_t lane_at, int s, int d) {
+        s16x4 part[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const uint32_t turned = lane_at ^ (d % 4 * 4 ^ value_turn<T, kRowBytes>(b * 8)) * 16;
+            part[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (Q38_LDS s16x4 *)(uintptr_t)(turned + (s * 16 + b * 8) * kRowBytes + d / 4 * 256));
+        }
+        return __builtin_bit_cast(u32x4, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+
+    /* one tile of each part at a time; where a part has none left it waits with the others */
+    if (from + (int)part * kKeys <= to) {
+        load(false, from + part * kKeys, 0);
+        load(true, from + part * kKeys, 0);
+    }
     uint32_t buffer = 0;
-    for (int key = from; key <= to; key += kKeys, buffer ^= 1) {
+    for (int tile = from; tile <= to; tile += kParts * kKeys, buffer ^= 1) {
+        const int key = tile + part * kKeys;
         tile_barrier();
-        if (key + kKeys <= to) load(key + kKeys, buffer ^ 1);
+        if (key + kParts * kKeys <= to) {
+            load(false, key + kParts * kKeys, buffer ^ 1);
+            load(true, key + kParts * kKeys, buffer ^ 1);
+        }
         if (key > highest || key + kKeys <= lowest) continue;
-        const uint32_t key_at = tiles_at + buffer * (2 * kHalf), value_at = key_at + kHalf;
-        f32x16 score[kKeys / 32][NQ] = {};
+        uint32_t key_at = tiles_at + buffer * kHalf + key_lane_at, value_at = tiles_at + (2 + buffer) * kHalf + value_lane_at;
+        asm volatile("" : "+v"(key_at), "+v"(value_at));     /* turned anew for each tile: places kept would fill registers */
+        f32x16 score[kTiles] = {};
 #pragma unroll
-        for (int t = 0; t < kKeys / 32; ++t)
+        for (int u = 0; u < kSteps; ++u)
 #pragma unroll
-            for (int u = 0; u < kSteps; ++u) {
-                const uint32_t r = t * 32 + low;
-                const u32x4 k = lds_read<u32x4>(key_at + r * kRowBytes + ((2 * u + half) ^ key_turn<kRowBytes>(r)) * 16);
-#pragma unroll
-                for (int q = 0; q < NQ; ++q) score[t][q] = multiply<T>(k, query[q][u], score[t][q]);
-            }
+            for (int t = 0; t < kTiles; ++t) score[t] = multiply<T>(key_piece(key_at, t, u), query[u], score[t]);
         if (key < latest || key + kKeys - 1 > earliest) {
+            const uint32_t span = row - start, begin = key + 4 * half - start;
 #pragma unroll
-            for (int q = 0; q < NQ; ++q) {
-                const uint32_t span = row[q] - start[q], base = key + 4 * half - start[q];
+            for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-                for (int t = 0; t < kKeys / 32; ++t)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (base + (t * 32 + r / 4 * 8 + r % 4) > span) score[t][q][r] = -INFINITY;
-            }
+                for (int r = 0; r < 16; ++r)
+                    if (begin + (t * 32 + r / 4 * 8 + r % 4) > span) score[t][r] = -INFINITY;
         }
-        u32x4 weight[NQ][kKeys / 16];
+        float most = score[0][0];
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-            float most = score[0][q][0];
+        for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-            for (int t = 0; t < kKeys / 32; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) most = fmaxf(most, score[t][q][r]);
-            most = halves_max(most) * scale;
-            if (__any(most > top[q] + 8.0f)) {
-                const float higher = fmaxf(top[q], most);
-                const float shrink = __builtin_amdgcn_exp2f(top[q] - (higher == -INFINITY ? 0.0f : higher));
-                top[q] = higher;
-                total[q] *= shrink;
-#pragma unroll
-                for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) out[q][d][r] *= shrink;
-            }
+            for (int r = 0; r < 16; ++r) most = fmaxf(most, score[t][r]);
+        most = halves_max(most) * scale;
+        if (__any(most > top + 8.0f)) {
+            const float before = top;
+            top = fmaxf(top, most);
             /* nothing but -infinity so far: differences would be NaN, weights are 0 */
-            const float base = top[q] == -INFINITY ? 0.0f : top[q];
+            base = top == -INFINITY ? 0.0f : top;
+            const float shrink = __builtin_amdgcn_exp2f(before - base);
+            total *= shrink;
 #pragma unroll
-            for (int t = 0; t < kKeys / 32; ++t) {
+            for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    score[t][q][r] = __builtin_amdgcn_exp2f(fmaf(score[t][q][r], scale, -base));
-                    total[q] += score[t][q][r];
-                }
-                if constexpr (sizeof(T) == 2) {
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        T e[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) e[j] = static_cast<T>(score[t][q][s * 8 + j]);
-                        weight[q][t * 2 + s] = __builtin_bit_cast(u32x4, e);
-                    }
-                }
-            }
+                for (int r = 0; r < 16; ++r) out[d][r] *= shrink;
         }
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                score[t][r] = __builtin_amdgcn_exp2f(fmaf(score[t][r], scale, -base));
+                total += score[t][r];
+            }
         if constexpr (sizeof(T) == 2) {
-            /* a transposed read: 16 lanes name four rows of 16 neighbours, four lanes a row,
-             * and get a column of four each */
-            const uint32_t i = lane & 15, d16 = lane >> 4 & 1;
 #pragma unroll
-            for (int s = 0; s < kKeys / 16; ++s)
+            for (int s = 0; s < kKeys / 16; ++s) {
+                T e[8];
 #pragma unroll
-                for (int d = 0; d < D / 32; ++d) {
-                    s16x4 part[2];
+                for (int j = 0; j < 8; ++j) e[j] = static_cast<T>(score[s / 2][s % 2 * 8 + j]);
+                const u32x4 weight = __builtin_bit_cast(u32x4, e);
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const uint32_t r = s * 16 + b * 8 + half * 4 + i / 4, piece = d * 4 + d16 * 2 + (i & 3) / 2;
-                        const uint32_t place = r * kRowBytes + (piece ^ value_turn<T, kRowBytes>(r)) * 16 + (i & 1) * 8;
-                        part[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Q38_LDS s16x4 *)(uintptr_t)(value_at + place));
-                    }
-                    const u32x4 v = __builtin_bit_cast(u32x4, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                    for (int q = 0; q < NQ; ++q) out[q][d] = multiply<T>(v, weight[q][s], out[q][d]);
-                }
+                for (int d = 0; d < D / 32; ++d) out[d] = multiply<T>(value_piece(value_at, s, d), weight, out[d]);
+            }
         } else {
 #pragma unroll
             for (int r = 0; r < 16; ++r)
 #pragma unroll
-                for (int d = 0; d < D / 32; ++d) {
-                    const uint32_t place = (r / 4 * 8 + half * 4 + r % 4) * kRowBytes + (d * 32 + low) * 4;
-                    const float v = lds_read<float>(value_at + place);
+                for (int d = 0; d < D / 32; ++d)
+                    out[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(
+                        lds_read<float>(value_at + (r / 4 * 8 + r % 4) * kRowBytes + d * 128), score[0][r], out[d], 0, 0, 0);
+        }
+    }
+
+    if constexpr (kParts > 1) {
+        tile_barrier();                                      /* the tiles have been read */
+        f32x4 *sums = reinterpret_cast<f32x4 *>(tiles) + (wave * (D / 8)) * 64 + lane;
+        float *statistics = reinterpret_cast<float *>(tiles + D / 2 * 256 * kWaves) + wave * 128 + lane;
+        if (part) {
 #pragma unroll
-                    for (int q = 0; q < NQ; ++q)
-                        out[q][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, score[0][q][r], out[q][d], 0, 0, 0);
-                }
+            for (int i = 0; i < D / 8; ++i)
+                sums[i * 64] = f32x4{out[i / 4][i % 4 * 4], out[i / 4][i % 4 * 4 + 1], out[i / 4][i % 4 * 4 + 2], out[i / 4][i % 4 * 4 + 3]};
+            statistics[0] = top;
+            statistics[64] = total;
+        }
+        __syncthreads();
+        if (part) return;
+        const float other = statistics[0], higher = fmaxf(top, other), both = higher == -INFINITY ? 0.0f : higher;
+        const float mine = __builtin_amdgcn_exp2f(top - both), theirs = __builtin_amdgcn_exp2f(other - both);
+        total = total * mine + statistics[64] * theirs;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+            const f32x4 v = sums[i * 64];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out[i / 4][i % 4 * 4 + j] = out[i / 4][i % 4 * 4 + j] * mine + v[j] * theirs;
         }
     }
 
     /* A weight of 0 times a value that is not finite is NaN, so such values of rows that a
      * column does not see have got into its sums.  Whatever came out not finite is done
      * again, row by row, from the rows that it sees. */
+    const float inverse = 1.0f / halves_sum(total);
+    float nothing = 0.0f;
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-        const float inverse = 1.0f / halves_sum(total[q]);
-        float nothing = 0.0f;
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            out[d][r] *= inverse;
+            nothing = fmaf(out[d][r], 0.0f, nothing);
+        }
+    const uint64_t found = __ballot(owned && nothing != 0.0f);
+    uint32_t again = (uint32_t)(found | found >> 32);
+    if (owned && !(again >> low & 1)) {
+        T *to_row = static_cast<T *>(a.output) + (uint64_t)row * a.output_row + (uint64_t)head * D;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                out[q][d][r] *= inverse;
-                nothing = fmaf(out[q][d][r], 0.0f, nothing);
-            }
-        const uint64_t found = __ballot(owned[q] && nothing != 0.0f);
-        uint32_t again = (uint32_t)(found | found >> 32);
-        if (owned[q] && !(again >> low & 1)) {
-            T *to_row = static_cast<T *>(a.output) + (uint64_t)row[q] * a.output_row + (uint64_t)head[q] * D;
-#pragma unroll
-            for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint32_t channel = d * 32 + r * 8 + half * 4;
-                    T e[4];
-                    if (a.gate) {
-                        const T *gate = static_cast<const T *>(a.gate) + query_at[q] + channel;
-                        if constexpr (kWhole && sizeof(T) == 2) {
-                            *reinterpret_cast<layer_u32x2 *>(e) = *reinterpret_cast<const layer_u32x2 *>(gate);
-                        } else if constexpr (kWhole) {
-                            *reinterpret_cast<u32x4 *>(e) = *reinterpret_cast<const u32x4 *>(gate);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) e[j] = gate[j];
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float v = out[q][d][r * 4 + j];
-                        if (a.gate) v *= __builtin_amdgcn_rcpf(1.0f + __expf(-static_cast<float>(e[j])));
-                        e[j] = static_cast<T>(v);
-                    }
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t channel = d * 32 + r * 8 + half * 4;
+                T e[4];
+                if (a.gate) {
+                    const T *gate = static_cast<const T *>(a.gate) + query_at + channel;
                     if constexpr (kWhole && sizeof(T) == 2) {
-                        *reinterpret_cast<layer_u32x2 *>(to_row + channel) = *reinterpret_cast<const layer_u32x2 *>(e);
+                        *reinterpret_cast<layer_u32x2 *>(e) = *reinterpret_cast<const layer_u32x2 *>(gate);
                     } else if constexpr (kWhole) {
-                        *reinterpret_cast<u32x4 *>(to_row + channel) = *reinterpret_cast<const u32x4 *>(e);
+                        *reinterpret_cast<u32x4 *>(e) = *reinterpret_cast<const u32x4 *>(gate);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) to_row[channel + j] = e[j];
+                        for (int j = 0; j < 4; ++j) e[j] = gate[j];
                     }
                 }
-        }
-        while (again) {
-            const uint32_t column = first + q * 32 + __builtin_ctz(again);
-            again &= again - 1;
-            attend_row<T, D, kWhole>(a, column / group, kv * group + column % group, lane);
-        }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float v = out[d][r * 4 + j];
+                    if (a.gate) v *= __builtin_amdgcn_rcpf(1.0f + __expf(-static_cast<float>(e[j])));
+                    e[j] = static_cast<T>(v);
+                }
+                if constexpr (kWhole && sizeof(T) == 2) {
+                    *reinterpret_cast<layer_u32x2 *>(to_row + channel) = *reinterpret_cast<const layer_u32x2 *>(e);
+                } else if constexpr (kWhole) {
+                    *reinterpret_cast<u32x4 *>(to_row + channel) = *reinterpret_cast<const u32x4 *>(e);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) to_row[channel + j] = e[j];
+                }
+            }
+    }
+    while (again) {
+        const uint32_t which = first + __builtin_ctz(again);
+        again &= again - 1;
+        attend_row<T, D, kWhole>(a, row0 + which / group, kv * group + which % group, lane);
     }
 }
 
 template <typename T, int D>
 bool attention(const PromptAttention &a, hipStream_t stream)
 {
+    /* 16-byte aligned rows, eight of which 32 bits span */
     const auto whole = [](const void *p, uint64_t stride) {
-        return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * sizeof(T) % 16 == 0;
+        return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * sizeof(T) % 16 == 0 && stride < 1u << 26;
     };
     const bool wide = whole(a.query, a.query_row) && whole(a.gate, a.query_head) && whole(a.key, a.key_row) &&
                       whole(a.value, a.value_row) && whole(a.output, a.output_row);
@@ -565,9 +616,20 @@ bool attention(const PromptAttention &a, hipStream_t stream)
     if (a.rows <= (sizeof(T) == 4 ? 128 : 64))
         return launch_kernel(wide ? row_kernel<T, D, true> : row_kernel<T, D, false>, dim3(layer_up(a.rows * a.heads, 4)), dim3(256),
                              stream, a);
+    /* a tile more for each sequence where tiles follow them */
     const uint32_t columns = a.rows * (a.heads / a.kv_heads);
-    const dim3 grid(layer_up(columns, PromptTile<T, D>::kColumns) * a.kv_heads);
-    return launch_kernel(wide ? prompt_kernel<T, D, true> : prompt_kernel<T, D, false>, grid, dim3(PromptTile<T, D>::kWaves * 64), stream, a);
+    const dim3 grid((layer_up(columns, PromptTile<T, D>::kColumns) + (a.count <= 64 ? a.count : 0)) * a.kv_heads);
+    /* Tiles that do not fill the card twice over: both halves of the registers go to one of them,
+     * unless keys are few.  Two parts against one, in us: bf16, 24 heads of 256, 1024 tokens (192
+     * tiles) 45 against 62, 2048 (384) 81 against 119, 3500 (660) 198 against 203, 24 prompts of up to 333 (520)
+     * 55 against 34; 32 heads of 128, 512 tokens (128) 17 against 18, 2048 (512) 53 against 58, 3500 (880)
+     * 130 against 118, 100 (32) 10.8 against 9.6. */
+    if constexpr (D * sizeof(T) < 1024)
+        if (grid.x <= 512 + a.count * a.kv_heads && a.rows >= 256 * a.count)
+            return launch_kernel(wide ? prompt_kernel<T, D, true, 2> : prompt_kernel<T, D, false, 2>, grid,
+                                 dim3(PromptTile<T, D>::kWaves * 128), stream, a);
+    return launch_kernel(wide ? prompt_kernel<T, D, true, 1> : prompt_kernel<T, D, false, 1>, grid,
+                         dim3(PromptTile<T, D>::kWaves * 64), stream, a);
 }
 
 template <typename T>
