@@ -80,25 +80,43 @@ struct ProductPlan {
 };
 inline ProductPlan plan_product(uint32_t tokens, uint32_t inputs, uint32_t outputs)
 {
+    /* A second launch costs 4 us, which small matrices do not repay: few tokens by 16 rows a
+     * workgroup, its wavefronts each a part of the inputs, against tiles, in us: 1 token, 5120 x 5120
+     * 8.3 against 11.4, 17408 x 5120 22 against 18; 4 tokens, 5120 x 5120 9.8 against 11.3, 5120 x 14336
+     * 16.7 against 14.7; 16 tokens, 5120 x 1024 7.6 against 11.6; 8 tokens, 5120 x 14336 18 against 15. */
+    const uint64_t codes = (uint64_t)inputs * outputs;
+    if ((tokens <= 4 && codes <= 1u << 25) || (tokens <= 16 && codes <= 1u << 23) || inputs < kE4M3Block)
+        return {kProductFew, 0, 1, 0};
+    /* One workgroup of tiles to a compute unit.  Of the tiles that do not fill a round, each is cut
+     * into as many parts as there are units, of four blocks of inputs or more. */
+    constexpr uint32_t kUnits = 256;
     const uint32_t blocks = e4m3_blocks(inputs);
-#ifndef Q38_FEW
-#define Q38_FEW 4
-#endif
-    if (tokens <= Q38_FEW || inputs < kE4M3Block) return {kProductFew, 0, 1, 0};
-    const auto tiles_of = [&](uint32_t tile) {
-        return (uint64_t)layer_up(outputs, kProductRows[tile]) * layer_up(tokens, kProductTokens[tile]);
+    const auto cut = [&](uint32_t tile) {
+        const uint64_t tiles = (uint64_t)layer_up(outputs, kProductRows[tile]) * layer_up(tokens, kProductTokens[tile]), rest = tiles % kUnits;
+        uint64_t splits = rest ? kUnits / rest : 1;
+        if (splits > blocks / 4) splits = blocks / 4;
+        if (splits < 2) return ProductPlan{tile, (uint32_t)tiles, 1, 0};
+        return ProductPlan{tile, (uint32_t)(tiles - rest), (uint32_t)splits, rest * splits * kProductRows[tile] * kProductTokens[tile] * 4};
     };
-    uint32_t tile = tokens <= 16 ? kProductTile16 : tokens <= 64 ? kProductTile64 : tokens <= 128 || tiles_of(kProductTile256) < 192 ? kProductTile128 : kProductTile256;
-#ifdef Q38_TILE
-    tile = Q38_TILE;
-#endif
-    /* workgroups that the card holds at once */
-    const uint32_t slots = tile == kProductTile256 ? 256 : 512;
-    const uint64_t tiles = tiles_of(tile), rest = tiles % slots;
-    uint64_t splits = rest ? slots / rest : 1;
-    if (splits > blocks / 4) splits = blocks / 4;
-    if (splits < 2) return {tile, (uint32_t)tiles, 1, 0};
-    return {tile, (uint32_t)(tiles - rest), (uint32_t)splits, rest * splits * kProductRows[tile] * kProductTokens[tile] * 4};
+    if (tokens <= 16) return cut(kProductTile16);
+    /* Larger tiles move fewer bytes for a product but cut the work into larger pieces: the least of what
+     * they take is taken.  A block of inputs takes 0.5, 0.82, 2.05 us (its products), or 0.84, 0.84, 1.68
+     * where the matrix comes from memory for one tile of tokens; the second launch takes 6 us, the parts' sums
+     * 1 us for 4 MB.  In us by tiles of 64, 128, 256 tokens: 80 x 5120 x 34816 59, 48, 69; 512 x 17408 x
+     * 5120 100, 100, 69; 768 x 5120 x 14336 119, 91, 74; 1024 x 2048 x 2048 11, 25, 26; 512 x 5120 x 5120
+     * 33, 31, 35; 2048 x 5120 x 5120 104, 83, 70. */
+    ProductPlan best = {};
+    float least = 0.0f;
+    for (uint32_t tile = kProductTile64; tile <= kProductTile256; ++tile) {
+        const ProductPlan plan = cut(tile);
+        const float products = tile == kProductTile64 ? 0.5f : tile == kProductTile128 ? 0.82f : 2.05f;
+        const float memory = kProductRows[tile] * (0.84f / 128) / layer_up(tokens, kProductTokens[tile]);
+        const uint32_t rounds = plan.whole / kUnits + (plan.splits == 1 && plan.whole % kUnits ? 1 : 0);
+        float us = (products > memory ? products : memory) * (rounds * blocks + (plan.splits > 1 ? layer_up(blocks, plan.splits) : 0));
+        if (plan.splits > 1) us += 6.0f + plan.bytes * 2.5e-7f;
+        if (tile == kProductTile64 || us < least) best = plan, least = us;
+    }
+    return best;
 }
 
 struct PromptAttention {

@@ -189,8 +189,8 @@ struct ProductTile {
     static_assert(WN * 16 <= (int)kE4M3Block && kE4M3Block % (WN * 16) == 0, "a wavefront's rows have one factor");
 };
 using Tile256 = ProductTile<8, 4, 2, 4, 2>;
-using Tile128 = ProductTile<4, 4, 2, 2, 2>;
-using Tile64 = ProductTile<2, 4, 4, 1, 3>;
+using Tile128 = ProductTile<4, 4, 2, 2, 3>;
+using Tile64 = ProductTile<2, 4, 4, 1, 4>;
 using Tile16 = ProductTile<2, 1, 4, 1, 4>;
 template <typename Tile>
 constexpr bool tile_is(int tile) { return (int)kProductRows[tile] == Tile::kRows && (int)kProductTokens[tile] == Tile::kTokens; }
@@ -378,8 +378,15 @@ __global__ void __launch_bounds__(256) join_kernel(ProductE4M3 a, ProductPlan pl
     const uint32_t token = tile.m * Tile::kTokens + four / (Tile::kRows / 4), row = tile.n * Tile::kRows + four % (Tile::kRows / 4) * 4;
     if (token >= a.tokens || row >= a.outputs) return;
     const f32x4 *part = reinterpret_cast<const f32x4 *>(a.partial) + (uint64_t)rest * plan.splits * kFours + four;
-    f32x4 sum = part[0];
-    for (uint32_t s = 1; s < plan.splits; ++s) sum += part[(uint64_t)s * kFours];
+    f32x4 sum = {};
+    for (uint32_t s = 0; s < plan.splits; s += 4) {
+        f32x4 v[4];                                          /* asked for together */
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) v[i] = part[(uint64_t)min(s + i, plan.splits - 1) * kFours];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+            if (s + i < plan.splits) sum += v[i];
+    }
     store_four<T>(a, token, row, sum);
 }
 

@@ -97,10 +97,11 @@ def scale_pitch(width):
 def _e4m3(x, rows, width, index, into):
     """new rows in 8 bits of x's shape, or the caller's"""
     if into is None:
-        return E4M3Rows(torch.empty_like(x, dtype=_CODES, memory_format=torch.contiguous_format),
-                        x.new_empty((rows, scale_pitch(width)), dtype=_SCALES))
-    _check_e4m3(into, rows, width, index)
-    return E4M3Rows(*into)
+        into = (torch.empty_like(x, dtype=_CODES, memory_format=torch.contiguous_format),
+                x.new_empty((rows, -(-width // 512) * 4), dtype=_SCALES))
+    else:
+        _check_e4m3(into, rows, width, index)
+    return tuple.__new__(E4M3Rows, into)
 
 
 def _check_e4m3(rows8, rows, width, index):
@@ -118,7 +119,7 @@ def quantize(x, gate=None, out=None):
     rows, width, stride, kind, index = _rows(x, "x")
     gate_row = 0 if gate is None else _alike(gate, "gate", x, index)
     out = _e4m3(x, rows, width, index, out)
-    _call("q38hip_quantize_e4m3", index, out.codes.data_ptr(), out.scales.data_ptr(), x.data_ptr(), stride,
+    _call("q38hip_quantize_e4m3", index, out[0].data_ptr(), out[1].data_ptr(), x.data_ptr(), stride,
           None if gate is None else gate.data_ptr(), gate_row, kind, width, rows)
     return out
 
@@ -133,8 +134,10 @@ def rms_norm(x, weight, eps=1e-6, addend=None, offset=0.0, e4m3=False, out=None,
     if addend is not None:
         addend_row, added = _alike(addend, "addend", x, index), addend.data_ptr()
         if total is None:
-            total = torch.empty_like(x, memory_format=torch.contiguous_format)
-        total_row, sum_at = _alike(total, "total", x, index), total.data_ptr()
+            total, total_row = torch.empty_like(x, memory_format=torch.contiguous_format), width
+        else:
+            total_row = stride if total is x else _alike(total, "total", x, index)
+        sum_at = total.data_ptr()
     elif total is None:
         addend_row = total_row = 0
         added = sum_at = None
@@ -142,11 +145,13 @@ def rms_norm(x, weight, eps=1e-6, addend=None, offset=0.0, e4m3=False, out=None,
         raise ValueError("total needs an addend")
     if e4m3:
         out = _e4m3(x, rows, width, index, out)
-        to, to_row, codes, scales = None, 0, out.codes.data_ptr(), out.scales.data_ptr()
+        to, to_row, codes, scales = None, 0, out[0].data_ptr(), out[1].data_ptr()
     else:
         if out is None:
-            out = torch.empty_like(x, memory_format=torch.contiguous_format)
-        to_row, to, codes, scales = _alike(out, "out", x, index), out.data_ptr(), None, None
+            out, to_row = torch.empty_like(x, memory_format=torch.contiguous_format), width
+        else:
+            to_row = _alike(out, "out", x, index)
+        to, codes, scales = out.data_ptr(), None, None
     _call("q38hip_rms_norm", index, to, to_row, codes, scales, sum_at, total_row, x.data_ptr(), stride, added, addend_row, kind,
           weight.data_ptr(), weight_kind, offset, eps, width, rows)
     return out if addend is None else (out, total)

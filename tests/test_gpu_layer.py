@@ -131,7 +131,7 @@ def test_norm_extremes(device):
 
 # ---- product -----------------------------------------------------------------------
 
-PRODUCTS = [(1, 16, 1), (1, 128, 16), (1, 5120, 17), (2, 144, 130), (3, 1168, 100), (16, 2048, 256), (17, 400, 128), (33, 1024, 300),
+PRODUCTS = [(1, 16, 1), (1, 128, 16), (1, 5120, 17), (2, 144, 130), (3, 1168, 100), (16, 2048, 256), (9, 4112, 2050), (3, 17408, 2000), (17, 400, 128), (33, 1024, 300),
             (48, 17408, 144), (64, 640, 129), (65, 256, 513), (100, 1280, 1000), (128, 128, 128), (200, 2064, 260), (257, 896, 511),
             (300, 4096, 256), (512, 384, 1024), (700, 528, 770), (2100, 272, 6010), (1030, 768, 10300)]
 
