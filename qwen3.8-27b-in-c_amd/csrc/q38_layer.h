@@ -2,10 +2,17 @@
  * kernels, launchers and checks share. */
 #pragma once
 
-#include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include "q38hip.h"
+
+/* what is plain C++ here is checked on the CPU too */
+#if defined(__HIPCC__)
+#include <hip/hip_runtime.h>
+#define Q38_LAYER_HD __host__ __device__ __forceinline__
+#else
+#define Q38_LAYER_HD inline
+#endif
 
 namespace q38 {
 
@@ -14,8 +21,6 @@ constexpr int kLayerF32 = 0, kLayerF16 = 1, kLayerBF16 = 30;
 
 /* elements that share a scale */
 constexpr uint32_t kE4M3Block = 128;
-
-#define Q38_LAYER_HD __host__ __device__ __forceinline__
 
 Q38_LAYER_HD constexpr uint32_t layer_up(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
 
@@ -119,6 +124,27 @@ inline ProductPlan plan_product(uint32_t tokens, uint32_t inputs, uint32_t outpu
     return best;
 }
 
+/* tile `place` of a product of tiles_n by tiles_m tiles: bands of four tiles of tokens,
+ * along the rows */
+struct TilePlace {
+    uint32_t n, m;
+};
+Q38_LAYER_HD TilePlace tile_place(uint32_t place, uint32_t tiles_n, uint32_t tiles_m)
+{
+    constexpr uint32_t kHigh = 4;
+    const uint32_t band = place / (kHigh * tiles_n), left = tiles_m - band * kHigh, high = left < kHigh ? left : kHigh;
+    place -= band * kHigh * tiles_n;
+    return {place / high, band * kHigh + place % high};
+}
+/* item `index` of `all` that workgroups take in turn: each of the eight dies, which workgroups go
+ * round, gets a run of neighbouring items, so that its cache serves what they share */
+Q38_LAYER_HD uint32_t die_place(uint32_t index, uint32_t all)
+{
+    constexpr uint32_t kDies = 8;
+    const uint32_t die = index % kDies, share = all / kDies, more = all % kDies;
+    return die * share + (die < more ? die : more) + index / kDies;
+}
+
 struct PromptAttention {
     void *output;
     const void *query, *gate, *key, *value;
@@ -129,11 +155,13 @@ struct PromptAttention {
     int type;
 };
 
+#if defined(__HIPCC__)
 bool launch_quantize_e4m3(const QuantizeRows &a, int type, hipStream_t stream);
 bool launch_rms_norm(const NormRows &a, int type, hipStream_t stream);
 bool launch_rotary(const Rotary &a, int type, hipStream_t stream);
 uint64_t product_e4m3_workspace_bytes(uint32_t tokens, uint64_t inputs, uint32_t outputs);
 bool launch_product_e4m3(const ProductE4M3 &a, hipStream_t stream);
 bool launch_prompt_attention(const PromptAttention &a, hipStream_t stream);
+#endif
 
 }  // namespace q38

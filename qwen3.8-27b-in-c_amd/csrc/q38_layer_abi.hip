@@ -164,6 +164,7 @@ extern "C" int q38hip_prompt_attention(void *output, uint64_t output_row_stride,
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return abi_fail("head_dim must be 64, 128 or 256");
     if (!heads || !kv_heads || heads % kv_heads) return abi_fail("heads must be a multiple of kv_heads");
     if (!count || !total_rows) return abi_fail("bad row arguments");
+    if (heads > 65535) return abi_fail("more than 65535 heads");
     if (count > kMost || total_rows > kMost || (uint64_t)total_rows * heads > 1u << 30)
         return abi_fail("more than 2^24 rows or sequences, or 2^30 query rows");
     if (heads > 1 && query_head_stride < head_dim) return abi_fail("query head stride too small");

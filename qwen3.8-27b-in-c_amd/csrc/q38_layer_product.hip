@@ -202,18 +202,6 @@ static_assert(tile_is<Tile256>(kProductTile256) && tile_is<Tile128>(kProductTile
  * 20..27, then the others) find places of their own modulo 256 bytes. */
 __device__ __forceinline__ uint32_t piece_turn(uint32_t row) { return row >> 1 & 7; }
 
-/* tile `place`: bands of four tiles of tokens, along the rows */
-struct TilePlace {
-    uint32_t n, m;
-};
-__device__ __forceinline__ TilePlace tile_place(uint32_t place, uint32_t tiles_n, uint32_t tiles_m)
-{
-    constexpr uint32_t kHigh = 4;
-    const uint32_t band = place / (kHigh * tiles_n), high = min(kHigh, tiles_m - band * kHigh);
-    place -= band * kHigh * tiles_n;
-    return {place / high, band * kHigh + place % high};
-}
-
 /* The first plan.whole tiles are formed by a workgroup each; of the others plan.splits
  * workgroups sum a part of the inputs each (a block at least), into
  * a.partial[tile][split][token][row].  Blocks of inputs go through stages of LDS: one is
@@ -227,13 +215,8 @@ __global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t tiles_n = layer_up(a.outputs, Tile::kRows), tiles_m = layer_up(a.tokens, Tile::kTokens);
 
-    /* Workgroups go round the eight dies; each die gets a run of neighbouring tiles, so that its
-     * cache serves their rows to several of them. */
-    constexpr uint32_t kDies = 8;
     const bool whole = blockIdx.x < plan.whole;
-    const uint32_t index = whole ? blockIdx.x : blockIdx.x - plan.whole, all = whole ? plan.whole : gridDim.x - plan.whole;
-    const uint32_t die = index % kDies, share = all / kDies, more = all % kDies;
-    const uint32_t place = die * share + min(die, more) + index / kDies;
+    const uint32_t place = whole ? die_place(blockIdx.x, plan.whole) : die_place(blockIdx.x - plan.whole, gridDim.x - plan.whole);
     const uint32_t rest = place / plan.splits, splits = whole ? 1 : plan.splits, split = whole ? 0 : place - rest * splits;
     const TilePlace tile = tile_place(whole ? place : plan.whole + rest, tiles_n, tiles_m);
     const uint32_t row0 = tile.n * Tile::kRows, token0 = tile.m * Tile::kTokens;

@@ -133,7 +133,10 @@ def test_norm_extremes(device):
 
 PRODUCTS = [(1, 16, 1), (1, 128, 16), (1, 5120, 17), (2, 144, 130), (3, 1168, 100), (16, 2048, 256), (9, 4112, 2050), (3, 17408, 2000), (17, 400, 128), (33, 1024, 300),
             (48, 17408, 144), (64, 640, 129), (65, 256, 513), (100, 1280, 1000), (128, 128, 128), (200, 2064, 260), (257, 896, 511),
-            (300, 4096, 256), (512, 384, 1024), (700, 528, 770), (2100, 272, 6010), (1030, 768, 10300)]
+            (300, 4096, 256), (512, 384, 1024), (700, 528, 770), (2100, 272, 6010), (1030, 768, 10300),
+            # every tile size whole, cut along the inputs, and both
+            (9, 400, 33000), (9, 1040, 33300), (17, 912, 33320), (66, 144, 17160), (199, 912, 17160), (66, 3600, 6050), (17, 912, 35340),
+            (516, 912, 22210), (199, 6672, 10090)]
 
 
 def _factors(rng, tokens, inputs, outputs):
@@ -143,8 +146,12 @@ def _factors(rng, tokens, inputs, outputs):
     return rows8, weight, scales
 
 
+def _to_bytes(t):
+    return t.view(torch.uint8)
+
+
 def _bytes(t):
-    return t.view(torch.uint8).cpu().numpy()
+    return _to_bytes(t).cpu().numpy()
 
 
 @pytest.mark.parametrize("tokens,inputs,outputs", PRODUCTS)
@@ -240,7 +247,8 @@ PROMPTS = [
     # heads, kv_heads, dim, lengths
     (1, 1, 64, [1]), (24, 4, 256, [37]), (4, 2, 128, [1, 2, 3, 1, 1]), (8, 2, 128, [63, 64, 65, 15, 16, 17, 31, 33]),
     (16, 16, 64, [130, 40]), (12, 1, 128, [300]), (5, 5, 256, [190]), (40, 8, 64, [90, 0, 200, 0, 0, 7]), (6, 2, 64, [1] * 70),
-    (2, 1, 256, [129, 127, 128]), (3, 3, 128, [257, 255]), (6, 1, 256, [513]), (2, 2, 64, [1030]), (7, 7, 128, [700, 1, 411]),
+    (2, 1, 256, [129, 127, 128]), (12, 2, 256, [200, 150, 90, 10]), (6, 2, 64, [0, 33, 5, 1] * 18), (8, 2, 128, [2, 40, 0, 17, 90] * 14),
+    (4, 1, 256, [25, 1, 70] * 22), (5, 5, 128, [300, 280]), (3, 3, 128, [257, 255]), (6, 1, 256, [513]), (2, 2, 64, [1030]), (7, 7, 128, [700, 1, 411]),
 ]
 
 
@@ -285,6 +293,46 @@ def test_attention_in_wider_rows(device, dtype):
     assert (room == 5).all() and not owned[:3].any() and not owned[109:].any()
 
 
+def _hidden(device, lengths, dim, dtype, at, where, bad):
+    """sequence `at` has a value of its own at row `where` that is not finite: rows before it and other sequences are as without"""
+    rng = np.random.default_rng(dim + len(lengths))
+    starts = kc.offsets(lengths)
+    q, k, v, _ = _prompt(rng, 4, 2, dim, starts[-1], dtype)
+    words = kc.words(starts, device)
+    want, mass, size, _ = lc.attention(f64(q), f64(k), f64(v), starts, dim ** -0.5)
+    bound = lc.attention_bound(want, mass, size, dtype, max(lengths))
+    lc.check(layer.attention(q, k, v, words), want, bound)
+    row, end = starts[at] + where, starts[at + 1]
+    v[row, 1, 5] = bad
+    got = layer.attention(q, k, v, words)
+    keep = [c for c in range(dim) if c != 5]
+    for part in (np.s_[:row], np.s_[row:end, :2], np.s_[row:end, 2:, keep], np.s_[end:]):
+        lc.check(got[part], want[part], bound[part])
+    assert not torch.isfinite(got[row:end, 2:, 5]).any()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("lengths,at,where", [([700], 0, 430), ([280, 290], 1, 3), ([9, 30] * 40, 13, 7)], ids=["one", "two", "eighty"])
+def test_attention_hidden_values(device, lengths, at, where, dtype):
+    """one prompt whose keys go in parts, two, and more sequences than lanes"""
+    for dim, bad in ((64, np.nan), (128, np.inf), (256, -np.inf)):
+        _hidden(device, lengths, dim, dtype, at, where, bad)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+@pytest.mark.parametrize("rows,count", [(40, 3), (300, 3), (300, 90)])
+def test_attention_bad_offsets_stay_inside(device, rows, count, dtype):
+    """Offsets that decrease, negative ones and ones behind the rows: what is written is the call's own output, nothing around it."""
+    rng = np.random.default_rng(rows + count)
+    q, k, v, _ = _prompt(rng, 4, 2, 64, rows, dtype)
+    room = torch.full((rows + 2, 4, 64), 3.0, dtype=dtype, device=device)
+    for _ in range(4):
+        starts = rng.integers(-2 * rows, 3 * rows, size=count + 1)
+        layer.attention(q, k, v, kc.words(starts.tolist(), device), out=room[1:-1])
+        torch.cuda.synchronize()
+        assert (room[0] == 3).all() and (room[-1] == 3).all()
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("dim", [64, 128, 256])
 def test_attention_hidden_rows_have_no_part(device, dim, dtype):
@@ -319,6 +367,40 @@ def test_attention_hidden_rows_have_no_part(device, dim, dtype):
     want, mass, size, _ = lc.attention(f64(q3), f64(k3), f64(v), starts, dim ** -0.5)
     size = np.minimum(size, 500.0)              # of the rows whose weights are not all or nothing
     lc.check(got[70:], want[70:], lc.attention_bound(want, mass, size, dtype, 100)[70:])
+
+
+# ---- far rows ---------------------------------------------------------------------------
+
+
+def test_offsets_beyond_32_bits(device):
+    """rows whose places pass 2^32 bytes"""
+    rng = np.random.default_rng(8)
+    rows, stride = 140, 1 << 25
+    big = torch.empty(rows * stride, dtype=BF16, device=device)
+    wide = big.as_strided((rows, 768), (stride, 1))
+    near = _normal(rng, rows, 768, dtype=BF16)
+    wide.copy_(near)
+    got, want = layer.quantize(wide[:, :512], gate=wide[:, 256:]), layer.quantize(near[:, :512], gate=near[:, 256:])
+    assert all(torch.equal(_to_bytes(a), _to_bytes(b)) for a, b in zip(got, want))
+    weight = _normal(rng, 512)
+    assert torch.equal(layer.rms_norm(wide[:, :512], weight), layer.rms_norm(near[:, :512].contiguous(), weight))
+    heads = lambda x: (x[:, :512].unflatten(1, (8, 64)), x[:, 512:640].unflatten(1, (2, 64)), x[:, 640:].unflatten(1, (2, 64)))  # noqa: E731
+    positions, frequencies = torch.arange(rows, dtype=torch.int32, device=device), layer.rotary_frequencies(64, device=device)[0]
+    assert torch.equal(layer.rotary(heads(wide)[0], positions, frequencies), layer.rotary(heads(near)[0], positions, frequencies))
+    words = kc.words([0, 100, 140], device)
+    assert torch.equal(layer.attention(*heads(wide), words), layer.attention(*heads(near), words))
+    layer.attention(*heads(near), words, out=heads(wide)[0])
+    assert torch.equal(heads(wide)[0], layer.attention(*heads(near), words))
+    del big, wide
+    tokens, inputs = 900000, 5120
+    codes = torch.zeros(tokens, inputs, dtype=torch.uint8, device=device)
+    scales = torch.zeros(tokens, layer.scale_pitch(inputs), dtype=torch.uint8, device=device)
+    last, matrix, factors = _factors(rng, 300, inputs, 24)
+    codes[-300:], scales[-300:] = last.codes.view(torch.uint8), last.scales.view(torch.uint8)
+    got = layer.product((codes.view(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu)), matrix, factors, F32)
+    want, mass = lc.product(_bytes(last.codes), _bytes(last.scales), _bytes(matrix), factors.cpu().numpy())
+    lc.check(got[-300:], want, lc.product_bound(want, mass, inputs, F32))
+    assert (got[:-300] == 0).all()
 
 
 # ---- as programs use them -------------------------------------------------------------

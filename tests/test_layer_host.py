@@ -3,6 +3,7 @@ include/q38hip.h, q38hip/layer.py), and the frequencies of rotary positions."""
 import ctypes
 import math
 import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -92,7 +93,7 @@ def test_attention_refuses():
         dict(dim=512), dict(heads=0), dict(kv_heads=0), dict(heads=3), dict(count=0), dict(rows=0), dict(count=BIG), dict(rows=BIG),
         dict(heads=1 << 20, kv_heads=2, rows=1 << 12, output_row=1 << 30), dict(query_head=127), dict(query_row=127), dict(key_row=255),
         dict(value_row=255), dict(output_row=511), dict(output=P + 1), dict(gate=P + 1), dict(key=P + 1), dict(starts=P + 2),
-        dict(scale=math.nan)])
+        dict(scale=math.nan), dict(heads=65536, kv_heads=65536, rows=1)])
 
 
 def test_python_refuses():
@@ -131,3 +132,68 @@ def test_frequencies():
     assert (np.diff(share) <= 2.0 ** -22).all() and share.min() >= 0.25 * (1 - 2.0 ** -23)
     same, magnitude = layer.rotary_frequencies(64, 1e6, factor=1.0, original=original)
     assert magnitude == 1.0 and torch.equal(same, plain)
+
+
+PLAN_CHECK = r"""
+#include <cstdio>
+#include <vector>
+#include "q38_layer.h"
+using namespace q38;
+#define CHECK(x) do { if (!(x)) { std::printf("line %d: %s (%u %u %u)\n", __LINE__, #x, m, k, n); return 1; } } while (0)
+static uint32_t state = 777;
+static uint32_t draw(uint32_t n) { state = state * 1664525u + 1013904223u; return (state >> 8) % n; }
+int main()
+{
+    unsigned seen[5][3] = {};
+    uint32_t m = 0, k = 0, n = 0;
+    for (int i = 0; i < 30000; ++i) {
+        m = draw(3) ? 1 + draw(1 + draw(5000)) : 1 + draw(70);
+        k = 16 * (1 + draw(1 + draw(1200)));
+        n = 1 + draw(1 + draw(40000));
+        const ProductPlan p = plan_product(m, k, n);
+        const uint32_t blocks = e4m3_blocks(k);
+        CHECK(p.tile <= kProductTile256);
+        if (p.tile == kProductFew) { CHECK(m <= 16 || k < 128); CHECK(p.splits == 1 && p.bytes == 0); ++seen[0][0]; continue; }
+        CHECK(k >= 128);
+        const uint32_t tiles_n = layer_up(n, kProductRows[p.tile]), tiles_m = layer_up(m, kProductTokens[p.tile]);
+        const uint64_t tiles = (uint64_t)tiles_n * tiles_m, rest = tiles - p.whole;
+        CHECK(p.whole <= tiles && p.splits >= 1 && (p.splits == 1) == (rest == 0));
+        CHECK(p.splits == 1 || blocks / p.splits >= 4);
+        CHECK(p.bytes == (p.splits == 1 ? 0 : rest * p.splits * kProductRows[p.tile] * kProductTokens[p.tile] * 4));
+        ++seen[p.tile][p.splits == 1 ? 0 : p.whole ? 1 : 2];
+        /* every tile once, whole or cut, and every block of inputs of a cut one once */
+        if (i % 16 == 0) {
+            std::vector<unsigned> got(tiles);
+            for (uint32_t b = 0; b < p.whole; ++b) {
+                const TilePlace t = tile_place(die_place(b, p.whole), tiles_n, tiles_m);
+                CHECK(t.n < tiles_n && t.m < tiles_m);
+                got[t.n + (uint64_t)t.m * tiles_n] += blocks;
+            }
+            const uint32_t all = (uint32_t)rest * p.splits;
+            for (uint32_t b = 0; b < all; ++b) {
+                const uint32_t place = die_place(b, all), tile = place / p.splits, split = place % p.splits;
+                const TilePlace t = tile_place(p.whole + tile, tiles_n, tiles_m);
+                const uint32_t from = (uint64_t)blocks * split / p.splits, to = (uint64_t)blocks * (split + 1) / p.splits;
+                CHECK(t.n < tiles_n && t.m < tiles_m && from < to);
+                got[t.n + (uint64_t)t.m * tiles_n] += to - from;
+            }
+            for (unsigned g : got) CHECK(g == blocks);
+        }
+    }
+    for (int t = 0; t < 5; ++t) std::printf("%u %u %u\n", seen[t][0], seen[t][1], seen[t][2]);
+    return 0;
+}
+"""
+
+
+def test_product_plans(tmp_path):
+    """every tile of a product is formed once, every plan is met by some size"""
+    source = tmp_path / "plan.cpp"
+    source.write_text(PLAN_CHECK)
+    program = str(tmp_path / "plan")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-I" + os.path.join(ROOT, "include"),
+                    "-I" + os.path.join(ROOT, "qwen3.8-27b-in-c_amd", "csrc"), str(source), "-o", program], check=True)
+    run = subprocess.run([program], capture_output=True, text=True)
+    assert run.returncode == 0, run.stdout
+    seen = [[int(v) for v in line.split()] for line in run.stdout.split("\n") if line]
+    assert seen[0][0] and all(all(row) for row in seen[1:]), seen
