@@ -49,6 +49,7 @@ extern "C" int q38hip_quantize_e4m3(uint8_t *codes, uint8_t *scales, const void 
     if (const char *fault = rows_fault(width, rows)) return abi_fail(fault);
     if (rows > 1 && (x_row_stride < width || (gate && gate_row_stride < width))) return abi_fail("row stride too small");
     if (!element_aligned(x, type) || !element_aligned(gate, type)) return abi_fail("rows must be aligned to their elements");
+    if (codes == x || codes == gate) return abi_fail("codes must not be an input");
     if (!q38::layer_launch_holds((uint64_t)rows * q38::quantize_parts(width), 256)) return abi_fail("more rows than a launch holds");
     const q38::QuantizeRows a = {codes, scales, x, gate, x_row_stride, gate_row_stride, (uint32_t)width,
                                  q38::e4m3_pitch(width), rows};
@@ -119,6 +120,7 @@ extern "C" int q38hip_gemm_e4m3(void *output, uint32_t type, uint64_t output_row
     if (!aligned(codes, 16) || !aligned(weight, 16)) return abi_fail("codes must be 16-byte aligned");
     if (!aligned(scales, 4) || !aligned(weight_scales, 4)) return abi_fail("scales must be 4-byte aligned");
     if (!element_aligned(output, type)) return abi_fail("output must be aligned to its elements");
+    if (output == codes || output == weight) return abi_fail("output must not be an input");
     if (q38::product_e4m3_workspace_bytes(batch_size, input_length, rows) && !workspace)
         return abi_fail("this product needs a workspace");
     if (!aligned(workspace, 16)) return abi_fail("workspace must be 16-byte aligned");
@@ -174,6 +176,7 @@ extern "C" int q38hip_prompt_attention(void *output, uint64_t output_row_stride,
     if (!element_aligned(output, type) || !element_aligned(query, type) || !element_aligned(gate, type) ||
         !element_aligned(key, type) || !element_aligned(value, type) || !aligned(row_starts, 4))
         return abi_fail("rows must be aligned to their elements");
+    if (output == query || output == gate || output == key || output == value) return abi_fail("output must not be an input");
     if (!std::isfinite(scale)) return abi_fail("scale must be finite");
     /* weights are equal where the scale is 0 (and where it is so small); a product with
      * -infinity must not become NaN there */

@@ -242,7 +242,7 @@ template <typename T, int D>
 struct PromptTile {
     static constexpr int kWaves = 4;
     /* Wavefronts of a SIMD, which share 512 registers a lane: two hide each other's softmax
-     * (bf16, 256-wide heads, 8197 tokens: 835 us, one with twice the keys 1187).  The queries and sums
+     * (bf16, 256-wide heads, 8197 tokens: 724 us, one with twice the keys 858).  The queries and sums
      * of 256-wide fp32 heads alone fill the registers of one. */
     static constexpr int kPerUnit = D * sizeof(T) == 1024 ? 1 : 2;
     static constexpr int kKeys = sizeof(T) == 4 || D == 256 ? 32 : 64;

@@ -206,6 +206,22 @@ def test_product_extremes(device, tokens):
     assert np.array_equal(np.isnan(got), bad)
 
 
+def test_product_of_many_tokens(device):
+    """more tiles of tokens than 16 bits count: each token's sums are its own, so parts of the batch give the same bits"""
+    rng = np.random.default_rng(9)
+    tokens, inputs, outputs = 65536 * 64 + 70, 32, 18
+    codes = torch.randint(0, 0x78, (tokens, inputs), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+    scales = torch.randint(120, 130, (tokens, 4), dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
+    _, weight, factors = _factors(rng, 1, inputs, outputs)
+    got = layer.product((codes, scales), weight, factors)
+    for first in range(0, tokens, 1 << 20):
+        part = slice(first, min(first + (1 << 20), tokens))
+        assert torch.equal(layer.product((codes[part], scales[part]), weight, factors), got[part])
+    tail = slice(tokens - 5, tokens)
+    want, mass = lc.product(_bytes(codes[tail]), _bytes(scales[tail]), _bytes(weight), factors.cpu().numpy())
+    lc.check(got[tail], want, lc.product_bound(want, mass, inputs, BF16))
+
+
 # ---- rotary positions ----------------------------------------------------------------
 
 ROTARIES = [(1, 1, 64, 32), (3, 4, 256, 32), (5, 2, 80, 10), (2, 3, 96, 48), (70, 28, 256, 32), (4, 1, 7, 3), (2, 2, 1024, 512),

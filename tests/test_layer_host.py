@@ -40,11 +40,12 @@ def test_pitch():
 
 
 def test_quantize_refuses():
-    good = dict(codes=P, scales=P, x=P, x_row=128, gate=None, gate_row=0, type=0, width=128, rows=2, stream=None)
+    good = dict(codes=2 * P, scales=3 * P, x=P, x_row=128, gate=None, gate_row=0, type=0, width=128, rows=2, stream=None)
     _refused("q38hip_quantize_e4m3", good, [
         dict(codes=None), dict(scales=None), dict(x=None), dict(type=2), dict(width=0), dict(rows=0), dict(width=BIG, x_row=BIG),
         dict(rows=BIG), dict(x_row=127), dict(gate=P, gate_row=127), dict(x=P + 2), dict(x=P + 1, type=1), dict(gate=P + 2, gate_row=128),
-        dict(rows=1 << 23, width=1 << 18, x_row=1 << 18), dict(rows=1 << 24, width=4096, x_row=4096)])
+        dict(rows=1 << 23, width=1 << 18, x_row=1 << 18), dict(rows=1 << 24, width=4096, x_row=4096), dict(codes=P),
+        dict(gate=2 * P, gate_row=128)])
 
 
 def test_norm_refuses():
@@ -62,13 +63,14 @@ def test_norm_refuses():
 
 
 def test_product_refuses():
-    good = dict(output=P, type=30, output_row=256, codes=P, scales=P, tokens=2, inputs=128, weight=P, weight_scales=P, rows=256,
+    good = dict(output=4 * P, type=30, output_row=256, codes=P, scales=P, tokens=2, inputs=128, weight=2 * P, weight_scales=P, rows=256,
                 workspace=None, stream=None)
     _refused("q38hip_gemm_e4m3", good, [
         dict(output=None), dict(type=8), dict(output_row=255), dict(codes=None), dict(scales=None), dict(weight=None),
         dict(weight_scales=None), dict(tokens=0), dict(inputs=0), dict(rows=0), dict(inputs=120), dict(inputs=129), dict(tokens=BIG),
         dict(inputs=BIG), dict(rows=BIG, output_row=BIG), dict(tokens=1 << 20, rows=1 << 20, output_row=1 << 20), dict(codes=P + 8),
-        dict(weight=P + 4), dict(scales=P + 2), dict(weight_scales=P + 2), dict(output=P + 1), dict(workspace=P + 8)])
+        dict(weight=P + 4), dict(scales=P + 2), dict(weight_scales=P + 2), dict(output=P + 1), dict(workspace=P + 8),
+        dict(output=P), dict(output=2 * P)])
     lib = layer._lib()
     for sizes in ((0, 128, 16), (1, 0, 16), (1, 128, 0), (1, 100, 16), (BIG, 128, 16)):
         assert lib.q38hip_gemm_e4m3_workspace_bytes(*sizes) == 0 and q38hip.last_error()
@@ -86,14 +88,15 @@ def test_rotary_refuses():
 
 
 def test_attention_refuses():
-    good = dict(output=P, output_row=512, query=P, gate=None, query_row=512, query_head=128, key=P, key_row=256, value=P,
+    good = dict(output=2 * P, output_row=512, query=P, gate=None, query_row=512, query_head=128, key=P, key_row=256, value=P,
                 value_row=256, type=30, heads=4, kv_heads=2, dim=128, scale=1.0, starts=P, count=1, rows=8, stream=None)
     _refused("q38hip_prompt_attention", good, [
         dict(output=None), dict(query=None), dict(key=None), dict(value=None), dict(starts=None), dict(type=2), dict(dim=96),
         dict(dim=512), dict(heads=0), dict(kv_heads=0), dict(heads=3), dict(count=0), dict(rows=0), dict(count=BIG), dict(rows=BIG),
         dict(heads=1 << 20, kv_heads=2, rows=1 << 12, output_row=1 << 30), dict(query_head=127), dict(query_row=127), dict(key_row=255),
         dict(value_row=255), dict(output_row=511), dict(output=P + 1), dict(gate=P + 1), dict(key=P + 1), dict(starts=P + 2),
-        dict(scale=math.nan), dict(heads=65536, kv_heads=65536, rows=1)])
+        dict(scale=math.nan), dict(heads=65536, kv_heads=65536, rows=1), dict(output=P), dict(gate=2 * P), dict(key=2 * P),
+        dict(value=2 * P)])
 
 
 def test_python_refuses():
