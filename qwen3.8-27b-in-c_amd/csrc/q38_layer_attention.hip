@@ -228,11 +228,10 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v)
     v = max(v, (uint32_t)dpp_move<0x143, 0xC>(0, (int)v));
     return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
+/* the least of numbers above -2^30 */
 __device__ __forceinline__ int wave_min(int v)
 {
-#pragma unroll
-    for (int i = 1; i < 64; i *= 2) v = min(v, __shfl_xor(v, i));
-    return v;
+    return (int)(0x7fffffffu - wave_max_u32(0x7fffffffu - (uint32_t)v));
 }
 
 /* Sizes of a workgroup: kWaves wavefronts of 32 columns, tiles of kKeys keys.  A
@@ -302,7 +301,11 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
     const uint32_t group = a.heads / a.kv_heads, kv = blockIdx.x % a.kv_heads, place = blockIdx.x / a.kv_heads;
     /* workgroups of one key/value head are eight apart where they can be, on one die's cache */
     uint32_t first, columns, row0 = 0;       /* this wavefront's first column, of how many from row row0 on */
-    int start = 0, owner = 0;                /* of the column's sequence */
+    int start = 0;                           /* of the column's sequence */
+    bool owned = true;
+    /* some column of the workgroup sees keys from .. to, of the wavefront lowest .. highest, and all of
+     * the wavefront see latest .. earliest */
+    int from = INT32_MAX, to = -1, lowest = INT32_MAX, highest = -1, latest = 0, earliest = INT32_MAX;
     if (a.count <= 64) {
         /* A lane to a sequence.  Tiles that see most first: tile d of any sequence, as many as it
          * has, before tile d - 1 of any; behind(d) tiles are d or later of theirs. */
@@ -324,7 +327,13 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
         row0 = __builtin_amdgcn_readlane(begin, sequence);
         columns = (__builtin_amdgcn_readlane(end, sequence) - row0) * group;
         first = low_d * Tile::kColumns + wave * 32;
-        start = row0;
+        start = from = latest = row0;
+        to = row0 + (min((low_d + 1) * Tile::kColumns, columns) - 1) / group;
+        if (first < columns) {
+            lowest = row0;
+            highest = row0 + min(first + 31, columns - 1) / group;
+            earliest = row0 + first / group;
+        }
     } else {
         columns = a.rows * group;
         first = (gridDim.x / a.kv_heads - 1 - place) * Tile::kColumns + wave * 32;
@@ -332,7 +341,7 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
     const uint32_t column = min(first + low, columns - 1), row = row0 + column / group, head = kv * group + column % group;
     if (a.count > 64) {
         const int row_first = (int)(min(first, columns - 1) / group), row_last = (int)(min(first + 31, columns - 1) / group);
-        owner = -1;
+        int owner = -1;
         uint32_t at = 0, end = a.count + 1;                  /* the last sequence at or before the first row */
         while (at < end) {
             const uint32_t mid = (at + end) / 2;
@@ -352,21 +361,21 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
             }
         }
         start = min(max(start, 0), (int)row);
-    }
-    const bool owned = first + low < columns && owner >= 0 && owner < (int)a.count;
-    /* the wavefront's keys: some column sees lowest .. highest, all see latest .. earliest */
-    const int lowest = __builtin_amdgcn_readfirstlane(wave_min(owned ? start : INT32_MAX));
-    const int highest = -__builtin_amdgcn_readfirstlane(wave_min(owned ? -(int)row : 1));
-    const int latest = -__builtin_amdgcn_readfirstlane(wave_min(owned ? -start : 0));
-    const int earliest = __builtin_amdgcn_readfirstlane(wave_min(owned ? (int)row : INT32_MAX));
-    if (lane == 0) ranges[wave][0] = lowest, ranges[wave][1] = highest;
-    __syncthreads();
-    int from = INT32_MAX, to = -1;
+        owned = owner >= 0 && owner < (int)a.count && first + low < columns;
+        lowest = wave_min(owned ? start : INT32_MAX);
+        highest = -wave_min(owned ? -(int)row : 1);
+        latest = -wave_min(owned ? -start : 0);
+        earliest = wave_min(owned ? (int)row : INT32_MAX);
+        if (lane == 0) ranges[wave][0] = lowest, ranges[wave][1] = highest;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) from = min(from, ranges[w][0]), to = max(to, ranges[w][1]);
-    from = __builtin_amdgcn_readfirstlane(from);
-    to = __builtin_amdgcn_readfirstlane(to);
-    if (to < 0) return;
+        for (int w = 0; w < kWaves; ++w) from = min(from, ranges[w][0]), to = max(to, ranges[w][1]);
+        from = __builtin_amdgcn_readfirstlane(from);
+        to = __builtin_amdgcn_readfirstlane(to);
+        if (to < 0) return;
+    } else {
+        owned = first + low < columns;
+    }
 
     /* queries, 16 bytes of each 32, in registers throughout; a negative scale turns their sign */
     constexpr int E = 16 / (int)sizeof(T);
