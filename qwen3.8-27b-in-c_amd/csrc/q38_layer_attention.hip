@@ -234,6 +234,29 @@ __device__ __forceinline__ int wave_min(int v)
     return (int)(0x7fffffffu - wave_max_u32(0x7fffffffu - (uint32_t)v));
 }
 
+/* 16 bytes of a row, and to one */
+template <bool kWhole, typename T>
+__device__ __forceinline__ u32x4 load_piece(const T *from)
+{
+    if constexpr (kWhole) return *reinterpret_cast<const u32x4 *>(from);
+    T e[16 / sizeof(T)];
+#pragma unroll
+    for (int i = 0; i < 16 / (int)sizeof(T); ++i) e[i] = from[i];
+    return __builtin_bit_cast(u32x4, e);
+}
+template <bool kWhole, typename T>
+__device__ __forceinline__ void store_piece(T *to, u32x4 piece)
+{
+    if constexpr (kWhole) {
+        *reinterpret_cast<u32x4 *>(to) = piece;
+    } else {
+        T e[16 / sizeof(T)];
+        __builtin_memcpy(e, &piece, 16);
+#pragma unroll
+        for (int i = 0; i < 16 / (int)sizeof(T); ++i) to[i] = e[i];
+    }
+}
+
 /* Sizes of a workgroup: kWaves wavefronts of 32 columns, tiles of kKeys keys.  A
  * column is a row and one of the query heads that share a key/value head, columns of a
  * row next to each other, so all of a tile's columns read the same keys and values. */
@@ -338,7 +361,14 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
         columns = a.rows * group;
         first = (gridDim.x / a.kv_heads - 1 - place) * Tile::kColumns + wave * 32;
     }
-    const uint32_t column = min(first + low, columns - 1), row = row0 + column / group, head = kv * group + column % group;
+    struct Column {
+        uint32_t row, head;
+    };
+    const auto column = [&](uint32_t i) {                    /* the wavefront's i-th */
+        const uint32_t at = min(first + i, columns - 1);
+        return Column{row0 + at / group, kv * group + at % group};
+    };
+    const auto [row, head] = column(low);
     if (a.count > 64) {
         const int row_first = (int)(min(first, columns - 1) / group), row_last = (int)(min(first + 31, columns - 1) / group);
         int owner = -1;
@@ -385,14 +415,7 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
 #pragma unroll
     for (int u = 0; u < kSteps; ++u) {
         const T *p = static_cast<const T *>(a.query) + query_at + (2 * u + half) * E;
-        if constexpr (kWhole) {
-            query[u] = *reinterpret_cast<const u32x4 *>(p);
-        } else {
-            T e[E];
-#pragma unroll
-            for (int i = 0; i < E; ++i) e[i] = p[i];
-            query[u] = __builtin_bit_cast(u32x4, e);
-        }
+        query[u] = load_piece<kWhole>(p);
         if (a.scale < 0) query[u] ^= sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
     }
 
@@ -594,40 +617,57 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
         }
     const uint64_t found = __ballot(owned && nothing != 0.0f);
     uint32_t again = (uint32_t)(found | found >> 32);
-    if (owned && !(again >> low & 1)) {
-        T *to_row = static_cast<T *>(a.output) + (uint64_t)row * a.output_row + (uint64_t)head * D;
+    const uint32_t done = (uint32_t)__ballot(owned) & ~again;
+
+    /* A lane has four neighbours of a column at a time.  They go through LDS, where the wavefront's
+     * own part has room for kChannels of its columns in fp32, so that what is read of the gate and
+     * written is whole rows. */
+    constexpr int kChannels = kHalf / 128 < D ? kHalf / 128 : D, kPieces = kChannels / E, kRows = 64 / kPieces;
+    if constexpr (kParts == 1) tile_barrier();               /* the tiles have been read; of two parts each wavefront has read its own sums */
+    float *turned = reinterpret_cast<float *>(tiles + wave * (kParts == 1 ? kHalf : D * 128));
+    const auto place_of = [](uint32_t r, uint32_t four) { return r * kChannels + (four ^ (r & 15)) * 4; };
+    uint32_t own = low;
+    asm volatile("" : "+v"(own));                            /* formed again: kept, they would fill registers of the loop */
+    const auto [own_row, own_head] = column(own);
+    const uint64_t output_at = (uint64_t)own_row * a.output_row + (uint64_t)own_head * D;
+    const uint64_t gate_at = (uint64_t)own_row * a.query_row + (uint64_t)own_head * a.query_head;
+    T *const output = static_cast<T *>(a.output);
+    const T *const gate = static_cast<const T *>(a.gate);
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
+    for (int from_channel = 0; from_channel < D; from_channel += kChannels) {
+#pragma unroll
+        for (int d = 0; d < kChannels / 32; ++d)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const uint32_t channel = d * 32 + r * 8 + half * 4;
-                T e[4];
-                if (a.gate) {
-                    const T *gate = static_cast<const T *>(a.gate) + query_at + channel;
-                    if constexpr (kWhole && sizeof(T) == 2) {
-                        *reinterpret_cast<layer_u32x2 *>(e) = *reinterpret_cast<const layer_u32x2 *>(gate);
-                    } else if constexpr (kWhole) {
-                        *reinterpret_cast<u32x4 *>(e) = *reinterpret_cast<const u32x4 *>(gate);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) e[j] = gate[j];
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float v = out[d][r * 4 + j];
-                    if (a.gate) v *= __builtin_amdgcn_rcpf(1.0f + __expf(-static_cast<float>(e[j])));
-                    e[j] = static_cast<T>(v);
-                }
-                if constexpr (kWhole && sizeof(T) == 2) {
-                    *reinterpret_cast<layer_u32x2 *>(to_row + channel) = *reinterpret_cast<const layer_u32x2 *>(e);
-                } else if constexpr (kWhole) {
-                    *reinterpret_cast<u32x4 *>(to_row + channel) = *reinterpret_cast<const u32x4 *>(e);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) to_row[channel + j] = e[j];
-                }
+                const f32x16 &v = out[from_channel / 32 + d];
+                *reinterpret_cast<f32x4 *>(turned + place_of(low, d * 8 + r * 2 + half)) =
+                    f32x4{v[r * 4], v[r * 4 + 1], v[r * 4 + 2], v[r * 4 + 3]};
             }
+        const uint32_t channel = from_channel + lane % kPieces * E;
+        constexpr int kBatch = 32 / kRows < 8 ? 32 / kRows : 8;      /* of the gate, asked for together */
+#pragma unroll
+        for (int i = 0; i < 32; i += kBatch * kRows) {
+            T e[kBatch][E];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const uint64_t at = __shfl(gate_at, i + b * kRows + lane / kPieces);
+                if (gate) *reinterpret_cast<u32x4 *>(e[b]) = load_piece<kWhole>(gate + at + channel);
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const uint32_t r = i + b * kRows + lane / kPieces;
+                const uint64_t at = __shfl(output_at, r);
+#pragma unroll
+                for (int j = 0; j < E; j += 4) {
+                    const f32x4 four = *reinterpret_cast<const f32x4 *>(turned + place_of(r, (channel - from_channel + j) / 4));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        e[b][j + k] = static_cast<T>(
+                            gate ? four[k] * __builtin_amdgcn_rcpf(1.0f + __expf(-static_cast<float>(e[b][j + k]))) : four[k]);
+                }
+                if (done >> r & 1) store_piece<kWhole>(output + at + channel, __builtin_bit_cast(u32x4, e[b]));
+            }
+        }
     }
     while (again) {
         const uint32_t which = first + __builtin_ctz(again);
