@@ -686,12 +686,12 @@ bool attention(const PromptAttention &a, hipStream_t stream)
     };
     const bool wide = whole(a.query, a.query_row) && whole(a.gate, a.query_head) && whole(a.key, a.key_row) &&
                       whole(a.value, a.value_row) && whole(a.output, a.output_row);
-    /* Few rows have few keys.  A wavefront to a row and head, against tiles, in us: 24 heads of
-     * 256, fp32, 37 rows 5.9 against 28, 128 rows 21 against 48, 500 rows 197 against 154; bf16
-     * 64 rows 10.5 against 14.7, 128 rows 20.7 against 17.4; 32 heads of 128, bf16, 64 rows 7.1
-     * against 8.5, 128 rows 13.8 against 9.8, fp32 128 rows 18.5 against 24, 200 rows 39
-     * against 35. */
-    if (a.rows <= (sizeof(T) == 4 ? 128 : 64))
+    /* Few rows have few keys.  A wavefront to a row and head, against tiles, in us: 24 heads of 256
+     * on 4, fp32, 37 rows 5.9 against 27, 300 rows 82 against 92, 500 rows 197 against 140; bf16 64 rows
+     * 10.6 against 11.7, 128 rows 20.7 against 13.7; 32 heads of 128, bf16, 64 rows 7.1 against 7.6,
+     * 96 rows 10.7 against 8.8, fp32 128 rows 18 against 24, 200 rows 39 against 35; 16 of 64, fp32, 128
+     * rows 8.4 against 14.7, 300 rows 24 against 27. */
+    if (a.rows <= (sizeof(T) == 4 ? 64 + D : 64))
         return launch_kernel(wide ? row_kernel<T, D, true> : row_kernel<T, D, false>, dim3(layer_up(a.rows * a.heads, 4)), dim3(256),
                              stream, a);
     /* a tile more for each sequence where tiles follow them */
@@ -699,9 +699,9 @@ bool attention(const PromptAttention &a, hipStream_t stream)
     const dim3 grid((layer_up(columns, PromptTile<T, D>::kColumns) + (a.count <= 64 ? a.count : 0)) * a.kv_heads);
     /* Tiles that do not fill the card twice over: both halves of the registers go to one of them,
      * unless keys are few.  Two parts against one, in us: bf16, 24 heads of 256, 1024 tokens (192
-     * tiles) 45 against 62, 2048 (384) 81 against 119, 3500 (660) 198 against 203, 24 prompts of up to 333 (520)
-     * 55 against 34; 32 heads of 128, 512 tokens (128) 17 against 18, 2048 (512) 53 against 58, 3500 (880)
-     * 130 against 118, 100 (32) 10.8 against 9.6. */
+     * tiles) 38 against 42, 2048 (384) 70 against 86, 3500 (660) 179 against 163, 12 prompts of up to 300
+     * (244) 29 against 22; 32 heads of 128, 700 tokens (176) 18.3 against 19.4, 2700 (680) 84 against 69, 12
+     * prompts of up to 300 (328) 19 against 13; fp32, 2048 tokens (512) 283 against 365. */
     if constexpr (D * sizeof(T) < 1024)
         if (grid.x <= 512 + a.count * a.kv_heads && a.rows >= 256 * a.count)
             return launch_kernel(wide ? prompt_kernel<T, D, true, 2> : prompt_kernel<T, D, false, 2>, grid,

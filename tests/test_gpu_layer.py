@@ -265,6 +265,7 @@ PROMPTS = [
     (16, 16, 64, [130, 40]), (12, 1, 128, [300]), (5, 5, 256, [190]), (40, 8, 64, [90, 0, 200, 0, 0, 7]), (6, 2, 64, [1] * 70),
     (2, 1, 256, [129, 127, 128]), (12, 2, 256, [200, 150, 90, 10]), (6, 2, 64, [0, 33, 5, 1] * 18), (8, 2, 128, [2, 40, 0, 17, 90] * 14),
     (4, 1, 256, [25, 1, 70] * 22), (5, 5, 128, [300, 280]), (3, 3, 128, [257, 255]), (6, 1, 256, [513]), (2, 2, 64, [1030]), (7, 7, 128, [700, 1, 411]),
+    (4, 2, 256, [0, 330, 1, 0, 33]), (6, 3, 256, [2, 0, 9, 17] * 30),
 ]
 
 
