@@ -113,7 +113,9 @@ __device__ __forceinline__ void store_piece(const ProductE4M3 &a, uint32_t token
 }
 
 /* 16 matrix rows by 16 * M tokens to a workgroup, whose eight wavefronts take
- * every eighth block of inputs and are summed in LDS in their order. */
+ * every eighth block of inputs and are summed in LDS in their order: many short
+ * workgroups, whose loads are all in flight at once, for matrices that a second launch would
+ * not repay (one token, 5120 x 5120: 8.3 us). */
 template <typename T, int M>
 __global__ void __launch_bounds__(kWaves * 64) few_kernel(ProductE4M3 a)
 {
@@ -221,7 +223,14 @@ __device__ __forceinline__ uint32_t piece_turn(uint32_t row) { return row >> 1 &
 /* The first plan.whole tiles are formed by a workgroup each; of the others plan.splits
  * workgroups sum a part of the inputs each (a block at least), into
  * a.partial[tile][split][token][row].  Blocks of inputs go through stages of LDS: one is
- * read while the next ones are on their way. */
+ * read while the next ones are on their way.
+ *
+ * Few tokens are bound by the matrix: one token, 5120 x 34816, 35 us, 5.1 TB/s; 48 tokens, 17408 x
+ * 5120, 21.6 us with the join's 4.  4096 tokens, 5120 x 34816: 704 us, 2.07 PFLOP/s.  There copying
+ * the stages alone takes 640 us (330 if all came from the die's cache): a unit has room for one
+ * stage of 64 KiB ahead, which arrives about when it is due; products, sums and reads from LDS
+ * alone take 565, writing the results about 50.  The fma of each product's sums, under the next
+ * products, costs a seventh of the matrix unit's rate with two wavefronts to a SIMD, a third with one. */
 template <typename T, typename Tile>
 __global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a, ProductPlan plan)
 {
