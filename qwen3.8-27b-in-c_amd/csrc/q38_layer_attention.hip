@@ -11,8 +11,14 @@ namespace {
 /* First row of the sequence that owns `row`, or -1 where none does: the last
  * sequence that starts at or before it, so empty ones are passed over.  Always
  * in 0 .. row, whatever the words hold. */
-__device__ __forceinline__ int sequence_start(const PromptAttention &a, uint32_t row)
+__device__ __forceinline__ int sequence_start(const PromptAttention &a, uint32_t row, uint32_t lane)
 {
+    if (a.count < 64) {                         /* one load: an offset to a lane */
+        const int begin = a.row_starts[min(lane, a.count)];
+        const uint32_t low = __popcll(__ballot(lane <= a.count && begin <= (int)row));
+        if (low == 0 || low == a.count + 1) return -1;
+        return min(max(__builtin_amdgcn_readlane(begin, low - 1), 0), (int)row);
+    }
     uint32_t low = 0, high = a.count + 1;       /* row_starts[low - 1] <= row < row_starts[high] */
     while (low < high) {
         const uint32_t mid = (low + high) / 2;
@@ -43,7 +49,7 @@ template <typename T, int D, bool kWhole>
 __device__ __forceinline__ void attend_row(const PromptAttention &a, uint32_t row, uint32_t head, uint32_t lane)
 {
     constexpr int E = 16 / (int)sizeof(T), C = D / (4 * E), kChannels = D / 64;
-    const int start = sequence_start(a, row);
+    const int start = sequence_start(a, row, lane);
     if (start < 0) return;
     const auto sixteen = [=](const T *from) {
         if constexpr (kWhole) return *reinterpret_cast<const layer_u32x4 *>(from);
@@ -62,17 +68,33 @@ __device__ __forceinline__ void attend_row(const PromptAttention &a, uint32_t ro
 #pragma unroll
         for (int e = 0; e < E; ++e) q[c][e] = static_cast<float>(reinterpret_cast<const T *>(&raw)[e]) * a.scale;
     }
+    float gate[kChannels] = {};
+    if (a.gate) {
+#pragma unroll
+        for (int e = 0; e < kChannels; ++e)
+            gate[e] = static_cast<float>(static_cast<const T *>(a.gate)[query + channel + e]);
+    }
     for (uint32_t first = start; first <= row; first += 64) {
         float s[4];
 #pragma unroll
+        for (int u = 0; u < 4; ++u) s[u] = -INFINITY;
+        /* 16-bit keys are asked for 16 at a time while the last 16 are multiplied (24 heads of 256, 37 rows: 6.0
+         * instead of 8.1 us); for fp32 that costs registers and wavefronts (6.3 instead of 5.9) */
+        constexpr int kInFlight = sizeof(T) == 2 ? 2 : 1;
+        layer_u32x4 pieces[kInFlight][C];
+        const auto ask = [&](int u) {
+            const T *from = keys + (uint64_t)min(first + u * 16 + lane / 4, row) * a.key_row;
+#pragma unroll
+            for (int c = 0; c < C; ++c) pieces[u % kInFlight][c] = sixteen(from + c * 4 * E);
+        };
+        if (kInFlight > 1) ask(0);
+#pragma unroll
         for (int u = 0; u < 4; ++u) {
-            s[u] = -INFINITY;
+            const int next = u + kInFlight - 1;
+            if (next < 4 && first + next * 16 <= row) ask(next);
             if (first + u * 16 > row) continue;
             const uint32_t key = first + u * 16 + lane / 4;
-            const T *from = keys + (uint64_t)min(key, row) * a.key_row;
-            layer_u32x4 raw[C];
-#pragma unroll
-            for (int c = 0; c < C; ++c) raw[c] = sixteen(from + c * 4 * E);
+            const layer_u32x4 (&raw)[C] = pieces[u % kInFlight];
             float dot[2] = {};
 #pragma unroll
             for (int c = 0; c < C; ++c)
@@ -123,10 +145,7 @@ __device__ __forceinline__ void attend_row(const PromptAttention &a, uint32_t ro
 #pragma unroll
     for (int e = 0; e < kChannels; ++e) {
         float v = out[e] * inverse;
-        if (a.gate) {
-            const float g = static_cast<float>(static_cast<const T *>(a.gate)[query + channel + e]);
-            v *= __builtin_amdgcn_rcpf(1.0f + __expf(-g));
-        }
+        if (a.gate) v *= __builtin_amdgcn_rcpf(1.0f + __expf(-gate[e]));
         to[e] = static_cast<T>(v);
     }
 }
@@ -692,7 +711,7 @@ bool attention(const PromptAttention &a, hipStream_t stream)
                       whole(a.value, a.value_row) && whole(a.output, a.output_row);
     /* Few rows have few keys.  A wavefront to a row and head, against tiles, in us: 24 heads of 256
      * on 4, fp32, 37 rows 5.9 against 27, 300 rows 82 against 92, 500 rows 197 against 140; bf16 64 rows
-     * 10.6 against 11.7, 128 rows 20.7 against 13.7; 32 heads of 128, bf16, 64 rows 7.1 against 7.6,
+     * 8.1 against 11.7, 128 rows 20.7 against 13.7; 32 heads of 128, bf16, 64 rows 6.1 against 7.6,
      * 96 rows 10.7 against 8.8, fp32 128 rows 18 against 24, 200 rows 39 against 35; 16 of 64, fp32, 128
      * rows 8.4 against 14.7, 300 rows 24 against 27. */
     if (a.rows <= (sizeof(T) == 4 ? 64 + D : 64))
