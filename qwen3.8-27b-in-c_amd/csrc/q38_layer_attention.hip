@@ -326,7 +326,7 @@ __device__ __forceinline__ uint32_t value_turn(uint32_t row)
  * units idle (bf16, 24 heads of 256, 8197 tokens: 724 us, 797 with each read at its product).
  * That is 1.14 PFLOP/s, what a large library product of bf16 reaches; the matrix unit is busy 0.61
  * of the cycles.  fp32 (0.095 PFLOP/s of 0.154) is bound by the fp32 products themselves.  Many
- * short prompts are bound by what a tile does once: 12 of up to 1500 tokens, 32 heads of 128, 59 us.
+ * short prompts are bound by what a tile does once: 12 of up to 1500 tokens, 32 heads of 128, 57 us.
  *
  * With kParts = 2 the workgroup has twice the wavefronts; the second half of them takes
  * every other tile of keys for the same columns, and its sums join the first's through LDS. */
