@@ -44,9 +44,9 @@ extern "C" int q38hip_quantize_e4m3(uint8_t *codes, uint8_t *scales, const void 
                                     const void *gate, uint64_t gate_row_stride, uint32_t type, uint64_t width,
                                     uint32_t rows, void *stream)
 {
+    if (const char *fault = rows_fault(width, rows)) return abi_fail(fault);
     if (!codes || !scales || !x) return abi_fail("bad quantize arguments");
     if (!element_type(type)) return abi_fail("rows must be F32, F16 or BF16");
-    if (const char *fault = rows_fault(width, rows)) return abi_fail(fault);
     if (rows > 1 && (x_row_stride < width || (gate && gate_row_stride < width))) return abi_fail("row stride too small");
     if (!element_aligned(x, type) || !element_aligned(gate, type)) return abi_fail("rows must be aligned to their elements");
     if (codes == x || codes == gate) return abi_fail("codes must not be an input");
@@ -62,10 +62,10 @@ extern "C" int q38hip_rms_norm(void *output, uint64_t output_row_stride, uint8_t
                                uint64_t addend_row_stride, uint32_t type, const void *weight, uint32_t weight_type,
                                float weight_offset, float eps, uint64_t width, uint32_t rows, void *stream)
 {
+    if (const char *fault = rows_fault(width, rows)) return abi_fail(fault);
     if (!x || !weight || (!output && !codes) || (!codes != !scales) || (!addend != !total))
         return abi_fail("bad norm arguments");
     if (!element_type(type) || !element_type(weight_type)) return abi_fail("rows and weight must be F32, F16 or BF16");
-    if (const char *fault = rows_fault(width, rows)) return abi_fail(fault);
     if (rows > 1 && (x_row_stride < width || (output && output_row_stride < width) ||
                      (addend && (addend_row_stride < width || total_row_stride < width))))
         return abi_fail("row stride too small");
@@ -73,6 +73,8 @@ extern "C" int q38hip_rms_norm(void *output, uint64_t output_row_stride, uint8_t
         !element_aligned(total, type) || !element_aligned(weight, weight_type))
         return abi_fail("rows must be aligned to their elements");
     if (output && output == total) return abi_fail("total and output must differ");
+    if (codes && (codes == x || codes == addend || codes == total || codes == output || codes == weight))
+        return abi_fail("codes must not be an input or another output");
     if (rows > 1 && ((total && ((total == x && total_row_stride != x_row_stride) ||
                                 (total == addend && total_row_stride != addend_row_stride))) ||
                      (output && ((output == x && output_row_stride != x_row_stride) ||
@@ -136,9 +138,9 @@ extern "C" int q38hip_rotary(void *output, uint64_t output_row_stride, uint64_t 
                              uint32_t head_dim, const int32_t *positions, const float *frequencies, uint32_t pairs,
                              int interleaved, float magnitude, void *stream)
 {
+    if (!rows || !heads || !head_dim || !pairs) return abi_fail("empty rows");
     if (!output || !x || !positions || !frequencies) return abi_fail("bad rotary arguments");
     if (!element_type(type)) return abi_fail("rows must be F32, F16 or BF16");
-    if (!rows || !heads || !head_dim || !pairs) return abi_fail("empty rows");
     if (rows > kMost) return abi_fail("more than 2^24 rows");
     if (head_dim > 1024 || (uint64_t)heads * head_dim > 1u << 20) return abi_fail("heads of more than 1024 or rows of more than 2^20 elements");
     if (2ull * pairs > head_dim) return abi_fail("more pairs than the head holds");
@@ -161,11 +163,11 @@ extern "C" int q38hip_prompt_attention(void *output, uint64_t output_row_stride,
                                        uint32_t heads, uint32_t kv_heads, uint32_t head_dim, float scale,
                                        const int32_t *row_starts, uint32_t count, uint32_t total_rows, void *stream)
 {
+    if (!count || !total_rows) return abi_fail("no sequences or no rows");
     if (!output || !query || !key || !value || !row_starts) return abi_fail("bad attention arguments");
     if (!element_type(type)) return abi_fail("rows must be F32, F16 or BF16");
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return abi_fail("head_dim must be 64, 128 or 256");
     if (!heads || !kv_heads || heads % kv_heads) return abi_fail("heads must be a multiple of kv_heads");
-    if (!count || !total_rows) return abi_fail("bad row arguments");
     if (heads > 65535) return abi_fail("more than 65535 heads");
     if (count > kMost || total_rows > kMost || (uint64_t)total_rows * heads > 1u << 30)
         return abi_fail("more than 2^24 rows or sequences, or 2^30 query rows");

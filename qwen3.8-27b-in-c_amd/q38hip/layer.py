@@ -3,9 +3,10 @@ that bring their own model: norm, projections in 8 bits, rotary positions and
 the attention of packed prompts.
 
 Functions check shapes and types on the host, enqueue on torch's current stream
-of their tensors' device and read nothing back.  Rows in 8 bits are a pair
-(codes, scales): float8_e4m3fn [rows, width] and float8_e8m0fnu [rows, blocks of
-128 rounded up to a multiple of 4].
+of their tensors' device and read nothing back; there is at least one row, and
+results carry no gradient.  Rows in 8 bits are a pair (codes, scales):
+float8_e4m3fn [rows, width] and float8_e8m0fnu [rows, blocks of 128 rounded up to
+a multiple of 4].
 
     y, x = layer.rms_norm(x, weight, addend=attended, e4m3=True)     # x + addend, and its norm in 8 bits
     both = layer.product(y, gate_up, gate_up_scales)                 # bfloat16 [rows, 2 * hidden]
@@ -162,7 +163,7 @@ _WORKSPACES = {}
 
 def product(rows8, weight, weight_scales, dtype=torch.bfloat16, out=None):
     """Rows in 8 bits [rows, inputs] times weight [outputs, inputs] (float8_e4m3fn) with weight_scales [ceil(outputs /
-    128), ceil(inputs / 128)] (float32): [rows, outputs] of dtype."""
+    128), ceil(inputs / 128)] (float32): [rows, outputs] of dtype, or of out's."""
     codes = rows8[0]
     if codes.dim() != 2 or weight.dim() != 2:
         raise ValueError("expected codes [rows, inputs] and weight [outputs, inputs]")

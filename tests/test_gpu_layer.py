@@ -575,6 +575,8 @@ def test_python_refuses(device):
     for call in (lambda: layer.rotary(heads, words, torch.ones(33, device=device)), lambda: layer.attention(heads, heads[:, :3], heads[:, :3], words),
                  lambda: layer.quantize(x[:1].expand(3, 256)),
                  lambda: layer.product((rows8.codes[:, :120].contiguous(), rows8.scales), w8[:, :120].contiguous(), ws[:, :1].contiguous()),
-                 lambda: layer.rms_norm(x, weight, eps=-1.0)):
+                 lambda: layer.rms_norm(x, weight, eps=-1.0), lambda: layer.quantize(x[:0]), lambda: layer.rms_norm(x[:0], weight),
+                 lambda: layer.product(layer.E4M3Rows(rows8.codes[:0], rows8.scales[:0]), w8, ws), lambda: layer.rotary(heads[:0], words[:0], f),
+                 lambda: layer.attention(heads[:0], heads[:0], heads[:0], words), lambda: layer.attention(heads, heads, heads, words, out=heads)):
         with pytest.raises(RuntimeError):
             call()

@@ -59,7 +59,9 @@ def test_norm_refuses():
         dict(added, total=P), dict(added, total=2 * P, total_row=512), dict(added, total=4 * P, total_row=512),
         dict(output=2 * P, output_row=512), dict(added, output=4 * P, output_row=512), dict(eps=-1.0), dict(eps=math.nan),
         dict(eps=math.inf), dict(offset=math.nan), dict(x=2 * P + 1), dict(weight=3 * P + 2), dict(output=P + 1),
-        dict(added, addend=4 * P + 1), dict(added, total=5 * P + 1), dict(rows=1 << 23, width=16384, x_row=16384, output_row=16384)])
+        dict(added, addend=4 * P + 1), dict(added, total=5 * P + 1),
+        dict(codes=2 * P, scales=7 * P), dict(codes=P, scales=7 * P), dict(added, codes=4 * P, scales=7 * P),
+        dict(added, codes=5 * P, scales=7 * P), dict(rows=1 << 23, width=16384, x_row=16384, output_row=16384)])
 
 
 def test_product_refuses():
