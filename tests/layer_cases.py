@@ -164,6 +164,21 @@ def attention(query, key, value, starts, scale, gate=None):
     return want, mass, size, first >= 0
 
 
+def attention_of(query, key, value, at, scale):
+    """attention() of one sequence, for its rows `at`: query holds those, key and value all rows"""
+    heads, group = query.shape[1], query.shape[1] // key.shape[1]
+    want, mass, size = np.empty(query.shape), np.empty(query.shape), np.empty(query.shape[:2])
+    hidden = np.arange(len(key)) > np.asarray(at)[:, None]
+    for h in range(heads):
+        q, k, v = query[:, h], key[:, h // group], value[:, h // group]
+        scores = np.where(hidden, -np.inf, q @ k.T * scale)
+        size[:, h] = np.where(hidden, 0, np.abs(q) @ np.abs(k).T * abs(scale)).max(1)
+        weight = np.exp(scores - scores.max(1, keepdims=True))
+        weight /= weight.sum(1, keepdims=True)
+        want[:, h], mass[:, h] = weight @ v, weight @ np.abs(v)
+    return want, mass, size
+
+
 def attention_bound(want, mass, size, dtype, longest):
     """Scores: exact products, fp32 sums of up to 256 terms (2^-24 of their sum
     each at most, 2^-24 * 32 in the mean), roundings of the scaling and of the difference to

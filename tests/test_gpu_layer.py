@@ -386,6 +386,19 @@ def test_attention_hidden_rows_have_no_part(device, dim, dtype):
     lc.check(got[70:], want[70:], lc.attention_bound(want, mass, size, dtype, 100)[70:])
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(4, 2, 64, BF16), (2, 1, 128, torch.float16), (3, 1, 256, BF16), (1, 1, 128, F32)], ids=str)
+def test_attention_of_a_long_prompt(device, heads, kv_heads, dim, dtype):
+    """33001 tokens behind a short prompt, at rows near tile ends and spread over it"""
+    rng = np.random.default_rng(dim)
+    starts, n = [0, 19, 33020], 33001
+    q, k, v, _ = _prompt(rng, heads, kv_heads, dim, 33020, dtype)
+    got = layer.attention(q, k, v, kc.words(starts, device))
+    at = np.array([0, 1, 31, 32, 33, 63, 64, 127, 128, 4095, 4096, 16383, 16384, 32767, 32768, 33000] + list(rng.integers(0, n, size=16)))
+    rows = torch.from_numpy(at + 19).to(device)
+    want, mass, size = lc.attention_of(f64(q[rows]), f64(k[19:]), f64(v[19:]), at, dim ** -0.5)
+    lc.check(got[rows], want, lc.attention_bound(want, mass, size, dtype, n))
+
+
 # ---- far rows ---------------------------------------------------------------------------
 
 
