@@ -157,22 +157,19 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(NormRows a)
 
 /* ---- rotary positions ------------------------------------------------------ */
 
-/* A workgroup takes a row, or a part of one.  Its angles are formed once, in fp64, reduced to a
- * turn and their sines and cosines kept in LDS for all heads; a thread then
+/* A workgroup takes a row, `parts` of them share one, or it takes `group` short rows.  Their angles are
+ * formed once, in fp64, reduced to a turn and their sines and cosines kept in LDS for all heads; a thread then
  * takes eight pairs (or eight channels that are copied) of a head at a time.  Bound by bytes:
  * 8192 bf16 rows of 40 heads of 128 move 168 MB in 33 us, 5.1 TB/s; few rows by the latency of their
  * angles (16 rows 2.7 us). */
-template <typename T, bool kInterleaved, bool kWhole>
-__global__ void __launch_bounds__(256) rotary_kernel(Rotary a, uint32_t parts, uint32_t items, uint32_t turned_items, uint32_t pass_items)
+template <typename T, bool kInterleaved, bool kWhole, bool kGroup>
+__global__ void __launch_bounds__(256) rotary_kernel(Rotary a, uint32_t parts, uint32_t group, uint32_t items, uint32_t turned_items, uint32_t pass_items)
 {
     __shared__ float cosine[512], sine[512];
-    const uint32_t part = blockIdx.x % parts;
-    const uint64_t row = blockIdx.x / parts;
-    const T *x = static_cast<const T *>(a.x) + row * a.x_row;
-    T *out = static_cast<T *>(a.output) + row * a.output_row;
-    const double position = (double)a.positions[row];
-    for (uint32_t i = threadIdx.x; i < a.pairs; i += blockDim.x) {
-        const double turns = position * (double)a.frequencies[i] * 0.15915494309189533577;
+    const uint32_t part = blockIdx.x % parts, row0 = blockIdx.x / parts * group, rows = kGroup ? min(group, a.rows - row0) : 1;
+    for (uint32_t i = threadIdx.x; i < rows * a.pairs; i += blockDim.x) {
+        const uint32_t r = kGroup ? i / a.pairs : 0;
+        const double turns = (double)a.positions[row0 + r] * (double)a.frequencies[i - r * a.pairs] * 0.15915494309189533577;
         float s, c;
         sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
         sine[i] = s * a.magnitude;
@@ -180,10 +177,11 @@ __global__ void __launch_bounds__(256) rotary_kernel(Rotary a, uint32_t parts, u
     }
     __syncthreads();
     const uint32_t per_head = turned_items + pass_items;
-    for (uint32_t item = part * blockDim.x + threadIdx.x; item < items; item += parts * blockDim.x) {
+    for (uint32_t i = part * blockDim.x + threadIdx.x; i < rows * items; i += parts * blockDim.x) {
+        const uint32_t r = kGroup ? i / items : 0, item = i - r * items, angles = r * a.pairs;
         const uint32_t head = item / per_head, place = item - head * per_head;
-        const T *from = x + head * a.x_head;
-        T *to = out + head * a.output_head;
+        const T *from = static_cast<const T *>(a.x) + (uint64_t)(row0 + r) * a.x_row + head * a.x_head;
+        T *to = static_cast<T *>(a.output) + (uint64_t)(row0 + r) * a.output_row + head * a.output_head;
         if (place >= turned_items) {
             const uint32_t at = 2 * a.pairs + (place - turned_items) * 8, some = min(8u, a.head_dim - at);
             float v[8];
@@ -195,7 +193,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(Rotary a, uint32_t parts, u
             layer_load8<T, kWhole>(v, from + at, some);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t pair = min(at / 2 + i, a.pairs - 1);
+                const uint32_t pair = angles + min(at / 2 + i, a.pairs - 1);
                 const float c = cosine[pair], s = sine[pair];
                 u[2 * i] = v[2 * i] * c - v[2 * i + 1] * s;
                 u[2 * i + 1] = v[2 * i + 1] * c + v[2 * i] * s;
@@ -208,7 +206,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(Rotary a, uint32_t parts, u
             layer_load8<T, kWhole>(w, from + a.pairs + at, some);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const uint32_t pair = min(at + i, a.pairs - 1);
+                const uint32_t pair = angles + min(at + i, a.pairs - 1);
                 const float c = cosine[pair], s = sine[pair];
                 p[i] = v[i] * c - w[i] * s;
                 q[i] = w[i] * c + v[i] * s;
@@ -277,14 +275,29 @@ bool rotary(const Rotary &a, hipStream_t stream)
     const bool wide = a.head_dim % 8 == 0 && a.pairs % (a.interleaved ? 4 : 8) == 0 && whole<T>(a.x, a.x_row, a.rows) &&
                       whole<T>(a.output, a.output_row, a.rows) && whole<T>(a.x, a.x_head, a.heads) &&
                       whole<T>(a.output, a.output_head, a.heads);
-    const auto kernel = a.interleaved ? (wide ? rotary_kernel<T, true, true> : rotary_kernel<T, true, false>)
-                                      : (wide ? rotary_kernel<T, false, true> : rotary_kernel<T, false, false>);
     const uint32_t threads = items >= 256 ? 256 : up(items, 64) * 64;
     /* Rows that leave units idle have a workgroup for each 256 of their items, each with angles of its own: 16 fp32
      * rows of 28 heads of 256 2.7 us against 4.2, 200 rows 4.4 against 4.7, 300 bf16 rows of 40 heads of 128 no
      * different. */
     const uint32_t parts = a.rows < 256 ? up(items, 256) : 1;
-    return launch_kernel(kernel, dim3(a.rows * parts), dim3(threads), stream, a, parts, items, turned, pass);
+    /* Short rows by as many to a workgroup as it has threads and room for angles, while four workgroups to a unit are
+     * left: 60000 fp32 rows of one head of 80 23 us against 54; with 64 items a row (8192 bf16 rows of 8 heads of 128)
+     * 6.9 against 6.3. */
+    uint32_t group = items <= 32 ? 256 / items : 1;
+    if (group > 512 / a.pairs) group = 512 / a.pairs;
+    if (group > a.rows / 1024) group = a.rows / 1024;
+    const auto go = [&](auto kernel, uint32_t workgroups, uint32_t size) {
+        return launch_kernel(kernel, dim3(workgroups), dim3(size), stream, a, parts, group, items, turned, pass);
+    };
+    if (group > 1) {
+        const auto kernel = a.interleaved ? (wide ? rotary_kernel<T, true, true, true> : rotary_kernel<T, true, false, true>)
+                                          : (wide ? rotary_kernel<T, false, true, true> : rotary_kernel<T, false, false, true>);
+        return go(kernel, up(a.rows, group), 256);
+    }
+    group = 1;
+    const auto kernel = a.interleaved ? (wide ? rotary_kernel<T, true, true, false> : rotary_kernel<T, true, false, false>)
+                                      : (wide ? rotary_kernel<T, false, true, false> : rotary_kernel<T, false, false, false>);
+    return go(kernel, a.rows * parts, threads);
 }
 
 }  // namespace

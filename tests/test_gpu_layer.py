@@ -225,7 +225,7 @@ def test_product_of_many_tokens(device):
 # ---- rotary positions ----------------------------------------------------------------
 
 ROTARIES = [(1, 1, 64, 32), (3, 4, 256, 32), (5, 2, 80, 10), (2, 3, 96, 48), (70, 28, 256, 32), (4, 1, 7, 3), (2, 2, 1024, 512),
-            (9, 40, 128, 64), (1, 16, 64, 31)]
+            (9, 40, 128, 64), (1, 16, 64, 31), (4100, 1, 80, 20), (3001, 2, 10, 5), (2500, 1, 256, 128)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
