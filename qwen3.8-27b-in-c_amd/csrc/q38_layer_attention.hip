@@ -199,6 +199,12 @@ __device__ __forceinline__ void tile_barrier()
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+/* the same for what was read from and written to LDS alone */
+__device__ __forceinline__ void lds_barrier()
+{
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 /* c + A B over 16 bytes of a row from each lane: A's rows and B's columns are
  * lane % 32, the inner index is the lane's half and the place in the 16 bytes, in both
  * alike.  Element r of c is row 8 (r / 4) + 4 (lane / 32) + r % 4, column lane % 32. */
@@ -280,18 +286,20 @@ __device__ __forceinline__ void store_piece(T *to, u32x4 piece)
 
 /* Sizes of a workgroup: kWaves wavefronts of 32 columns, tiles of kKeys keys.  A
  * column is a row and one of the query heads that share a key/value head, columns of a
- * row next to each other, so all of a tile's columns read the same keys and values. */
-template <typename T, int D>
+ * row next to each other, so all of a tile's columns read the same keys and values.
+ * With kShares = 4 the four wavefronts share 32 columns: each takes a fourth of the channels in both products,
+ * and the parts of the scores are joined through LDS. */
+template <typename T, int D, int kShares>
 struct PromptTile {
     static constexpr int kWaves = 4;
     /* Wavefronts of a SIMD, which share 512 registers a lane: two hide each other's softmax
      * (bf16, 256-wide heads, 8197 tokens: 724 us, one with twice the keys 858).  The queries and sums
      * of 256-wide fp32 heads alone fill the registers of one. */
-    static constexpr int kPerUnit = D * sizeof(T) == 1024 ? 1 : 2;
+    static constexpr int kPerUnit = D * sizeof(T) / kShares == 1024 ? 1 : 2;
     static constexpr int kKeys = sizeof(T) == 4 || D == 256 ? 32 : 64;
     static constexpr int kRowBytes = D * (int)sizeof(T);
     static constexpr int kHalf = kKeys * kRowBytes;          /* keys or values of a tile */
-    static constexpr uint32_t kColumns = kWaves * 32;
+    static constexpr uint32_t kColumns = kWaves / kShares * 32;
 };
 
 /* Where 16-byte piece `piece` of row `row` lies in its row in LDS.  Keys are read
@@ -330,21 +338,23 @@ __device__ __forceinline__ uint32_t value_turn(uint32_t row)
  *
  * With kParts = 2 the workgroup has twice the wavefronts; the second half of them takes
  * every other tile of keys for the same columns, and its sums join the first's through LDS. */
-template <typename T, int D, bool kWhole, int kParts>
-__global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (PromptTile<T, D>::kPerUnit))
+template <typename T, int D, bool kWhole, int kParts, int kShares>
+__global__ void __launch_bounds__((PromptTile<T, D, kShares>::kWaves * 64 * kParts), (PromptTile<T, D, kShares>::kPerUnit))
     prompt_kernel(PromptAttention a)
 {
-    using Tile = PromptTile<T, D>;
+    using Tile = PromptTile<T, D, kShares>;
     constexpr int kWaves = Tile::kWaves, kRowBytes = Tile::kRowBytes, kKeys = Tile::kKeys, kHalf = Tile::kHalf;
     constexpr int kSteps = kRowBytes / 32;                   /* 16 bytes a lane each */
     constexpr int kTiles = kKeys / 32, kAhead = 3;
+    constexpr int kOwnSteps = kSteps / kShares, kOwn = D / kShares;      /* of the wavefront's channels */
+    static_assert(kShares == 1 || (kOwnSteps == 8 && kParts == 1 && kTiles == 1), "shares of 256 bytes");
     /* of each part keys and values, two of each; then the second part's sums and statistics */
     constexpr int kTilesBytes = kParts * 4 * kHalf, kJoinBytes = kParts > 1 ? (D / 2 + 2) * 256 * kWaves : 0;
     __shared__ __align__(1024) uint8_t tiles[kTilesBytes > kJoinBytes ? kTilesBytes : kJoinBytes];
     __shared__ int ranges[kWaves][2];
     const uint32_t lane = threadIdx.x & 63, part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / kWaves;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % kWaves;
-    const uint32_t half = lane >> 5, low = lane & 31;
+    const uint32_t half = lane >> 5, low = lane & 31, share = wave % kShares;
     const uint32_t group = a.heads / a.kv_heads, kv = blockIdx.x % a.kv_heads, place = blockIdx.x / a.kv_heads;
     /* workgroups of one key/value head are eight apart where they can be, on one die's cache */
     uint32_t first, columns, row0 = 0;       /* this wavefront's first column, of how many from row row0 on */
@@ -373,7 +383,7 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
         const uint32_t sequence = __builtin_ctzll(others);
         row0 = __builtin_amdgcn_readlane(begin, sequence);
         columns = (__builtin_amdgcn_readlane(end, sequence) - row0) * group;
-        first = low_d * Tile::kColumns + wave * 32;
+        first = low_d * Tile::kColumns + wave / kShares * 32;
         start = from = latest = row0;
         to = row0 + (min((low_d + 1) * Tile::kColumns, columns) - 1) / group;
         if (first < columns) {
@@ -383,7 +393,7 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
         }
     } else {
         columns = a.rows * group;
-        first = (gridDim.x / a.kv_heads - 1 - place) * Tile::kColumns + wave * 32;
+        first = (gridDim.x / a.kv_heads - 1 - place) * Tile::kColumns + wave / kShares * 32;
     }
     struct Column {
         uint32_t row, head;
@@ -433,12 +443,12 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
 
     /* queries, 16 bytes of each 32, in registers throughout; a negative scale turns their sign */
     constexpr int E = 16 / (int)sizeof(T);
-    u32x4 query[kSteps];
+    u32x4 query[kOwnSteps];
     const uint64_t query_at = (uint64_t)row * a.query_row + (uint64_t)head * a.query_head;
     const float scale = fabsf(a.scale);
 #pragma unroll
-    for (int u = 0; u < kSteps; ++u) {
-        const T *p = static_cast<const T *>(a.query) + query_at + (2 * u + half) * E;
+    for (int u = 0; u < kOwnSteps; ++u) {
+        const T *p = static_cast<const T *>(a.query) + query_at + share * kOwn + (2 * u + half) * E;
         query[u] = load_piece<kWhole>(p);
         if (a.scale < 0) query[u] ^= sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
     }
@@ -486,7 +496,7 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
         }
     };
 
-    f32x16 out[D / 32] = {};
+    f32x16 out[kOwn / 32] = {};
     float top = -INFINITY, base = 0.0f, total = 0.0f;
 
     /* piece 2 u + half of key row 32 t + low; `lane_at` holds what is the lane's of its place */
@@ -525,19 +535,41 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
             load(false, key + kParts * kKeys, buffer ^ 1);
             load(true, key + kParts * kKeys, buffer ^ 1);
         }
-        if (key > highest || key + kKeys <= lowest) continue;
-        uint32_t key_at = tiles_at + buffer * kHalf + key_lane_at, value_at = tiles_at + (2 + buffer) * kHalf + value_lane_at;
+        const bool sees = key <= highest && key + kKeys > lowest;
+        if (kShares == 1 && !sees) continue;
+        uint32_t key_at = tiles_at + buffer * kHalf + key_lane_at + share * 256;
+        uint32_t value_at = tiles_at + (2 + buffer) * kHalf + value_lane_at + share * (kOwn * (uint32_t)sizeof(T));
         asm volatile("" : "+v"(key_at), "+v"(value_at));     /* turned anew for each tile: places kept would fill registers */
         f32x16 score[kTiles] = {};
         u32x4 ahead[kAhead + 1];                             /* pieces that are asked for before their products */
+        if (sees) {
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) ahead[i] = key_piece(key_at, i % kTiles, i / kTiles);
+            for (int i = 0; i < kAhead; ++i) ahead[i] = key_piece(key_at, i % kTiles, i / kTiles);
 #pragma unroll
-        for (int i = 0; i < kTiles * kSteps; ++i) {
-            const int j = i + kAhead;
-            if (j < kTiles * kSteps) ahead[j % (kAhead + 1)] = key_piece(key_at, j % kTiles, j / kTiles);
-            score[i % kTiles] = multiply<T>(ahead[i % (kAhead + 1)], query[i / kTiles], score[i % kTiles]);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int i = 0; i < kTiles * kOwnSteps; ++i) {
+                const int j = i + kAhead;
+                if (j < kTiles * kOwnSteps) ahead[j % (kAhead + 1)] = key_piece(key_at, j % kTiles, j / kTiles);
+                score[i % kTiles] = multiply<T>(ahead[i % (kAhead + 1)], query[i / kTiles], score[i % kTiles]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if constexpr (kShares > 1) {
+            /* the tile's keys have been read: their place takes the parts of the scores */
+            const auto part_of = [&](uint32_t w, int i) { return tiles_at + buffer * kHalf + w * 4096 + i * 1024 + lane * 16; };
+            lds_barrier();
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *(Q38_LDS f32x4 *)(uintptr_t)part_of(wave, i) = f32x4{score[0][4 * i], score[0][4 * i + 1], score[0][4 * i + 2], score[0][4 * i + 3]};
+            lds_barrier();
+            if (!sees) continue;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f32x4 sum = lds_read<f32x4>(part_of(wave - share, i));
+#pragma unroll
+                for (int w = 1; w < kShares; ++w) sum += lds_read<f32x4>(part_of(wave - share + w, i));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) score[0][4 * i + j] = sum[j];
+            }
         }
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -565,7 +597,7 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
             const float shrink = __builtin_amdgcn_exp2f(before - base);
             total *= shrink;
 #pragma unroll
-            for (int d = 0; d < D / 32; ++d)
+            for (int d = 0; d < kOwn / 32; ++d)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) out[d][r] *= shrink;
         }
@@ -597,7 +629,7 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
 #pragma unroll
             for (int r = 0; r < 16; ++r)
 #pragma unroll
-                for (int d = 0; d < D / 32; ++d)
+                for (int d = 0; d < kOwn / 32; ++d)
                     out[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(
                         lds_read<float>(value_at + (r / 4 * 8 + r % 4) * kRowBytes + d * 128), score[0][r], out[d], 0, 0, 0);
         }
@@ -633,7 +665,7 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
     const float inverse = 1.0f / halves_sum(total);
     float nothing = 0.0f;
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d)
+    for (int d = 0; d < kOwn / 32; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             out[d][r] *= inverse;
@@ -641,14 +673,23 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
         }
     const uint64_t found = __ballot(owned && nothing != 0.0f);
     uint32_t again = (uint32_t)(found | found >> 32);
+    if constexpr (kShares > 1) {                             /* in any share's channels */
+        if (lane == 0) ranges[wave][0] = (int)again;
+        __syncthreads();
+        again = 0;
+#pragma unroll
+        for (int w = 0; w < kShares; ++w) again |= (uint32_t)ranges[wave - share + w][0];
+        again = __builtin_amdgcn_readfirstlane(again);
+    }
     const uint32_t done = (uint32_t)__ballot(owned) & ~again;
 
     /* A lane has four neighbours of a column at a time.  They go through LDS, where the wavefront's
      * own part has room for kChannels of its columns in fp32, so that what is read of the gate and
      * written is whole rows. */
-    constexpr int kChannels = kHalf / 128 < D ? kHalf / 128 : D, kPieces = kChannels / E, kRows = 64 / kPieces;
+    constexpr int kRoom = kParts == 1 ? 4 * kHalf / kWaves : D * 128;
+    constexpr int kChannels = kRoom / 128 < kOwn ? kRoom / 128 : kOwn, kPieces = kChannels / E, kRows = 64 / kPieces;
     if constexpr (kParts == 1) tile_barrier();               /* the tiles have been read; of two parts each wavefront has read its own sums */
-    float *turned = reinterpret_cast<float *>(tiles + wave * (kParts == 1 ? kHalf : D * 128));
+    float *turned = reinterpret_cast<float *>(tiles + wave * kRoom);
     const auto place_of = [](uint32_t r, uint32_t four) { return r * kChannels + (four ^ (r & 15)) * 4; };
     uint32_t own = low;
     asm volatile("" : "+v"(own));                            /* formed again: kept, they would fill registers of the loop */
@@ -658,7 +699,7 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
     T *const output = static_cast<T *>(a.output);
     const T *const gate = static_cast<const T *>(a.gate);
 #pragma unroll
-    for (int from_channel = 0; from_channel < D; from_channel += kChannels) {
+    for (int from_channel = 0; from_channel < kOwn; from_channel += kChannels) {
 #pragma unroll
         for (int d = 0; d < kChannels / 32; ++d)
 #pragma unroll
@@ -667,7 +708,7 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
                 *reinterpret_cast<f32x4 *>(turned + place_of(low, d * 8 + r * 2 + half)) =
                     f32x4{v[r * 4], v[r * 4 + 1], v[r * 4 + 2], v[r * 4 + 3]};
             }
-        const uint32_t channel = from_channel + lane % kPieces * E;
+        const uint32_t piece = lane % kPieces * E, channel = share * kOwn + from_channel + piece;
         constexpr int kBatch = 32 / kRows < 8 ? 32 / kRows : 8;      /* of the gate, asked for together */
 #pragma unroll
         for (int i = 0; i < 32; i += kBatch * kRows) {
@@ -683,7 +724,7 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
                 const uint64_t at = __shfl(output_at, r);
 #pragma unroll
                 for (int j = 0; j < E; j += 4) {
-                    const f32x4 four = *reinterpret_cast<const f32x4 *>(turned + place_of(r, (channel - from_channel + j) / 4));
+                    const f32x4 four = *reinterpret_cast<const f32x4 *>(turned + place_of(r, (piece + j) / 4));
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         e[b][j + k] = static_cast<T>(
@@ -693,7 +734,7 @@ __global__ void __launch_bounds__((PromptTile<T, D>::kWaves * 64 * kParts), (Pro
             }
         }
     }
-    while (again) {
+    while (again && share == 0) {
         const uint32_t which = first + __builtin_ctz(again);
         again &= again - 1;
         attend_row<T, D, kWhole>(a, row0 + which / group, kv * group + which % group, lane);
@@ -718,8 +759,16 @@ bool attention(const PromptAttention &a, hipStream_t stream)
         return launch_kernel(wide ? row_kernel<T, D, true> : row_kernel<T, D, false>, dim3(layer_up(a.rows * a.heads, 4)), dim3(256),
                              stream, a);
     /* a tile more for each sequence where tiles follow them */
-    const uint32_t columns = a.rows * (a.heads / a.kv_heads);
-    const dim3 grid((layer_up(columns, PromptTile<T, D>::kColumns) + (a.count <= 64 ? a.count : 0)) * a.kv_heads);
+    const uint32_t columns = a.rows * (a.heads / a.kv_heads), more = a.count <= 64 ? a.count : 0;
+    const auto tiles = [&](uint32_t size) { return dim3((layer_up(columns, size) + more) * a.kv_heads); };
+    const dim3 grid = tiles(PromptTile<T, D, 1>::kColumns);
+    /* A tile of 256-wide fp32 heads takes 8.6 us for 32 keys, so where there are fewer tiles than units,
+     * columns are shared: 5 heads on 5, 1375 tokens (60 tiles) 140 us against 364, 24 on 4, 1000 (192)
+     * 175 against 272, 2048 (384) 637 against 540. */
+    if constexpr (D * sizeof(T) == 1024)
+        if (grid.x <= 256 + a.count * a.kv_heads)
+            return launch_kernel(wide ? prompt_kernel<T, D, true, 1, 4> : prompt_kernel<T, D, false, 1, 4>,
+                                 tiles(PromptTile<T, D, 4>::kColumns), dim3(256), stream, a);
     /* Tiles that do not fill the card twice over: both halves of the registers go to one of them,
      * unless keys are few.  Two parts against one, in us: bf16, 24 heads of 256, 1024 tokens (192
      * tiles) 38 against 42, 2048 (384) 70 against 86, 3500 (660) 179 against 163, 12 prompts of up to 300
@@ -727,10 +776,9 @@ bool attention(const PromptAttention &a, hipStream_t stream)
      * prompts of up to 300 (328) 19 against 13; fp32, 2048 tokens (512) 283 against 365. */
     if constexpr (D * sizeof(T) < 1024)
         if (grid.x <= 512 + a.count * a.kv_heads && a.rows >= 256 * a.count)
-            return launch_kernel(wide ? prompt_kernel<T, D, true, 2> : prompt_kernel<T, D, false, 2>, grid,
-                                 dim3(PromptTile<T, D>::kWaves * 128), stream, a);
-    return launch_kernel(wide ? prompt_kernel<T, D, true, 1> : prompt_kernel<T, D, false, 1>, grid,
-                         dim3(PromptTile<T, D>::kWaves * 64), stream, a);
+            return launch_kernel(wide ? prompt_kernel<T, D, true, 2, 1> : prompt_kernel<T, D, false, 2, 1>, grid,
+                                 dim3(512), stream, a);
+    return launch_kernel(wide ? prompt_kernel<T, D, true, 1, 1> : prompt_kernel<T, D, false, 1, 1>, grid, dim3(256), stream, a);
 }
 
 template <typename T>

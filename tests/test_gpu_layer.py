@@ -266,6 +266,7 @@ PROMPTS = [
     (2, 1, 256, [129, 127, 128]), (12, 2, 256, [200, 150, 90, 10]), (6, 2, 64, [0, 33, 5, 1] * 18), (8, 2, 128, [2, 40, 0, 17, 90] * 14),
     (4, 1, 256, [25, 1, 70] * 22), (5, 5, 128, [300, 280]), (3, 3, 128, [257, 255]), (6, 1, 256, [513]), (2, 2, 64, [1030]), (7, 7, 128, [700, 1, 411]),
     (4, 2, 256, [0, 330, 1, 0, 33]), (6, 3, 256, [2, 0, 9, 17] * 30),
+    (24, 4, 256, [1100, 700]), (3, 1, 256, [7, 50, 0, 120] * 20), (16, 8, 256, [400, 5, 1, 64, 32, 31]),
 ]
 
 
@@ -386,7 +387,7 @@ def test_attention_hidden_rows_have_no_part(device, dim, dtype):
     lc.check(got[70:], want[70:], lc.attention_bound(want, mass, size, dtype, 100)[70:])
 
 
-@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(4, 2, 64, BF16), (2, 1, 128, torch.float16), (3, 1, 256, BF16), (1, 1, 128, F32)], ids=str)
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(4, 2, 64, BF16), (2, 1, 128, torch.float16), (3, 1, 256, BF16), (1, 1, 128, F32), (2, 1, 256, F32)], ids=str)
 def test_attention_of_a_long_prompt(device, heads, kv_heads, dim, dtype):
     """33001 tokens behind a short prompt, at rows near tile ends and spread over it"""
     rng = np.random.default_rng(dim)
