@@ -751,11 +751,12 @@ bool attention(const PromptAttention &a, hipStream_t stream)
     const bool wide = whole(a.query, a.query_row) && whole(a.gate, a.query_head) && whole(a.key, a.key_row) &&
                       whole(a.value, a.value_row) && whole(a.output, a.output_row);
     /* Few rows have few keys.  A wavefront to a row and head, against tiles, in us: 24 heads of 256
-     * on 4, fp32, 37 rows 5.9 against 27, 300 rows 82 against 92, 500 rows 197 against 140; bf16 64 rows
-     * 8.1 against 11.7, 128 rows 20.7 against 13.7; 32 heads of 128, bf16, 64 rows 6.1 against 7.6,
-     * 96 rows 10.7 against 8.8, fp32 128 rows 18 against 24, 200 rows 39 against 35; 16 of 64, fp32, 128
-     * rows 8.4 against 14.7, 300 rows 24 against 27. */
-    if (a.rows <= (sizeof(T) == 4 ? 64 + D : 64))
+     * on 4, fp32, 64 rows 9.5 against 11.5, 128 rows 21 against 18; 5 of 256 on 5, fp32, 320 rows 32 against 35;
+     * 24 of 256 bf16, 64 rows 8.1 against 11.7, 128 rows 20.7 against 13.7; 32 of 128, bf16, 64 rows 6.1
+     * against 7.6, 128 rows 13.8 against 8.8, fp32 128 rows 18 against 24, 200 rows 39 against 35; 16 of 64, fp32,
+     * 128 rows 8.4 against 14.7. */
+    constexpr uint32_t kFew = sizeof(T) == 4 ? 64 + D : 64, kFewWaves = D * sizeof(T) == 1024 ? 2048 : 5120;
+    if (a.rows <= kFew && (sizeof(T) == 2 || a.rows * a.heads <= kFewWaves))
         return launch_kernel(wide ? row_kernel<T, D, true> : row_kernel<T, D, false>, dim3(layer_up(a.rows * a.heads, 4)), dim3(256),
                              stream, a);
     /* a tile more for each sequence where tiles follow them */
