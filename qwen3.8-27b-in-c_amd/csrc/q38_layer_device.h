@@ -10,11 +10,11 @@ namespace q38 {
 typedef uint32_t layer_u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t layer_u32x2 __attribute__((ext_vector_type(2)));
 
-/* eight neighbours at any place of an element: the compiler makes wide accesses of it,
+/* N neighbours at any place of an element: the compiler makes wide accesses of it,
  * which this target takes at any address */
-template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) LayerEight {
-    T e[8];
+template <typename T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) LayerSome {
+    T e[N];
 };
 
 /* Eight neighbouring elements, or `some` of them.  Whole: 16-byte aligned and all there.
@@ -32,7 +32,7 @@ __device__ __forceinline__ void layer_load8(float v[8], const T *from, uint32_t 
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(e[i]);
     } else if (some == 8) {
-        const LayerEight<T> raw = *reinterpret_cast<const LayerEight<T> *>(from);
+        const LayerSome<T, 8> raw = *reinterpret_cast<const LayerSome<T, 8> *>(from);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(raw.e[i]);
     } else {
@@ -53,10 +53,10 @@ __device__ __forceinline__ void layer_store8(T *to, const float v[8], uint32_t s
 #pragma unroll
         for (int i = 0; i < kWords; ++i) reinterpret_cast<layer_u32x4 *>(to)[i] = raw[i];
     } else if (some == 8) {
-        LayerEight<T> raw;
+        LayerSome<T, 8> raw;
 #pragma unroll
         for (int i = 0; i < 8; ++i) raw.e[i] = static_cast<T>(v[i]);
-        *reinterpret_cast<LayerEight<T> *>(to) = raw;
+        *reinterpret_cast<LayerSome<T, 8> *>(to) = raw;
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -112,7 +112,7 @@ __device__ __forceinline__ void e4m3_store8(uint8_t *to, layer_u32x2 codes, uint
     if constexpr (kWhole) {
         *reinterpret_cast<layer_u32x2 *>(to) = codes;
     } else if (some == 8) {
-        *reinterpret_cast<LayerEight<uint8_t> *>(to) = __builtin_bit_cast(LayerEight<uint8_t>, codes);
+        *reinterpret_cast<LayerSome<uint8_t, 8> *>(to) = __builtin_bit_cast(LayerSome<uint8_t, 8>, codes);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)

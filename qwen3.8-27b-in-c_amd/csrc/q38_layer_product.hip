@@ -82,13 +82,14 @@ __device__ __forceinline__ void store_output(const ProductE4M3 &a, uint32_t toke
 template <typename T>
 __device__ __forceinline__ void store_four(const ProductE4M3 &a, uint32_t token, uint32_t row, f32x4 v)
 {
-    if (a.wide && row + 4 <= a.outputs) {
-        T e[4];
+    if (row + 4 <= a.outputs) {
+        LayerSome<T, 4> some;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = static_cast<T>(v[i]);
+        for (int i = 0; i < 4; ++i) some.e[i] = static_cast<T>(v[i]);
         T *to = static_cast<T *>(a.output) + (uint64_t)token * a.output_row + row;
-        if constexpr (sizeof(T) == 2) *reinterpret_cast<layer_u32x2 *>(to) = __builtin_bit_cast(layer_u32x2, e);
-        else *reinterpret_cast<layer_u32x4 *>(to) = __builtin_bit_cast(layer_u32x4, e);
+        struct Aligned { LayerSome<T, 4> some; } __attribute__((aligned(4 * sizeof(T))));
+        if (a.wide) *reinterpret_cast<Aligned *>(to) = Aligned{some};
+        else *reinterpret_cast<LayerSome<T, 4> *>(to) = some;
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -101,14 +102,17 @@ template <typename T>
 __device__ __forceinline__ void store_piece(const ProductE4M3 &a, uint32_t token, uint32_t row, layer_u32x4 piece)
 {
     constexpr uint32_t E = 16 / sizeof(T);
+    T *to = static_cast<T *>(a.output) + (uint64_t)token * a.output_row + row;
     if (a.wide && row + E <= a.outputs) {
-        *reinterpret_cast<layer_u32x4 *>(static_cast<T *>(a.output) + (uint64_t)token * a.output_row + row) = piece;
+        *reinterpret_cast<layer_u32x4 *>(to) = piece;
+    } else if (row + E <= a.outputs) {
+        *reinterpret_cast<LayerSome<T, E> *>(to) = __builtin_bit_cast(LayerSome<T, E>, piece);
     } else {
         T e[E];
         __builtin_memcpy(e, &piece, 16);
 #pragma unroll
         for (uint32_t i = 0; i < E; ++i)
-            if (row + i < a.outputs) static_cast<T *>(a.output)[(uint64_t)token * a.output_row + row + i] = e[i];
+            if (row + i < a.outputs) to[i] = e[i];
     }
 }
 
