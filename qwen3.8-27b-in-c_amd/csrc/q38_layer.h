@@ -71,7 +71,6 @@ struct ProductE4M3 {
     float *partial;
     uint32_t tokens, inputs, outputs, blocks, pitch;
     int type;
-    bool wide;             /* rows of the output are 16-byte aligned */
 };
 
 /* How a product is cut: tiles of so many matrix rows by tokens; `whole` of them have

@@ -128,8 +128,7 @@ extern "C" int q38hip_gemm_e4m3(void *output, uint32_t type, uint64_t output_row
     if (!aligned(workspace, 16)) return abi_fail("workspace must be 16-byte aligned");
     const q38::ProductE4M3 a = {output, output_row_stride, codes, scales, weight, weight_scales,
                                 static_cast<float *>(workspace), batch_size, (uint32_t)input_length, rows,
-                                q38::e4m3_blocks(input_length), q38::e4m3_pitch(input_length), (int)type,
-                                aligned(output, 16) && output_row_stride % (type == (uint32_t)q38::kLayerF32 ? 4 : 8) == 0};
+                                q38::e4m3_blocks(input_length), q38::e4m3_pitch(input_length), (int)type};
     return q38::launch_product_e4m3(a, static_cast<hipStream_t>(stream)) ? 1 : abi_fail("product kernel failed");
 }
 

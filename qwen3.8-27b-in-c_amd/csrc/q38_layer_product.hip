@@ -78,7 +78,7 @@ __device__ __forceinline__ void store_output(const ProductE4M3 &a, uint32_t toke
     static_cast<T *>(a.output)[(uint64_t)token * a.output_row + row] = static_cast<T>(v);
 }
 
-/* four neighbouring rows' outputs of a token, as far as there are rows */
+/* four neighbouring rows' outputs of a token, as far as there are rows; at any alignment of elements */
 template <typename T>
 __device__ __forceinline__ void store_four(const ProductE4M3 &a, uint32_t token, uint32_t row, f32x4 v)
 {
@@ -86,10 +86,7 @@ __device__ __forceinline__ void store_four(const ProductE4M3 &a, uint32_t token,
         LayerSome<T, 4> some;
 #pragma unroll
         for (int i = 0; i < 4; ++i) some.e[i] = static_cast<T>(v[i]);
-        T *to = static_cast<T *>(a.output) + (uint64_t)token * a.output_row + row;
-        struct Aligned { LayerSome<T, 4> some; } __attribute__((aligned(4 * sizeof(T))));
-        if (a.wide) *reinterpret_cast<Aligned *>(to) = Aligned{some};
-        else *reinterpret_cast<LayerSome<T, 4> *>(to) = some;
+        *reinterpret_cast<LayerSome<T, 4> *>(static_cast<T *>(a.output) + (uint64_t)token * a.output_row + row) = some;
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -103,9 +100,7 @@ __device__ __forceinline__ void store_piece(const ProductE4M3 &a, uint32_t token
 {
     constexpr uint32_t E = 16 / sizeof(T);
     T *to = static_cast<T *>(a.output) + (uint64_t)token * a.output_row + row;
-    if (a.wide && row + E <= a.outputs) {
-        *reinterpret_cast<layer_u32x4 *>(to) = piece;
-    } else if (row + E <= a.outputs) {
+    if (row + E <= a.outputs) {
         *reinterpret_cast<LayerSome<T, E> *>(to) = __builtin_bit_cast(LayerSome<T, E>, piece);
     } else {
         T e[E];
