@@ -89,7 +89,7 @@ inline ProductPlan plan_product(uint32_t tokens, uint32_t inputs, uint32_t outpu
      * 8.3 against 11.4, 17408 x 5120 22 against 18; 4 tokens, 5120 x 5120 9.8 against 11.3, 5120 x 14336
      * 16.7 against 14.7; 16 tokens, 5120 x 1024 7.6 against 11.6; 8 tokens, 5120 x 14336 18 against 15. */
     const uint64_t codes = (uint64_t)inputs * outputs;
-    if ((tokens <= 4 && codes <= 1u << 25) || (tokens <= 16 && codes <= 1u << 23) || inputs < kE4M3Block)
+    if ((tokens <= 4 && codes <= 1u << 25) || (tokens <= 16 && codes <= 1u << 23))
         return {kProductFew, 0, 1, 0};
     /* One workgroup of tiles to a compute unit.  Of the tiles that do not fill a round, each is cut
      * into as many parts as there are units, of four blocks of inputs or more. */

@@ -111,26 +111,20 @@ __device__ __forceinline__ void store_piece(const ProductE4M3 &a, uint32_t token
     }
 }
 
-/* 16 matrix rows by 16 * M tokens to a workgroup, whose eight wavefronts take
+/* 16 matrix rows by up to 16 tokens to a workgroup, whose eight wavefronts take
  * every eighth block of inputs and are summed in LDS in their order: many short
  * workgroups, whose loads are all in flight at once, for matrices that a second launch would
  * not repay (one token, 5120 x 5120: 8.3 us). */
-template <typename T, int M>
+template <typename T>
 __global__ void __launch_bounds__(kWaves * 64) few_kernel(ProductE4M3 a)
 {
-    __shared__ float sums[kWaves][M * 4][64];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t row0 = blockIdx.x * 16, token0 = blockIdx.y * (16 * M);
+    __shared__ float sums[kWaves][4][64];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row0 = blockIdx.x * 16;
     const uint8_t *matrix = a.weight + (uint64_t)min(row0 + lane % 16, a.outputs - 1) * a.inputs;
-    const uint8_t *codes[M], *scales[M];
-#pragma unroll
-    for (int m = 0; m < M; ++m) {
-        const uint64_t token = min(token0 + m * 16 + lane % 16, a.tokens - 1);
-        codes[m] = a.codes + token * a.inputs;
-        scales[m] = a.scales + token * a.pitch;
-    }
+    const uint64_t mine = min(lane % 16, a.tokens - 1);
+    const uint8_t *codes = a.codes + mine * a.inputs, *scales = a.scales + mine * a.pitch;
     const float *weight_scales = a.weight_scales + (uint64_t)(row0 / kE4M3Block) * a.blocks;
-    f32x4 sum[M] = {};
+    f32x4 sum = {};
     for (uint32_t b = wave; b < a.blocks; b += kWaves) {
         const uint32_t at = b * kE4M3Block + lane / 16 * 16;
         const bool low = at < a.inputs, high = at + 64 < a.inputs;
@@ -139,28 +133,21 @@ __global__ void __launch_bounds__(kWaves * 64) few_kernel(ProductE4M3 a)
             const i32x4 h = high ? *reinterpret_cast<const i32x4 *>(row + at + 64) : i32x4{};
             return both(l, h);
         };
-        const i32x8 w = load(matrix);
+        const i32x8 w = load(matrix), token = load(codes);
         const float s = weight_scales[b];
-#pragma unroll
-        for (int m = 0; m < M; ++m) {
-            const i32x8 token = load(codes[m]);
-            if constexpr (std::is_same_v<T, float>) sum[m] = add_exact(sum[m], w, token, scales[m][b], s);
-            else sum[m] = add_scaled(sum[m], block_product(w, token, scales[m][b]), s);
-        }
+        if constexpr (std::is_same_v<T, float>) sum = add_exact(sum, w, token, scales[b], s);
+        else sum = add_scaled(sum, block_product(w, token, scales[b]), s);
     }
 #pragma unroll
-    for (int m = 0; m < M; ++m)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sums[wave][m * 4 + r][lane] = sum[m][r];
+    for (int r = 0; r < 4; ++r) sums[wave][r][lane] = sum[r];
     __syncthreads();
-    /* output i of 256 M: token i / 16, matrix row i % 16 */
-    for (uint32_t i = threadIdx.x; i < 256 * M; i += kWaves * 64) {
-        const uint32_t r = i % 16, t = i / 16;
-        float v = 0.0f;
+    /* an output to a thread: token i / 16, matrix row i % 16 */
+    const uint32_t r = threadIdx.x % 16, t = threadIdx.x / 16;
+    if (t >= a.tokens || row0 + r >= a.outputs) return;
+    float v = 0.0f;
 #pragma unroll
-        for (uint32_t w = 0; w < kWaves; ++w) v += sums[w][t / 16 * 4 + r % 4][r / 4 * 16 + t % 16];
-        if (token0 + t < a.tokens && row0 + r < a.outputs) store_output<T>(a, token0 + t, row0 + r, v);
-    }
+    for (uint32_t w = 0; w < kWaves; ++w) v += sums[w][r % 4][r / 4 * 16 + t];
+    store_output<T>(a, t, row0 + r, v);
 }
 
 /* ---- tiles --------------------------------------------------------------------- */
@@ -248,13 +235,15 @@ __global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a
 
     /* what this lane copies: 8 rows of 128 bytes at a time */
     const uint8_t *matrix = a.weight + (uint64_t)row0 * a.inputs, *codes = a.codes + (uint64_t)token0 * a.inputs;
+    /* rows shorter than a block lie at the end of the stage's, their first codes before them too */
+    const uint32_t missing = __builtin_amdgcn_readfirstlane(a.inputs < kE4M3Block ? kE4M3Block - a.inputs : 0);
     uint32_t offset[kRowParts + kTokenParts];
 #pragma unroll
     for (int i = 0; i < kRowParts + kTokenParts; ++i) {
         const bool token = i >= kRowParts;
         const uint32_t r = ((token ? i - kRowParts : i) * kWaveCount + wave) * 8 + lane / 8;
         const uint32_t last = (token ? a.tokens - token0 : a.outputs - row0) - 1;
-        offset[i] = min(r, last) * a.inputs + ((lane & 7) ^ piece_turn(r)) * 16;
+        offset[i] = min(r, last) * a.inputs + max(((lane & 7) ^ piece_turn(r)) * 16, missing) - missing;
     }
     const uint32_t stages_at = (uint32_t)(uintptr_t)(Q38_LDS const void *)stages;
     /* wavefront w copies the words of tokens 64 w on, the last one the factors */
@@ -268,7 +257,7 @@ __global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a
         if (has_scales) copy_words_to_lds(scales + block / 4 * 4, scale_offset, stage_at + Tile::kScalesAt + wave * 256);
         if (wave == kWaveCount - 1) copy_words_to_lds(factors + block, factor_offset, stage_at + Tile::kFactorsAt);
         /* of a row's end the last 128 codes, so nothing behind it is read */
-        const uint32_t from = min(block * kE4M3Block, a.inputs - kE4M3Block);
+        const uint32_t from = min(block * kE4M3Block, a.inputs + missing - kE4M3Block);
 #pragma unroll
         for (int i = 0; i < kRowParts + kTokenParts; ++i)
             if (i < Tile::kLeast || (i - kRowParts) * kWaveCount + wave < Tile::kTokens / 8)
@@ -434,11 +423,7 @@ bool product(const ProductE4M3 &a, hipStream_t stream)
     if (plan.tile == kProductTile128) return tiled<T, Tile128>(a, plan, stream);
     if (plan.tile == kProductTile16) return tiled<T, Tile16>(a, plan, stream);
     if (plan.tile == kProductTile64) return tiled<T, Tile64>(a, plan, stream);
-    const uint32_t tiles = layer_up(a.outputs, 16);
-    const int m = a.tokens <= 16 ? 1 : a.tokens <= 32 ? 2 : 4;
-    const dim3 grid(tiles, layer_up(a.tokens, 16 * m));
-    const auto kernel = m == 1 ? few_kernel<T, 1> : m == 2 ? few_kernel<T, 2> : few_kernel<T, 4>;
-    return launch_kernel(kernel, grid, dim3(kWaves * 64), stream, a);
+    return launch_kernel(few_kernel<T>, dim3(layer_up(a.outputs, 16)), dim3(kWaves * 64), stream, a);
 }
 
 }  // namespace

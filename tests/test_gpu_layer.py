@@ -136,7 +136,9 @@ PRODUCTS = [(1, 16, 1), (1, 128, 16), (1, 5120, 17), (2, 144, 130), (3, 1168, 10
             (300, 4096, 256), (512, 384, 1024), (700, 528, 770), (2100, 272, 6010), (1030, 768, 10300),
             # every tile size whole, cut along the inputs, and both
             (9, 400, 33000), (9, 1040, 33300), (17, 912, 33320), (66, 144, 17160), (199, 912, 17160), (66, 3600, 6050), (17, 912, 35340),
-            (516, 912, 22210), (199, 6672, 10090)]
+            (516, 912, 22210), (199, 6672, 10090),
+            # rows shorter than a block, for every tile
+            (16, 16, 40), (9, 112, 76000), (40, 16, 300), (150, 48, 520), (300, 80, 2600), (600, 96, 140), (4096, 112, 4100)]
 
 
 def _factors(rng, tokens, inputs, outputs):
