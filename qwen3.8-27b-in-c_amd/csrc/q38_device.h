@@ -110,4 +110,27 @@ __device__ __forceinline__ float sqrt_rn(float a) { return __builtin_sqrtf(a); }
 __device__ __forceinline__ float fmul_rn(float a, float b) { return __fmul_rn(a, b); }
 __device__ __forceinline__ float fadd_rn(float a, float b) { return __fadd_rn(a, b); }
 
+/* e^-a for a of 0 to 256 as the result, 0.7 to 1.42, times 2^n.  log2(e) is in two
+ * parts, so the error does not grow with a. */
+__device__ __forceinline__ float exp_fraction(float a, int &n)
+{
+    constexpr float kHigh = 1.44269502f, kLow = 1.92596299e-8f;
+    const float whole = __builtin_rintf(-a * kHigh);
+    n = (int)whole;
+    return __builtin_amdgcn_exp2f(fmaf(-a, kLow, fmaf(-a, kHigh, -whole)));
+}
+
+/* 1 / (1 + e^-x) within 2^-21 of itself, or, where it is subnormal, 2^-149.
+ * With E = e^-|x| it is 1 / (1 + E), for negative x E / (1 + E): nothing
+ * overflows.  E is 0 in fp32 from |x| = 104 on, so x ends at 128 (a NaN stays one). */
+__device__ __forceinline__ float sigmoid_f32(float x)
+{
+    float a = fabsf(x);
+    if (a > 128.0f) a = 128.0f;
+    int n;
+    const float part = exp_fraction(a, n), e = ldexpf(part, n), d = 1.0f + e;
+    const float first = __builtin_amdgcn_rcpf(d), inverse = fmaf(first, fmaf(-d, first, 1.0f), first);
+    return x < 0.0f ? e * inverse : inverse;
+}
+
 }  // namespace q38

@@ -156,7 +156,7 @@ __device__ __forceinline__ void attend_row(const PromptAttention &a, uint32_t ro
 #pragma unroll
     for (int e = 0; e < kChannels; ++e) {
         float v = out[e] * inverse;
-        if (a.gate) v *= __builtin_amdgcn_rcpf(1.0f + __expf(-gate[e]));
+        if (a.gate) v *= sigmoid_f32(gate[e]);
         to[e] = static_cast<T>(v);
     }
 }
@@ -735,11 +735,13 @@ __global__ void __launch_bounds__((PromptTile<T, D, kShares>::kWaves * 64 * kPar
                 const uint64_t at = __shfl(output_at, r);
 #pragma unroll
                 for (int j = 0; j < E; j += 4) {
-                    const f32x4 four = *reinterpret_cast<const f32x4 *>(turned + place_of(r, (piece + j) / 4));
+                    f32x4 four = *reinterpret_cast<const f32x4 *>(turned + place_of(r, (piece + j) / 4));
+                    if (gate) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        e[b][j + k] = static_cast<T>(
-                            gate ? four[k] * __builtin_amdgcn_rcpf(1.0f + __expf(-static_cast<float>(e[b][j + k]))) : four[k]);
+                        for (int k = 0; k < 4; ++k) four[k] *= sigmoid_f32(static_cast<float>(e[b][j + k]));
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) e[b][j + k] = static_cast<T>(four[k]);
                 }
                 if (done >> r & 1) store_piece<kWhole>(output + at + channel, __builtin_bit_cast(u32x4, e[b]));
             }

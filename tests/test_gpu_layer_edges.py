@@ -47,3 +47,36 @@ def test_infinite_values(device, form, dim, dtype):
     assert np.array_equal(np.isinf(got) * np.sign(got), infinite)
     far = np.abs(got - want)[infinite == 0] / bound[infinite == 0]
     assert far.max() <= 1, "worst %g of its bound" % far.max()
+
+
+# ---- gates of all sizes -----------------------------------------------------------------
+
+GATES = [0.0, 1.0, -1.0, 20.0, -20.0, -40.0, 40.0, -60.0, -80.0, 87.0, -87.0, 87.5, -87.5, 88.0, -88.0, 89.0, -89.0, 90.0, -90.0, 95.0, -95.0, 100.0,
+         -100.0, 103.0, -103.0, 104.0, -104.0, 1e4, -1e4, 5e4, -5e4, 1e9, -1e9, 1e30, -1e30, 3e38, -3e38, np.inf, -np.inf, np.nan]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_gates_of_all_sizes(device, form, dim, dtype):
+    """Rows of a sequence have one value, a small whole number times a power of two, and keys of 0: weights are equal and sums exact, which
+    leaves three roundings (the total's inverse, its product, the gate's) beside the sigmoid.  That is good to 2^-21, or to its
+    smallest step where it is subnormal in fp32."""
+    rng = np.random.default_rng(dim)
+    lengths = FORMS[form]
+    starts = kc.offsets(lengths)
+    q = _normal(rng, starts[-1], 4, dim, dtype=dtype)
+    k = torch.zeros(starts[-1], 2, dim, dtype=dtype, device=device)
+    one = torch.from_numpy(rng.integers(1, 9, size=(len(lengths), 2, dim)) * np.exp2(rng.integers(-3, 4, size=(len(lengths), 2, dim))))
+    v = one.repeat_interleave(torch.tensor(lengths), 0).to(dtype).to(device)
+    at = torch.arange(starts[-1])[:, None, None] + torch.arange(4)[:, None] + torch.arange(dim)
+    gate = torch.tensor(GATES, dtype=torch.float64)[at % len(GATES)].to(dtype)
+    got = f64(layer.attention(q, k, v, kc.words(starts, device), gate=gate.to(device)))
+    g, value = gate.double().numpy(), f64(v).repeat(2, 1)
+    with np.errstate(over="ignore"):
+        want = value / (1 + np.exp(-g))
+    number = ~np.isnan(g)
+    assert np.array_equal(np.isnan(got), ~number)
+    bound = np.abs(want) * (2.0 ** -21 + 3 * 2.0 ** -24) + 2.0 ** -149 * (1 + value) + lc.rounding(want, dtype) * 1.01
+    far = np.abs(got - want)[number] / bound[number]
+    assert far.max() <= 1, "worst %g of its bound" % far.max()
