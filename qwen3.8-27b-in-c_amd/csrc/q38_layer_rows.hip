@@ -14,6 +14,17 @@ constexpr auto up = layer_up;
 
 /* ---- rows into 8 bits ------------------------------------------------------ */
 
+/* x * g / (1 + e^-g) for g below kFarGate, where e^-g is all of the divisor: e^g leaves fp32's range long before the product
+ * does, so its power of two is applied in two halves.  Nothing is left below -256 for any x. */
+constexpr float kFarGate = -80.0f;
+__device__ __forceinline__ float times_far_silu(float x, float g)
+{
+    if (g == -INFINITY) return g - g;                        /* -infinity / infinity */
+    int n;
+    const float a = fminf(-g, 256.0f), part = exp_fraction(a, n);
+    return ldexpf(x * ldexpf(-a * part, n / 2), n - n / 2);
+}
+
 /* A thread takes eight neighbours, 16 lanes a block.  A row has `parts`
  * workgroups of 256 threads.  Bound by bytes: SwiGLU of 4096 bf16 rows of 17408 moves 357
  * MB in 61 us, 5.8 TB/s; 48 rows 3 us, a launch's latency. */
@@ -30,8 +41,17 @@ __global__ void __launch_bounds__(256) quantize_kernel(QuantizeRows a, uint32_t 
         if constexpr (kGate) {
             float g[8];
             layer_load8<T, kWhole>(g, static_cast<const T *>(a.gate) + row * a.gate_row + at, some);
+            float least = g[0];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] *= g[i] * __builtin_amdgcn_rcpf(1.0f + __expf(-g[i]));
+            for (int i = 1; i < 8; ++i) least = fminf(least, g[i]);
+            if (least < kFarGate) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    v[i] = g[i] < kFarGate ? times_far_silu(v[i], g[i]) : v[i] * (g[i] * __builtin_amdgcn_rcpf(1.0f + __expf(-g[i])));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] *= g[i] * __builtin_amdgcn_rcpf(1.0f + __expf(-g[i]));
+            }
             if constexpr (!kWhole) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = (uint32_t)i < some ? v[i] : 0.0f;

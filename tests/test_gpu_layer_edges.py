@@ -80,3 +80,21 @@ def test_gates_of_all_sizes(device, form, dim, dtype):
     bound = np.abs(want) * (2.0 ** -21 + 3 * 2.0 ** -24) + 2.0 ** -149 * (1 + value) + lc.rounding(want, dtype) * 1.01
     far = np.abs(got - want)[number] / bound[number]
     assert far.max() <= 1, "worst %g of its bound" % far.max()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+@pytest.mark.parametrize("width", [1024, 1001])
+def test_swiglu_of_far_gates(device, width, dtype):
+    """Gates whose sigmoid leaves fp32's range and values that bring the product back into it, a block of 128 of each size; gates so
+    far that nothing is left.  The error of e^-g: up to -80 its argument's two roundings (2^-18 each of an argument below 128, times
+    ln 2), beyond that less."""
+    rng = np.random.default_rng(width)
+    sizes = np.array([-60.0, -80.0, -86.0, -88.0, -95.0, -104.0, -120.0, 100.0])
+    gate = torch.from_numpy(np.repeat(sizes, 128)[:width] + rng.uniform(-0.9, 0.9, size=(3, width))).to(dtype).to(device)
+    x = torch.from_numpy(rng.normal(size=(3, width)) * np.where(np.repeat(sizes, 128)[:width] < 0, 3e37, 1.0)).to(dtype).to(device)
+    lc.check_quantized(layer.quantize(x, gate=gate), f64(x) * lc.silu(f64(gate)), 2.0 ** -17)
+    for far in (-250.0, -1e4, -3e38):
+        got = layer.quantize(x, gate=torch.full_like(gate, far))
+        assert (got.codes.float() == 0).all() and (got.scales.view(torch.uint8)[:, :-(-width // 128)] == 27).all()
+    got = layer.quantize(x, gate=torch.full_like(gate, -np.inf))
+    assert (got.scales.view(torch.uint8)[:, :-(-width // 128)] == 255).all()
