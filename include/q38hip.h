@@ -471,7 +471,8 @@ int q38hip_rotary(void *output, uint64_t output_row_stride, uint64_t output_head
  * rows of key, value and output are their strides apart, heads head_dim, which
  * is 64, 128 or 256, of at most 65535 heads.  Scores, statistics and sums are in
  * fp32; in the second product the weights of 16-bit rows have 8 (BF16) or 11 (F16)
- * bits. */
+ * bits, those of F16 below 2^-9 of the largest weight of the same 32 or 64 keys
+ * fewer (they are off by up to 2^-20 of that one). */
 int q38hip_prompt_attention(void *output, uint64_t output_row_stride, const void *query, const void *gate,
                             uint64_t query_row_stride, uint64_t query_head_stride, const void *key,
                             uint64_t key_row_stride, const void *value, uint64_t value_row_stride, uint32_t type,

@@ -337,8 +337,8 @@ __device__ __forceinline__ uint32_t value_turn(uint32_t row)
  * each half of the wavefront, the keys that the second product, O^T = V^T P^T, takes
  * from that half: the weights go from one product to the other in registers.  So
  * statistics and rescaling are per lane; one exchange between the halves joins a
- * maximum.  The maximum that weights are relative to is raised only where a score
- * exceeds it by more than 2^8: then the sums are rescaled.
+ * maximum.  The maximum that weights are relative to is moved only where a score
+ * exceeds it by more than 2^8 (fp16: or a tile's largest is 2^12 below): then the sums are rescaled.
  *
  * Pieces of keys and values are read from LDS kAhead products early, the first of the
  * values before the softmax: a product that waits for a read of its own leaves the matrix
@@ -509,6 +509,14 @@ __global__ void __launch_bounds__((PromptTile<T, D, kShares>::kWaves * 64 * kPar
 
     f32x16 out[kOwn / 32] = {};
     float top = -INFINITY, base = 0.0f, total = 0.0f;
+    /* Weights of fp16 rows are relative to 2^(top - 7), so at most 2^15, and the largest of each tile is at least 2^-5:
+     * top follows the tiles' maxima down too (as far as `least`, 2^40 below the highest that it was), so that the
+     * small weights beside a far larger one, thousands of which count, keep their 11 bits.  Within a tile those below
+     * 2^-14 are in steps of 2^-24.  32 heads of 128, 8192 tokens: 550 us, 545 with weights relative to 2^top alone;
+     * with kFall = 8, which scores of ordinary spread meet, 556. */
+    constexpr bool kNarrow = std::is_same_v<T, _Float16>;
+    constexpr float kBelow = kNarrow ? 7.0f : 0.0f, kFall = 12.0f;
+    float least = -INFINITY;
 
     /* piece 2 u + half of key row 32 t + low; `lane_at` holds what is the lane's of its place */
     const uint32_t key_lane_at = low * kRowBytes + (half ^ key_turn<kRowBytes>(low)) * 16;
@@ -600,12 +608,14 @@ __global__ void __launch_bounds__((PromptTile<T, D, kShares>::kWaves * 64 * kPar
 #pragma unroll
             for (int r = 0; r < 16; ++r) most = fmaxf(most, score[t][r]);
         most = halves_max(most) * scale;
-        if (__any(most > top + 8.0f)) {
+        if constexpr (kNarrow) most = fmaxf(most, least);
+        if (__any(kNarrow ? (most > top + 8.0f || most < top - kFall) : most > top + 8.0f)) {
             const float before = top;
-            top = fmaxf(top, most);
+            top = kNarrow && most < top - kFall ? most : fmaxf(top, most);
+            least = fmaxf(least, top - 40.0f);
             /* nothing but -infinity so far: differences would be NaN, weights are 0 */
-            base = top == -INFINITY ? 0.0f : top;
-            const float shrink = __builtin_amdgcn_exp2f(before - base);
+            base = top == -INFINITY ? 0.0f : top - kBelow;
+            const float shrink = __builtin_amdgcn_exp2f(before - kBelow - base);
             total *= shrink;
 #pragma unroll
             for (int d = 0; d < kOwn / 32; ++d)

@@ -98,3 +98,64 @@ def test_swiglu_of_far_gates(device, width, dtype):
         assert (got.codes.float() == 0).all() and (got.scales.view(torch.uint8)[:, :-(-width // 128)] == 27).all()
     got = layer.quantize(x, gate=torch.full_like(gate, -np.inf))
     assert (got.scales.view(torch.uint8)[:, :-(-width // 128)] == 255).all()
+
+
+# ---- attention: keys far above the others --------------------------------------------------
+
+
+def _step_bound(v, tokens, low):
+    """What fp16 weights add beside half a step each: a step's weights (up to 64 keys) are off by up to 2^-20 of the step's
+    largest one, which is 1 (relative to the row's largest) in the step that holds that key and `low` in the others."""
+    return (64 + tokens * low) * 2.0 ** -20 * np.abs(v).max()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv_heads,tokens", [(2, 1, 8192), (16, 4, 8192), (2, 2, 300)], ids=["two parts", "one part", "short"])
+@pytest.mark.parametrize("gap", [10.0, 17.5, 21.0])
+def test_sink(device, gap, heads, kv_heads, tokens, dim):
+    """One key whose score is `gap` above all others' and whose value is 0, as the values of the 63 behind it: the thousands of small
+    weights keep the bits of their type"""
+    rng = np.random.default_rng(dim)
+    q = torch.ones(tokens, heads, dim, dtype=F16, device=device)
+    k = torch.zeros(tokens, kv_heads, dim, dtype=F16, device=device)
+    k[0] = gap * dim ** -0.5
+    v = (_normal(rng, tokens, kv_heads, dim) * 500 + 3000).to(F16)
+    v[:64] = 0
+    got = layer.attention(q, k, v, kc.words([0, tokens], device))
+    at = np.array([0, 63, 64, 65, 100, 130, tokens // 2, tokens - 2, tokens - 1])
+    want, mass, size = lc.attention_of(f64(q[at]), f64(k), f64(v), at, dim ** -0.5)
+    lc.check(got[at], want, lc.attention_bound(want, mass, size, F16, tokens) + tokens * np.exp(-gap) * 2.0 ** -24 * f64(v).max())
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lengths", [[1300], [200, 150, 310], [25, 90] * 33], ids=["two parts", "one part", "many"])
+def test_scores_that_rise_and_fall(device, lengths, dim):
+    """Steps of keys whose scores are 20 above or below the last step's, so what weights are relative to goes up and down.  Each
+    step's weights are off by 2^-20 of its largest beside half a step of their own, and no step's largest is above the row's."""
+    rng = np.random.default_rng(dim)
+    starts = kc.offsets(lengths)
+    rows = starts[-1]
+    q = _normal(rng, rows, 4, dim) * 0.3
+    q[..., 0] = dim ** 0.5
+    k, v = _normal(rng, rows, 2, dim) * 0.3, _normal(rng, rows, 2, dim)
+    k[..., 0] = torch.from_numpy(np.repeat(rng.uniform(-20, 20, size=-(-rows // 32)), 32)[:rows, None]).to(device)
+    q, k, v = q.to(F16), k.to(F16), v.to(F16)
+    want, mass, size, _ = lc.attention(f64(q), f64(k), f64(v), starts, dim ** -0.5)
+    bound = lc.attention_bound(want, mass, size, F16, max(lengths)) + max(lengths) * 2.0 ** -20 * np.abs(f64(v)).max()
+    lc.check(layer.attention(q, k, v, kc.words(starts, device)), want, bound)
+
+
+def test_sink_within_a_step(device):
+    """the small weights of the sink's own step of keys"""
+    rng = np.random.default_rng(1)
+    for dim in (64, 128, 256):
+        lengths = [70] * 5
+        starts = kc.offsets(lengths)
+        q = torch.ones(350, 2, dim, dtype=F16, device=device)
+        k = torch.zeros(350, 1, dim, dtype=F16, device=device)
+        k[starts[:-1]] = 12.0 * dim ** -0.5
+        v = (_normal(rng, 350, 1, dim) + 5).to(F16)
+        v[starts[:-1]] = 0
+        want, mass, size, _ = lc.attention(f64(q), f64(k), f64(v), starts, dim ** -0.5)
+        bound = lc.attention_bound(want, mass, size, F16, 70) + _step_bound(f64(v), 70, np.exp(-12))
+        lc.check(layer.attention(q, k, v, kc.words(starts, device)), want, bound)
