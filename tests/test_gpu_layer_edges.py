@@ -159,3 +159,52 @@ def test_sink_within_a_step(device):
         want, mass, size, _ = lc.attention(f64(q), f64(k), f64(v), starts, dim ** -0.5)
         bound = lc.attention_bound(want, mass, size, F16, 70) + _step_bound(f64(v), 70, np.exp(-12))
         lc.check(layer.attention(q, k, v, kc.words(starts, device)), want, bound)
+
+
+# ---- product: what 16-bit outputs keep --------------------------------------------------------
+
+# every tile size whole, cut along the inputs, and both; few tokens; rows that end inside a block
+SIZES = [(1, 5120, 17), (4, 2048, 256), (9, 4112, 2050), (3, 17408, 2000), (9, 400, 33000), (33, 1024, 300), (48, 17408, 144), (65, 256, 513), (100, 1280, 1000),
+         (128, 128, 128), (200, 2064, 260), (257, 896, 511), (300, 4096, 256), (66, 3600, 6050), (516, 912, 2210), (700, 528, 770), (1030, 768, 1030),
+         (300, 80, 2600)]
+
+
+def _half_step(want, dtype):
+    return np.exp2(np.floor(np.log2(np.maximum(np.abs(want), torch.finfo(dtype).smallest_normal)))) * torch.finfo(dtype).eps / 2
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("tokens,inputs,outputs", SIZES)
+def test_product_of_16_bit_outputs(device, tokens, inputs, outputs, dtype):
+    """The error of all outputs together: 1e-4 of the result's norm, three times what the header states for such factors, and the
+    rounding, whose square is a third of the half step's on average and, over n outputs, 8 / sqrt(n) more of it at most (its standard
+    deviation is 0.9 / sqrt(n))."""
+    rng = np.random.default_rng(tokens + inputs + outputs)
+    rows8 = layer.quantize(_normal(rng, tokens, inputs) * torch.from_numpy(np.exp(0.7 * rng.normal(size=inputs))).float().to(device))
+    weight = (_normal(rng, outputs, inputs) * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+    scales = torch.from_numpy(np.exp(rng.normal(size=(-(-outputs // 128), -(-inputs // 128)))) * 0.01).float().to(device)
+    to_bytes = lambda t: t.view(torch.uint8).cpu().numpy()  # noqa: E731
+    want, _ = lc.product(to_bytes(rows8.codes), to_bytes(rows8.scales), to_bytes(weight), scales.cpu().numpy())
+    want *= 2.0 ** -8                                # within fp16's range
+    got = f64(layer.product(rows8, weight, scales * 2.0 ** -8, dtype))
+    most = (1e-4 * np.linalg.norm(want)) ** 2 + (_half_step(want, dtype) ** 2).sum() / 3 * (1 + 8 / np.sqrt(want.size))
+    assert ((got - want) ** 2).sum() <= most, "%g of its bound" % np.sqrt(((got - want) ** 2).sum() / most)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("tokens,inputs,outputs", SIZES)
+def test_product_of_small_whole_numbers(device, tokens, inputs, outputs, dtype):
+    """codes of -4 to 4, whose products span five bits, and scales that are powers of two: sums are exact, so every output is the exact
+    one, rounded once"""
+    rng = np.random.default_rng(tokens)
+    blocks = -(-inputs // 128)
+    codes = torch.from_numpy(rng.integers(-4, 5, size=(tokens, inputs))).float().to(torch.float8_e4m3fn).to(device)
+    weight = torch.from_numpy(rng.integers(-4, 5, size=(outputs, inputs))).float().to(torch.float8_e4m3fn).to(device)
+    scales = np.zeros((tokens, lc.pitch(inputs)), dtype=np.uint8)
+    scales[:, :blocks] = rng.integers(125, 128, size=(tokens, blocks))
+    factors = np.exp2(rng.integers(-2, 2, size=(-(-outputs // 128), blocks))).astype(np.float32)
+    rows8 = (codes, torch.from_numpy(scales).to(device).view(torch.float8_e8m0fnu))
+    to_bytes = lambda t: t.view(torch.uint8).cpu().numpy()  # noqa: E731
+    want, _ = lc.product(to_bytes(codes), scales, to_bytes(weight), factors)
+    got = layer.product(rows8, weight, torch.from_numpy(factors).to(device), dtype)
+    assert torch.equal(got.cpu(), torch.from_numpy(want).to(dtype))
