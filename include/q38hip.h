@@ -417,7 +417,8 @@ int q38hip_kv_attention(const Q38KVPages *cache, uint32_t layer, void *output, c
 uint32_t q38hip_e4m3_scale_pitch(uint64_t width);
 
 /* Rows into 8 bits: x, or x * silu(gate) where gate is not NULL (gate / (1 +
- * e^-gate), the middle of a SwiGLU).  width and rows up to 2^24. */
+ * e^-gate), the middle of a SwiGLU).  width up to 2^24, rows * ceil(width /
+ * 2048) below 2^24. */
 int q38hip_quantize_e4m3(uint8_t *codes, uint8_t *scales, const void *x, uint64_t x_row_stride, const void *gate,
                          uint64_t gate_row_stride, uint32_t type, uint64_t width, uint32_t rows, void *stream);
 
@@ -426,7 +427,8 @@ int q38hip_quantize_e4m3(uint8_t *codes, uint8_t *scales, const void *x, uint64_
  * (weight + weight_offset).  y goes to output, in `type`, where that is not
  * NULL, and to codes and scales where those are not NULL; one of them at least.
  * weight has `width` elements of weight_type.  total may be x or addend itself
- * (same pointer and stride), output x or addend, total not output. */
+ * (same pointer and stride), output x or addend, total not output.  width up to
+ * 2^24, rows below 2^24, with widths above 8192 below 2^22; 2^40 elements. */
 int q38hip_rms_norm(void *output, uint64_t output_row_stride, uint8_t *codes, uint8_t *scales, void *total,
                     uint64_t total_row_stride, const void *x, uint64_t x_row_stride, const void *addend,
                     uint64_t addend_row_stride, uint32_t type, const void *weight, uint32_t weight_type,
@@ -440,6 +442,7 @@ int q38hip_rms_norm(void *output, uint64_t output_row_stride, uint8_t *codes, ui
  * output is of `type`, rows output_row_stride elements apart.  Products of codes are
  * exact and their sums in fp32; for 16-bit outputs the matrix unit adds a block's
  * products at 13 bits below the largest of them (about 3e-5 of the result's norm).
+ * batch_size, input_length and rows up to 2^24, 2^36 outputs.
  * q38hip_gemm_e4m3_workspace_bytes: device memory for the call, 16-byte aligned
  * (0: none needed, or a bad call). */
 uint64_t q38hip_gemm_e4m3_workspace_bytes(uint32_t batch_size, uint64_t input_length, uint32_t rows);
@@ -453,7 +456,7 @@ int q38hip_gemm_e4m3(void *output, uint32_t type, uint64_t output_row_stride, co
  * 2i and 2i + 1 where interleaved is not 0, else i and i + pairs; channels from
  * 2 * pairs on are copied.  Angles are formed in fp64, so far positions keep
  * the accuracy of near ones.  output may be x itself (same pointer and strides).
- * 2 * pairs <= head_dim <= 1024, heads * head_dim <= 2^20. */
+ * 2 * pairs <= head_dim <= 1024, heads * head_dim <= 2^20, rows below 2^24. */
 int q38hip_rotary(void *output, uint64_t output_row_stride, uint64_t output_head_stride, const void *x,
                   uint64_t x_row_stride, uint64_t x_head_stride, uint32_t type, uint32_t rows, uint32_t heads,
                   uint32_t head_dim, const int32_t *positions, const float *frequencies, uint32_t pairs,
@@ -469,7 +472,8 @@ int q38hip_rotary(void *output, uint64_t output_row_stride, uint64_t output_head
  * key/value head h / (heads / kv_heads).  Head h of a row begins at row *
  * query_row_stride + h * query_head_stride elements of query and of gate;
  * rows of key, value and output are their strides apart, heads head_dim, which
- * is 64, 128 or 256, of at most 65535 heads.  Scores, statistics and sums are in
+ * is 64, 128 or 256, of at most 65535 heads; up to 2^24 rows and sequences,
+ * total_rows * heads up to 2^30.  Scores, statistics and sums are in
  * fp32; in the second product the weights of 16-bit rows have 8 (BF16) or 11 (F16)
  * bits, those of F16 below 2^-9 of the largest weight of the same 32 or 64 keys
  * fewer (they are off by up to 2^-20 of that one). */

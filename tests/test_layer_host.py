@@ -201,3 +201,47 @@ def test_product_plans(tmp_path):
     assert run.returncode == 0, run.stdout
     seen = [[int(v) for v in line.split()] for line in run.stdout.split("\n") if line]
     assert seen[0][0] and all(all(row) for row in seen[1:]), seen
+
+
+LIMIT_CHECK = r"""
+#include <cstdio>
+#include "q38_layer.h"
+using namespace q38;
+int main()
+{
+    const uint64_t widths[] = {1, 128, 2048, 2049, 4096, 8192, 8193, 17408, 1u << 20, 1u << 24};
+    for (uint64_t width : widths) {
+        const uint64_t parts = (width + 2047) / 2048, quantized = ((1u << 24) - 1) / parts, normed = width > 8192 ? (1u << 22) - 1 : (1u << 24) - 1;
+        if (!layer_launch_holds(quantized * quantize_parts(width), 256) || layer_launch_holds((quantized + 1) * quantize_parts(width), 256) ||
+            !layer_launch_holds(normed, norm_threads(width)) || layer_launch_holds(normed + 1, norm_threads(width))) {
+            std::printf("width %llu\n", (unsigned long long)width);
+            return 1;
+        }
+    }
+    return !layer_launch_holds((1u << 24) - 1, 256) || layer_launch_holds(1u << 24, 256);
+}
+"""
+
+
+def _run_cpp(tmp_path, text):
+    source, program = tmp_path / "check.cpp", str(tmp_path / "check")
+    source.write_text(text)
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-I" + os.path.join(ROOT, "include"),
+                    "-I" + os.path.join(ROOT, "qwen3.8-27b-in-c_amd", "csrc"), str(source), "-o", program], check=True)
+    run = subprocess.run([program], capture_output=True, text=True)
+    assert run.returncode == 0, run.stdout
+    return run.stdout
+
+
+def test_limits_are_the_documented_ones(tmp_path):
+    """the most rows that the header names fit a launch and one more does not; the calls refuse those"""
+    declared = " ".join(open(os.path.join(ROOT, "include", "q38hip.h")).read().replace("*", " ").split())
+    for limit in ("rows ceil(width / 2048) below 2^24", "rows below 2^24, with widths above 8192 below 2^22",
+                  "heads head_dim <= 2^20, rows below 2^24"):
+        assert limit in declared, limit
+    _run_cpp(tmp_path, LIMIT_CHECK)
+    norm = dict(output=P, output_row=8193, codes=None, scales=None, total=None, total_row=0, x=2 * P, x_row=8193, addend=None,
+                addend_row=0, type=30, weight=3 * P, weight_type=0, offset=0.0, eps=1e-6, width=8193, rows=1 << 22, stream=None)
+    _refused("q38hip_rms_norm", norm, [dict(), dict(width=1, rows=1 << 24)])
+    quantize = dict(codes=2 * P, scales=3 * P, x=P, x_row=2049, gate=None, gate_row=0, type=0, width=2049, rows=1 << 23, stream=None)
+    _refused("q38hip_quantize_e4m3", quantize, [dict(), dict(width=1, rows=1 << 24)])
