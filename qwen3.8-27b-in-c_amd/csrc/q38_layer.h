@@ -154,6 +154,45 @@ struct PromptAttention {
     int type;
 };
 
+/* How packed prompts are attended to: a wavefront to a row and head, or tiles of columns (a row and one
+ * of the heads that share keys and values), with the keys in two parts or the columns shared by four
+ * wavefronts. */
+enum { kPromptRows = 0, kPromptTiles, kPromptParts, kPromptShares };
+constexpr uint32_t kPromptColumns = 128, kPromptSharedColumns = 32;
+struct PromptPlan {
+    int form;
+    uint32_t workgroups;
+};
+inline PromptPlan plan_prompt(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t element, uint32_t count)
+{
+    /* Few rows have few keys.  A wavefront to a row and head, against tiles, in us: 24 heads of 256
+     * on 4, fp32, 64 rows 9.5 against 11.5, 128 rows 21 against 18; 5 of 256 on 5, fp32, 320 rows 32 against 35;
+     * 24 of 256 bf16, 64 rows 8.1 against 11.7, 128 rows 20.7 against 13.7; 32 of 128, bf16, 64 rows 6.1
+     * against 7.6, 128 rows 13.8 against 8.8, fp32 128 rows 18 against 24, 200 rows 39 against 35; 16 of 64, fp32,
+     * 128 rows 8.4 against 14.7. */
+    const bool full = element == 4 && head_dim == 256;
+    if (rows <= (element == 4 ? 64 + head_dim : 64) && (element == 2 || rows * heads <= (full ? 2048u : 5120u)))
+        return {kPromptRows, layer_up(rows * heads, 4)};
+    /* a tile more for each sequence where tiles follow them */
+    const uint32_t columns = rows * (heads / kv_heads), more = count <= 64 ? count : 0, spare = more * kv_heads;
+    const auto tiles = [&](uint32_t size) { return (layer_up(columns, size) + more) * kv_heads; };
+    const uint32_t workgroups = tiles(kPromptColumns);
+    /* A tile of 256-wide fp32 heads takes 8.6 us for 32 keys, so where there are fewer tiles than units,
+     * columns are shared: 5 heads on 5, 1375 tokens (60 tiles) 140 us against 364, 24 on 4, 1000 (192)
+     * 175 against 272, 2048 (384) 637 against 540.  Tiles that run over sequences see few keys each, so what matters is
+     * how evenly they fill the units: 24 on 4, 100 prompts, of 15 tokens (284) 42 against 49, 18 (340) 50 against 50,
+     * 24 (452) 65 against 58; 5 on 5, of 100 (395) 110 against 134. */
+    if (full && workgroups <= (more ? 256 + spare : 400)) return {kPromptShares, tiles(kPromptSharedColumns)};
+    /* Tiles that do not fill the card twice over: both halves of the registers go to one of them,
+     * unless keys are few.  Two parts against one, in us: bf16, 24 heads of 256, 1024 tokens (192
+     * tiles) 38 against 42, 2048 (384) 70 against 86, 3500 (660) 179 against 163, 12 prompts of up to 300
+     * (244) 29 against 22; 32 heads of 128, 700 tokens (176) 18.3 against 19.4, 2700 (680) 84 against 69, 12
+     * prompts of up to 300 (328) 19 against 13; fp32, 2048 tokens (512) 283 against 365; 66 prompts of 260, 4 heads on 4
+     * (540), bf16, 64-wide 24 against 17, 256-wide 63 against 48. */
+    if (!full && workgroups <= 512 + spare && rows >= 256ull * count) return {kPromptParts, workgroups};
+    return {kPromptTiles, workgroups};
+}
+
 #if defined(__HIPCC__)
 bool launch_quantize_e4m3(const QuantizeRows &a, int type, hipStream_t stream);
 bool launch_rms_norm(const NormRows &a, int type, hipStream_t stream);

@@ -764,6 +764,9 @@ __global__ void __launch_bounds__((PromptTile<T, D, kShares>::kWaves * 64 * kPar
     }
 }
 
+static_assert(PromptTile<float, 256, 1>::kColumns == kPromptColumns && PromptTile<float, 256, 4>::kColumns == kPromptSharedColumns,
+              "the plan's columns");
+
 template <typename T, int D>
 bool attention(const PromptAttention &a, hipStream_t stream)
 {
@@ -773,36 +776,14 @@ bool attention(const PromptAttention &a, hipStream_t stream)
     };
     const bool wide = whole(a.query, a.query_row) && whole(a.gate, a.query_head) && whole(a.key, a.key_row) &&
                       whole(a.value, a.value_row) && whole(a.output, a.output_row);
-    /* Few rows have few keys.  A wavefront to a row and head, against tiles, in us: 24 heads of 256
-     * on 4, fp32, 64 rows 9.5 against 11.5, 128 rows 21 against 18; 5 of 256 on 5, fp32, 320 rows 32 against 35;
-     * 24 of 256 bf16, 64 rows 8.1 against 11.7, 128 rows 20.7 against 13.7; 32 of 128, bf16, 64 rows 6.1
-     * against 7.6, 128 rows 13.8 against 8.8, fp32 128 rows 18 against 24, 200 rows 39 against 35; 16 of 64, fp32,
-     * 128 rows 8.4 against 14.7. */
-    constexpr uint32_t kFew = sizeof(T) == 4 ? 64 + D : 64, kFewWaves = D * sizeof(T) == 1024 ? 2048 : 5120;
-    if (a.rows <= kFew && (sizeof(T) == 2 || a.rows * a.heads <= kFewWaves))
-        return launch_kernel(wide ? row_kernel<T, D, true> : row_kernel<T, D, false>, dim3(layer_up(a.rows * a.heads, 4)), dim3(256),
-                             stream, a);
-    /* a tile more for each sequence where tiles follow them */
-    const uint32_t columns = a.rows * (a.heads / a.kv_heads), more = a.count <= 64 ? a.count : 0;
-    const auto tiles = [&](uint32_t size) { return dim3((layer_up(columns, size) + more) * a.kv_heads); };
-    const dim3 grid = tiles(PromptTile<T, D, 1>::kColumns);
-    /* A tile of 256-wide fp32 heads takes 8.6 us for 32 keys, so where there are fewer tiles than units,
-     * columns are shared: 5 heads on 5, 1375 tokens (60 tiles) 140 us against 364, 24 on 4, 1000 (192)
-     * 175 against 272, 2048 (384) 637 against 540. */
+    const PromptPlan plan = plan_prompt(a.rows, a.heads, a.kv_heads, D, sizeof(T), a.count);
+    const auto go = [&](auto kernel, uint32_t threads) { return launch_kernel(kernel, dim3(plan.workgroups), dim3(threads), stream, a); };
+    if (plan.form == kPromptRows) return go(wide ? row_kernel<T, D, true> : row_kernel<T, D, false>, 256);
     if constexpr (D * sizeof(T) == 1024)
-        if (grid.x <= 256 + a.count * a.kv_heads)
-            return launch_kernel(wide ? prompt_kernel<T, D, true, 1, 4> : prompt_kernel<T, D, false, 1, 4>,
-                                 tiles(PromptTile<T, D, 4>::kColumns), dim3(256), stream, a);
-    /* Tiles that do not fill the card twice over: both halves of the registers go to one of them,
-     * unless keys are few.  Two parts against one, in us: bf16, 24 heads of 256, 1024 tokens (192
-     * tiles) 38 against 42, 2048 (384) 70 against 86, 3500 (660) 179 against 163, 12 prompts of up to 300
-     * (244) 29 against 22; 32 heads of 128, 700 tokens (176) 18.3 against 19.4, 2700 (680) 84 against 69, 12
-     * prompts of up to 300 (328) 19 against 13; fp32, 2048 tokens (512) 283 against 365. */
+        if (plan.form == kPromptShares) return go(wide ? prompt_kernel<T, D, true, 1, 4> : prompt_kernel<T, D, false, 1, 4>, 256);
     if constexpr (D * sizeof(T) < 1024)
-        if (grid.x <= 512 + a.count * a.kv_heads && a.rows >= 256 * a.count)
-            return launch_kernel(wide ? prompt_kernel<T, D, true, 2, 1> : prompt_kernel<T, D, false, 2, 1>, grid,
-                                 dim3(512), stream, a);
-    return launch_kernel(wide ? prompt_kernel<T, D, true, 1, 1> : prompt_kernel<T, D, false, 1, 1>, grid, dim3(256), stream, a);
+        if (plan.form == kPromptParts) return go(wide ? prompt_kernel<T, D, true, 2, 1> : prompt_kernel<T, D, false, 2, 1>, 512);
+    return go(wide ? prompt_kernel<T, D, true, 1, 1> : prompt_kernel<T, D, false, 1, 1>, 256);
 }
 
 template <typename T>

@@ -208,3 +208,47 @@ def test_product_of_small_whole_numbers(device, tokens, inputs, outputs, dtype):
     want, _ = lc.product(to_bytes(codes), scales, to_bytes(weight), factors)
     got = layer.product(rows8, weight, torch.from_numpy(factors).to(device), dtype)
     assert torch.equal(got.cpu(), torch.from_numpy(want).to(dtype))
+
+
+# ---- attention: counts of sequences ---------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("count", [9, 32, 62, 63, 64, 65, 130])
+def test_counts_of_sequences(device, count, dim, dtype):
+    """short prompts, by rows and by tiles, empty ones among them, rows before the first and behind the last that none owns"""
+    rng = np.random.default_rng(count)
+    for most in (1, 40):
+        lengths = rng.integers(0, most + 1, size=count)
+        lengths[rng.integers(count)] = most
+        starts = [2] + [2 + n for n in kc.offsets(lengths)[1:]]
+        rows = starts[-1] + 3
+        q, k, v = (_normal(rng, rows, h, dim, dtype=dtype) for h in (4, 2, 2))
+        want, mass, size, owned = lc.attention(f64(q), f64(k), f64(v), starts, dim ** -0.5)
+        out = torch.full_like(q, 7.0)
+        layer.attention(q, k, v, kc.words(starts, device), out=out)
+        lc.check(out[owned], want[owned], lc.attention_bound(want, mass, size, dtype, most)[owned])
+        assert (out[~owned] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_many_long_sequences(device, dim, dtype):
+    """more sequences than lanes, of a length at which keys go in two parts"""
+    rng = np.random.default_rng(dim)
+    lengths = [256 + int(n) for n in rng.integers(0, 9, size=66)]
+    starts = kc.offsets(lengths)
+    q, k, v = (_normal(rng, starts[-1], 1, dim, dtype=dtype) for _ in range(3))
+    want, mass, size, _ = lc.attention(f64(q), f64(k), f64(v), starts, dim ** -0.5)
+    lc.check(layer.attention(q, k, v, kc.words(starts, device)), want, lc.attention_bound(want, mass, size, dtype, max(lengths)))
+
+
+@pytest.mark.parametrize("each", [21, 22], ids=["columns shared", "columns of a wavefront"])
+def test_many_short_fp32_sequences(device, each):
+    """100 prompts of 256-wide fp32 heads on both sides of the border between the two forms of tiles"""
+    rng = np.random.default_rng(each)
+    starts = kc.offsets([each] * 100)
+    q, k, v = (_normal(rng, starts[-1], h, 256) for h in (24, 4, 4))
+    want, mass, size, _ = lc.attention(f64(q), f64(k), f64(v), starts, 1 / 16)
+    lc.check(layer.attention(q, k, v, kc.words(starts, device)), want, lc.attention_bound(want, mass, size, F32, each))

@@ -245,3 +245,48 @@ def test_limits_are_the_documented_ones(tmp_path):
     _refused("q38hip_rms_norm", norm, [dict(), dict(width=1, rows=1 << 24)])
     quantize = dict(codes=2 * P, scales=3 * P, x=P, x_row=2049, gate=None, gate_row=0, type=0, width=2049, rows=1 << 23, stream=None)
     _refused("q38hip_quantize_e4m3", quantize, [dict(), dict(width=1, rows=1 << 24)])
+
+
+PROMPT_CHECK = r"""
+#include <cstdio>
+#include <initializer_list>
+#include "q38_layer.h"
+using namespace q38;
+#define CHECK(x) do { if (!(x)) { std::printf("line %d: %s\n", __LINE__, #x); return 1; } } while (0)
+int main()
+{
+    /* more sequences than lanes have no spare tiles: both sides of 400 and 512 real ones */
+    CHECK(plan_prompt(100 * 30, 24, 4, 256, 4, 100).form == kPromptTiles && plan_prompt(100 * 30, 24, 4, 256, 4, 100).workgroups == 564);
+    CHECK(plan_prompt(2133, 24, 4, 256, 4, 100).form == kPromptShares && plan_prompt(2133, 24, 4, 256, 4, 100).workgroups == 4 * 400);
+    CHECK(plan_prompt(2134, 24, 4, 256, 4, 100).form == kPromptTiles && plan_prompt(2134, 24, 4, 256, 4, 100).workgroups == 4 * 101);
+    CHECK(plan_prompt(65536, 1, 1, 128, 2, 100).form == kPromptParts && plan_prompt(65537, 1, 1, 128, 2, 100).form == kPromptTiles);
+    /* up to 64 they have one each for each key/value head */
+    CHECK(plan_prompt(1365, 24, 4, 256, 4, 10).form == kPromptShares && plan_prompt(1365, 24, 4, 256, 4, 10).workgroups == 4 * 266);
+    CHECK(plan_prompt(1366, 24, 4, 256, 4, 10).form == kPromptTiles && plan_prompt(1366, 24, 4, 256, 4, 10).workgroups == 4 * 75);
+    CHECK(plan_prompt(16384, 4, 4, 128, 2, 64).form == kPromptParts && plan_prompt(16385, 4, 4, 128, 2, 64).form == kPromptTiles);
+    /* keys that are few on average go in one part, whatever the count */
+    CHECK(plan_prompt(25599, 1, 1, 128, 2, 100).form == kPromptTiles && plan_prompt(25600, 1, 1, 128, 2, 100).form == kPromptParts);
+    CHECK(plan_prompt(1 << 16, 1, 1, 64, 2, 1 << 24).form == kPromptTiles);
+    CHECK(plan_prompt(300, 65535, 65535, 256, 4, 1 << 17).form == kPromptTiles);
+    /* every launch of the sizes that are taken holds its threads, and has a tile or a wavefront for every row and head */
+    for (uint32_t rows = 1; rows <= 1u << 24; rows += 1 + rows / 3)
+        for (uint32_t heads = 1; heads <= 65535; heads += 1 + heads / 2)
+            for (uint32_t kv = 1; kv <= heads; ++kv)
+                if (heads % kv == 0 && (uint64_t)rows * heads <= 1u << 30)
+                    for (uint32_t dim = 64; dim <= 256; dim *= 2)
+                        for (uint32_t element = 2; element <= 4; element += 2)
+                            for (uint32_t count : {1u, 64u, 65u, 1000u, 1u << 24}) {
+                                const PromptPlan p = plan_prompt(rows, heads, kv, dim, element, count);
+                                CHECK(layer_launch_holds(p.workgroups, p.form == kPromptParts ? 512 : 256));
+                                if (p.form == kPromptRows) { CHECK(p.workgroups * 4ull >= (uint64_t)rows * heads); continue; }
+                                const uint64_t tiles = ((uint64_t)rows * (heads / kv) + (p.form == kPromptShares ? 31 : 127)) / (p.form == kPromptShares ? 32 : 128);
+                                CHECK(p.workgroups == (tiles + (count <= 64 ? count : 0)) * kv);
+                            }
+    return 0;
+}
+"""
+
+
+def test_prompt_plans(tmp_path):
+    """which form of attention is taken on both sides of each border, and that all launches hold it"""
+    _run_cpp(tmp_path, PROMPT_CHECK)
