@@ -131,7 +131,9 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(NormRows a)
     sum = 0.0;
 #pragma unroll
     for (int w = 0; w < THREADS / 64; ++w) sum += partial[w];
-    const float inverse = (float)(1.0 / sqrt(sum / (double)a.width + (double)a.eps));
+    /* in two factors: the inverse of a row near the ends of fp32's range is outside of it, or subnormal */
+    int power;
+    const float inverse = (float)frexp(1.0 / sqrt(sum / (double)a.width + (double)a.eps), &power);
 
     const auto finish = [&](float v[8], uint32_t at) {
         const uint32_t some = at < a.width ? min(8u, a.width - at) : 0;
@@ -145,7 +147,7 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(NormRows a)
             else
                 layer_load8<__bf16, kWhole>(w, static_cast<const __bf16 *>(a.weight) + at, some);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = (uint32_t)i < some ? v[i] * inverse * (w[i] + a.offset) : 0.0f;
+            for (int i = 0; i < 8; ++i) v[i] = (uint32_t)i < some ? ldexpf(v[i], power) * inverse * (w[i] + a.offset) : 0.0f;
             if (a.output) layer_store8<T, kWhole>(static_cast<T *>(a.output) + row * a.output_row + at, v, some);
         }
         if (a.codes) {

@@ -210,6 +210,44 @@ def test_product_of_small_whole_numbers(device, tokens, inputs, outputs, dtype):
     assert torch.equal(got.cpu(), torch.from_numpy(want).to(dtype))
 
 
+# ---- norm: rows of all sizes -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+@pytest.mark.parametrize("width", [256, 2050, 8200, 24580])
+def test_norm_of_rows_of_all_sizes(device, width, dtype):
+    """rows whose inverse root leaves fp32's range, or is subnormal in it: the inverse rounded once, the weight's sum, two products"""
+    rng = np.random.default_rng(width)
+    sizes = np.array([1e-44, 1e-42, 1e-39, 1e-38, 1e-30, 1e30, 1e37, 1e38, 3.3e38])[0 if dtype == F32 else 2:]
+    x = torch.from_numpy(rng.uniform(0.5, 1.0, size=(len(sizes), width)) * sizes[:, None] * rng.choice([-1.0, 1.0], size=(1, width)))
+    x = x.to(dtype).to(device)
+    weight = _normal(rng, width)
+    want = lc.rms_norm(f64(x), f64(weight), 0.0, 0.0)
+    bound = np.abs(want) * 5 * 2.0 ** -24 + lc.rounding(want, dtype) * 1.01
+    lc.check(layer.rms_norm(x, weight, 0.0), want, bound)
+    lc.check_quantized(layer.rms_norm(x, weight, 0.0, e4m3=True), want, 5 * 2.0 ** -24)
+    assert torch.isnan(layer.rms_norm(torch.zeros_like(x), weight, 0.0)).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,width", [(1, 256), (3, 5120), (2, 2051), (2, 24584), (5, 30001)])
+def test_norm_in_both_forms(device, rows, width, dtype):
+    """the call that writes rows of the type and rows in 8 bits, in place too: what the calls that write one of them give"""
+    rng = np.random.default_rng(width)
+    x, addend, weight = _normal(rng, rows, width, dtype=dtype), _normal(rng, rows, width, dtype=dtype), _normal(rng, width)
+    kind, stream = {F32: 0, F16: 1, BF16: 30}[dtype], torch.cuda.current_stream().cuda_stream
+    plain, total = layer.rms_norm(x, weight, addend=addend)
+    rows8 = layer.rms_norm(x, weight, addend=addend, e4m3=True)[0]
+    for place in range(3):
+        given, added = x.clone(), addend.clone()
+        y, t = (torch.empty_like(x), added) if place == 0 else (given, torch.empty_like(x)) if place == 1 else (added, given)
+        codes, scales = torch.empty_like(rows8.codes), torch.empty_like(rows8.scales)
+        assert layer._lib().q38hip_rms_norm(y.data_ptr(), width, codes.data_ptr(), scales.data_ptr(), t.data_ptr(), width, given.data_ptr(), width,
+                                            added.data_ptr(), width, kind, weight.data_ptr(), 0, 0.0, 1e-6, width, rows, stream)
+        assert torch.equal(y, plain) and torch.equal(t, total)
+        assert torch.equal(codes.view(torch.uint8), rows8.codes.view(torch.uint8)) and torch.equal(scales.view(torch.uint8), rows8.scales.view(torch.uint8))
+
+
 # ---- attention: counts of sequences ---------------------------------------------------------------
 
 
