@@ -473,7 +473,7 @@ int q38hip_rotary(void *output, uint64_t output_row_stride, uint64_t output_head
  * query_row_stride + h * query_head_stride elements of query and of gate;
  * rows of key, value and output are their strides apart, heads head_dim, which
  * is 64, 128 or 256, of at most 65535 heads; up to 2^24 rows and sequences,
- * total_rows * heads up to 2^30.  Scores, statistics and sums are in
+ * total_rows * heads up to 2^30, scale up to 2^127.  Scores, statistics and sums are in
  * fp32; in the second product the weights of 16-bit rows have 8 (BF16) or 11 (F16)
  * bits, those of F16 below 2^-9 of the largest weight of the same 32 or 64 keys
  * fewer (they are off by up to 2^-20 of that one). */

@@ -178,10 +178,10 @@ extern "C" int q38hip_prompt_attention(void *output, uint64_t output_row_stride,
         !element_aligned(key, type) || !element_aligned(value, type) || !aligned(row_starts, 4))
         return abi_fail("rows must be aligned to their elements");
     if (output == query || output == gate || output == key || output == value) return abi_fail("output must not be an input");
-    if (!std::isfinite(scale)) return abi_fail("scale must be finite");
     /* weights are equal where the scale is 0 (and where it is so small); a product with
      * -infinity must not become NaN there */
     const float factor = scale * 1.44269504088896340736f;
+    if (!std::isfinite(factor)) return abi_fail("scale must be finite, at most 2^127");
     const q38::PromptAttention a = {output, query, gate, key, value, output_row_stride, query_row_stride,
                                     query_head_stride, key_row_stride, value_row_stride, row_starts, count, total_rows,
                                     heads, kv_heads, head_dim, std::fabs(factor) < 0x1p-126f ? 0x1p-126f : factor,

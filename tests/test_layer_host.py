@@ -290,3 +290,13 @@ int main()
 def test_prompt_plans(tmp_path):
     """which form of attention is taken on both sides of each border, and that all launches hold it"""
     _run_cpp(tmp_path, PROMPT_CHECK)
+
+
+def test_attention_refuses_scales_beyond_the_exponent():
+    """scores are taken times scale * log2(e), which has to be finite too"""
+    good = dict(output=2 * P, output_row=512, query=P, gate=None, query_row=512, query_head=128, key=P, key_row=256, value=P,
+                value_row=256, type=30, heads=4, kv_heads=2, dim=128, scale=1.0, starts=P, count=1, rows=8, stream=None)
+    _refused("q38hip_prompt_attention", good, [dict(scale=s) for s in (3e38, -3e38, 2.4e38, math.inf, -math.inf, math.nan)])
+    for scale in (3e38, math.inf):
+        assert layer._lib().q38hip_prompt_attention(*dict(good, scale=scale).values()) == 0
+        assert q38hip.last_error() == "scale must be finite, at most 2^127"
