@@ -201,9 +201,12 @@ def rotary_frequencies(turned, base=10000.0, factor=1.0, original=None, fast=32.
     """Frequencies of the turned / 2 pairs (float32) and the magnitude for rotary(): base^(-2i / turned).  With a factor
     above 1 for longer contexts: divided by it for all pairs where `original` is None; else, with `original` the context
     that the model was trained on, pairs that turn at least `fast` times within it stay, those that turn at most `slow`
-    times are divided, those between are blended linearly in the pair's index, and the magnitude is 0.1 ln(factor) + 1."""
-    if turned < 2 or turned % 2 or not base > 1 or not factor >= 1 or (original is not None and not original > 0):
-        raise ValueError("expected an even number of channels, a base above 1 and a factor of at least 1")
+    times are divided, those between are blended linearly in the pair's index, and the magnitude is 0.1 ln(factor) + 1 (the
+    method of Peng, Quesnelle, Fan and Shippole, "YaRN: Efficient Context Window Extension of Large Language Models", 2023)."""
+    if turned < 2 or turned % 2 or not 1 < base < math.inf or not 1 <= factor < math.inf or not math.inf > fast > slow > 0 or \
+            (original is not None and not 0 < original < math.inf):
+        raise ValueError("expected an even number of channels, a base above 1, a factor of at least 1, a context above 0 and fast above "
+                         "slow above 0")
     pairs = torch.arange(turned // 2, dtype=torch.float64)
     plain, magnitude = base ** (-2 * pairs / turned), 1.0
     frequencies = plain / factor
@@ -211,7 +214,8 @@ def rotary_frequencies(turned, base=10000.0, factor=1.0, original=None, fast=32.
         # pair i turns original * base^(-2i / turned) / (2 pi) times
         at = lambda turns: turned * math.log(original / (2 * math.pi * turns)) / (2 * math.log(base))  # noqa: E731
         low, high = max(math.floor(at(fast)), 0), min(math.ceil(at(slow)), turned - 1)
-        part = ((pairs - low) / max(high - low, 0.001)).clamp(0, 1)
+        # where not even pair 0 turns more than `slow` times all are divided
+        part = ((pairs - low) / max(high - low, 0.001)).clamp(0, 1) if high > 0 else torch.ones_like(pairs)
         frequencies = plain * (1 - part) + frequencies * part
         magnitude = 0.1 * math.log(factor) + 1
     return frequencies.float().to(device), magnitude

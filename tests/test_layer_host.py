@@ -300,3 +300,23 @@ def test_attention_refuses_scales_beyond_the_exponent():
     for scale in (3e38, math.inf):
         assert layer._lib().q38hip_prompt_attention(*dict(good, scale=scale).values()) == 0
         assert q38hip.last_error() == "scale must be finite, at most 2^127"
+
+
+def test_blended_frequencies_at_the_ends():
+    """contexts in which no pair turns `slow` times, or all turn `fast` times; the borders themselves; arguments that have no blend"""
+    plain = layer.rotary_frequencies(64, 1e4)[0]
+    for original in (1, 3, 6):                   # pair 0 turns original / (2 pi) < 1 times: all are divided
+        assert torch.equal(layer.rotary_frequencies(64, 1e4, factor=4.0, original=original)[0], layer.rotary_frequencies(64, 1e4, factor=4.0)[0])
+    for original in (10 ** 7, 10 ** 9):          # the last pair turns original / (2 pi) * 1e4^(-62 / 64) > 32 times: all stay
+        assert torch.equal(layer.rotary_frequencies(64, 1e4, factor=4.0, original=original)[0], plain)
+    for original in (7, 50, 200, 4096, 100000, 600000):
+        for turned in (2, 4, 64, 128):
+            want = 1e4 ** (-np.arange(0, turned, 2) / turned)
+            share = layer.rotary_frequencies(turned, 1e4, factor=4.0, original=original)[0].double().numpy() / want
+            turns = original * want / (2 * np.pi)
+            assert np.allclose(share[turns >= 32], 1, rtol=2.0 ** -23) and np.allclose(share[turns <= 1], 0.25, rtol=2.0 ** -23)
+            assert (np.diff(share) <= 2.0 ** -22).all() and (share <= 1 + 2.0 ** -23).all() and (share >= 0.25 - 2.0 ** -23).all()
+    for bad in (dict(fast=1.0, slow=1.0), dict(fast=1.0, slow=2.0), dict(slow=0.0), dict(slow=-1.0), dict(fast=math.nan), dict(fast=math.inf),
+                dict(original=math.nan), dict(original=math.inf), dict(factor=math.inf), dict(factor=math.nan), dict(base=math.inf)):
+        with pytest.raises(ValueError):
+            layer.rotary_frequencies(64, **dict(dict(factor=4.0, original=4096), **bad))
