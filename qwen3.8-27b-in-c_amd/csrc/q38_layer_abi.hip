@@ -1,6 +1,7 @@
 /* C ABI of a decoder layer's operators (declared in include/q38hip.h): checks
  * of what the host can see, then the launch. */
 #include <cmath>
+#include <initializer_list>
 
 #include "q38_kernels.h"
 #include "q38_layer.h"
@@ -20,6 +21,14 @@ bool aligned(const void *p, uintptr_t bytes) { return (reinterpret_cast<uintptr_
 
 /* elements of whole numbers of bytes */
 bool element_aligned(const void *p, uint32_t type) { return aligned(p, type == (uint32_t)q38::kLayerF32 ? 4 : 2); }
+
+/* an output or a workspace that begins where another tensor of the call does */
+bool among(const void *p, std::initializer_list<const void *> others)
+{
+    for (const void *other : others)
+        if (p && p == other) return true;
+    return false;
+}
 
 const char *rows_fault(uint64_t width, uint32_t rows)
 {
@@ -49,7 +58,7 @@ extern "C" int q38hip_quantize_e4m3(uint8_t *codes, uint8_t *scales, const void 
     if (!element_type(type)) return abi_fail("rows must be F32, F16 or BF16");
     if (rows > 1 && (x_row_stride < width || (gate && gate_row_stride < width))) return abi_fail("row stride too small");
     if (!element_aligned(x, type) || !element_aligned(gate, type)) return abi_fail("rows must be aligned to their elements");
-    if (codes == x || codes == gate) return abi_fail("codes must not be an input");
+    if (among(codes, {x, gate}) || among(scales, {x, gate, codes})) return abi_fail("codes and scales must not be an input or each other");
     if (!q38::layer_launch_holds((uint64_t)rows * q38::quantize_parts(width), 256)) return abi_fail("more rows than a launch holds");
     const q38::QuantizeRows a = {codes, scales, x, gate, x_row_stride, gate_row_stride, (uint32_t)width,
                                  q38::e4m3_pitch(width), rows};
@@ -72,9 +81,9 @@ extern "C" int q38hip_rms_norm(void *output, uint64_t output_row_stride, uint8_t
     if (!element_aligned(x, type) || !element_aligned(output, type) || !element_aligned(addend, type) ||
         !element_aligned(total, type) || !element_aligned(weight, weight_type))
         return abi_fail("rows must be aligned to their elements");
-    if (output && output == total) return abi_fail("total and output must differ");
-    if (codes && (codes == x || codes == addend || codes == total || codes == output || codes == weight))
-        return abi_fail("codes must not be an input or another output");
+    if (among(output, {total, weight}) || among(total, {weight})) return abi_fail("total and output must differ, and not be the weight");
+    if (among(codes, {x, addend, total, output, weight}) || among(scales, {x, addend, total, output, weight, codes}))
+        return abi_fail("codes and scales must not be an input or another output");
     if (rows > 1 && ((total && ((total == x && total_row_stride != x_row_stride) ||
                                 (total == addend && total_row_stride != addend_row_stride))) ||
                      (output && ((output == x && output_row_stride != x_row_stride) ||
@@ -122,7 +131,8 @@ extern "C" int q38hip_gemm_e4m3(void *output, uint32_t type, uint64_t output_row
     if (!aligned(codes, 16) || !aligned(weight, 16)) return abi_fail("codes must be 16-byte aligned");
     if (!aligned(scales, 4) || !aligned(weight_scales, 4)) return abi_fail("scales must be 4-byte aligned");
     if (!element_aligned(output, type)) return abi_fail("output must be aligned to its elements");
-    if (output == codes || output == weight) return abi_fail("output must not be an input");
+    if (among(output, {codes, scales, weight, weight_scales})) return abi_fail("output must not be an input");
+    if (among(workspace, {output, codes, scales, weight, weight_scales})) return abi_fail("workspace must be memory of its own");
     if (q38::product_e4m3_workspace_bytes(batch_size, input_length, rows) && !workspace)
         return abi_fail("this product needs a workspace");
     if (!aligned(workspace, 16)) return abi_fail("workspace must be 16-byte aligned");
@@ -149,6 +159,7 @@ extern "C" int q38hip_rotary(void *output, uint64_t output_row_stride, uint64_t 
     if (!aligned(positions, 4) || !aligned(frequencies, 4)) return abi_fail("positions and frequencies must be 4-byte aligned");
     if (output == x && ((rows > 1 && output_row_stride != x_row_stride) || (heads > 1 && output_head_stride != x_head_stride)))
         return abi_fail("rows turned in place must keep their strides");
+    if (among(output, {positions, frequencies})) return abi_fail("output must not be the positions or frequencies");
     if (!std::isfinite(magnitude)) return abi_fail("magnitude must be finite");
     if (!q38::layer_launch_holds(rows, 256)) return abi_fail("more rows than a launch holds");
     const q38::Rotary a = {output, x, output_row_stride, output_head_stride, x_row_stride, x_head_stride, rows, heads,
@@ -177,7 +188,7 @@ extern "C" int q38hip_prompt_attention(void *output, uint64_t output_row_stride,
     if (!element_aligned(output, type) || !element_aligned(query, type) || !element_aligned(gate, type) ||
         !element_aligned(key, type) || !element_aligned(value, type) || !aligned(row_starts, 4))
         return abi_fail("rows must be aligned to their elements");
-    if (output == query || output == gate || output == key || output == value) return abi_fail("output must not be an input");
+    if (among(output, {query, gate, key, value, row_starts})) return abi_fail("output must not be an input");
     /* weights are equal where the scale is 0 (and where it is so small); a product with
      * -infinity must not become NaN there */
     const float factor = scale * 1.44269504088896340736f;

@@ -320,3 +320,30 @@ def test_blended_frequencies_at_the_ends():
                 dict(original=math.nan), dict(original=math.inf), dict(factor=math.inf), dict(factor=math.nan), dict(base=math.inf)):
         with pytest.raises(ValueError):
             layer.rotary_frequencies(64, **dict(dict(factor=4.0, original=4096), **bad))
+
+
+def test_outputs_that_are_inputs_are_refused():
+    """every output and workspace against every other tensor of its call, but for what may be in place; the message says so"""
+    at = {name: (i + 1) * 16 * P for i, name in enumerate("abcdefghi")}
+    calls = {
+        "q38hip_quantize_e4m3": (dict(codes=at["a"], scales=at["b"], x=at["c"], x_row=128, gate=at["d"], gate_row=128, type=0, width=128, rows=2,
+                                      stream=None), ("codes", "scales"), ("x", "gate"), ()),
+        "q38hip_rms_norm": (dict(output=at["a"], output_row=256, codes=at["b"], scales=at["c"], total=at["d"], total_row=256, x=at["e"], x_row=256,
+                                 addend=at["f"], addend_row=256, type=30, weight=at["g"], weight_type=0, offset=0.0, eps=1e-6, width=256, rows=3,
+                                 stream=None), ("output", "codes", "scales", "total"), ("x", "addend", "weight"),
+                            (("output", "x"), ("output", "addend"), ("total", "x"), ("total", "addend"))),
+        "q38hip_gemm_e4m3": (dict(output=at["a"], type=30, output_row=256, codes=at["b"], scales=at["c"], tokens=2, inputs=128, weight=at["d"],
+                                  weight_scales=at["e"], rows=256, workspace=at["f"], stream=None), ("output", "workspace"),
+                             ("codes", "scales", "weight", "weight_scales"), ()),
+        "q38hip_rotary": (dict(output=at["a"], output_row=512, output_head=128, x=at["b"], x_row=512, x_head=128, type=1, rows=3, heads=4, dim=128,
+                               positions=at["c"], frequencies=at["d"], pairs=32, interleaved=0, magnitude=1.0, stream=None), ("output",),
+                          ("x", "positions", "frequencies"), (("output", "x"),)),
+        "q38hip_prompt_attention": (dict(output=at["a"], output_row=512, query=at["b"], gate=at["c"], query_row=512, query_head=128, key=at["d"],
+                                         key_row=256, value=at["e"], value_row=256, type=30, heads=4, kv_heads=2, dim=128, scale=1.0,
+                                         starts=at["f"], count=1, rows=8, stream=None), ("output",), ("query", "gate", "key", "value", "starts"), ())}
+    for name, (good, outputs, inputs, allowed) in calls.items():
+        for output in outputs:
+            for other in outputs + inputs:
+                if other != output and (output, other) not in allowed:
+                    _refused(name, good, [{output: good[other]}])
+                    assert " must " in q38hip.last_error() and "kernel failed" not in q38hip.last_error(), (name, output, other)
