@@ -60,16 +60,22 @@ __device__ __forceinline__ f32x4 add_scaled(f32x4 sum, f32x4 p, float factor)
     for (int r = 0; r < 4; ++r) sum[r] = fmaf(p[r], factor, sum[r]);
     return sum;
 }
-/* both for fp32 outputs */
+/* Both for fp32 outputs.  The token's power of two goes into its bf16 values as far as 2^-100 and 2^100, where those and
+ * their products with codes are normal, the rest of it into the block's factor. */
+__device__ __forceinline__ uint32_t token_scale(uint32_t scale) { return min(max(scale, 127u - 100), 127u + 100); }
+__device__ __forceinline__ float block_factor(uint32_t scale, float factor)
+{
+    return scale == 255u ? __uint_as_float(0x7fc00000u) : ldexpf(factor, (int)scale - (int)token_scale(scale));
+}
 __device__ __forceinline__ f32x4 add_exact(f32x4 sum, i32x8 matrix, i32x8 token, uint32_t scale, float factor)
 {
-    const float power = __uint_as_float(scale << 23);
+    const float power = __uint_as_float(token_scale(scale) << 23);
     f32x4 p = {};
 #pragma unroll
     for (int q = 0; q < 4; ++q)
         p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(decoded(matrix[2 * q], matrix[2 * q + 1], 1.0f),
                                                     decoded(token[2 * q], token[2 * q + 1], power), p, 0, 0, 0);
-    return add_scaled(sum, p, scale == 255u ? __uint_as_float(0x7fc00000u) : factor);
+    return add_scaled(sum, p, factor);
 }
 
 template <typename T>
@@ -135,7 +141,7 @@ __global__ void __launch_bounds__(kWaves * 64) few_kernel(ProductE4M3 a)
         };
         const i32x8 w = load(matrix), token = load(codes);
         const float s = weight_scales[b];
-        if constexpr (std::is_same_v<T, float>) sum = add_exact(sum, w, token, scales[b], s);
+        if constexpr (std::is_same_v<T, float>) sum = add_exact(sum, w, token, scales[b], block_factor(scales[b], s));
         else sum = add_scaled(sum, block_product(w, token, scales[b]), s);
     }
 #pragma unroll
@@ -312,11 +318,14 @@ __global__ void __launch_bounds__((Tile::kThreads), 2) tile_kernel(ProductE4M3 a
                 for (int i = 0; i < 8; ++i) token[m][i] = (i < 4 ? low : high) ? token[m][i] : 0;
         }
         if constexpr (std::is_same_v<T, float>) {
+            float factors[WM];
+#pragma unroll
+            for (int m = 0; m < WM; ++m) factors[m] = block_factor(scale[m], factor);
 #pragma unroll
             for (int n = 0; n < WN; ++n) {
                 const i32x8 rows = read(row_low, row_high, n);
 #pragma unroll
-                for (int m = 0; m < WM; ++m) sum[n][m] = add_exact(sum[n][m], rows, token[m], scale[m], factor);
+                for (int m = 0; m < WM; ++m) sum[n][m] = add_exact(sum[n][m], rows, token[m], scale[m], factors[m]);
             }
         } else {
             /* a product's result takes longer than the next product's start: the sums of one

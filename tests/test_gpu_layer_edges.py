@@ -248,6 +248,36 @@ def test_norm_in_both_forms(device, rows, width, dtype):
         assert torch.equal(codes.view(torch.uint8), rows8.codes.view(torch.uint8)) and torch.equal(scales.view(torch.uint8), rows8.scales.view(torch.uint8))
 
 
+# ---- product: scales of all sizes ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+@pytest.mark.parametrize("tokens,inputs", [(16, 384), (40, 384), (128, 384), (200, 656), (600, 656)])
+def test_product_of_all_scales(device, tokens, inputs, dtype):
+    """every scale byte, against matrix scales that bring the product back into fp32's range; NaN for 255"""
+    rng = np.random.default_rng(tokens)
+    blocks = -(-inputs // 128)
+    finite = np.array([c for c in range(256) if c & 0x7f != 0x7f], dtype=np.uint8)
+    codes, weight = finite[rng.integers(0, len(finite), size=(tokens, inputs))], finite[rng.integers(0, len(finite), size=(257, inputs))]
+    to = lambda a, t: torch.from_numpy(a).to(device).view(t)  # noqa: E731
+    for first in range(0, 256, tokens):
+        scales = np.zeros((tokens, lc.pitch(inputs)), dtype=np.uint8)
+        scales[:, :blocks] = ((first + np.arange(tokens)) % 256)[:, None]
+        for power in (-100, -30, 30, 100):
+            factors = np.full((3, blocks), 2.0 ** power, dtype=np.float32)
+            # a block's largest sum times both scales within fp32's range, and its smallest
+            e = scales[:, 0].astype(int) - 127
+            inside = (e + power >= -126 + 18) & (e + power <= 127 - 27) & (scales[:, 0] != 255)
+            # on the way to it: what is beyond 2^100 times the matrix's factor; for 16-bit outputs the sums times the tokens' alone
+            inside &= np.abs(power + e - e.clip(-100, 100)) <= 126 if dtype == F32 else (e >= -126 + 18) & (e <= 127 - 27)
+            got = layer.product((to(codes, torch.float8_e4m3fn), to(scales, torch.float8_e8m0fnu)), to(weight, torch.float8_e4m3fn),
+                                torch.from_numpy(factors).to(device), dtype)
+            assert torch.isnan(got[torch.from_numpy(scales[:, 0] == 255)]).all()
+            if inside.any():
+                want, mass = lc.product(codes[inside], scales[inside], weight, factors)
+                lc.check(got[torch.from_numpy(inside)], want, lc.product_bound(want, mass, inputs, dtype))
+
+
 # ---- attention: counts of sequences ---------------------------------------------------------------
 
 
