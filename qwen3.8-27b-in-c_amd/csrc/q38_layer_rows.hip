@@ -180,7 +180,8 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(NormRows a)
 /* ---- rotary positions ------------------------------------------------------ */
 
 /* A workgroup takes a row, `parts` of them share one, or it takes `group` short rows.  Their angles are
- * formed once, in fp64, reduced to a turn and their sines and cosines kept in LDS for all heads; a thread then
+ * formed once, in fp64, reduced to a turn and their sines and cosines, times the magnitude, rounded to fp32 and kept in
+ * LDS for all heads (all of it in fp64: 12.2 us instead of 10.5 for 60000 rows of one head of 80, else no time); a thread then
  * takes eight pairs (or eight channels that are copied) of a head at a time.  Bound by bytes:
  * 8192 bf16 rows of 40 heads of 128 move 168 MB in 33 us, 5.1 TB/s; few rows by the latency of their
  * angles (16 rows 2.7 us). */
@@ -192,10 +193,10 @@ __global__ void __launch_bounds__(256) rotary_kernel(Rotary a, uint32_t parts, u
     for (uint32_t i = threadIdx.x; i < rows * a.pairs; i += blockDim.x) {
         const uint32_t r = kGroup ? i / a.pairs : 0;
         const double turns = (double)a.positions[row0 + r] * (double)a.frequencies[i - r * a.pairs] * 0.15915494309189533577;
-        float s, c;
-        sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-        sine[i] = s * a.magnitude;
-        cosine[i] = c * a.magnitude;
+        double s, c;
+        sincospi(2.0 * (turns - rint(turns)), &s, &c);
+        sine[i] = (float)(s * (double)a.magnitude);
+        cosine[i] = (float)(c * (double)a.magnitude);
     }
     __syncthreads();
     const uint32_t per_head = turned_items + pass_items;

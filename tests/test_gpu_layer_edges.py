@@ -278,6 +278,22 @@ def test_product_of_all_scales(device, tokens, inputs, dtype):
                 lc.check(got[torch.from_numpy(inside)], want, lc.product_bound(want, mass, inputs, dtype))
 
 
+# ---- rotary positions: the last bits -----------------------------------------------------------
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("rows,heads,dim,pairs,magnitude", [(7, 3, 256, 32, 1.0), (300, 2, 128, 64, 1.1386), (5000, 1, 80, 20, 1.25)])
+def test_rotary_rounds_its_factors_once(device, rows, heads, dim, pairs, magnitude, interleaved):
+    """Sine and cosine times the magnitude are rounded to fp32 once, from fp64; then two products and a sum."""
+    rng = np.random.default_rng(rows)
+    x = _normal(rng, rows, heads, dim)
+    frequencies, _ = layer.rotary_frequencies(2 * pairs, 1e6, device=device)
+    positions = rng.integers(0, 1 << 20, size=rows).astype(np.int32)
+    want, size = lc.rotary(f64(x), positions, f64(frequencies), interleaved, np.float64(np.float32(magnitude)))
+    bound = size * (2 * 2.0 ** -24 + 2 * np.pi * (1 << 20) / 6 * 2.0 ** -52) + lc.rounding(want, F32) * 1.01
+    lc.check(layer.rotary(x, kc.words(positions, device), frequencies, interleaved, magnitude), want, bound)
+
+
 # ---- attention: counts of sequences ---------------------------------------------------------------
 
 
