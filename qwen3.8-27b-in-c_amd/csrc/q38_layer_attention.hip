@@ -115,6 +115,8 @@ __device__ __forceinline__ void attend_row(const PromptAttention &a, uint32_t ro
         total *= shrink;
 #pragma unroll
         for (int u = 0; u < 4; ++u) total += s[u] = __builtin_amdgcn_exp2f(s[u] - base);
+        /* a score that is NaN: so are all channels, whatever follows */
+        if (kHidden && __any(total != total)) break;
 #pragma unroll
         for (int e = 0; e < kChannels; ++e) out[e] *= shrink;
 #pragma unroll
@@ -136,12 +138,17 @@ __device__ __forceinline__ void attend_row(const PromptAttention &a, uint32_t ro
                     for (int e = 0; e < kChannels; ++e) v[j][e] = from[e];
                 }
             }
+            const auto add = [&](auto all) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float weight = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(s[u]), j * 4));
+                for (int j = 0; j < 16; ++j) {
+                    const float weight = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(s[u]), j * 4));
 #pragma unroll
-                for (int e = 0; e < kChannels; ++e) out[e] = fmaf(weight, !kHidden || (uint32_t)j < seen ? static_cast<float>(v[j][e]) : 0.0f, out[e]);
-            }
+                    for (int e = 0; e < kChannels; ++e)
+                        out[e] = fmaf(weight, all || (uint32_t)j < seen ? static_cast<float>(v[j][e]) : 0.0f, out[e]);
+                }
+            };
+            if (!kHidden || seen >= 16) add(std::true_type());
+            else add(std::false_type());
         }
     }
     /* the four lanes of a score each counted it */
@@ -682,7 +689,9 @@ __global__ void __launch_bounds__((PromptTile<T, D, kShares>::kWaves * 64 * kPar
 
     /* A weight of 0 times a value that is not finite is NaN, so such values of rows that a
      * column does not see have got into its sums.  Whatever came out not finite is done
-     * again, row by row, from the rows that it sees. */
+     * again, row by row, from the rows that it sees: a tile's columns one after another, without the matrix unit.
+     * 24 heads of 256, bf16, 8197 tokens: 0.70 ms, with a NaN among the first row's values 41, its keys 1.0, both of the
+     * middle row 26 (2048 tokens: 0.08, 4.2, 0.24, 2.2). */
     const float inverse = 1.0f / halves_sum(total);
     float nothing = 0.0f;
 #pragma unroll

@@ -49,6 +49,30 @@ def test_infinite_values(device, form, dim, dtype):
     assert far.max() <= 1, "worst %g of its bound" % far.max()
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_keys_that_are_not_numbers(device, form, dim, dtype):
+    """rows that see such a key are NaN in all channels, others are as without"""
+    rng = np.random.default_rng(dim)
+    lengths = FORMS[form]
+    starts = kc.offsets(lengths)
+    rows = starts[-1]
+    q, k, v = (_normal(rng, rows, h, dim, dtype=dtype) for h in (4, 2, 2))
+    want, mass, size, _ = lc.attention(f64(q), f64(k), f64(v), starts, dim ** -0.5)
+    bound = lc.attention_bound(want, mass, size, dtype, max(lengths))
+    for share in (0.0, 0.1, 0.6):
+        k2, bad = k.clone(), np.zeros(want.shape, dtype=bool)
+        for a, b in zip(starts, starts[1:]):
+            row = a + int(share * (b - a))
+            k2[row, 1, 3] = np.nan
+            bad[row:b, 2:] = True
+        got = f64(layer.attention(q, k2, v, kc.words(starts, device)))
+        assert np.array_equal(np.isnan(got), bad)
+        far = np.abs(got - want)[~bad] / bound[~bad]
+        assert far.max() <= 1, "worst %g of its bound" % far.max()
+
+
 # ---- gates of all sizes -----------------------------------------------------------------
 
 GATES = [0.0, 1.0, -1.0, 20.0, -20.0, -40.0, 40.0, -60.0, -80.0, 87.0, -87.0, 87.5, -87.5, 88.0, -88.0, 89.0, -89.0, 90.0, -90.0, 95.0, -95.0, 100.0,
