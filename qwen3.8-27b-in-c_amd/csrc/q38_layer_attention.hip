@@ -184,6 +184,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -241,6 +243,16 @@ __device__ __forceinline__ f32x16 multiply(u32x4 rows, u32x4 columns, f32x16 c)
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, rows), __builtin_bit_cast(bf16x8, columns), c,
                                                        0, 0, 0);
     }
+}
+
+/* c + the two 16-bit numbers of a word, within 2^-22 of the sum */
+template <typename T>
+__device__ __forceinline__ float add_pair(uint32_t pair, float c)
+{
+    if constexpr (std::is_same_v<T, _Float16>)
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), f16x2{(_Float16)1.0f, (_Float16)1.0f}, c, false);
+    else
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), bf16x2{(__bf16)1.0f, (__bf16)1.0f}, c, false);
 }
 
 /* the value of both halves of the wavefront, in both */
@@ -634,17 +646,23 @@ __global__ void __launch_bounds__((PromptTile<T, D, kShares>::kWaves * 64 * kPar
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 score[t][r] = __builtin_amdgcn_exp2f(fmaf(score[t][r], scale, -base));
-                total += score[t][r];
+                if constexpr (sizeof(T) == 4) total += score[t][r];
             }
         if constexpr (sizeof(T) == 2) {
+            /* Weights are rounded to the values' type, which the matrix unit wants: half a step of each, which mostly
+             * cancels over the keys.  The total sums them as they are rounded, so that equal values stay what they are. */
             u32x4 weight[kKeys / 16];
+            float sums[4] = {total, 0.0f, 0.0f, 0.0f};       /* four chains: one would be waited for */
 #pragma unroll
             for (int s = 0; s < kKeys / 16; ++s) {
                 T e[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) e[j] = static_cast<T>(score[s / 2][s % 2 * 8 + j]);
                 weight[s] = __builtin_bit_cast(u32x4, e);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sums[j] = add_pair<T>(weight[s][j], sums[j]);
             }
+            total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < kKeys / 16 * (D / 32); ++i) {

@@ -185,6 +185,23 @@ def test_sink_within_a_step(device):
         lc.check(layer.attention(q, k, v, kc.words(starts, device)), want, bound)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_equal_values_stay(device, form, dim, dtype):
+    """Rows whose values are all equal give that value, whatever the weights: they are divided by the sum of what multiplies the
+    values.  In fp32 sums of n weights and terms are off by 2^-24 sqrt(n) each in the mean, four times that at most, and the
+    division and its product by two roundings; 16-bit results round that away."""
+    rng = np.random.default_rng(dim)
+    lengths = FORMS[form]
+    starts = kc.offsets(lengths)
+    q, k = _normal(rng, starts[-1], 4, dim, scale=3.0, dtype=dtype), _normal(rng, starts[-1], 2, dim, dtype=dtype)
+    v = _normal(rng, len(lengths), 2, dim).repeat_interleave(torch.tensor(lengths, device=device), 0).to(dtype)
+    got, want = f64(layer.attention(q, k, v, kc.words(starts, device))), f64(v).repeat(2, 1)
+    bound = np.abs(want) * (8 * 2.0 ** -24 * np.sqrt(max(lengths)) + 2 * 2.0 ** -24) if dtype == F32 else np.zeros_like(want)
+    assert (np.abs(got - want) <= bound).all(), "worst %g of the value" % (np.abs(got - want) / np.abs(want)).max()
+
+
 # ---- product: what 16-bit outputs keep --------------------------------------------------------
 
 # every tile size whole, cut along the inputs, and both; few tokens; rows that end inside a block
