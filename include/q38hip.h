@@ -459,8 +459,8 @@ int q38hip_gemm_e4m3(void *output, uint32_t type, uint64_t output_row_stride, co
  * positions[row] * frequencies[i] radians and multiplied by magnitude: (a, b)
  * becomes magnitude * (a cos - b sin, b cos + a sin).  The pair is channels
  * 2i and 2i + 1 where interleaved is not 0, else i and i + pairs; channels from
- * 2 * pairs on are copied.  Angles are formed in fp64, so far positions keep
- * the accuracy of near ones.  output may be x itself (same pointer and strides).
+ * 2 * pairs on are copied.  Angles and their sines and cosines are formed in fp64, so
+ * far positions keep the accuracy of near ones.  output may be x itself (same pointer and strides).
  * 2 * pairs <= head_dim <= 1024, heads * head_dim <= 2^20, rows below 2^24. */
 int q38hip_rotary(void *output, uint64_t output_row_stride, uint64_t output_head_stride, const void *x,
                   uint64_t x_row_stride, uint64_t x_head_stride, uint32_t type, uint32_t rows, uint32_t heads,
