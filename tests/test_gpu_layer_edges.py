@@ -377,3 +377,108 @@ def test_many_short_fp32_sequences(device, each):
     q, k, v = (_normal(rng, starts[-1], h, 256) for h in (24, 4, 4))
     want, mass, size, _ = lc.attention(f64(q), f64(k), f64(v), starts, 1 / 16)
     lc.check(layer.attention(q, k, v, kc.words(starts, device)), want, lc.attention_bound(want, mass, size, F32, each))
+
+
+# ---- attention: scales, hidden keys, offsets that change under a graph ---------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_scales_of_all_signs(device, form, dim, dtype):
+    """negative, zero, so small that all weights are equal, and so large that one is all"""
+    rng = np.random.default_rng(dim)
+    lengths = FORMS[form]
+    starts = kc.offsets(lengths)
+    q, k, v = (_normal(rng, starts[-1], h, dim, dtype=dtype) for h in (4, 2, 2))
+    for scale in (-dim ** -0.5, 0.0, 1e-42, -1e-30, 2.0):
+        want, mass, size, _ = lc.attention(f64(q), f64(k), f64(v), starts, scale)
+        lc.check(layer.attention(q, k, v, kc.words(starts, device), scale=scale), want, lc.attention_bound(want, mass, size, dtype, max(lengths)))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_keys_of_minus_infinity(device, form, dim, dtype):
+    """keys whose scores are -infinity have no part; a row that sees nothing else is NaN"""
+    rng = np.random.default_rng(dim)
+    lengths = FORMS[form]
+    starts = kc.offsets(lengths)
+    rows = starts[-1]
+    q, k, v = (_normal(rng, rows, h, dim, dtype=dtype) for h in (4, 2, 2))
+    q[..., 0] = q[..., 0].abs() + 0.25
+    hidden = rng.random(rows) < 0.3
+    for a, b in zip(starts, starts[1:]):
+        hidden[a:min(a + 3, b)] = True                   # the first rows see nothing
+        hidden[a + 3:min(a + 4, b)] = False
+    want, mass, size = np.full(q.shape, np.nan), np.full(q.shape, np.nan), np.zeros((rows, 4))
+    query, key, value = f64(q), f64(k), f64(v)
+    for a, b in zip(starts, starts[1:]):
+        seen = ~hidden[a:b] & np.tri(b - a, dtype=bool)
+        some = seen.any(1)
+        for h in range(4):
+            n, m, o = query[a:b, h], key[a:b, h // 2], value[a:b, h // 2]
+            scores = np.where(seen, n @ m.T * dim ** -0.5, -np.inf)[some]
+            weight = np.exp(scores - scores.max(1, keepdims=True))
+            weight /= weight.sum(1, keepdims=True)
+            want[a:b, h][some], mass[a:b, h][some] = weight @ o, weight @ np.abs(o)
+            size[a:b, h] = np.where(seen, np.abs(n) @ np.abs(m).T * dim ** -0.5, 0).max(1)
+    k[torch.from_numpy(np.flatnonzero(hidden)).to(device), :, 0] = -np.inf
+    got = f64(layer.attention(q, k, v, kc.words(starts, device)))
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    far = np.abs(got - want) / lc.attention_bound(want, mass, size, dtype, max(lengths))
+    assert np.nanmax(far) <= 1, "worst %g of its bound" % np.nanmax(far)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+@pytest.mark.parametrize("count,rows", [(3, 40), (4, 700), (64, 600), (80, 900)])
+def test_offsets_change_under_a_graph(device, count, rows, dtype):
+    """a captured call reads the offsets when it is replayed"""
+    rng = np.random.default_rng(count)
+    q, k, v = (_normal(rng, rows, h, 128, dtype=dtype) for h in (4, 2, 2))
+    words, out = torch.zeros(count + 1, dtype=torch.int32, device=device), torch.empty_like(q)
+    side = torch.cuda.Stream(device=device)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer.attention(q, k, v, words, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer.attention(q, k, v, words, out=out)
+    for _ in range(4):
+        starts = np.sort(rng.integers(0, rows + 1, size=count + 1))
+        words.copy_(kc.words(starts.tolist(), device))
+        out.fill_(7.0)
+        graph.replay()
+        want, mass, size, owned = lc.attention(f64(q), f64(k), f64(v), starts.tolist(), 128 ** -0.5)
+        lc.check(out[owned], want[owned], lc.attention_bound(want, mass, size, dtype, rows)[owned])
+        assert (out[~owned] == 7).all()
+
+
+# ---- product: codes that are not numbers, in every type and tile ------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("tokens,inputs,outputs", [(3, 400, 40), (16, 80, 33000), (40, 400, 300), (128, 144, 8200), (300, 912, 5000), (520, 400, 513)])
+def test_product_of_codes_that_are_not_numbers(device, tokens, inputs, outputs, dtype):
+    """a NaN code of a token or of a matrix row, a NaN scale of either, an infinite scale: theirs are the only outputs that are not finite"""
+    rng = np.random.default_rng(tokens)
+    blocks = -(-inputs // 128)
+    codes, weight = rng.integers(0x20, 0x50, size=(tokens, inputs)).astype(np.uint8), rng.integers(0x20, 0x50, size=(outputs, inputs)).astype(np.uint8)
+    scales = np.zeros((tokens, lc.pitch(inputs)), dtype=np.uint8)
+    scales[:, :blocks] = 120
+    factors = np.full((-(-outputs // 128), blocks), 0.01, dtype=np.float32)
+    for last in (False, True):                       # in the first block, and in the last, which may be part of one
+        c, w, s, f = codes.copy(), weight.copy(), scales.copy(), factors.copy()
+        at, block = (inputs - 1, blocks - 1) if last else (5, 0)
+        c[1, at], w[outputs - 7, at], s[2, block] = 0x7f, 0xff, 255
+        bad = np.zeros((tokens, outputs), dtype=bool)
+        bad[1], bad[2], bad[:, outputs - 7] = True, True, True
+        infinite = np.zeros_like(bad)
+        if len(f) > 2:
+            f[0, block], f[1, block] = np.nan, np.inf
+            bad[:, :128], infinite[:, 128:256] = True, True
+        to = lambda a, t: torch.from_numpy(a).to(device).view(t)  # noqa: E731
+        got = f64(layer.product((to(c, torch.float8_e4m3fn), to(s, torch.float8_e8m0fnu)), to(w, torch.float8_e4m3fn),
+                                torch.from_numpy(f).to(device), dtype))
+        assert np.array_equal(np.isnan(got), bad) and np.array_equal(np.isinf(got), infinite & ~bad)
