@@ -482,3 +482,91 @@ def test_product_of_codes_that_are_not_numbers(device, tokens, inputs, outputs, 
         got = f64(layer.product((to(c, torch.float8_e4m3fn), to(s, torch.float8_e8m0fnu)), to(w, torch.float8_e4m3fn),
                                 torch.from_numpy(f).to(device), dtype))
         assert np.array_equal(np.isnan(got), bad) and np.array_equal(np.isinf(got), infinite & ~bad)
+
+
+# ---- calls in other layouts ----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows", [1, 7, 300, 3000])
+def test_heads_before_rows(device, rows, dtype):
+    """queries (and gates) laid out [heads, rows, head_dim]: the same bits as [rows, heads, head_dim]"""
+    rng = np.random.default_rng(rows)
+    frequencies, positions = layer.rotary_frequencies(64, device=device)[0], torch.arange(rows, dtype=torch.int32, device=device)
+    words = kc.words([0, rows // 3, rows], device)
+    q, gate, k, v = (_normal(rng, rows, h, 128, dtype=dtype) for h in (4, 4, 2, 2))
+    other = lambda x: x.transpose(0, 1).contiguous().transpose(0, 1)  # noqa: E731
+    for interleaved in (False, True):
+        want = layer.rotary(q, positions, frequencies, interleaved)
+        assert torch.equal(layer.rotary(other(q), positions, frequencies, interleaved), want)
+        turned = other(q)
+        layer.rotary(turned, positions, frequencies, interleaved, out=turned)
+        assert torch.equal(turned, want)
+        into = other(torch.zeros_like(q))
+        layer.rotary(q, positions, frequencies, interleaved, out=into)
+        assert torch.equal(into, want)
+    assert torch.equal(layer.attention(other(q), k, v, words, gate=other(gate)), layer.attention(q, k, v, words, gate=gate))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("width", [128, 1000, 24600])
+def test_norm_weights_of_all_types(device, width, dtype):
+    """weights of another type than the rows', at any element"""
+    rng = np.random.default_rng(width)
+    x = _normal(rng, 5, width, dtype=dtype)
+    for kind in TYPES:
+        weight = _normal(rng, width + 3, dtype=kind)
+        for first in (0, 1, 3):
+            part = weight[first:first + width]
+            want = lc.rms_norm(f64(x), f64(part), 1e-6, 0.5)
+            bound = np.abs(want) * 5 * 2.0 ** -24 + lc.rounding(want, dtype) * 1.01
+            lc.check(layer.rms_norm(x, part, offset=0.5), want, bound)
+            lc.check_quantized(layer.rms_norm(x, part, offset=0.5, e4m3=True), want, 5 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,width", [(1, 128), (3, 1001), (40, 5120), (2, 24600)])
+def test_given_outputs(device, rows, width, dtype):
+    """results into the caller's tensors, in wider rows, and in place: the same bits as into new ones"""
+    rng = np.random.default_rng(width)
+    x, addend, weight = _normal(rng, rows, width, dtype=dtype), _normal(rng, rows, width, dtype=dtype), _normal(rng, width)
+    same = lambda a, b: torch.equal(a.codes.view(torch.uint8), b.codes.view(torch.uint8)) and \
+        torch.equal(a.scales.view(torch.uint8), b.scales.view(torch.uint8))  # noqa: E731
+    into = lambda: (torch.zeros(rows, width, dtype=torch.float8_e4m3fn, device=device),  # noqa: E731
+                    torch.ones(rows, layer.scale_pitch(width), dtype=torch.float8_e8m0fnu, device=device))
+    want = layer.quantize(x, gate=addend)
+    given = into()
+    got = layer.quantize(x, gate=addend, out=given)
+    assert same(got, want) and got.codes is given[0] and got.scales is given[1]
+    want, total = layer.rms_norm(x, weight, addend=addend, e4m3=True)
+    room = torch.full((rows, width + 5), 3.0, dtype=dtype, device=device)
+    got, summed = layer.rms_norm(x, weight, addend=addend, e4m3=True, out=into(), total=room[:, 2:width + 2])
+    assert same(got, want) and torch.equal(summed, total) and (room[:, :2] == 3).all() and (room[:, width + 2:] == 3).all()
+    want, total = layer.rms_norm(x, weight, addend=addend)
+    room.fill_(3.0)
+    got, summed = layer.rms_norm(x, weight, addend=addend, out=room[:, 1:width + 1])
+    assert torch.equal(got, want) and torch.equal(summed, total) and (room[:, :1] == 3).all() and (room[:, width + 1:] == 3).all()
+    for out, total_at in ((0, 1), (1, 0), (0, None), (1, None), (None, 0), (None, 1)):
+        pair = (x.clone(), addend.clone())
+        got, summed = layer.rms_norm(pair[0], weight, addend=pair[1], out=None if out is None else pair[out],
+                                     total=None if total_at is None else pair[total_at])
+        assert torch.equal(got, want) and torch.equal(summed, total)
+    plain, alone = layer.rms_norm(x, weight), x.clone()
+    assert layer.rms_norm(alone, weight, out=alone) is alone and torch.equal(alone, plain)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("tokens,inputs,outputs", [(1, 5120, 37), (3, 17408, 2001), (40, 400, 301), (200, 912, 1001), (600, 528, 770)])
+def test_product_into_rows_at_any_element(device, tokens, inputs, outputs, dtype):
+    """outputs that begin at odd elements in rows of odd length, nothing beside them written"""
+    rng = np.random.default_rng(tokens)
+    rows8 = layer.quantize(_normal(rng, tokens, inputs))
+    weight = (_normal(rng, outputs, inputs) * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+    scales = torch.full((-(-outputs // 128), -(-inputs // 128)), 1e-4, device=device)
+    want = layer.product(rows8, weight, scales, dtype)
+    for before, behind in ((1, 2), (3, 0), (0, 1)):
+        room = torch.full((tokens, before + outputs + behind), 3.0, dtype=dtype, device=device)
+        layer.product(rows8, weight, scales, out=room[:, before:before + outputs])
+        assert torch.equal(room[:, before:before + outputs], want)
+        room[:, before:before + outputs] = 3.0
+        assert (room == 3).all()
