@@ -471,10 +471,11 @@ int q38hip_rotary(void *output, uint64_t output_row_stride, uint64_t output_head
  * row_starts[i] .. row_starts[i + 1] - 1 of total_rows (device words,
  * non-decreasing).  output[row][head] = sum softmax(scale q.k) v over the rows
  * of its sequence up to itself, times sigmoid(gate) where gate is not NULL.
- * What other sequences and later rows hold, NaN included, has no part in it;
- * rows that see a value that is not finite are formed one by one, which makes a
- * prompt in which most do take up to 60 times as long (0.7 to 41 ms for 8197
- * bf16 tokens of 24 heads of 256), less where it is keys that are NaN.
+ * What other sequences and later rows hold, NaN included, has no part in it.
+ * Calls with values or keys that are not finite take longer: 3 to 8 times where
+ * many rows see them, and the up to 64 rows before such a one are formed one by one
+ * (0.3 ms each at 4096 tokens of 24 heads of 256), as all rows are that see infinite
+ * keys, or infinite values of F16 (up to 60 times as long).
  * Rows that no sequence owns are not written.  Where row_starts decrease, what
  * is written to rows of the output is unspecified.  Query head h reads
  * key/value head h / (heads / kv_heads).  Head h of a row begins at row *

@@ -350,6 +350,51 @@ __device__ __forceinline__ uint32_t value_turn(uint32_t row)
     return kRowBytes >= 256 ? (row & 3) << 2 | (row >> 2 & 3) : (row >> 1 & 1) << 2 | (row >> 2 & 3);
 }
 
+/* What is not finite among the values and keys of rows first .. last, of which all columns of a wavefront see latest ..
+ * earliest.  values: no row that a column may not see has one, and the others are too small for a sum of them to overflow
+ * (weights are below 2^9; fp16 rows' are larger, but their values end at 2^16), so what a column's sums make of the values that it sees is
+ * right.  fp16 weights may be 0 where they are small, times an infinity NaN: infinities do not count as right there.  key:
+ * the first row with a NaN among its keys, which makes all channels of a column that sees it NaN.  One more pass over the rows by
+ * each wavefront: 24 heads of 256, bf16, 8197 tokens 0.75 ms, with a NaN among the first row's values or keys 3.3, both of the
+ * middle row 6.0; 2048 tokens 0.08 and 0.39.  Without it every column that sees one is done again: 41 ms, 4.2. */
+struct Seen {
+    bool values;
+    int key;
+};
+template <typename T, int D, bool kWhole>
+__device__ __forceinline__ Seen look_over(const PromptAttention &a, uint32_t kv, int first, int last, int latest, int earliest, uint32_t lane)
+{
+    constexpr int E = 16 / (int)sizeof(T), kPieces = D / E, kRows = 64 / kPieces, kInFlight = 4;
+    const uint64_t at = kv * D + lane % kPieces * E;
+    const T *keys = static_cast<const T *>(a.key) + at, *values = static_cast<const T *>(a.value) + at;
+    uint32_t largest = 0, other = 0;
+    int key = INT32_MAX;
+    for (int from = first; from <= last; from += kInFlight * kRows) {
+        u32x4 k[kInFlight], v[kInFlight];
+#pragma unroll
+        for (int i = 0; i < kInFlight; ++i) {
+            const uint64_t row = min(from + i * kRows + (int)(lane / kPieces), last);
+            k[i] = load_piece<kWhole>(keys + row * a.key_row);
+            v[i] = load_piece<kWhole>(values + row * a.value_row);
+        }
+#pragma unroll
+        for (int i = 0; i < kInFlight; ++i) {
+            const int row = min(from + i * kRows + (int)(lane / kPieces), last);
+            const bool hidden = row < latest || row > earliest;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float x = static_cast<float>(reinterpret_cast<const T *>(&k[i])[e]);
+                const uint32_t bits = __float_as_uint(static_cast<float>(reinterpret_cast<const T *>(&v[i])[e])) & 0x7fffffffu;
+                if (x != x) key = min(key, row);
+                if (bits < 0x7f800000u) largest = max(largest, bits);
+                else if (hidden || (std::is_same_v<T, _Float16> && bits == 0x7f800000u)) other = 1;
+            }
+        }
+    }
+    key = wave_min(key);
+    return {wave_max_u32(other) == 0 && __uint_as_float(wave_max_u32(largest)) * (float)(last - first + 1) < 0x1p118f, key};
+}
+
 /* Causal attention of a tile of columns.
  *
  * S^T = K Q^T leaves each lane the scores of one column, and its result has, in
@@ -560,6 +605,7 @@ __global__ void __launch_bounds__((PromptTile<T, D, kShares>::kWaves * 64 * kPar
         return __builtin_bit_cast(u32x4, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
     };
 
+    const uint32_t span = row - start;
     /* one tile of each part at a time; where a part has none left it waits with the others */
     if (from + (int)part * kKeys <= to) {
         load(false, from + part * kKeys, 0);
@@ -614,7 +660,7 @@ __global__ void __launch_bounds__((PromptTile<T, D, kShares>::kWaves * 64 * kPar
             for (int i = 0; i < kAhead; ++i) ahead[i] = value_piece(value_at, i / (D / 32), i % (D / 32));
         }
         if (key < latest || key + kKeys - 1 > earliest) {
-            const uint32_t span = row - start, begin = key + 4 * half - start;
+            const uint32_t begin = key + 4 * half - start;
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
 #pragma unroll
@@ -706,10 +752,9 @@ __global__ void __launch_bounds__((PromptTile<T, D, kShares>::kWaves * 64 * kPar
     }
 
     /* A weight of 0 times a value that is not finite is NaN, so such values of rows that a
-     * column does not see have got into its sums.  Whatever came out not finite is done
-     * again, row by row, from the rows that it sees: a tile's columns one after another, without the matrix unit.
-     * 24 heads of 256, bf16, 8197 tokens: 0.70 ms, with a NaN among the first row's values 41, its keys 1.0, both of the
-     * middle row 26 (2048 tokens: 0.08, 4.2, 0.24, 2.2). */
+     * column does not see have got into its sums.  What came out not finite for another reason stays; the rest is done
+     * again, row by row, from the rows that it sees: a tile's columns one after another, without the matrix unit (4096
+     * tokens, 24 heads of 256: 0.3 ms a column). */
     const float inverse = 1.0f / halves_sum(total);
     float nothing = 0.0f;
 #pragma unroll
@@ -728,6 +773,13 @@ __global__ void __launch_bounds__((PromptTile<T, D, kShares>::kWaves * 64 * kPar
 #pragma unroll
         for (int w = 0; w < kShares; ++w) again |= (uint32_t)ranges[wave - share + w][0];
         again = __builtin_amdgcn_readfirstlane(again);
+    }
+    if (again) {
+        /* of the tiles that the wavefront took */
+        const int v0 = from + (lowest - from) / kKeys * kKeys, v1 = min(from + (highest - from) / kKeys * kKeys + kKeys - 1, to);
+        const Seen seen = look_over<T, D, kWhole>(a, kv, v0, v1, latest, earliest, lane);
+        const bool summed = inverse > 0.0f && inverse < INFINITY;
+        again &= ~(uint32_t)__ballot((seen.values && summed) || (uint32_t)(seen.key - start) <= span);
     }
     const uint32_t done = (uint32_t)__ballot(owned) & ~again;
 

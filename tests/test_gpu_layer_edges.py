@@ -73,6 +73,58 @@ def test_keys_that_are_not_numbers(device, form, dim, dtype):
         assert far.max() <= 1, "worst %g of its bound" % far.max()
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_values_that_are_not_numbers(device, form, dim, dtype):
+    """NaN and infinities among values at random places, next to each other and far apart: a channel of a row is NaN where it sees one
+    NaN or two infinities of different signs, infinite where it sees infinities of one, and as without elsewhere"""
+    rng = np.random.default_rng(dim)
+    lengths = FORMS[form]
+    starts = kc.offsets(lengths)
+    rows = starts[-1]
+    q, k, v = (_normal(rng, rows, h, dim, dtype=dtype) for h in (4, 2, 2))
+    want, mass, size, _ = lc.attention(f64(q), f64(k), f64(v), starts, dim ** -0.5)
+    bound = lc.attention_bound(want, mass, size, dtype, max(lengths))
+    for kinds in ((np.nan,), (np.inf, -np.inf), (np.nan, np.inf, -np.inf)):
+        v2, seen = v.clone(), np.zeros((3,) + want.shape, dtype=bool)
+        for a, b in zip(starts, starts[1:]):
+            for row in rng.integers(a, b, size=4):
+                channel, kind = int(rng.integers(dim // 2)), int(rng.integers(len(kinds)))
+                v2[row, 1, channel] = kinds[kind]
+        given = f64(v2)[:, 1]
+        for a, b in zip(starts, starts[1:]):
+            for i, found in enumerate((np.isnan(given[a:b]), given[a:b] == np.inf, given[a:b] == -np.inf)):
+                seen[i, a:b, 2:] = np.logical_or.accumulate(found, 0)[:, None]
+        nan = seen[0] | seen[1] & seen[2]
+        got = f64(layer.attention(q, k, v2, kc.words(starts, device)))
+        assert np.array_equal(np.isnan(got), nan)
+        assert np.array_equal(got == np.inf, seen[1] & ~nan) and np.array_equal(got == -np.inf, seen[2] & ~nan)
+        rest = ~seen.any(0)
+        far = np.abs(got - want)[rest] / bound[rest]
+        assert far.max() <= 1, "worst %g of its bound" % far.max()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lengths", [[700], [300, 70, 260], [25, 90] * 33], ids=["two parts", "one part", "many"])
+def test_sums_beyond_the_range_beside_a_nan(device, lengths, dim, dtype):
+    """Values of 1e35 whose weights are up to 2^7 before they are divided: the sums of a tile leave fp32, the result does not.  A NaN in
+    another channel, which all rows see, changes nothing.  Weights as in attention_bound, of terms that are all alike."""
+    starts = kc.offsets(lengths)
+    rows = starts[-1]
+    q, k = torch.zeros(rows, 2, dim, dtype=dtype, device=device), torch.zeros(rows, 1, dim, dtype=dtype, device=device)
+    q[..., 0] = 1.0
+    for a, b in zip(starts, starts[1:]):
+        k[a + 16:b, 0, 0] = 4.5 * dim ** 0.5         # 2^6.5
+    v = torch.full((rows, 1, dim), 1e35, dtype=dtype, device=device)
+    v[starts[:-1], 0, 3] = float("nan")
+    got = f64(layer.attention(q, k, v, kc.words(starts, device)))
+    assert np.isnan(got[..., 3]).all()
+    want, rest = float(v[1, 0, 0].double()), [c for c in range(dim) if c != 3]
+    assert np.abs(got[..., rest] / want - 1).max() <= 2.0 ** -14 + (lc.HALF_STEP[BF16] if dtype == BF16 else 0)
+
+
 # ---- gates of all sizes -----------------------------------------------------------------
 
 GATES = [0.0, 1.0, -1.0, 20.0, -20.0, -40.0, 40.0, -60.0, -80.0, 87.0, -87.0, 87.5, -87.5, 88.0, -88.0, 89.0, -89.0, 90.0, -90.0, 95.0, -95.0, 100.0,
